@@ -55,6 +55,14 @@ _OP_NAMES = (
     "patch_merge_norm_3d",
     "proj_out_norm_3d",
     "window_linear",
+    "relative_position_bias",
+    "relative_position_bias_backward",
+    "swin_window_attention_qkv_backward",
+    "norm_gate_residual",
+    "norm_gate_residual_backward",
+    "gelu_checkpoint",
+    "gelu_checkpoint_backward",
+    "restore_activation",
 )
 
 
@@ -299,6 +307,21 @@ from .block_fusion import (  # noqa: E402
     patch_merge_norm_3d,
     proj_out_norm_3d,
 )
+from .training import (  # noqa: E402
+    relative_position_buckets,
+    relative_position_bias,
+    relative_position_bias_backward,
+    swin_window_attention_train,
+    swin_window_attention_backward,
+    norm_gate_residual,
+    norm_gate_residual_backward,
+    gelu_checkpoint,
+    gelu_checkpoint_backward,
+    restore_activation,
+    checkpointed_mlp,
+    enable_training_kernels,
+    disable_training_kernels,
+)
 
 
 def device_status(clear: bool = False, device: torch.device | int | None = None) -> int:
@@ -353,6 +376,19 @@ __all__ = [
     "patch_merge_norm_3d",
     "proj_out_norm_3d",
     "window_linear",
+    "relative_position_buckets",
+    "relative_position_bias",
+    "relative_position_bias_backward",
+    "swin_window_attention_train",
+    "swin_window_attention_backward",
+    "norm_gate_residual",
+    "norm_gate_residual_backward",
+    "gelu_checkpoint",
+    "gelu_checkpoint_backward",
+    "restore_activation",
+    "checkpointed_mlp",
+    "enable_training_kernels",
+    "disable_training_kernels",
     "patch_monai_swin_unetr",
     "unpatch_monai_swin_unetr",
     "clear_mask_cache",

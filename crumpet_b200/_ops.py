@@ -136,6 +136,31 @@ def capi() -> ctypes.CDLL:
         lib.crumpet_roi_accumulate.restype = i32
         lib.crumpet_roi_argmax.argtypes = [vp, vp, vp, vp, vp, vp] + [i64] * 4 + [vp]
         lib.crumpet_roi_argmax.restype = i32
+        f32 = ctypes.c_float
+        lib.crumpet_relative_position_bias.argtypes = [vp, i32, vp, i32, i64, i64, vp, i64, vp]
+        lib.crumpet_relative_position_bias.restype = i32
+        lib.crumpet_relative_position_bias_backward.argtypes = [
+            vp, i32, i64, vp, i32, i64, vp, i64, vp, i64, vp, i64, vp, vp]
+        lib.crumpet_relative_position_bias_backward.restype = i32
+        lib.crumpet_window_attention_backward_shares.argtypes = [i64] * 4 + [i32]
+        lib.crumpet_window_attention_backward_shares.restype = i64
+        lib.crumpet_swin_window_attention_qkv_backward.argtypes = (
+            [vp] * 6 + [i32, i64, vp, i64] + [i64] * 9 + [i32] + [i64] * 4 + [f32, vp])
+        lib.crumpet_swin_window_attention_qkv_backward.restype = i32
+        lib.crumpet_norm_gate_residual.argtypes = (
+            [vp] * 4 + [i32, i32, vp, vp, i64] + [vp] * 4 + [f32, i64, i64, vp])
+        lib.crumpet_norm_gate_residual.restype = i32
+        lib.crumpet_norm_gate_residual_backward_partials.argtypes = [i64, i64]
+        lib.crumpet_norm_gate_residual_backward_partials.restype = i64
+        lib.crumpet_norm_gate_residual_backward.argtypes = (
+            [vp] * 11 + [i32, i32, vp, vp, i64] + [vp] * 3 + [f32, vp, i64, i64, vp])
+        lib.crumpet_norm_gate_residual_backward.restype = i32
+        lib.crumpet_gelu_checkpoint.argtypes = [vp] * 4 + [i32, i64, i64, vp]
+        lib.crumpet_gelu_checkpoint.restype = i32
+        lib.crumpet_gelu_checkpoint_backward.argtypes = [vp] * 5 + [i32, i64, i64, vp]
+        lib.crumpet_gelu_checkpoint_backward.restype = i32
+        lib.crumpet_restore_activation.argtypes = [vp] * 3 + [i32, i64, i64, vp]
+        lib.crumpet_restore_activation.restype = i32
         lib.crumpet_last_error.argtypes = []
         lib.crumpet_last_error.restype = ctypes.c_char_p
         lib.crumpet_abi_version.argtypes = []

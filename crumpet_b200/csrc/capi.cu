@@ -432,6 +432,281 @@ int crumpet_roi_argmax(uint8_t* labels, float* logits, const float* acc, const f
                            static_cast<cudaStream_t>(stream));
 }
 
+int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
+                                   int64_t table_rows, int64_t H, const int* pairs, int64_t npairs,
+                                   void* stream) {
+  if (int e = check_dtype(out_dtype)) return e;
+  if (int e = check_dtype(table_dtype)) return e;
+  if (H < 0 || npairs < 0) return set_error(kErrInvalid, "H and npairs must be non-negative");
+  if (H == 0 || npairs == 0) return kOk;
+  if (table_rows < 1 || table_rows > 0x7fffffff || npairs > 0x7fffffff || H > 0xffff)
+    return set_error(kErrInvalid, "relative position bias: table_rows, npairs or H out of range");
+  if (!bias || !table || !pairs) return set_error(kErrInvalid, "null tensor pointer");
+  return launch_relative_position_bias(bias, out_dtype, table, table_dtype, pairs, npairs,
+                                       table_rows, H, static_cast<cudaStream_t>(stream));
+}
+
+int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, int64_t H,
+                                            const void* grad, int grad_dtype, int64_t slabs,
+                                            const int* order, int64_t npairs, const int* items,
+                                            int64_t n_items, const int* multi, int64_t n_multi,
+                                            float* partial, void* stream) {
+  if (int e = check_dtype(table_dtype)) return e;
+  if (int e = check_dtype(grad_dtype)) return e;
+  if (H < 0 || npairs < 0 || n_items < 0 || n_multi < 0)
+    return set_error(kErrInvalid, "H, npairs, n_items and n_multi must be non-negative");
+  if (H == 0 || n_items == 0) return kOk;
+  if (npairs > 0x7fffffff || H > 0xffff || n_items > 0x7fffffff || slabs < 0 || slabs > 0x7fffffff)
+    return set_error(kErrInvalid, "relative position bias: npairs, H, items or slabs out of range");
+  if (!grad_table || !items || (npairs > 0 && (!grad || !order)) ||
+      (n_multi > 0 && (!multi || !partial)))
+    return set_error(kErrInvalid, "null tensor pointer");
+  BiasGradArgs a{};
+  a.grad_table = grad_table;
+  a.table_dtype = table_dtype;
+  a.grad = grad;
+  a.grad_dtype = grad_dtype;
+  a.slabs = slabs;
+  a.npairs = npairs;
+  a.H = H;
+  a.order = order;
+  a.items = items;
+  a.multi = multi;
+  a.n_items = n_items;
+  a.n_multi = n_multi;
+  a.partial = partial;
+  return launch_relative_position_bias_grad(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N, int64_t head_dim,
+                                                 int dtype) {
+  if (B < 0 || H < 1 || N < 1) return 0;
+  return attention_grad_tensor_path(dtype, N, head_dim) ? attention_grad_shares(B, H, N)
+                                                        : attention_grad_shares_simt(B, H, N);
+}
+
+int crumpet_swin_window_attention_qkv_backward(
+    void* grad_qkv, float* grad_bias, float* stats, const void* grad_out, const void* qkv,
+    const void* bias_table, int table_f32, int64_t table_rows, const int* pairs, int64_t shares,
+    int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d, int64_t ws_h, int64_t ws_w,
+    int64_t ss_d, int64_t ss_h, int64_t ss_w, int dtype, int64_t B, int64_t H, int64_t N,
+    int64_t head_dim, float scale, void* stream) {
+  if (int e = check_dtype(dtype)) return e;
+  if (!simt_attention_head_dim(head_dim))
+    return set_error(kErrUnsupported,
+                     "window attention requires a power-of-two head_dim between 16 and 256");
+  if (B < 0 || H < 1 || N < 1) return set_error(kErrInvalid, "B must be >= 0, H and N >= 1");
+  if (!(scale > 0.f) || !(scale < 1e30f))
+    return set_error(kErrUnsupported, "window attention requires a finite scale > 0");
+  if (B > 0x7fffffff || H > 0xffff || N > 46340)
+    return set_error(kErrInvalid, "B, H or N too large");
+  const bool shifted = (ss_d | ss_h | ss_w) != 0;
+  if (shifted) {
+    const int64_t ws[3] = {ws_d, ws_h, ws_w}, ss[3] = {ss_d, ss_h, ss_w};
+    if (nw_d < 1 || nw_h < 1 || nw_w < 1 || ws_d < 1 || ws_h < 1 || ws_w < 1 ||
+        ws_d * ws_h * ws_w != N)
+      return set_error(kErrInvalid, "analytic mask geometry does not match N");
+    if (nw_d > 0xffff || nw_h > 0xffff || nw_w > 0xffff || nw_d * nw_h * nw_w > 0x7fffffff)
+      return set_error(kErrInvalid, "too many windows per axis");
+    for (int a = 0; a < 3; ++a)
+      if (ss[a] < 0 || ss[a] >= ws[a])
+        return set_error(kErrInvalid, "analytic mask shift must satisfy 0 <= shift < window");
+  }
+  const bool sized = attention_grad_tensor_path(dtype, N, head_dim);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(grad_qkv) |
+                         reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(qkv);
+  if (shares < 1 || shares > 0xffff || shares > (B > 0 ? B : 1))
+    return set_error(kErrInvalid, "shares must be between 1 and the number of windows");
+  if (H * ((N + 63) / 64) * shares > 0x7fffffff)
+    return set_error(kErrInvalid, "too many windows x heads for one launch");
+  if (!grad_bias) return set_error(kErrInvalid, "null tensor pointer");
+  if (B == 0) {  // no window: no gradient of the bias
+    const cudaError_t e = cudaMemsetAsync(grad_bias, 0, size_t(shares * H * N * N) * sizeof(float),
+                                          static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? kOk : set_cuda_error(e, "window attention backward memset");
+  }
+  if (!grad_qkv || !stats || !grad_out || !qkv || !bias_table || !pairs)
+    return set_error(kErrInvalid, "null tensor pointer");
+  if (table_rows < 1) return set_error(kErrInvalid, "relative position bias table has no rows");
+  if (reinterpret_cast<uintptr_t>(stats) & 7u)
+    return set_error(kErrInvalid, "stats must be 8-byte aligned");
+  AttnGradArgs a{};
+  a.grad_qkv = grad_qkv;
+  a.grad_bias = grad_bias;
+  a.stats = stats;
+  a.grad_out = grad_out;
+  a.qkv = qkv;
+  a.table = bias_table;
+  a.table_f32 = table_f32 != 0 || dtype == kF32;
+  a.pairs = pairs;
+  a.nwin[0] = nw_d;
+  a.nwin[1] = nw_h;
+  a.nwin[2] = nw_w;
+  a.win[0] = ws_d;
+  a.win[1] = ws_h;
+  a.win[2] = ws_w;
+  a.shift[0] = ss_d;
+  a.shift[1] = ss_h;
+  a.shift[2] = ss_w;
+  a.B = B;
+  a.H = H;
+  a.N = N;
+  a.head_dim = head_dim;
+  a.shares = shares;
+  a.scale = scale;
+  a.dtype = dtype;
+  if (sized && (bits & 15u) == 0) return launch_attention_grad(a, static_cast<cudaStream_t>(stream));
+  return launch_attention_grad_simt(a, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+int check_norm_gate(int dtype, int stream_dtype, const float* row_scale, int64_t samples,
+                    const float* post_w, const float* post_b, float eps, int64_t M, int64_t C) {
+  if (int e = check_dtype(dtype)) return e;
+  if (stream_dtype != dtype && stream_dtype != kF32)
+    return set_error(kErrInvalid, "the residual stream must be float32 or of the branch's dtype");
+  if (M < 0 || C < 1 || C > 4096) return set_error(kErrInvalid, "norm_gate_residual needs 1 <= C <= 4096");
+  if (!(eps > 0.f)) return set_error(kErrInvalid, "eps must be positive");
+  if (row_scale && (samples < 1 || M % samples))
+    return set_error(kErrInvalid, "the rows must divide evenly among the samples of row_scale");
+  if ((post_w == nullptr) != (post_b == nullptr))
+    return set_error(kErrInvalid, "post weight and bias must both be given or both be NULL");
+  return kOk;
+}
+
+}  // namespace
+
+int crumpet_norm_gate_residual(void* out, void* normed, const void* branch, const void* residual,
+                               int dtype, int stream_dtype, const float* gate,
+                               const float* row_scale, int64_t samples, const float* post_w,
+                               const float* post_b, const float* pre_w, const float* pre_b,
+                               float eps, int64_t M, int64_t C, void* stream) {
+  if (int e = check_norm_gate(dtype, stream_dtype, row_scale, samples, post_w, post_b, eps, M, C))
+    return e;
+  if ((pre_w == nullptr) != (pre_b == nullptr))
+    return set_error(kErrInvalid, "pre weight and bias must both be given or both be NULL");
+  if (M == 0) return kOk;
+  if (!out || !branch || !residual || (pre_w && !normed))
+    return set_error(kErrInvalid, "null tensor pointer");
+  NormGateArgs n{};
+  n.branch = branch;
+  n.residual = residual;
+  n.out = out;
+  n.normed = normed;
+  n.gate = gate;
+  n.row_scale = row_scale;
+  n.post_w = post_w;
+  n.post_b = post_b;
+  n.pre_w = pre_w;
+  n.pre_b = pre_b;
+  n.M = M;
+  n.C = C;
+  n.samples = row_scale ? samples : 1;
+  n.eps = eps;
+  n.dtype = dtype;
+  n.stream_dtype = stream_dtype;
+  return launch_norm_gate(n, static_cast<cudaStream_t>(stream));
+}
+
+int64_t crumpet_norm_gate_residual_backward_partials(int64_t M, int64_t C) {
+  return norm_gate_backward_partials(M, C);
+}
+
+int crumpet_norm_gate_residual_backward(
+    void* grad_residual, void* grad_branch, float* grad_gate, float* grad_post_w,
+    float* grad_post_b, float* grad_pre_w, float* grad_pre_b, const void* grad_out,
+    const void* grad_normed, const void* out, const void* branch, int dtype, int stream_dtype,
+    const float* gate, const float* row_scale, int64_t samples, const float* post_w,
+    const float* post_b, const float* pre_w, float eps, float* partial, int64_t M, int64_t C,
+    void* stream) {
+  if (int e = check_norm_gate(dtype, stream_dtype, row_scale, samples, post_w, post_b, eps, M, C))
+    return e;
+  if ((gate && !grad_gate) || (post_w && (!grad_post_w || !grad_post_b)) ||
+      (pre_w && (!grad_pre_w || !grad_pre_b)))
+    return set_error(kErrInvalid, "null tensor pointer");
+  if (M == 0) {  // no rows: the sums over them are zero
+    float* const sums[5] = {gate ? grad_gate : nullptr, post_w ? grad_post_w : nullptr,
+                            post_w ? grad_post_b : nullptr, pre_w ? grad_pre_w : nullptr,
+                            pre_w ? grad_pre_b : nullptr};
+    for (float* s : sums) {
+      if (!s) continue;
+      const cudaError_t e =
+          cudaMemsetAsync(s, 0, size_t(C) * sizeof(float), static_cast<cudaStream_t>(stream));
+      if (e != cudaSuccess) return set_cuda_error(e, "norm gate residual backward memset");
+    }
+    return kOk;
+  }
+  if (!grad_residual || !grad_branch || !grad_out || (pre_w && (!grad_normed || !out)) ||
+      ((gate || post_w) && !branch) || ((gate || post_w || pre_w) && !partial))
+    return set_error(kErrInvalid, "null tensor pointer");
+  NormGateArgs n{};
+  n.branch = branch;
+  n.out = const_cast<void*>(out);  // only read by the backward
+  n.grad_out = grad_out;
+  n.grad_normed = grad_normed;
+  n.grad_residual = grad_residual;
+  n.grad_branch = grad_branch;
+  n.partial = partial;
+  n.grad_gate = grad_gate;
+  n.grad_post_w = grad_post_w;
+  n.grad_post_b = grad_post_b;
+  n.grad_pre_w = grad_pre_w;
+  n.grad_pre_b = grad_pre_b;
+  n.gate = gate;
+  n.row_scale = row_scale;
+  n.post_w = post_w;
+  n.post_b = post_b;
+  n.pre_w = pre_w;
+  n.M = M;
+  n.C = C;
+  n.samples = row_scale ? samples : 1;
+  n.eps = eps;
+  n.dtype = dtype;
+  n.stream_dtype = stream_dtype;
+  return launch_norm_gate_backward(n, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+int check_kept(int dtype, int64_t M, int64_t C) {
+  if (int e = check_dtype(dtype)) return e;
+  if (M < 0 || C < 0) return set_error(kErrInvalid, "M and C must be non-negative");
+  if (C > (1 << 24)) return set_error(kErrInvalid, "C must be at most 2^24");
+  return kOk;
+}
+
+}  // namespace
+
+int crumpet_gelu_checkpoint(void* y, int8_t* kept, uint8_t* scales, const void* x, int dtype,
+                            int64_t M, int64_t C, void* stream) {
+  if (int e = check_kept(dtype, M, C)) return e;
+  if (M == 0 || C == 0) return kOk;
+  if (!y || !kept || !scales || !x) return set_error(kErrInvalid, "null tensor pointer");
+  return launch_gelu_checkpoint(y, kept, scales, x, dtype, M, C,
+                                static_cast<cudaStream_t>(stream));
+}
+
+int crumpet_gelu_checkpoint_backward(void* grad_x, void* again, const void* grad_y,
+                                     const int8_t* kept, const uint8_t* scales, int dtype,
+                                     int64_t M, int64_t C, void* stream) {
+  if (int e = check_kept(dtype, M, C)) return e;
+  if (M == 0 || C == 0) return kOk;
+  if (!grad_x || !again || !grad_y || !kept || !scales)
+    return set_error(kErrInvalid, "null tensor pointer");
+  return launch_gelu_checkpoint_backward(grad_x, again, grad_y, kept, scales, dtype, M, C,
+                                         static_cast<cudaStream_t>(stream));
+}
+
+int crumpet_restore_activation(void* x, const int8_t* kept, const uint8_t* scales, int dtype,
+                               int64_t M, int64_t C, void* stream) {
+  if (int e = check_kept(dtype, M, C)) return e;
+  if (M == 0 || C == 0) return kOk;
+  if (!x || !kept || !scales) return set_error(kErrInvalid, "null tensor pointer");
+  return launch_restore_activation(x, kept, scales, dtype, M, C,
+                                   static_cast<cudaStream_t>(stream));
+}
+
 int crumpet_test_stall_attention(int enable) { return set_attention_test_stall(enable); }
 
 int crumpet_device_status(int clear) {

@@ -135,6 +135,77 @@ int launch_window_attention_static_tiles(const AttnArgs& a, cudaStream_t stream)
 bool simt_attention_head_dim(int64_t head_dim);
 int launch_window_attention_simt(const AttnArgs& a, cudaStream_t stream);
 
+// Gradient of the packed-qkv window attention.  `grad_bias` receives `shares` parts of the
+// bias gradient, each [H, N, N] summed over the windows of that share; `stats` is scratch.
+struct AttnGradArgs {
+  void* grad_qkv;        // [B, N, 3, H, head_dim]
+  float* grad_bias;      // [shares, H, N, N]
+  float* stats;          // [3, B, H, N] floats
+  const void* grad_out;  // [B, N, H * head_dim]
+  const void* qkv;       // [B, N, 3, H, head_dim]
+  const void* table;     // [T, H]
+  bool table_f32;
+  const int* pairs;      // [N, N] buckets in [0, T)
+  int64_t nwin[3], win[3], shift[3];
+  int64_t B, H, N, head_dim, shares;
+  float scale;
+  int dtype;
+};
+bool attention_grad_tensor_path(int dtype, int64_t N, int64_t head_dim);
+int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
+int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N);
+int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
+int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream);
+
+// Relative-position bias by buckets: bias[h, p] = table[pairs[p], h] and the table's gradient
+// from `slabs` parts of grad [H, npairs].
+int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
+                                  const int* pairs, int64_t npairs, int64_t rows, int64_t H,
+                                  cudaStream_t stream);
+struct BiasGradArgs {
+  void* grad_table;  // [T, H]
+  int table_dtype;
+  const void* grad;  // [slabs, H, npairs]
+  int grad_dtype;
+  int64_t slabs, npairs, H;
+  const int* order;  // [npairs] pairs sorted by bucket
+  const int* items;  // [n_items][3]: bucket (-1: one of several items), begin, end
+  const int* multi;  // [n_multi][3]: bucket of several items, first item, last item + 1
+  int64_t n_items, n_multi;
+  float* partial;    // [n_items, H] (n_multi > 0)
+};
+int launch_relative_position_bias_grad(const BiasGradArgs& a, cudaStream_t stream);
+
+// Post-norm, gate, residual scale, residual add and next norm (norm_gate.cu).  Null: absent.
+struct NormGateArgs {
+  const void* branch;
+  const void* residual;
+  void* out;
+  void* normed;
+  const void* grad_out;
+  const void* grad_normed;
+  void* grad_residual;
+  void* grad_branch;
+  float* partial;
+  float *grad_gate, *grad_post_w, *grad_post_b, *grad_pre_w, *grad_pre_b;
+  const float *gate, *row_scale, *post_w, *post_b, *pre_w, *pre_b;
+  int64_t M, C, samples;
+  float eps;
+  int dtype, stream_dtype;
+};
+int64_t norm_gate_backward_partials(int64_t M, int64_t C);
+int launch_norm_gate(const NormGateArgs& n, cudaStream_t stream);
+int launch_norm_gate_backward(const NormGateArgs& n, cudaStream_t stream);
+
+// GELU with its input kept in 8 bits (act_checkpoint.cu).
+int launch_gelu_checkpoint(void* y, int8_t* kept, uint8_t* scales, const void* x, int dtype,
+                           int64_t M, int64_t C, cudaStream_t stream);
+int launch_gelu_checkpoint_backward(void* grad_x, void* again, const void* grad_y,
+                                    const int8_t* kept, const uint8_t* scales, int dtype,
+                                    int64_t M, int64_t C, cudaStream_t stream);
+int launch_restore_activation(void* x, const int8_t* kept, const uint8_t* scales, int dtype,
+                              int64_t M, int64_t C, cudaStream_t stream);
+
 // Test hook: while enabled, attention launches issue no TMA loads (every wait in
 // the kernel expires after its time limit).  Returns the previous setting.
 int set_attention_test_stall(int enable);

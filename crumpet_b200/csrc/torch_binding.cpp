@@ -3,7 +3,8 @@
 // Same op names, schemas and tags as the reference registration
 // (torch-ext/torch_binding.cpp:9-39), CUDA implementations only, plus
 // fused_swin_attention, which the reference exposes only as a Python/Triton
-// function (torch-ext/crumpet/fused_attention.py:149-226).  Every impl checks
+// function (torch-ext/crumpet/fused_attention.py:149-226), and ops without a reference
+// counterpart.  Every impl checks
 // the tensors, takes the current stream and calls the C ABI in
 // libcrumpet_b200.so; ops never allocate (outputs are preallocated `Tensor!`).
 #include <ATen/ATen.h>
@@ -582,6 +583,238 @@ void roi_normalize(at::Tensor& logits, const at::Tensor& acc, const at::Tensor& 
   roi_argmax_impl(nullptr, logits.data_ptr<float>(), acc, count_d, count_h, count_w);
 }
 
+// ---- training operators -------------------------------------------------------------
+
+void check_int32(const at::Tensor& t, const char* name) {
+  check_cuda_contig(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be an int32 tensor");
+}
+
+void check_f32(const at::Tensor& t, int64_t n, const char* name) {
+  check_cuda_contig(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == n, name,
+              " must be a float32 tensor of ", n, " elements");
+}
+
+// The float32 [n] vector of an optional tensor, or null.
+float* optional_f32(const at::Tensor& ref, const c10::optional<at::Tensor>& t, int64_t n,
+                    const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_f32(*t, n, name);
+  same_device(ref, *t, name);
+  return t->data_ptr<float>();
+}
+
+void relative_position_bias(at::Tensor& bias, const at::Tensor& table, const at::Tensor& pairs) {
+  check_cuda_contig(bias, "bias");
+  check_cuda_contig(table, "table");
+  check_int32(pairs, "pairs");
+  TORCH_CHECK(table.dim() == 2, "table must be [buckets, heads]");
+  TORCH_CHECK(bias.numel() == pairs.numel() * table.size(1), "bias must be [heads, pairs]");
+  same_device(bias, table, "table");
+  same_device(bias, pairs, "pairs");
+  const c10::cuda::CUDAGuard guard(bias.device());
+  check_rc(crumpet_relative_position_bias(bias.data_ptr(), dtype_code(bias), table.data_ptr(),
+                                          dtype_code(table), table.size(0), table.size(1),
+                                          pairs.data_ptr<int>(), pairs.numel(), cur_stream(bias)));
+}
+
+void relative_position_bias_backward(at::Tensor& grad_table, const at::Tensor& grad,
+                                     const at::Tensor& order, const at::Tensor& items,
+                                     const at::Tensor& multi,
+                                     const c10::optional<at::Tensor>& partial) {
+  check_cuda_contig(grad_table, "grad_table");
+  check_cuda_contig(grad, "grad");
+  check_int32(order, "order");
+  check_int32(items, "items");
+  check_int32(multi, "multi");
+  TORCH_CHECK(grad_table.dim() == 2, "grad_table must be [buckets, heads]");
+  TORCH_CHECK(items.dim() == 2 && items.size(1) == 3 && multi.dim() == 2 && multi.size(1) == 3,
+              "items and multi must be [n, 3]");
+  const int64_t H = grad_table.size(1), pairs = order.numel();
+  TORCH_CHECK(H * pairs == 0 ? grad.numel() == 0 : grad.numel() % (H * pairs) == 0,
+              "grad must be [slabs, heads, pairs]");
+  same_device(grad_table, grad, "grad");
+  same_device(grad_table, order, "order");
+  same_device(grad_table, items, "items");
+  same_device(grad_table, multi, "multi");
+  float* part = optional_f32(grad_table, partial, items.size(0) * H, "partial");
+  const c10::cuda::CUDAGuard guard(grad_table.device());
+  check_rc(crumpet_relative_position_bias_backward(
+      grad_table.data_ptr(), dtype_code(grad_table), H, grad.data_ptr(), dtype_code(grad),
+      H * pairs == 0 ? 0 : grad.numel() / (H * pairs), order.data_ptr<int>(), pairs,
+      items.data_ptr<int>(), items.size(0), multi.data_ptr<int>(), multi.size(0), part,
+      cur_stream(grad_table)));
+}
+
+void swin_window_attention_qkv_backward(at::Tensor& grad_qkv, at::Tensor& grad_bias,
+                                        at::Tensor& stats, const at::Tensor& grad_out,
+                                        const at::Tensor& qkv, const at::Tensor& table,
+                                        const at::Tensor& pairs, at::IntArrayRef num_windows,
+                                        at::IntArrayRef window_size, at::IntArrayRef shift_size,
+                                        double scale) {
+  check_cuda_contig(grad_qkv, "grad_qkv");
+  check_cuda_contig(grad_out, "grad_out");
+  check_cuda_contig(qkv, "qkv");
+  check_cuda_contig(table, "table");
+  check_int32(pairs, "pairs");
+  TORCH_CHECK(qkv.dim() == 5 && qkv.size(2) == 3, "qkv must have shape [B, N, 3, H, head_dim]");
+  const int64_t B = qkv.size(0), N = qkv.size(1), H = qkv.size(3), Dh = qkv.size(4);
+  TORCH_CHECK(grad_qkv.sizes() == qkv.sizes() && grad_qkv.scalar_type() == qkv.scalar_type(),
+              "grad_qkv must have the shape and dtype of qkv");
+  TORCH_CHECK(grad_out.numel() == B * N * H * Dh && grad_out.scalar_type() == qkv.scalar_type(),
+              "grad_out must be [B, N, H * head_dim] in the dtype of qkv");
+  TORCH_CHECK(table.dim() == 2 && table.size(1) == H, "table must be [buckets, H]");
+  TORCH_CHECK(table.scalar_type() == at::kFloat || table.scalar_type() == qkv.scalar_type(),
+              "table must be float32 or of the dtype of qkv");
+  TORCH_CHECK(pairs.numel() == N * N, "pairs must be [N, N]");
+  check_cuda_contig(grad_bias, "grad_bias");
+  TORCH_CHECK(grad_bias.scalar_type() == at::kFloat && grad_bias.dim() == 4 &&
+                  grad_bias.size(1) == H && grad_bias.size(2) == N && grad_bias.size(3) == N,
+              "grad_bias must be a float32 [shares, H, N, N] tensor");
+  check_f32(stats, 3 * B * H * N, "stats");
+  TORCH_CHECK(num_windows.size() == 3 && window_size.size() == 3 && shift_size.size() == 3,
+              "num_windows, window_size and shift_size take three values");
+  same_device(qkv, grad_qkv, "grad_qkv");
+  same_device(qkv, grad_bias, "grad_bias");
+  same_device(qkv, stats, "stats");
+  same_device(qkv, grad_out, "grad_out");
+  same_device(qkv, table, "table");
+  same_device(qkv, pairs, "pairs");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  check_rc(crumpet_swin_window_attention_qkv_backward(
+      grad_qkv.data_ptr(), grad_bias.data_ptr<float>(), stats.data_ptr<float>(),
+      grad_out.data_ptr(), qkv.data_ptr(), table.data_ptr(),
+      table.scalar_type() == at::kFloat ? 1 : 0, table.size(0), pairs.data_ptr<int>(),
+      grad_bias.size(0), num_windows[0], num_windows[1], num_windows[2], window_size[0],
+      window_size[1], window_size[2], shift_size[0], shift_size[1], shift_size[2],
+      dtype_code(qkv), B, H, N, Dh, static_cast<float>(scale), cur_stream(qkv)));
+}
+
+// Rows of `t` must be a contiguous [M, C] (any leading dims) of the dtype of `like`.
+void check_rows(const at::Tensor& ref, const at::Tensor& t, const at::Tensor& like,
+                const char* name) {
+  check_cuda_contig(t, name);
+  same_device(ref, t, name);
+  TORCH_CHECK(t.sizes() == ref.sizes() && t.scalar_type() == like.scalar_type(), name,
+              " must have the shape of branch and its stream's dtype");
+}
+
+void norm_gate_residual(at::Tensor& out, const c10::optional<at::Tensor>& normed,
+                        const at::Tensor& branch, const at::Tensor& residual,
+                        const c10::optional<at::Tensor>& gate,
+                        const c10::optional<at::Tensor>& row_scale,
+                        const c10::optional<at::Tensor>& post_w,
+                        const c10::optional<at::Tensor>& post_b,
+                        const c10::optional<at::Tensor>& pre_w,
+                        const c10::optional<at::Tensor>& pre_b, double eps) {
+  check_cuda_contig(branch, "branch");
+  TORCH_CHECK(branch.dim() >= 1, "branch must be [..., C]");
+  const int64_t C = branch.size(-1), M = C ? branch.numel() / C : 0;
+  check_rows(branch, residual, residual, "residual");
+  check_rows(branch, out, residual, "out");
+  void* normed_ptr = nullptr;
+  if (normed.has_value() && normed->defined()) {
+    check_rows(branch, *normed, branch, "normed");
+    normed_ptr = normed->data_ptr();
+  }
+  const int64_t samples = row_scale.has_value() && row_scale->defined() ? row_scale->numel() : 1;
+  const c10::cuda::CUDAGuard guard(branch.device());
+  check_rc(crumpet_norm_gate_residual(
+      out.data_ptr(), normed_ptr, branch.data_ptr(), residual.data_ptr(), dtype_code(branch),
+      dtype_code(residual), optional_f32(branch, gate, C, "gate"),
+      optional_f32(branch, row_scale, samples, "row_scale"), samples,
+      optional_f32(branch, post_w, C, "post weight"), optional_f32(branch, post_b, C, "post bias"),
+      optional_f32(branch, pre_w, C, "pre weight"), optional_f32(branch, pre_b, C, "pre bias"),
+      static_cast<float>(eps), M, C, cur_stream(branch)));
+}
+
+void norm_gate_residual_backward(at::Tensor& grad_residual, at::Tensor& grad_branch,
+                                 const c10::optional<at::Tensor>& sums,
+                                 const c10::optional<at::Tensor>& partial,
+                                 const at::Tensor& grad_out,
+                                 const c10::optional<at::Tensor>& grad_normed,
+                                 const at::Tensor& out, const at::Tensor& branch,
+                                 const c10::optional<at::Tensor>& gate,
+                                 const c10::optional<at::Tensor>& row_scale,
+                                 const c10::optional<at::Tensor>& post_w,
+                                 const c10::optional<at::Tensor>& post_b,
+                                 const c10::optional<at::Tensor>& pre_w, double eps) {
+  check_cuda_contig(branch, "branch");
+  TORCH_CHECK(branch.dim() >= 1, "branch must be [..., C]");
+  const int64_t C = branch.size(-1), M = C ? branch.numel() / C : 0;
+  check_rows(branch, grad_out, out, "grad_out");
+  check_rows(branch, out, out, "out");
+  check_rows(branch, grad_residual, out, "grad_residual");
+  check_rows(branch, grad_branch, branch, "grad_branch");
+  const void* gn = nullptr;
+  if (grad_normed.has_value() && grad_normed->defined()) {
+    check_rows(branch, *grad_normed, branch, "grad_normed");
+    gn = grad_normed->data_ptr();
+  }
+  float* part = optional_f32(branch, partial, crumpet_norm_gate_residual_backward_partials(M, C),
+                             "partial");
+  float* s = optional_f32(branch, sums, 5 * C, "sums");  // gate, post w, post b, pre w, pre b
+  float* at_[5];
+  for (int q = 0; q < 5; ++q) at_[q] = s ? s + q * C : nullptr;
+  const int64_t samples = row_scale.has_value() && row_scale->defined() ? row_scale->numel() : 1;
+  const c10::cuda::CUDAGuard guard(branch.device());
+  check_rc(crumpet_norm_gate_residual_backward(
+      grad_residual.data_ptr(), grad_branch.data_ptr(), at_[0], at_[1], at_[2], at_[3], at_[4],
+      grad_out.data_ptr(), gn, out.data_ptr(), branch.data_ptr(), dtype_code(branch),
+      dtype_code(out), optional_f32(branch, gate, C, "gate"),
+      optional_f32(branch, row_scale, samples, "row_scale"), samples,
+      optional_f32(branch, post_w, C, "post weight"), optional_f32(branch, post_b, C, "post bias"),
+      optional_f32(branch, pre_w, C, "pre weight"), static_cast<float>(eps), part, M, C,
+      cur_stream(branch)));
+}
+
+// int8 [.., C] and uint8 [.., ceil(C / 32)] of an activation [.., C]
+void check_kept(const at::Tensor& x, const at::Tensor& kept, const at::Tensor& scales) {
+  check_cuda_contig(x, "x");
+  check_cuda_contig(kept, "kept");
+  check_cuda_contig(scales, "scales");
+  same_device(x, kept, "kept");
+  same_device(x, scales, "scales");
+  TORCH_CHECK(x.dim() >= 1, "x must be [..., C]");
+  TORCH_CHECK(kept.scalar_type() == at::kChar && kept.numel() == x.numel(),
+              "kept must be an int8 tensor of x's elements");
+  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
+  TORCH_CHECK(scales.scalar_type() == at::kByte && scales.numel() == M * ((C + 31) / 32),
+              "scales must be a uint8 tensor of one element per 32 channels");
+}
+
+void gelu_checkpoint(at::Tensor& y, at::Tensor& kept, at::Tensor& scales, const at::Tensor& x) {
+  check_kept(x, kept, scales);
+  check_rows(x, y, x, "y");
+  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(crumpet_gelu_checkpoint(y.data_ptr(), kept.data_ptr<int8_t>(),
+                                   scales.data_ptr<uint8_t>(), x.data_ptr(), dtype_code(x), M, C,
+                                   cur_stream(x)));
+}
+
+void gelu_checkpoint_backward(at::Tensor& grad_x, at::Tensor& again, const at::Tensor& grad_y,
+                              const at::Tensor& kept, const at::Tensor& scales) {
+  check_kept(grad_y, kept, scales);
+  check_rows(grad_y, grad_x, grad_y, "grad_x");
+  check_rows(grad_y, again, grad_y, "again");
+  const int64_t C = grad_y.size(-1), M = C ? grad_y.numel() / C : 0;
+  const c10::cuda::CUDAGuard guard(grad_y.device());
+  check_rc(crumpet_gelu_checkpoint_backward(
+      grad_x.data_ptr(), again.data_ptr(), grad_y.data_ptr(), kept.data_ptr<int8_t>(),
+      scales.data_ptr<uint8_t>(), dtype_code(grad_y), M, C, cur_stream(grad_y)));
+}
+
+void restore_activation(at::Tensor& x, const at::Tensor& kept, const at::Tensor& scales) {
+  check_kept(x, kept, scales);
+  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(crumpet_restore_activation(x.data_ptr(), kept.data_ptr<int8_t>(),
+                                      scales.data_ptr<uint8_t>(), dtype_code(x), M, C,
+                                      cur_stream(x)));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(crumpet_ops, ops) {
@@ -656,6 +889,34 @@ TORCH_LIBRARY(crumpet_ops, ops) {
       "roi_normalize(Tensor! logits, Tensor acc, Tensor count_d, Tensor count_h, "
       "Tensor count_w) -> ()",
       kTags);
+  ops.def("relative_position_bias(Tensor! bias, Tensor table, Tensor pairs) -> ()", kTags);
+  ops.def(
+      "relative_position_bias_backward(Tensor! grad_table, Tensor grad, Tensor order, "
+      "Tensor items, Tensor multi, Tensor(a!)? partial) -> ()",
+      kTags);
+  ops.def(
+      "swin_window_attention_qkv_backward(Tensor(a!) grad_qkv, Tensor(b!) grad_bias, "
+      "Tensor(c!) stats, Tensor grad_out, Tensor qkv, Tensor table, Tensor pairs, "
+      "int[] num_windows, int[] window_size, int[] shift_size, float scale) -> ()",
+      kTags);
+  ops.def(
+      "norm_gate_residual(Tensor(a!) out, Tensor(b!)? normed, Tensor branch, Tensor residual, "
+      "Tensor? gate, Tensor? row_scale, Tensor? post_w, Tensor? post_b, Tensor? pre_w, "
+      "Tensor? pre_b, float eps) -> ()",
+      kTags);
+  ops.def(
+      "norm_gate_residual_backward(Tensor(a!) grad_residual, Tensor(b!) grad_branch, "
+      "Tensor(c!)? sums, Tensor(d!)? partial, Tensor grad_out, Tensor? grad_normed, Tensor out, "
+      "Tensor branch, Tensor? gate, Tensor? row_scale, Tensor? post_w, Tensor? post_b, "
+      "Tensor? pre_w, float eps) -> ()",
+      kTags);
+  ops.def(
+      "gelu_checkpoint(Tensor(a!) y, Tensor(b!) kept, Tensor(c!) scales, Tensor x) -> ()", kTags);
+  ops.def(
+      "gelu_checkpoint_backward(Tensor(a!) grad_x, Tensor(b!) again, Tensor grad_y, Tensor kept, "
+      "Tensor scales) -> ()",
+      kTags);
+  ops.def("restore_activation(Tensor! x, Tensor kept, Tensor scales) -> ()", kTags);
 }
 
 TORCH_LIBRARY_IMPL(crumpet_ops, CUDA, ops) {
@@ -679,4 +940,12 @@ TORCH_LIBRARY_IMPL(crumpet_ops, CUDA, ops) {
   ops.impl("roi_accumulate", &roi_accumulate);
   ops.impl("roi_argmax", &roi_argmax);
   ops.impl("roi_normalize", &roi_normalize);
+  ops.impl("relative_position_bias", &relative_position_bias);
+  ops.impl("relative_position_bias_backward", &relative_position_bias_backward);
+  ops.impl("swin_window_attention_qkv_backward", &swin_window_attention_qkv_backward);
+  ops.impl("norm_gate_residual", &norm_gate_residual);
+  ops.impl("norm_gate_residual_backward", &norm_gate_residual_backward);
+  ops.impl("gelu_checkpoint", &gelu_checkpoint);
+  ops.impl("gelu_checkpoint_backward", &gelu_checkpoint_backward);
+  ops.impl("restore_activation", &restore_activation);
 }

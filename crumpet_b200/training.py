@@ -1,0 +1,727 @@
+"""Training operators of a Swin block, with their gradients.
+
+The reference's patch runs eager torch in training (torch-ext/crumpet/monai_patch.py:137-151),
+and so do the patched methods here unless :func:`enable_training_kernels` is called on a model.
+The operators behind it, each usable by itself:
+
+* :func:`relative_position_buckets` / :func:`relative_position_bias`: the learned
+  relative-position bias ``table[index]`` per head and the gradient of its table;
+* :func:`swin_window_attention_train`: window attention from the packed qkv with that bias and
+  the shifted-window mask, differentiable in qkv and the table.  Nothing but its inputs is kept
+  for the backward pass;
+* :func:`norm_gate_residual`: post-norm, gate, per-sample residual scale, residual add and the
+  next norm in one pass each way;
+* :func:`gelu_checkpoint` / :func:`checkpointed_mlp`: GELU whose input is kept in 8 bits, and
+  the MLP around it.
+
+``*_backward`` functions are the gradients as plain calls, for programs that do without
+autograd.  All run on the current CUDA stream and return without waiting for it; results do not
+change from run to run (no atomics).  CUDA tensors only, as elsewhere in the package.
+"""
+
+from __future__ import annotations
+
+import sys
+import types
+from typing import NamedTuple, Sequence
+
+import torch
+import torch.nn.functional as F
+
+from . import _ops as _native
+from . import profiling as _prof
+from .fused_attention import (_ATTN_DTYPES, attention_bias_tiles, head_dim_supported,
+                              swin_window_attention_qkv, tensor_core_attention)
+
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+GROUP = 32  # neighbouring channels that share one scale of an 8-bit checkpoint
+MAX_CHANNELS = 4096  # of norm_gate_residual
+_ITEM = 1024  # most pairs of one bucket that one warp sums
+
+
+def _require_cuda(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError(f"crumpet_b200 runs {what} on CUDA devices only (got {t.device})")
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------ relative-position bias
+class RelativePositionBuckets(NamedTuple):
+    """A fixed bucket index ``[rows, cols]``, laid out once for the bias and its gradient
+    (:func:`relative_position_buckets`)."""
+
+    index: torch.Tensor  # int64 [rows, cols]
+    pairs: torch.Tensor  # int32 [rows, cols]: the same
+    order: torch.Tensor  # int32 [rows * cols]: the pairs sorted by bucket
+    items: torch.Tensor  # int32 [n, 3]: bucket (-1: one of several items), begin, end
+    multi: torch.Tensor  # int32 [m, 3]: bucket of several items, its first item, past its last
+    num_buckets: int
+
+
+def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> RelativePositionBuckets:
+    """Lay out ``index`` (integers ``[rows, cols]`` in ``[0, num_buckets)``, the bucket of every
+    query / key pair) for :func:`relative_position_bias` and
+    :func:`swin_window_attention_train`.  Made once for a module's index (for a window clamped
+    to a smaller volume, of its slice ``index[:n, :n]``): it sorts the pairs and checks their
+    values, which waits for the device."""
+    if index.ndim != 2 or index.is_floating_point() or index.is_complex() or index.dtype == torch.bool:
+        raise ValueError("index must be an integer tensor [rows, cols]")
+    num_buckets = int(num_buckets)
+    if num_buckets < 1:
+        raise ValueError("num_buckets must be positive")
+    if index.numel() >= 2 ** 31 or num_buckets >= 2 ** 31:
+        raise ValueError("index must hold fewer than 2^31 pairs and buckets")
+    index = index.detach().long().contiguous()
+    flat = index.reshape(-1)
+    if flat.numel() and (int(flat.min()) < 0 or int(flat.max()) >= num_buckets):
+        raise ValueError(f"index values must lie in [0, {num_buckets})")
+    order = torch.sort(flat, stable=True).indices
+    count = torch.bincount(flat, minlength=num_buckets)
+    begin = torch.cumsum(count, 0) - count
+    parts = torch.clamp((count + _ITEM - 1) // _ITEM, min=1)  # an empty bucket has one item too
+    bucket = torch.repeat_interleave(torch.arange(num_buckets, device=index.device), parts)
+    first = torch.cumsum(parts, 0) - parts
+    part = torch.arange(bucket.numel(), device=index.device) - first[bucket]
+    lo = begin[bucket] + part * _ITEM
+    hi = torch.minimum(lo + _ITEM, (begin + count)[bucket])
+    several = parts > 1
+    items = torch.stack((torch.where(several[bucket], -1, bucket), lo, hi), 1)
+    which = torch.nonzero(several).reshape(-1)
+    multi = torch.stack((which, first[which], (first + parts)[which]), 1)
+    return RelativePositionBuckets(index, index.int(), order.int(), items.int().contiguous(),
+                                   multi.int().contiguous(), num_buckets)
+
+
+def _check_table(table: torch.Tensor, buckets: RelativePositionBuckets) -> int:
+    if table.ndim != 2 or int(table.shape[0]) != buckets.num_buckets:
+        raise ValueError(f"table must have shape [{buckets.num_buckets}, heads]")
+    if table.dtype not in _DTYPES:
+        raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
+    return int(table.shape[1])
+
+
+def _bias_forward(table, buckets, dtype):
+    heads = int(table.shape[1])
+    bias = torch.empty((heads, *buckets.pairs.shape), dtype=dtype, device=table.device)
+    token = _prof.kernel_begin("relative_position_bias", lambda: {
+        "bytes": bias.numel() * bias.element_size() + buckets.pairs.numel() * 4})
+    _native.require().relative_position_bias(bias, table.contiguous(), buckets.pairs)
+    _prof.count("relative_position_bias")
+    _prof.kernel_end(token)
+    return bias
+
+
+def _table_gradient(grad, heads, buckets, dtype):
+    """[buckets, heads] from grad [slabs *, heads, rows, cols]."""
+    grad_table = torch.empty((buckets.num_buckets, heads), dtype=dtype, device=grad.device)
+    partial = None
+    if buckets.multi.shape[0]:
+        partial = torch.empty(buckets.items.shape[0] * heads, dtype=torch.float32,
+                              device=grad.device)
+    token = _prof.kernel_begin("relative_position_bias_backward", lambda: {
+        "bytes": grad.numel() * grad.element_size() + buckets.order.numel() * 4})
+    _native.require().relative_position_bias_backward(grad_table, grad, buckets.order,
+                                                      buckets.items, buckets.multi, partial)
+    _prof.count("relative_position_bias_backward")
+    _prof.kernel_end(token)
+    return grad_table
+
+
+class _Bias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, buckets, dtype):
+        ctx.buckets, ctx.dtype = buckets, table.dtype
+        return _bias_forward(table, buckets, dtype)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return relative_position_bias_backward(grad, ctx.buckets, ctx.dtype), None, None
+
+
+def relative_position_bias(table: torch.Tensor, buckets: RelativePositionBuckets,
+                           dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``table[index].permute(2, 0, 1)`` as a contiguous ``[heads, rows, cols]`` in ``dtype``
+    (default: the table's), differentiable in ``table [num_buckets, heads]``."""
+    _check_table(table, buckets)
+    dtype = table.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
+    if table.device.type == "meta":
+        return torch.empty((int(table.shape[1]), *buckets.pairs.shape), dtype=dtype, device="meta")
+    _require_cuda("relative_position_bias", table, buckets.pairs)
+    if _needs_grad(table):
+        return _Bias.apply(table, buckets, dtype)
+    return _bias_forward(table, buckets, dtype)
+
+
+def relative_position_bias_backward(grad_bias: torch.Tensor, buckets: RelativePositionBuckets,
+                                    dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Gradient of the table, ``[num_buckets, heads]`` in ``dtype`` (default: ``grad_bias``'s),
+    from the gradient ``[heads, rows, cols]`` of the bias: per bucket the fp32 sum over its
+    pairs, rounded once."""
+    if grad_bias.ndim != 3 or tuple(grad_bias.shape[1:]) != tuple(buckets.pairs.shape):
+        raise ValueError(f"grad_bias must have shape [heads, {', '.join(map(str, buckets.pairs.shape))}]")
+    dtype = grad_bias.dtype if dtype is None else dtype
+    if grad_bias.dtype not in _DTYPES or dtype not in _DTYPES:
+        raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
+    _require_cuda("relative_position_bias_backward", grad_bias, buckets.order)
+    return _table_gradient(grad_bias.contiguous(), int(grad_bias.shape[0]), buckets, dtype)
+
+
+# ------------------------------------------------------------------------- window attention
+def _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale):
+    if qkv.ndim != 5 or qkv.shape[2] != 3:
+        raise ValueError("qkv must have shape [B, N, 3, H, head_dim]")
+    B, N, _, H, D = (int(s) for s in qkv.shape)
+    if qkv.dtype not in _ATTN_DTYPES:
+        raise TypeError("window attention supports torch.float32, torch.float16 and torch.bfloat16")
+    if not head_dim_supported(D):
+        raise ValueError("window attention requires a power-of-two head_dim between 16 and 256")
+    if _check_table(table, buckets) != H:
+        raise ValueError(f"table must have shape [{buckets.num_buckets}, {H}]")
+    if tuple(buckets.pairs.shape) != (N, N):
+        raise ValueError(f"buckets must be made of an index [{N}, {N}] (index[:n, :n] of a "
+                         "clamped window)")
+    num_windows, shift_size = tuple(map(int, num_windows)), tuple(map(int, shift_size))
+    window_size = (N, 1, 1) if window_size is None else tuple(map(int, window_size))
+    if not len(num_windows) == len(window_size) == len(shift_size) == 3:
+        raise ValueError("num_windows, window_size and shift_size must contain exactly three values")
+    if min(num_windows) < 1 or min(window_size) < 1:
+        raise ValueError("num_windows and window_size values must be positive")
+    if window_size[0] * window_size[1] * window_size[2] != N:
+        raise ValueError(f"window_size must hold N = {N} tokens")
+    if any(not 0 <= s < w for s, w in zip(shift_size, window_size)):
+        raise ValueError("shift_size must satisfy 0 <= shift < window_size")
+    if any(shift_size) and B % (num_windows[0] * num_windows[1] * num_windows[2]):
+        raise ValueError("B must be a multiple of the number of windows")
+    scale = 1.0 / (D ** 0.5) if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("window attention requires a finite scale > 0")
+    _require_cuda("window attention", qkv, table, buckets.pairs)
+    return num_windows, window_size, shift_size, scale
+
+
+def _attention_table(table, dtype):
+    table = table.detach()
+    return (table if table.dtype in (torch.float32, dtype) else table.float()).contiguous()
+
+
+def _attention_forward(qkv, table, buckets, place):
+    num_windows, window_size, shift_size, scale = place
+    qkv = qkv.contiguous()
+    N, D = int(qkv.shape[1]), int(qkv.shape[4])
+    tiles = None
+    if tensor_core_attention(qkv.dtype, N, D) and qkv.numel() and qkv.data_ptr() % 16 == 0:
+        # the table changes every step, so its operands are built every step
+        tiles = attention_bias_tiles(table, buckets.index, N, scale, qkv.dtype)
+    return swin_window_attention_qkv(qkv, _attention_table(table, qkv.dtype), buckets.index,
+                                     num_windows, window_size, shift_size, scale, bias_tiles=tiles)
+
+
+def _attention_backward(grad_out, qkv, table, buckets, place):
+    num_windows, window_size, shift_size, scale = place
+    qkv, grad_out = qkv.contiguous(), grad_out.contiguous()
+    B, N, _, H, D = (int(s) for s in qkv.shape)
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[qkv.dtype]
+    with torch.cuda.device(qkv.device):
+        shares = int(_native.capi().crumpet_window_attention_backward_shares(B, H, N, D, code))
+    grad_qkv = torch.empty_like(qkv)
+    grad_bias = torch.empty((shares, H, N, N), dtype=torch.float32, device=qkv.device)
+    stats = torch.empty(3 * B * H * N, dtype=torch.float32, device=qkv.device)
+    token = _prof.kernel_begin("swin_window_attention_qkv_backward", lambda: {
+        "bytes": 7 * B * H * N * D * qkv.element_size(), "flops": 10 * B * H * N * N * D,
+        "exps": B * H * N * N})
+    _native.require().swin_window_attention_qkv_backward(
+        grad_qkv, grad_bias, stats, grad_out, qkv, _attention_table(table, qkv.dtype),
+        buckets.pairs, num_windows, window_size, shift_size, scale)
+    _prof.count("swin_window_attention_qkv_backward")
+    _prof.kernel_end(token)
+    return grad_qkv, _table_gradient(grad_bias, H, buckets, table.dtype)
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, table, buckets, place):
+        ctx.save_for_backward(qkv, table)
+        ctx.buckets, ctx.place = buckets, place
+        return _attention_forward(qkv, table, buckets, place)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        qkv, table = ctx.saved_tensors
+        return (*_attention_backward(grad_out, qkv, table, ctx.buckets, ctx.place), None, None)
+
+
+def swin_window_attention_train(
+    qkv: torch.Tensor,
+    table: torch.Tensor,
+    buckets: RelativePositionBuckets,
+    num_windows: Sequence[int] = (1, 1, 1),
+    window_size: Sequence[int] | None = None,
+    shift_size: Sequence[int] = (0, 0, 0),
+    scale: float | None = None,
+) -> torch.Tensor:
+    """:func:`~crumpet_b200.swin_window_attention_qkv` for training: the same result, from
+    ``qkv [B, N, 3, H, head_dim]``, the bias ``table [num_buckets, H]`` and its ``buckets``
+    (of the ``[N, N]`` index), differentiable in ``qkv`` and ``table``."""
+    place = _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale)
+    if _needs_grad(qkv, table):
+        return _WindowAttention.apply(qkv, table, buckets, place)
+    return _attention_forward(qkv, table, buckets, place)
+
+
+def swin_window_attention_backward(
+    grad_out: torch.Tensor,
+    qkv: torch.Tensor,
+    table: torch.Tensor,
+    buckets: RelativePositionBuckets,
+    num_windows: Sequence[int] = (1, 1, 1),
+    window_size: Sequence[int] | None = None,
+    shift_size: Sequence[int] = (0, 0, 0),
+    scale: float | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(grad_qkv, grad_table)`` of :func:`swin_window_attention_train` from ``grad_out
+    [B, N, H * head_dim]`` and the forward's own arguments, in the dtypes of ``qkv`` and
+    ``table``."""
+    place = _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale)
+    B, N, _, H, D = (int(s) for s in qkv.shape)
+    if tuple(grad_out.shape) != (B, N, H * D) or grad_out.dtype != qkv.dtype:
+        raise ValueError(f"grad_out must have shape {(B, N, H * D)} and the dtype of qkv")
+    _require_cuda("window attention", grad_out)
+    return _attention_backward(grad_out, qkv, table, buckets, place)
+
+
+# ------------------------------------------------- norms, gate and residual between branches
+class NormGateGrads(NamedTuple):
+    """Gradients of :func:`norm_gate_residual`; None where the argument was not given."""
+
+    residual: torch.Tensor
+    branch: torch.Tensor
+    gate: torch.Tensor | None
+    post_weight: torch.Tensor | None
+    post_bias: torch.Tensor | None
+    pre_weight: torch.Tensor | None
+    pre_bias: torch.Tensor | None
+
+
+def _vector(t, n, device, what):
+    if t is None:
+        return None
+    if tuple(t.shape) != (n,) or not t.is_floating_point():
+        raise ValueError(f"{what} must be a floating-point tensor of shape ({n},)")
+    return t.detach().to(device=device, dtype=torch.float32).contiguous()
+
+
+def _check_norm_gate(branch, stream, gate, row_scale, post_norm, pre_norm, eps):
+    if branch.ndim < 1 or branch.shape != stream.shape:
+        raise ValueError("branch and the residual stream must share a shape [..., C]")
+    if branch.dtype not in _DTYPES or stream.dtype not in (branch.dtype, torch.float32):
+        raise TypeError("norm_gate_residual takes float32, float16 or bfloat16 branches and a "
+                        "residual stream in float32 or the branch's dtype")
+    C = int(branch.shape[-1])
+    if not 1 <= C <= MAX_CHANNELS:
+        raise ValueError(f"norm_gate_residual needs 1 to {MAX_CHANNELS} channels")
+    if not eps > 0:
+        raise ValueError("eps must be positive")
+    for name, norm in (("post_norm", post_norm), ("pre_norm", pre_norm)):
+        if norm is not None and len(norm) != 2:
+            raise ValueError(f"{name} must be a (weight, bias) pair")
+    rows = branch.numel() // C
+    if row_scale is not None and (row_scale.ndim != 1 or not row_scale.numel()
+                                  or rows % row_scale.numel()):
+        raise ValueError("row_scale must be one value per sample, the rows a multiple of it")
+    _require_cuda("norm_gate_residual", branch, stream)
+    dev = branch.device
+    post = post_norm or (None, None)
+    pre = pre_norm or (None, None)
+    return (_vector(gate, C, dev, "gate"),
+            None if row_scale is None else _vector(row_scale, row_scale.numel(), dev, "row_scale"),
+            _vector(post[0], C, dev, "post_norm weight"), _vector(post[1], C, dev, "post_norm bias"),
+            _vector(pre[0], C, dev, "pre_norm weight"), _vector(pre[1], C, dev, "pre_norm bias"))
+
+
+def _norm_gate_forward(branch, residual, params, eps):
+    branch, residual = branch.contiguous(), residual.contiguous()
+    out = torch.empty_like(residual)
+    normed = None if params[4] is None else torch.empty_like(branch)
+    token = _prof.kernel_begin("norm_gate_residual", lambda: {
+        "bytes": sum(t.numel() * t.element_size() for t in (branch, residual, out, normed)
+                     if t is not None)})
+    _native.require().norm_gate_residual(out, normed, branch, residual, *params, float(eps))
+    _prof.count("norm_gate_residual")
+    _prof.kernel_end(token)
+    return out, normed
+
+
+def _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps):
+    gate, row_scale, post_w, post_b, pre_w, _ = params
+    branch, out, grad_out = branch.contiguous(), out.contiguous(), grad_out.contiguous()
+    grad_normed = None if pre_w is None else grad_normed.contiguous()
+    C = int(branch.shape[-1])
+    grad_residual, grad_branch = torch.empty_like(out), torch.empty_like(branch)
+    sums = partial = None
+    if gate is not None or post_w is not None or pre_w is not None:
+        with torch.cuda.device(branch.device):
+            n = int(_native.capi().crumpet_norm_gate_residual_backward_partials(
+                branch.numel() // C, C))
+        sums = torch.empty((5, C), dtype=torch.float32, device=branch.device)
+        partial = torch.empty(n, dtype=torch.float32, device=branch.device)
+    token = _prof.kernel_begin("norm_gate_residual_backward", lambda: {
+        "bytes": sum(t.numel() * t.element_size() for t in (
+            grad_out, grad_normed, out if pre_w is not None else None,
+            branch if gate is not None or post_w is not None else None, grad_residual,
+            grad_branch) if t is not None)})
+    _native.require().norm_gate_residual_backward(
+        grad_residual, grad_branch, sums, partial, grad_out, grad_normed, out, branch, gate,
+        row_scale, post_w, post_b, pre_w, float(eps))
+    _prof.count("norm_gate_residual_backward")
+    _prof.kernel_end(token)
+    given = (gate, post_w, post_w, pre_w, pre_w)
+    return NormGateGrads(grad_residual, grad_branch,
+                         *(None if g is None else sums[i] for i, g in enumerate(given)))
+
+
+class _NormGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, branch, residual, gate, post_w, post_b, pre_w, pre_b, row_scale, params, eps):
+        out, normed = _norm_gate_forward(branch, residual, params, eps)
+        ctx.save_for_backward(branch if gate is not None or post_w is not None else None, out,
+                              *params)
+        ctx.eps, ctx.branch_dtype = eps, branch.dtype
+        ctx.dtypes = tuple(None if t is None else t.dtype
+                           for t in (gate, post_w, post_b, pre_w, pre_b))
+        if normed is None:
+            return out
+        return out, normed
+
+    @staticmethod
+    def backward(ctx, grad_out, grad_normed=None):
+        branch, out, *params = ctx.saved_tensors
+        if branch is None:  # not read
+            branch = torch.empty_like(out, dtype=ctx.branch_dtype)
+        g = _norm_gate_backward(grad_out, grad_normed, out, branch, params, ctx.eps)
+        vectors = (None if t is None else t.to(dt) for t, dt in zip(g[2:], ctx.dtypes))
+        return (g.branch, g.residual, *vectors, None, None, None)
+
+
+def norm_gate_residual(
+    branch: torch.Tensor,
+    residual: torch.Tensor,
+    gate: torch.Tensor | None = None,
+    row_scale: torch.Tensor | None = None,
+    post_norm: tuple[torch.Tensor, torch.Tensor] | None = None,
+    pre_norm: tuple[torch.Tensor, torch.Tensor] | None = None,
+    eps: float = 1e-5,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``(out, normed)`` of ``out = residual + row_scale * gate * post_norm(branch)`` and
+    ``normed = pre_norm(out)``.
+
+    ``branch [..., C]``; ``residual`` has its shape, in its dtype or float32 (the stream under
+    autocast), and gives ``out``'s dtype; ``normed`` (None without ``pre_norm``) has the
+    branch's.  ``post_norm`` / ``pre_norm`` are the (weight, bias) of a LayerNorm over C with
+    ``eps``, ``gate [C]`` a layer scale, ``row_scale [samples]`` a factor per sample (drop path:
+    0 or 1 / keep; the leading dimensions are cut evenly).  Differentiable in all but
+    ``row_scale``.  C at most 4096.
+    """
+    if branch.device.type == "meta":
+        return (torch.empty_like(residual), None if pre_norm is None else torch.empty_like(branch))
+    params = _check_norm_gate(branch, residual, gate, row_scale, post_norm, pre_norm, eps)
+    post, pre = post_norm or (None, None), pre_norm or (None, None)
+    if _needs_grad(branch, residual, gate, *post, *pre):
+        res = _NormGate.apply(branch, residual, gate, *post, *pre, row_scale, params, eps)
+        return res if pre_norm is not None else (res, None)
+    return _norm_gate_forward(branch, residual, params, eps)
+
+
+def norm_gate_residual_backward(
+    grad_out: torch.Tensor,
+    grad_normed: torch.Tensor | None,
+    out: torch.Tensor,
+    branch: torch.Tensor,
+    gate: torch.Tensor | None = None,
+    row_scale: torch.Tensor | None = None,
+    post_norm: tuple[torch.Tensor, torch.Tensor] | None = None,
+    pre_norm: tuple[torch.Tensor, torch.Tensor] | None = None,
+    eps: float = 1e-5,
+) -> NormGateGrads:
+    """Gradients of :func:`norm_gate_residual` from those of its results, its own ``out`` and
+    the forward's arguments; ``grad_normed`` is None without ``pre_norm``.  The norms' and the
+    gate's gradients are float32."""
+    params = _check_norm_gate(branch, out, gate, row_scale, post_norm, pre_norm, eps)
+    if grad_out.shape != out.shape or grad_out.dtype != out.dtype:
+        raise ValueError("grad_out must have the shape and dtype of out")
+    if (grad_normed is None) != (pre_norm is None):
+        raise ValueError("grad_normed belongs to pre_norm: give both or neither")
+    if grad_normed is not None and (grad_normed.shape != branch.shape
+                                    or grad_normed.dtype != branch.dtype):
+        raise ValueError("grad_normed must have the shape and dtype of branch")
+    _require_cuda("norm_gate_residual", grad_out, grad_normed)
+    return _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps)
+
+
+# -------------------------------------------------------------- 8-bit activation checkpoints
+class KeptActivation(NamedTuple):
+    """An activation ``[..., C]`` in 8 bits: per 32 neighbouring channels one power of two
+    ``2^(scales - 127)`` and int8 multiples of it (``scales`` 255: the group held an infinity
+    or NaN and reads back as NaN)."""
+
+    kept: torch.Tensor    # int8 [..., C]
+    scales: torch.Tensor  # uint8 [..., ceil(C / 32)]
+    dtype: torch.dtype
+
+
+def gelu_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, KeptActivation]:
+    """``gelu(x)`` (exact, as ``torch.nn.GELU()``) and ``x`` in 8 bits for
+    :func:`gelu_checkpoint_backward`.  Called outside autograd (:func:`checkpointed_mlp` is the
+    differentiable form)."""
+    if x.ndim < 1 or x.dtype not in _DTYPES:
+        raise TypeError("gelu_checkpoint takes float32, float16 or bfloat16 tensors [..., C]")
+    if _needs_grad(x):
+        raise RuntimeError("gelu_checkpoint is not differentiable by itself; use "
+                           "checkpointed_mlp, or call it under torch.no_grad()")
+    _require_cuda("gelu_checkpoint", x)
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    kept = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], -(-x.shape[-1] // GROUP)), dtype=torch.uint8,
+                         device=x.device)
+    token = _prof.kernel_begin("gelu_checkpoint", lambda: {
+        "bytes": x.numel() * (2 * x.element_size() + 1) + scales.numel()})
+    _native.require().gelu_checkpoint(y, kept, scales, x)
+    _prof.count("gelu_checkpoint")
+    _prof.kernel_end(token)
+    return y, KeptActivation(kept, scales, x.dtype)
+
+
+def gelu_checkpoint_backward(grad_y: torch.Tensor, kept: KeptActivation
+                             ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(grad_x, again)`` from the gradient of ``y``: with ``u`` the kept input, ``grad_y *
+    gelu'(u)`` and ``gelu(u)``, the input of the next Linear's weight gradient."""
+    if grad_y.shape != kept.kept.shape or grad_y.dtype != kept.dtype:
+        raise ValueError("grad_y must have the shape and dtype of the kept activation")
+    _require_cuda("gelu_checkpoint_backward", grad_y)
+    grad_y = grad_y.contiguous()
+    grad_x, again = torch.empty_like(grad_y), torch.empty_like(grad_y)
+    token = _prof.kernel_begin("gelu_checkpoint_backward", lambda: {
+        "bytes": grad_y.numel() * (3 * grad_y.element_size() + 1) + kept.scales.numel()})
+    _native.require().gelu_checkpoint_backward(grad_x, again, grad_y, kept.kept, kept.scales)
+    _prof.count("gelu_checkpoint_backward")
+    _prof.kernel_end(token)
+    return grad_x, again
+
+
+def restore_activation(kept: KeptActivation) -> torch.Tensor:
+    """The kept activation in its own dtype."""
+    _require_cuda("restore_activation", kept.kept)
+    x = torch.empty(kept.kept.shape, dtype=kept.dtype, device=kept.kept.device)
+    _native.require().restore_activation(x, kept.kept, kept.scales)
+    _prof.count("restore_activation")
+    return x
+
+
+class _Mlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, dtype):
+        xc, w1c, w2c = x.to(dtype), w1.to(dtype), w2.to(dtype)
+        # outside autocast: the operands are already in the compute dtype
+        with torch.autocast("cuda", enabled=False):
+            u = F.linear(xc, w1c, None if b1 is None else b1.to(dtype))
+            y, kept = gelu_checkpoint(u)
+            out = F.linear(y, w2c, None if b2 is None else b2.to(dtype))
+        ctx.save_for_backward(xc, w1c, w2c, kept.kept, kept.scales)
+        ctx.dtypes = tuple(None if t is None else t.dtype for t in (x, w1, b1, w2, b2))
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, w1, w2, kept, scales = ctx.saved_tensors
+        with torch.autocast("cuda", enabled=False):
+            rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+            grad = grad.to(x.dtype)
+            grad_u, y = gelu_checkpoint_backward(grad @ w2, KeptActivation(kept, scales, x.dtype))
+            grads = (grad_u @ w1, rows(grad_u).t() @ rows(x), rows(grad_u).sum(0),
+                     rows(grad).t() @ rows(y), rows(grad).sum(0))
+        return (*(None if dt is None else g.to(dt) for g, dt in zip(grads, ctx.dtypes)), None)
+
+
+def checkpointed_mlp(x: torch.Tensor, weight1: torch.Tensor, bias1: torch.Tensor | None,
+                     weight2: torch.Tensor, bias2: torch.Tensor | None) -> torch.Tensor:
+    """``linear2(gelu(linear1(x)))`` that keeps its hidden activation in 8 bits (a byte and
+    1/32 per element instead of the Linear's output and GELU's) for the backward pass.
+
+    Computes in the autocast dtype under autocast, else in ``x``'s.  The forward result is the
+    unquantised one; the gradients of ``x``, ``weight1``, ``bias1`` and ``weight2`` see the
+    hidden activation as 8 bits keep it.
+    """
+    if weight1.ndim != 2 or weight2.ndim != 2 or int(weight1.shape[1]) != int(x.shape[-1]) \
+            or int(weight2.shape[1]) != int(weight1.shape[0]):
+        raise ValueError("weight1 must be [hidden, C] and weight2 [out, hidden]")
+    _require_cuda("checkpointed_mlp", x, weight1, weight2)
+    dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    if dtype not in _DTYPES:
+        raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
+    return _Mlp.apply(x, weight1, bias1, weight2, bias2, dtype)
+
+
+# ------------------------------------------------------------------- a Swin stage in training
+_BUCKETS_ATTR = "_crumpet_buckets"
+_FORWARD_ATTR = "_crumpet_eager_forward"
+
+
+def _module_buckets(attn, n: int) -> RelativePositionBuckets:
+    """The buckets of the module's own index for windows of n tokens, laid out on first use and
+    again if the index tensor is replaced or written to."""
+    index = attn.relative_position_index
+    kept = getattr(attn, _BUCKETS_ATTR, None)
+    if kept is None or kept[0] is not index or kept[1] != index._version:
+        kept = (index, index._version, {})
+        object.__setattr__(attn, _BUCKETS_ATTR, kept)
+    if n not in kept[2]:
+        kept[2][n] = relative_position_buckets(index[:n, :n],
+                                               attn.relative_position_bias_table.shape[0])
+    return kept[2][n]
+
+
+def _off(module) -> bool:
+    """Whether a dropout-like module (or None) does nothing."""
+    return module is None or isinstance(module, torch.nn.Identity) \
+        or getattr(module, "p", None) == 0.0
+
+
+def _fits(norm, C: int) -> bool:
+    return (isinstance(norm, torch.nn.LayerNorm) and tuple(norm.normalized_shape) == (C,)
+            and norm.weight is not None and norm.bias is not None)
+
+
+def _block_trains(blk, C: int) -> bool:
+    """Whether the training kernels compute exactly what the block does."""
+    attn, mlp = blk.attn, blk.mlp
+    act = getattr(mlp, "fn", None)
+    path = getattr(blk, "drop_path", None)
+    heads = int(attn.num_heads)
+    return (C <= MAX_CHANNELS and _fits(blk.norm1, C) and _fits(blk.norm2, C)
+            and C % heads == 0 and head_dim_supported(C // heads)
+            and _off(attn.attn_drop) and _off(attn.proj_drop)
+            and isinstance(act, torch.nn.GELU) and act.approximate == "none"
+            and _off(getattr(mlp, "drop1", None)) and _off(getattr(mlp, "drop2", None))
+            and (_off(path) or (hasattr(path, "drop_prob") and getattr(path, "scale_by_keep", True)))
+            and not getattr(blk, "use_checkpoint", False))
+
+
+def _path_scale(blk, samples: int, device) -> torch.Tensor | None:
+    """Drop path's factor per sample: 0, or 1 / keep with probability keep."""
+    drop = float(getattr(getattr(blk, "drop_path", None), "drop_prob", 0.0) or 0.0)
+    if drop == 0.0:
+        return None
+    keep = 1.0 - drop
+    kept = torch.rand(samples, device=device) < keep
+    return kept.float() / keep if keep > 0 else kept.float()
+
+
+def _train_branch(blk, normed, window_size, shift_size):
+    """The attention branch of a block from norm1's output: pad, roll + partition, qkv, window
+    attention, proj, back."""
+    from . import fused_shift_partition_3d, fused_unshift_unpartition_3d
+
+    attn = blk.attn
+    b, d, h, w, c = normed.shape
+    pad = [-s % ws for s, ws in zip((d, h, w), window_size)]
+    if any(pad):
+        normed = F.pad(normed, (0, 0, 0, pad[2], 0, pad[1], 0, pad[0]))
+    dims = tuple(int(s) for s in normed.shape[1:4])
+    windows = fused_shift_partition_3d(normed, window_size, shift_size)
+    n, heads = int(windows.shape[1]), int(attn.num_heads)
+    qkv = attn.qkv(windows).view(windows.shape[0], n, 3, heads, c // heads)
+    num_windows = tuple(s // ws for s, ws in zip(dims, window_size))
+    out = swin_window_attention_train(qkv, attn.relative_position_bias_table,
+                                      _module_buckets(attn, n), num_windows, window_size,
+                                      shift_size, attn.scale)
+    out = attn.proj(out)
+    x = fused_unshift_unpartition_3d(out, b, *dims, c, window_size, shift_size)
+    return x[:, :d, :h, :w].contiguous() if any(pad) else x
+
+
+def _train_layer(layer, x, get_window_size):
+    """A Swin stage (channels-first in and out) on the training operators: between two branches
+    one :func:`norm_gate_residual` adds the residual and takes the next norm."""
+    b, c, d, h, w = (int(s) for s in x.shape)
+    x = x.permute(0, 2, 3, 4, 1).contiguous()
+    blocks = list(layer.blocks)
+    compute = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    normed = blocks[0].norm1(x).to(compute)
+    for i, blk in enumerate(blocks):
+        window_size, shift_size = get_window_size((d, h, w), blk.window_size, blk.shift_size)
+        window_size, shift_size = tuple(map(int, window_size)), tuple(map(int, shift_size))
+        branch = _train_branch(blk, normed, window_size, shift_size)
+        x, normed = norm_gate_residual(
+            branch, x, row_scale=_path_scale(blk, b, x.device),
+            pre_norm=(blk.norm2.weight, blk.norm2.bias), eps=blk.norm2.eps)
+        mlp = blk.mlp
+        branch = checkpointed_mlp(normed, mlp.linear1.weight, mlp.linear1.bias, mlp.linear2.weight,
+                                  mlp.linear2.bias)
+        after = blocks[i + 1].norm1 if i + 1 < len(blocks) else None
+        x, normed = norm_gate_residual(
+            branch, x, row_scale=_path_scale(blk, b, x.device),
+            pre_norm=None if after is None else (after.weight, after.bias),
+            eps=blk.norm2.eps if after is None else after.eps)
+    if layer.downsample is not None:
+        x = layer.downsample(x)
+    return x.permute(0, 4, 1, 2, 3).contiguous()
+
+
+def _layer_forward(layer, x):
+    eager = layer.__dict__[_FORWARD_ATTR]
+    swin = sys.modules[type(layer).__module__]
+    c = int(x.shape[1]) if x.dim() == 5 else 0
+    if (x.dim() != 5 or not x.is_cuda or not layer.training or x.dtype not in _DTYPES
+            or not all(_block_trains(blk, c) for blk in layer.blocks)):
+        return eager(x) if eager is not None else type(layer).forward(layer, x)
+    if torch.is_autocast_enabled("cuda") and x.dtype not in (torch.float32,
+                                                            torch.get_autocast_dtype("cuda")):
+        x = x.float()
+    return _train_layer(layer, x, swin.get_window_size)
+
+
+def _layers(model):
+    return [m for m in model.modules()
+            if hasattr(m, "blocks") and hasattr(m, "downsample") and hasattr(m, "window_size")
+            and hasattr(sys.modules[type(m).__module__], "get_window_size")]
+
+
+def enable_training_kernels(model: torch.nn.Module) -> int:
+    """Run the Swin stages (``BasicLayer`` of MONAI or of ``crumpet_b200.swin_unetr``) of
+    ``model`` on the training operators while they are in training mode, on CUDA; returns how
+    many.  A stage with what they do not compute (attention, projection or MLP dropout,
+    activation checkpointing, another activation or norm) keeps its own forward, and so does
+    eval mode.  Undone by :func:`disable_training_kernels`."""
+    layers = _layers(model)
+    for layer in layers:
+        if _FORWARD_ATTR not in layer.__dict__:
+            layer.__dict__[_FORWARD_ATTR] = layer.__dict__.get("forward")
+            layer.__dict__["forward"] = types.MethodType(_layer_forward, layer)
+    return len(layers)
+
+
+def disable_training_kernels(model: torch.nn.Module) -> int:
+    """Undo :func:`enable_training_kernels`; returns how many stages it changed back."""
+    layers = [m for m in model.modules() if _FORWARD_ATTR in m.__dict__]
+    for layer in layers:
+        eager = layer.__dict__.pop(_FORWARD_ATTR)
+        layer.__dict__.pop("forward", None)
+        if eager is not None:
+            layer.__dict__["forward"] = eager
+    return len(layers)
+
+
+__all__ = [
+    "RelativePositionBuckets", "relative_position_buckets", "relative_position_bias",
+    "relative_position_bias_backward", "swin_window_attention_train",
+    "swin_window_attention_backward", "NormGateGrads", "norm_gate_residual",
+    "norm_gate_residual_backward", "KeptActivation", "gelu_checkpoint",
+    "gelu_checkpoint_backward", "restore_activation", "checkpointed_mlp",
+    "enable_training_kernels", "disable_training_kernels",
+]

@@ -385,6 +385,99 @@ CRUMPET_API int crumpet_roi_argmax(uint8_t* labels, float* logits, const float* 
                                    int64_t W, void* stream);
 
 /*
+ * ---- Training operators (no reference counterpart: its patch runs eager torch in training,
+ * torch-ext/crumpet/monai_patch.py:137-151).
+ *
+ * Learned relative-position bias by buckets:
+ *   bias[h, p] = table[pairs[p], h]             for H heads and npairs (query, key) pairs
+ *   grad_table[t, h] = sum over pairs p of bucket t of grad[h, p]
+ * table [table_rows, H] and bias [H, npairs] in their dtypes; pairs int32, every value in
+ * [0, table_rows) (the caller has checked them).  The gradient wants the pairs sorted by bucket
+ * (`order`, int32 [npairs]) and cut into items: int32 triples (bucket, begin, end) into order,
+ * in the order of the buckets, every bucket (an empty one too) with one item at least.  A
+ * bucket of several items is written as -1 in them and listed in `multi`, int32 triples
+ * (bucket, first item, last item + 1); then `partial` is fp32 scratch [n_items, H].  grad is
+ * the sum of `slabs` tensors [H, npairs], one after another.  Sums are fp32 in a fixed order.
+ */
+CRUMPET_API int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
+                                               int table_dtype, int64_t table_rows, int64_t H,
+                                               const int* pairs, int64_t npairs, void* stream);
+CRUMPET_API int crumpet_relative_position_bias_backward(
+    void* grad_table, int table_dtype, int64_t H, const void* grad, int grad_dtype, int64_t slabs,
+    const int* order, int64_t npairs, const int* items, int64_t n_items, const int* multi,
+    int64_t n_multi, float* partial, void* stream);
+
+/*
+ * Gradient of crumpet_swin_window_attention_qkv: from grad_out [B, N, H * head_dim] and the
+ * forward's qkv, table and geometry (arguments as there; pairs int32 [N, N] holds the buckets
+ * index[:N, :N], every value in [0, table_rows)), writes grad_qkv [B, N, 3, H, head_dim] and
+ * grad_bias fp32 [shares, H, N, N], whose sum over the shares is the gradient of the bias
+ * (pass it on to crumpet_relative_position_bias_backward with slabs = shares).  `shares` is
+ * what crumpet_window_attention_backward_shares gives for these sizes; `stats` is fp32
+ * scratch of 3 * B * H * N elements.  The bias is used as the table has it (the forward rounds
+ * it to dtype); the row statistics are taken again in fp32.  dtype, head_dim and N as for the
+ * forward: F16 / BF16 with head_dim 16 or 32, N <= 352 and 16-byte aligned tensors run the
+ * tensor-core kernels, every other call an fp32 SIMT kernel.
+ */
+CRUMPET_API int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N,
+                                                             int64_t head_dim, int dtype);
+CRUMPET_API int crumpet_swin_window_attention_qkv_backward(
+    void* grad_qkv, float* grad_bias, float* stats, const void* grad_out, const void* qkv,
+    const void* bias_table, int table_f32, int64_t table_rows, const int* pairs, int64_t shares,
+    int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d, int64_t ws_h, int64_t ws_w,
+    int64_t ss_d, int64_t ss_h, int64_t ss_w, int dtype, int64_t B, int64_t H, int64_t N,
+    int64_t head_dim, float scale, void* stream);
+
+/*
+ * The passes between two branches of a block, for M rows (tokens) of C channels:
+ *   n      = LN(branch; post_w, post_b), or branch where post_w is NULL
+ *   out    = residual + row_scale[sample] * gate * n   (each factor 1 where NULL), rounded
+ *   normed = LN(out; pre_w, pre_b)                     (not written where pre_w is NULL)
+ * branch and normed in dtype, residual and out in stream_dtype (dtype, or F32); gate and the
+ * norms' weights and biases fp32 [C]; row_scale fp32 [samples], M a multiple of samples and
+ * the rows of a sample one after another.  1 <= C <= 4096, eps > 0.  LN as in
+ * crumpet_norm_shift_partition_3d; it reads out as stored.
+ *
+ * Backward: from grad_out (stream_dtype), grad_normed (dtype, with pre_w), the forward's out
+ * (with pre_w) and branch (with gate or post_w), writes grad_residual (stream_dtype),
+ * grad_branch (dtype) and, for what is given, the fp32 [C] gradients of gate, post and pre
+ * weight and bias.  `partial` is fp32 scratch of
+ * crumpet_norm_gate_residual_backward_partials(M, C) elements.  Sums in a fixed order.
+ */
+CRUMPET_API int crumpet_norm_gate_residual(void* out, void* normed, const void* branch,
+                                           const void* residual, int dtype, int stream_dtype,
+                                           const float* gate, const float* row_scale,
+                                           int64_t samples, const float* post_w,
+                                           const float* post_b, const float* pre_w,
+                                           const float* pre_b, float eps, int64_t M, int64_t C,
+                                           void* stream);
+CRUMPET_API int64_t crumpet_norm_gate_residual_backward_partials(int64_t M, int64_t C);
+CRUMPET_API int crumpet_norm_gate_residual_backward(
+    void* grad_residual, void* grad_branch, float* grad_gate, float* grad_post_w,
+    float* grad_post_b, float* grad_pre_w, float* grad_pre_b, const void* grad_out,
+    const void* grad_normed, const void* out, const void* branch, int dtype, int stream_dtype,
+    const float* gate, const float* row_scale, int64_t samples, const float* post_w,
+    const float* post_b, const float* pre_w, float eps, float* partial, int64_t M, int64_t C,
+    void* stream);
+
+/*
+ * GELU (exact, by the normal distribution) whose input is kept in 8 bits for the backward:
+ *   y = gelu(x);  kept int8 [M, C], scales uint8 [M, ceil(C / 32)]
+ * Per 32 neighbouring channels of a row, s = 2^(scale - 127) is the least power of two (not
+ * below 2^-126) with max|x| <= 127 s, and kept = rint(x / s); scale 255 marks a group with an
+ * infinity or NaN, which reads back as NaN.  Backward, with u = kept * s:
+ *   grad_x = grad_y * gelu'(u), again = gelu(u)   (the weight gradient's input)
+ * crumpet_restore_activation writes u itself.  x, y, grad_*, again and u in dtype; C <= 2^24.
+ */
+CRUMPET_API int crumpet_gelu_checkpoint(void* y, int8_t* kept, uint8_t* scales, const void* x,
+                                        int dtype, int64_t M, int64_t C, void* stream);
+CRUMPET_API int crumpet_gelu_checkpoint_backward(void* grad_x, void* again, const void* grad_y,
+                                                 const int8_t* kept, const uint8_t* scales,
+                                                 int dtype, int64_t M, int64_t C, void* stream);
+CRUMPET_API int crumpet_restore_activation(void* x, const int8_t* kept, const uint8_t* scales,
+                                           int dtype, int64_t M, int64_t C, void* stream);
+
+/*
  * Device error word: non-zero once a kernel of this library gave up on a
  * bounded wait (bit 1: it then drained its work, freed its tensor memory and
  * returned without completing its output) or met a relative-position index
