@@ -1019,13 +1019,17 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
   }
 }
 
-// Prebuilt bias tiles: block `pair` (= h * MT + mt) writes the tile the attention kernel
-// would gather for that (head, query tile), in the same shared-memory image.
+// Prebuilt bias tiles: the blocks (pair, .) with pair = h * MT + mt write the tile the attention
+// kernel would gather for that (head, query tile), in the same shared-memory image.  Training
+// rebuilds the tiles every step, so a tile is spread over kTileBlocks blocks: the gathers are
+// latency, and one block per tile left most of the GPU idle (46 us at 3 heads x 343 tokens).
+constexpr int kTileBlocks = 11;
 template <int NPAD, bool BF16>
 __global__ void __launch_bounds__(256) bias_tile_kernel(const KParams p, uint8_t* tiles) {
   const int pair = blockIdx.x;
   const int h = pair / p.MT, mt = pair - h * p.MT;
-  build_bias_tile<NPAD, BF16>(p, h, mt, threadIdx.x, blockDim.x,
+  build_bias_tile<NPAD, BF16>(p, h, mt, blockIdx.y * blockDim.x + threadIdx.x,
+                              gridDim.y * blockDim.x,
                               tiles + size_t(pair) * size_t(Cfg<NPAD, 16>::BIAS_BYTES));
 }
 
@@ -1245,9 +1249,9 @@ int64_t bias_tile_bytes(int npad) { return int64_t(npad / 8) * (kBM / 8) * 128; 
 template <int NPAD>
 int launch_bias_tiles_npad(uint8_t* tiles, const KParams& kp, int dtype, cudaStream_t stream) {
   if (dtype == kBF16)
-    bias_tile_kernel<NPAD, true><<<kp.P, 256, 0, stream>>>(kp, tiles);
+    bias_tile_kernel<NPAD, true><<<dim3(kp.P, kTileBlocks), 256, 0, stream>>>(kp, tiles);
   else
-    bias_tile_kernel<NPAD, false><<<kp.P, 256, 0, stream>>>(kp, tiles);
+    bias_tile_kernel<NPAD, false><<<dim3(kp.P, kTileBlocks), 256, 0, stream>>>(kp, tiles);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "bias tile launch");
   return kOk;
@@ -1354,8 +1358,9 @@ int read_device_error(bool clear) {
     cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
   }
   const int lin = read_linear_error(clear);  // the Linear kernel's own word
-  if (lin < 0) return -1;
-  return v | lin;
+  const int grad = read_attention_grad_error(clear);  // the gradient kernels'
+  if (lin < 0 || grad < 0) return -1;
+  return v | lin | grad;
 }
 
 }  // namespace crumpet

@@ -14,21 +14,23 @@
 // the next, rather than in tensor memory, from which every element would be read and written
 // back for the arithmetic.
 //
-// Two kernels, each with CTAs of 64 rows x all columns of one head, which walk the windows of
-// their share one after another (so what belongs to the head -- the bias, and the sum dbias
-// -- stays on the SM):
-//   * rows kernel (64 query rows, all keys): row statistics, dq and dbias.  Every warp holds
-//     a 16 x WC tile of scores and of dp in registers (WC <= 88 keys), so each exponential is
-//     taken once and the statistics (row maximum, row sum, delta) are exchanged between the
-//     CG warps of a row through shared memory.  The bias tile and the dbias sums of the CTA
-//     (2 x 64 x 352 fp32 = 176 KB) sit in tensor memory, used here as a second register file:
-//     the bias is loaded straight into the accumulators of q k^T, dbias is read, added to and
-//     written back once per window.
-//   * columns kernel (64 key rows, all queries): dk and dv from the transposed scores with the
-//     statistics of the first kernel; its bias tile stays in registers.
-// The windows' K, V (or Q, dO) rows come in through cp.async, one window ahead.  No wait
+// Two kernels; a CTA takes some rows x all columns of one head and walks the windows of its
+// share one after another, so what belongs to the head -- the bias, and the sum dbias -- stays
+// on the SM, in tensor memory, used here as a second register file:
+//   * rows kernel (64 query rows, all keys): row statistics, dq and dbias.  A warp holds a
+//     16 x WC tile of scores and of dp in registers (WC <= 88 keys), so each exponential is
+//     taken once; the CG warps of a row exchange (maximum, sum, sum of p dp) through shared
+//     memory at one barrier per window, behind which they also join the dq of the window
+//     before.  The bias goes from tensor memory straight into the accumulators of q k^T; dbias
+//     is read from it, added to and written back once per window (2 x 64 x 352 fp32).
+//   * columns kernel: dk and dv from the transposed scores with the statistics of the first
+//     kernel; a warp takes 16 keys x all queries, so nothing is exchanged between warps.
+// TMA brings the windows' rows into a ring of stages; the last warp that has read a stage
+// refills it, so warps drift apart by up to a ring and no warp waits only to copy.  Waits for
+// the loads are bounded like the forward kernel's (2 s, then the device error word).  No wait
 // depends on another CTA; sums have a fixed order, so results do not change from run to run.
 #include <cmath>
+#include <mutex>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -36,35 +38,53 @@
 
 namespace crumpet {
 
+static __device__ int g_grad_error;  // 1: a bounded wait of these kernels expired
+
 namespace {
 
 using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kRG = 4;         // row groups of 16 rows per CTA
-constexpr int kBR = 16 * kRG;  // rows per CTA
+constexpr int kRG = 4;         // row groups of 16 rows per CTA of the rows kernel
+constexpr int kBR = 16 * kRG;  // its rows
+constexpr int kSmemBudget = 227 * 1024 - 1024;  // per SM, less what the CTAs reserve
 
 struct GradParams {
-  const uint16_t* qkv;   // [B, N, 3, H, HD]
-  const uint16_t* dout;  // [B, N, H, HD]
   uint16_t* dqkv;        // [B, N, 3, H, HD]
   float* dbias;          // [S, H, N, N]
-  float2* stats;         // [B, H, N]: (log2 of the row's sum of exponentials, delta)
-  float* amax;           // [B, H, N]: largest |do| of the row (fp16 only)
+  float2* stats;         // [B, H, NS]: (log2 of the row's sum of exponentials, delta)
+  float* amax;           // [B, H, groups of 16 rows]: their largest |do| (fp16 only)
   const void* table;     // [T, H]: fp32 (table_f32) or the element type
   const int* pairs;      // [N, N]: bucket of every (query, key) pair, in [0, T)
   int table_f32;
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
   int analytic;
-  int B, H, N, RB, S;    // RB = row blocks, S = shares the windows are split into
+  int B, H, N, NS;       // NS = N rounded up to 2: rows of stats start on 16 bytes
+  int RB, S;             // row blocks, and shares that the windows are split into
   float scale;
 };
 
-// One padded token count: CG warps share a row's columns, WC columns (NT tiles of 8) each.
+// What both kernels share: token rows in shared memory as TMA writes them, HD * 2 bytes each in
+// the 32- or 64-byte swizzle, whose permuted 16-byte chunks let eight rows of an ldmatrix phase
+// fall into different banks.
+template <int HD>
+struct Rows {
+  static constexpr int BYTES = HD * 2;
+  static constexpr int KS = HD / 16;  // depth steps of a product over the channels
+  // offset of 16-byte chunk c of row r, for rows counted from a multiple of 8
+  __device__ static __forceinline__ uint32_t at(int r, int c) {
+    const int sw = HD == 16 ? (r >> 2) & 1 : (r >> 1) & 3;
+    return uint32_t(r * BYTES + ((c ^ sw) << 4));
+  }
+};
+
+// Boxes of a TMA load of `rows` token rows: equal, at most 256 rows.
+__host__ __device__ constexpr int box_rows(int rows) { return rows > 256 ? rows / 2 : rows; }
+
+// Rows kernel: CG warps share a row's NPAD columns, WC columns (NT tiles of 8) each.
 template <int NPAD_, int HD_>
-struct Shape {
-  static constexpr int NPAD = NPAD_;
-  static constexpr int HD = HD_;
+struct RowsShape {
+  static constexpr int NPAD = NPAD_, HD = HD_;
   static constexpr int CG = NPAD == 64 ? 1 : NPAD == 128 ? 2 : 4;
   static constexpr int WC = NPAD / CG;
   static constexpr int NT = WC / 8;
@@ -72,30 +92,64 @@ struct Shape {
   static constexpr int WARPS = kRG * CG;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int MINB = 512 / THREADS;  // 128 registers per thread
-  static constexpr int KS = HD / 16;          // depth steps of a product over the channels
-  // Row pitch in shared memory: 16 bytes past the row, so the eight 16-byte rows that an
-  // ldmatrix phase reads fall into different banks (pitch 48: 0, 48, 96, 16, 64, ...).
-  static constexpr int PITCH = HD * 2 + 16;
-  static constexpr int COLS_BYTES = NPAD * PITCH;  // one column-side tensor of a window
-  static constexpr int ROWS_BYTES = kBR * PITCH;   // one row-side tensor of a window
-  static constexpr int STAGE = 2 * COLS_BYTES + 2 * ROWS_BYTES;
-  // tensor memory: WC/2 fp32 of bias and of dbias per thread and warp, four warps per lane
+  static constexpr int COLS = NPAD * HD * 2;  // bytes of K or V of a window
+  static constexpr int ROWS = kBR * HD * 2;   // bytes of the CTA's rows of Q or dO
+  static constexpr int STAGE = 2 * COLS + 2 * ROWS;
+  // tensor memory: WC/2 fp32 of bias and of dbias per thread and warp, the CG warps of a lane
   // quarter side by side
-  static constexpr int TM_WARP = WC;
-  static constexpr int TM_USED = TM_WARP * CG;
+  static constexpr int TM_USED = WC * CG;
   static constexpr uint32_t TM_COLS = TM_USED <= 64 ? 64 : TM_USED <= 128 ? 128
                                       : TM_USED <= 256 ? 256 : 512;
-  static constexpr int RED_ROWS = WARPS * 16 * HD * 4;      // partial dq of every warp
-  static constexpr int RED_COLS = 2 * WARPS * 16 * HD * 4;  // partial dk and dv
-  static constexpr int EXCH = 3 * kBR * CG * 4;             // row maximum, sum, delta partials
-  static constexpr int SMEM_ROWS = 2 * STAGE + RED_ROWS + EXCH + NPAD + 16;
-  static constexpr int SMEM_COLS = 2 * STAGE + 2 * NPAD * 12 + RED_COLS + NPAD + 16;
-  static_assert(SMEM_ROWS <= 232448 && SMEM_COLS <= 232448, "shared memory budget");
+  static constexpr int PITCH = HD + 8;                      // floats per row of partial dq
+  static constexpr int RED = 2 * WARPS * 16 * PITCH * 4;    // partial dq, two windows
+  static constexpr int EXCH = 2 * CG * kBR * 16;            // row statistics, two windows
+  static constexpr int MASK = NPAD * 16;                    // mask features of the columns
+  static constexpr int FIXED = RED + EXCH + MASK + 1024 + 256;
+  static constexpr int FIT = (kSmemBudget / MINB - FIXED) / STAGE;
+  static constexpr int STAGES = FIT > 4 ? 4 : FIT;
+  static constexpr int SMEM = STAGES * STAGE + FIXED;
+  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory budget");
+};
+
+// Columns kernel: a warp takes 16 keys and all NPAD queries, NT tiles of 8.
+template <int NPAD_, int HD_>
+struct ColsShape {
+  static constexpr int NPAD = NPAD_, HD = HD_;
+  static constexpr int NT = NPAD / 8;
+  static_assert(NT % 2 == 0, "tiles are taken in pairs");
+  static constexpr int WARPS = NPAD == 352 ? 11 : NPAD == 224 ? 7 : 4;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int MINB = NPAD == 352 ? 1 : NPAD == 224 ? 2 : 4;  // CTAs per SM
+  static constexpr int BR = 16 * WARPS;  // rows (keys) per CTA
+  // Tensor memory: 4 fp32 of the bias per thread and tile, the warps of a lane quarter side by
+  // side; the tiles that do not fit stay in registers (2 of 44 where three warps share 512).
+  static constexpr int QUARTER = (WARPS + 3) / 4;
+  static constexpr int TT = 512 / MINB / (4 * QUARTER) < NT ? 512 / MINB / (4 * QUARTER) / 2 * 2 : NT;
+  static constexpr int TM_USED = 4 * TT * QUARTER;
+  static constexpr uint32_t TM_COLS = TM_USED <= 32 ? 32 : TM_USED <= 64 ? 64
+                                      : TM_USED <= 128 ? 128 : TM_USED <= 256 ? 256 : 512;
+  static_assert(TM_COLS * MINB <= 512 && NT - TT <= 2, "tensor memory budget");
+  static constexpr int COLS = NPAD * HD * 2;  // bytes of Q or dO of a window
+  static constexpr int ROWS = BR * HD * 2;    // bytes of the CTA's rows of K or V
+  static constexpr int STAT = NPAD * 8;       // statistics of the window's rows
+  static constexpr int STAGE = (2 * COLS + 2 * ROWS + STAT + 1023) / 1024 * 1024;
+  static constexpr int MASK = NPAD * 16;
+  static constexpr int FIXED = MASK + 1024 + 256;
+  static constexpr int FIT = (kSmemBudget / MINB - FIXED) / STAGE;
+  static constexpr int STAGES = FIT > 4 ? 4 : FIT;
+  static constexpr int SMEM = STAGES * STAGE + FIXED;
+  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory budget");
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float rcp(float x) {  // within 1 ulp
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -161,15 +215,48 @@ __device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(b0));
 }
 
-__device__ __forceinline__ void tm_ld4(uint32_t t, float* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3])
-               : "r"(t));
+// 4 NT consecutive tensor-memory columns of this thread's lane (widths are powers of two)
+template <int N>
+__device__ __forceinline__ void tm_ld(uint32_t t, float* r) {
+  if constexpr (N >= 32) {
+    tmem_ld32(t, reinterpret_cast<uint32_t*>(r));
+    tm_ld<N - 32>(t + 32, r + 32);
+  } else if constexpr (N >= 16) {
+    tmem_ld16(t, reinterpret_cast<uint32_t(&)[16]>(*r));
+    tm_ld<N - 16>(t + 16, r + 16);
+  } else if constexpr (N >= 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]),
+                   "=f"(r[6]), "=f"(r[7])
+                 : "r"(t));
+    tm_ld<N - 8>(t + 8, r + 8);
+  } else if constexpr (N >= 4) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3])
+                 : "r"(t));
+    tm_ld<N - 4>(t + 4, r + 4);
+  }
 }
-__device__ __forceinline__ void tm_st4(uint32_t t, const float* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(t), "f"(r[0]),
-               "f"(r[1]), "f"(r[2]), "f"(r[3])
-               : "memory");
+template <int N>
+__device__ __forceinline__ void tm_st(uint32_t t, const float* r) {
+  if constexpr (N >= 32) {
+    tmem_st32(t, reinterpret_cast<const uint32_t*>(r));
+    tm_st<N - 32>(t + 32, r + 32);
+  } else if constexpr (N >= 16) {
+    tmem_st16(t, reinterpret_cast<const uint32_t*>(r));
+    tm_st<N - 16>(t + 16, r + 16);
+  } else if constexpr (N >= 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t),
+                 "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]),
+                 "f"(r[7])
+                 : "memory");
+    tm_st<N - 8>(t + 8, r + 8);
+  } else if constexpr (N >= 4) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(t), "f"(r[0]),
+                 "f"(r[1]), "f"(r[2]), "f"(r[3])
+                 : "memory");
+    tm_st<N - 4>(t + 4, r + 4);
+  }
 }
 // Waits for the loads that filled `v`; the values pass through the statement, so no use of
 // them can be scheduled before it.
@@ -182,19 +269,30 @@ __device__ __forceinline__ void tm_wait(float (&v)[NT][4]) {
     for (int e = 0; e < 4; ++e) asm volatile("" : "+f"(v[t][e]));
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+// The two values of a row in a fragment, for the packed fp32 arithmetic (two per instruction)
+__device__ __forceinline__ float2 two(const float (&v)[4], int row) {
+  return make_float2(v[2 * row], v[2 * row + 1]);
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void put(float (&v)[4], int row, float2 x) {
+  v[2 * row] = x.x;
+  v[2 * row + 1] = x.y;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_wait_all() {
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Untiled copy global -> shared (16-byte aligned, a multiple of 16 bytes), counted on `bar`
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
+
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -215,27 +313,49 @@ __device__ __forceinline__ uint32_t last_axes(const GradParams& p, int b) {
          (uint32_t(p.ssw != 0 && iw == p.nww - 1) << 2);
 }
 
-// bias[h, i, j] / scale, as the accumulators of q k^T start; -inf past the last key, so the
-// padded columns' exponentials are 0.
-template <bool BF16>
-__device__ __forceinline__ float bias_start(const GradParams& p, int h, int i, int j, float inv) {
-  if (j >= p.N || i >= p.N) return 0.f;
-  const long long t = p.pairs[(long long)i * p.N + j];
-  const float v = p.table_f32
-                      ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
-                      : elem_f32<BF16>(__ldg(static_cast<const uint16_t*>(p.table) + t * p.H + h));
-  return v * inv;
+// The accumulators that q k^T starts from: bias[h, i, j] / scale, -inf past the last column (its
+// exponentials are 0), 0 in padded rows.  `at(t, e)` gives the (query, key) of a value; two rounds
+// of independent gathers, since a CTA does nothing else meanwhile.
+template <int NT, bool BF16, bool COLS>
+__device__ __forceinline__ void start_values(const GradParams& p, int h, int row0, int col0,
+                                             float (&v)[NT][4]) {
+  int at[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = row0 + (e < 2 ? 0 : 8), c = col0 + 8 * t + (e & 1);
+      at[t][e] = r < p.N && c < p.N ? __ldg(p.pairs + (COLS ? c * p.N + r : r * p.N + c)) : -1;
+    }
+  const float inv = 1.f / p.scale;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = col0 + 8 * t + (e & 1);
+      float x = c < p.N ? 0.f : -INFINITY;
+      if (at[t][e] >= 0) {
+        const long long i = (long long)at[t][e] * p.H + h;
+        x = inv * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + i)
+                               : elem_f32<BF16>(__ldg(static_cast<const uint16_t*>(p.table) + i)));
+      }
+      v[t][e] = x;
+    }
 }
 
-// Copies of `rows` token rows of one head (row stride in elements) into pitched shared memory.
-template <int HD, int PITCH>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const uint16_t* src, long long stride,
-                                          int rows, int tid, int threads) {
-  constexpr int CH = HD / 8;  // 16-byte chunks per row
-  for (int c = tid; c < rows * CH; c += threads) {
-    const int r = c / CH, k = c % CH;
-    cp16(dst + uint32_t(r * PITCH + k * 16), src + r * stride + k * 8);
-  }
+// Shifted-window mask as one more product of depth 8 in the windows that need it: per axis a
+// (of the lane's t4) a row token has the features (bit, 1 - bit) of its roll-side code and a
+// column token ((1 - bit) pen, bit pen), pen = elem(-100 / scale), so their product is pen where
+// the two tokens lie on different sides of the seam, else 0.  Element pairs as mma operands.
+template <bool BF16>
+__device__ __forceinline__ uint32_t row_feature(uint32_t code, int axis) {
+  const uint32_t one = BF16 ? 0x3F80u : 0x3C00u;
+  return axis > 2 ? 0u : (code >> axis) & 1u ? one : one << 16;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t col_feature(uint32_t code, int axis, float scale) {
+  const uint32_t pen = pack2<BF16>(-100.f / scale, 0.f) & 0xffffu;
+  return axis > 2 ? 0u : (code >> axis) & 1u ? pen << 16 : pen;
 }
 
 // 2^-(e + 4) for the exponent e of m: rows of do scaled by it have magnitudes below 1/8, so
@@ -247,18 +367,94 @@ __device__ __forceinline__ float grad_scale(float m) {
   return __uint_as_float((250u - e) << 23);  // 2^(127 - e - 4)
 }
 
+__device__ __forceinline__ float inverse_scale(float g) {  // 1 / g of a power of two
+  return __uint_as_float((254u << 23) - __float_as_uint(g));
+}
+
+// ------------------------------------------------------------------- ring of windows
+// The CTA's windows k = 0, 1, ... (window share + k S of the batch) pass through STAGES stages of
+// shared memory.  One thread issues a window's loads; the warps wait for its stage to be full,
+// and the last warp to have read a stage issues the window that comes next in it.
+constexpr int kMaxStages = 4;
+struct Tail {  // the CTA's shared words
+  uint64_t full[kMaxStages];
+  uint32_t done[kMaxStages];  // warps that have read the stage
+  uint32_t last[kMaxStages];  // the stage's window: axes with a roll seam (last_axes)
+  uint32_t tm_slot;
+  int abort;   // a wait expired: no more waiting, no more loads
+  int issued;  // windows whose loads were issued
+};
+
+__device__ __forceinline__ void init_tail(Tail* tail) {
+  for (int s = 0; s < kMaxStages; ++s) {
+    mbar_init(&tail->full[s], 1);
+    tail->done[s] = 0;
+  }
+  tail->abort = 0;
+  tail->issued = 0;
+  fence_mbar_init();
+}
+
+// Whether the stage of window k is full.  After a wait has expired the warps go on without
+// waiting, so they keep meeting at their barriers; what they compute is not used.
+template <int STAGES>
+__device__ __forceinline__ void wait_stage(Tail* tail, int k) {
+  mbar_wait(&tail->full[k % STAGES], uint32_t(k / STAGES) & 1u, &tail->abort);
+  __syncwarp();
+}
+
+// Counts this warp's reading of window k as finished; true for the lane that now has to issue
+// window k + STAGES.
+template <int STAGES>
+__device__ __forceinline__ bool release_stage(Tail* tail, int k, int count, uint32_t warps) {
+  __syncwarp();
+  if ((threadIdx.x & 31) != 0) return false;
+  __threadfence_block();  // this warp's reads come before the loads that follow the count
+  if (atomicAdd(&tail->done[k % STAGES], 1u) + 1u != warps) return false;
+  tail->done[k % STAGES] = 0;
+  __threadfence_block();
+  return k + STAGES < count && *reinterpret_cast<volatile int*>(&tail->abort) == 0;
+}
+
+// After the CTA's last barrier, by one thread: reports an expired wait, and lets loads that are
+// still in flight land (bounded) before the CTA's shared memory is given back.
+template <int STAGES>
+__device__ __forceinline__ void finish_ring(Tail* tail) {
+  if (tail->abort == 0) return;
+  atomicOr(&g_grad_error, 1);
+  for (int k = tail->issued - 1; k >= 0 && k >= tail->issued - STAGES; --k) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(&tail->full[k % STAGES], uint32_t(k / STAGES) & 1u))
+      if (globaltimer_ns() - t0 > kWaitLimitNs) break;
+  }
+}
+
+// TMA loads of ROWS token rows from row0 of (head h, window b), in equal boxes
+template <int HD, int ROWS>
+__device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, uint64_t* full,
+                                          int row0, int h, int b) {
+#pragma unroll
+  for (int r = 0; r < ROWS; r += box_rows(ROWS))
+    tma_load_4d(dst + r * HD * 2, map, full, 0, row0 + r, h, b);
+}
+
+struct Maps {  // q, k, v and do, in boxes of a window's (cols) and of a CTA's (rows) tokens
+  CUtensorMap q_cols, k_cols, v_cols, o_cols, q_rows, k_rows, v_rows, o_rows;
+};
+
 // ------------------------------------------------------------------------ rows kernel
 template <class S, bool BF16>
-__global__ void __launch_bounds__(S::THREADS, S::MINB) grad_rows_kernel(const GradParams p) {
-  constexpr int NT = S::NT, HD = S::HD, CG = S::CG, PITCH = S::PITCH;
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* red_b = smem + 2 * S::STAGE;
-  float* red = reinterpret_cast<float*>(red_b);                      // [warp][16][HD]
-  float* ex_max = reinterpret_cast<float*>(red_b + S::RED_ROWS);     // [64 rows][CG]
-  float* ex_sum = ex_max + kBR * CG;
-  float* ex_dp = ex_sum + kBR * CG;
-  uint8_t* code = reinterpret_cast<uint8_t*>(ex_dp + kBR * CG);      // [NPAD]
-  uint32_t* tm_slot = reinterpret_cast<uint32_t*>(code + S::NPAD);
+__global__ void __launch_bounds__(S::THREADS, S::MINB)
+grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
+  constexpr int NT = S::NT, HD = S::HD, CG = S::CG, PITCH = S::PITCH, STAGES = S::STAGES;
+  using R = Rows<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* red = reinterpret_cast<float*>(smem + STAGES * S::STAGE);       // [2][warp][16][PITCH]
+  float4* ex = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // [2][CG][64]
+  uint32_t* mask_s = reinterpret_cast<uint32_t*>(ex + 2 * CG * kBR);     // [NPAD][4]
+  Tail* tail = reinterpret_cast<Tail*>(mask_s + S::NPAD * 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rg = warp / CG, cg = warp % CG;
@@ -270,547 +466,623 @@ __global__ void __launch_bounds__(S::THREADS, S::MINB) grad_rows_kernel(const Gr
   const int row0 = rb * kBR;
   const int rows = min(kBR, p.N - row0);
   const bool live = rg * 16 < rows;
+  const uint32_t warps = uint32_t((rows + 15) / 16 * CG);  // live ones
+  const int count = (p.B - share + p.S - 1) / p.S;
   const int i0 = row0 + rg * 16 + g, i1 = i0 + 8;  // this thread's two query rows
   const int jb = cg * S::WC + 2 * t4;              // its first column; tile t adds 8 t
-  const float inv_scale = 1.f / p.scale;
   const float c1 = p.scale * kLog2e;
-  const float pen = -100.f * inv_scale;
 
-  // shared memory past the window's rows stays zero
-  for (int i = tid * 16; i < 2 * S::STAGE; i += S::THREADS * 16)
-    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
-  if (p.analytic)
-    for (int i = tid; i < S::NPAD; i += S::THREADS)
-      code[i] = i < p.N ? uint8_t(side_code(p, i)) : uint8_t(0);
+  auto issue = [&](int k) {
+    const int st = k % STAGES, b = share + k * p.S;
+    uint8_t* base = smem + st * S::STAGE;
+    uint64_t* full = &tail->full[st];
+    if (p.analytic) tail->last[st] = last_axes(p, b);
+    tail->issued = k + 1;
+    mbar_arrive_expect_tx(full, S::STAGE);
+    load_rows<HD, S::NPAD>(base, &maps.k_cols, full, 0, h, b);
+    load_rows<HD, S::NPAD>(base + S::COLS, &maps.v_cols, full, 0, h, b);
+    load_rows<HD, kBR>(base + 2 * S::COLS, &maps.q_rows, full, row0, h, b);
+    load_rows<HD, kBR>(base + 2 * S::COLS + S::ROWS, &maps.o_rows, full, row0, h, b);
+  };
+  if (tid == 0) {
+    init_tail(tail);
+    for (int k = 0; k < STAGES && k < count; ++k) issue(k);
+  }
+  uint32_t f0 = 0, f1 = 0;
+  if (p.analytic) {
+    for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
+      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4, p.scale) : 0u;
+    f0 = i0 < p.N ? row_feature<BF16>(side_code(p, i0), t4) : 0u;
+    f1 = i1 < p.N ? row_feature<BF16>(side_code(p, i1), t4) : 0u;
+  }
   if (warp == 0) {
-    tmem_alloc(tm_slot, S::TM_COLS);
+    tmem_alloc(&tail->tm_slot, S::TM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // a warp reads and writes the 32 tensor-memory lanes of its quarter
-  const uint32_t tm = *tm_slot + (uint32_t(32 * (warp & 3)) << 16) + uint32_t((warp >> 2) * S::TM_WARP);
+  const uint32_t tm =
+      tail->tm_slot + (uint32_t(32 * (warp & 3)) << 16) + uint32_t((warp >> 2) * S::WC);
   const uint32_t tm_bias = tm, tm_sum = tm + NT * 4;
+
   if (live) {
+    {
+      float v[NT][4];
+      start_values<NT, BF16, false>(p, h, i0, jb, v);
+      tm_st<NT * 4>(tm_bias, v[0]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[t][e] = 0.f;
+      tm_st<NT * 4>(tm_sum, v[0]);
+      tmem_wait_st();
+    }
+    const int width = p.H * HD, tok = 3 * width;  // elements per token of the output and of qkv
+    // dq of window k: the sum of the CG warps' parts
+    auto join = [&](int k) {
+      const float* all = red + ((k & 1) * S::WARPS + rg * CG) * 16 * PITCH;
+      uint16_t* to = p.dqkv + ((long long)(share + k * p.S) * p.N + row0 + rg * 16) * tok + h * HD;
+#pragma unroll
+      for (int o = cg * 32 + lane; o < 16 * HD / 2; o += 32 * CG) {
+        const int r = o / (HD / 2), c = (o % (HD / 2)) * 2;
+        float2 v = *reinterpret_cast<const float2*>(all + r * PITCH + c);
+#pragma unroll
+        for (int w = 1; w < CG; ++w)
+          v = __fadd2_rn(v, *reinterpret_cast<const float2*>(all + (w * 16 + r) * PITCH + c));
+        if (row0 + rg * 16 + r < p.N)
+          *reinterpret_cast<uint32_t*>(to + r * tok + c) = pack2<BF16>(v.x, v.y);
+      }
+    };
+
+    // lane parts of the ldmatrix addresses
+    const uint32_t a_off = R::at(rg * 16 + (lane & 15), lane >> 4);
+    const uint32_t a_off1 = HD == 32 ? R::at(rg * 16 + (lane & 15), (lane >> 4) + 2) : 0u;
+    const uint32_t col0 = uint32_t(cg * S::WC * R::BYTES);
+    const uint32_t b_off =
+        col0 + (HD == 16 ? R::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1)  // 2 tiles
+                         : R::at(lane & 7, lane >> 3));                          // 1 tile
+    const uint32_t bt_off = col0 + R::at(lane & 15, lane >> 4);
+    const uint32_t bt_off1 = HD == 32 ? col0 + R::at(lane & 15, (lane >> 4) + 2) : 0u;
+
 #pragma unroll 1
-    for (int t = 0; t < NT; ++t) {
-      float v[4];
+    for (int k = 0; k < count; ++k) {
+      // scores: the accumulators start at bias / scale
+      float s[NT][4];
+      wait_stage<STAGES>(tail, k);
+      tm_ld<NT * 4>(tm_bias, s[0]);
+      const uint32_t ks = smem_u32(smem) + uint32_t((k % STAGES) * S::STAGE);
+      const uint32_t vs = ks + S::COLS, qs = vs + S::COLS, gs = qs + S::ROWS;
+      {
+        uint32_t a[R::KS][4];
+        ldsm_x4(qs + a_off, a[0]);
+        if constexpr (HD == 32) ldsm_x4(qs + a_off1, a[1]);
+        tm_wait<NT>(s);
+        if constexpr (HD == 16) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = e < 2 ? i0 : i1, j = jb + 8 * t + (e & 1);
-        v[e] = j < p.N ? bias_start<BF16>(p, h, i, j, inv_scale) : -INFINITY;
-      }
-      tm_st4(tm_bias + 4 * t, v);
-      const float z[4] = {0.f, 0.f, 0.f, 0.f};
-      tm_st4(tm_sum + 4 * t, z);
-    }
-    tmem_wait_st();
-  }
-
-  const long long tok = 3LL * p.H * HD;  // elements per token of qkv
-  auto fetch = [&](int b, int st) {
-    const uint32_t base = smem_u32(smem) + uint32_t(st * S::STAGE);
-    const uint16_t* w = p.qkv + (long long)b * p.N * tok + h * HD;
-    copy_rows<HD, PITCH>(base, w + p.H * HD, tok, p.N, tid, S::THREADS);
-    copy_rows<HD, PITCH>(base + S::COLS_BYTES, w + 2 * p.H * HD, tok, p.N, tid, S::THREADS);
-    copy_rows<HD, PITCH>(base + 2 * S::COLS_BYTES, w + row0 * tok, tok, rows, tid, S::THREADS);
-    copy_rows<HD, PITCH>(base + 2 * S::COLS_BYTES + S::ROWS_BYTES,
-                         p.dout + ((long long)b * p.N + row0) * p.H * HD + h * HD, p.H * HD, rows,
-                         tid, S::THREADS);
-    cp_commit();
-  };
-
-  // lane parts of the ldmatrix addresses
-  const uint32_t a_off = uint32_t((lane & 15) * PITCH + (lane >> 4) * 16);             // A, rows
-  const uint32_t b_off = HD == 16 ? uint32_t(((lane & 7) + (lane >> 4) * 8) * PITCH +
-                                             ((lane >> 3) & 1) * 16)                   // 2 tiles
-                                  : uint32_t((lane & 7) * PITCH + (lane >> 3) * 16);   // 1 tile
-  const uint32_t bt_off = uint32_t((lane & 15) * PITCH + (lane >> 4) * 16);            // B, trans
-
-  int st = 0;
-  if (share < p.B) fetch(share, 0);
-  for (int b = share; b < p.B; b += p.S, st ^= 1) {
-    cp_wait_all();
-    __syncthreads();  // window b has landed; the other stage is no longer read
-    if (b + p.S < p.B) fetch(b + p.S, st ^ 1);
-    if (!live) continue;
-    const uint32_t ks = smem_u32(smem) + uint32_t(st * S::STAGE);
-    const uint32_t vs = ks + S::COLS_BYTES;
-    const uint32_t qs = vs + S::COLS_BYTES + uint32_t(rg * 16 * PITCH);
-    const uint32_t gs = qs + S::ROWS_BYTES;
-    const uint32_t col0 = uint32_t(cg * S::WC * PITCH);
-
-    // scores: the accumulators start at bias / scale
-    float s[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) tm_ld4(tm_bias + 4 * t, s[t]);
-    {
-      uint32_t a[S::KS][4];
-#pragma unroll
-      for (int k = 0; k < S::KS; ++k) ldsm_x4(qs + a_off + 32 * k, a[k]);
-      tm_wait<NT>(s);
-      if constexpr (HD == 16) {
-#pragma unroll
-        for (int t = 0; t < NT; t += 2) {
-          uint32_t bf[4];  // past the last tile: rows of the next warp or of V, not used
-          ldsm_x4(ks + col0 + uint32_t(8 * t * PITCH) + b_off, bf);
-          mma16<BF16>(s[t], a[0], bf[0], bf[1], s[t]);
-          if (t + 1 < NT) mma16<BF16>(s[t + 1], a[0], bf[2], bf[3], s[t + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint32_t bf[4];
-          ldsm_x4(ks + col0 + uint32_t(8 * t * PITCH) + b_off, bf);
-          mma16<BF16>(s[t], a[0], bf[0], bf[1], s[t]);
-          mma16<BF16>(s[t], a[1], bf[2], bf[3], s[t]);
-        }
-      }
-    }
-    if (p.analytic) {
-      const uint32_t last = last_axes(p, b);
-      if (last != 0) {  // padded rows (i >= N) take code 0: their results are not kept
-        const uint32_t r0 = i0 < p.N ? code[i0] : 0u, r1 = i1 < p.N ? code[i1] : 0u;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint32_t k0 = code[jb + 8 * t], k1 = code[jb + 8 * t + 1];
-          if ((r0 ^ k0) & last) s[t][0] += pen;
-          if ((r0 ^ k1) & last) s[t][1] += pen;
-          if ((r1 ^ k0) & last) s[t][2] += pen;
-          if ((r1 ^ k1) & last) s[t][3] += pen;
-        }
-      }
-    }
-    // row maxima over the CG warps of the row
-    float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
-      m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      m0 = fmaxf(m0, __shfl_xor_sync(~0u, m0, o));
-      m1 = fmaxf(m1, __shfl_xor_sync(~0u, m1, o));
-    }
-    const int lr0 = rg * 16 + g, lr1 = lr0 + 8;
-    if constexpr (CG > 1) {
-      if (t4 == 0) {
-        ex_max[lr0 * CG + cg] = m0;
-        ex_max[lr1 * CG + cg] = m1;
-      }
-      bar_sync(1 + rg, 32 * CG);
-#pragma unroll
-      for (int c = 0; c < CG; ++c) {
-        m0 = fmaxf(m0, ex_max[lr0 * CG + c]);
-        m1 = fmaxf(m1, ex_max[lr1 * CG + c]);
-      }
-    }
-    const float n0 = -m0 * c1, n1 = -m1 * c1;
-    float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      s[t][0] = ex2(fmaf(s[t][0], c1, n0));
-      s[t][1] = ex2(fmaf(s[t][1], c1, n0));
-      s[t][2] = ex2(fmaf(s[t][2], c1, n1));
-      s[t][3] = ex2(fmaf(s[t][3], c1, n1));
-      l0 += s[t][0] + s[t][1];
-      l1 += s[t][2] + s[t][3];
-    }
-    // dp = do v^T
-    float d[NT][4];
-    float g0 = 1.f, g1 = 1.f, am0 = 0.f, am1 = 0.f;
-    {
-      uint32_t a[S::KS][4];
-#pragma unroll
-      for (int k = 0; k < S::KS; ++k) ldsm_x4(gs + a_off + 32 * k, a[k]);
-      if constexpr (!BF16) {  // power-of-two scale of ds, from the row's largest |do|
-#pragma unroll
-        for (int k = 0; k < S::KS; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a[k][e]));
-            const float m = fmaxf(fabsf(v.x), fabsf(v.y));
-            if (e & 1) am1 = fmaxf(am1, m);
-            else am0 = fmaxf(am0, m);
+          for (int t = 0; t < NT; t += 2) {
+            uint32_t bf[4];  // past the last tile: rows of the next warp, V or Q, not used
+            ldsm_x4(ks + b_off + uint32_t(8 * t * R::BYTES), bf);
+            mma16<BF16>(s[t], a[0], bf[0], bf[1], s[t]);
+            if (t + 1 < NT) mma16<BF16>(s[t + 1], a[0], bf[2], bf[3], s[t + 1]);
           }
+        } else {
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
-          am1 = fmaxf(am1, __shfl_xor_sync(~0u, am1, o));
+          for (int t = 0; t < NT; ++t) {
+            uint32_t bf[4];
+            ldsm_x4(ks + b_off + uint32_t(8 * t * R::BYTES), bf);
+            mma16<BF16>(s[t], a[0], bf[0], bf[1], s[t]);
+            mma16<BF16>(s[t], a[1], bf[2], bf[3], s[t]);
+          }
         }
-        g0 = grad_scale(am0);
-        g1 = grad_scale(am1);
       }
-      const float z[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (HD == 16) {
+      if (p.analytic) {
+        const uint32_t last = tail->last[k % STAGES];
+        if (last != 0) {
+          const bool on = (last >> t4) & 1u;
+          const uint32_t a0 = on ? f0 : 0u, a1 = on ? f1 : 0u;
+          const uint32_t* mb = mask_s + (cg * S::WC + g) * 4 + t4;
 #pragma unroll
-        for (int t = 0; t < NT; t += 2) {
-          uint32_t bf[4];
-          ldsm_x4(vs + col0 + uint32_t(8 * t * PITCH) + b_off, bf);
-          mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
-          if (t + 1 < NT) mma16<BF16>(d[t + 1], a[0], bf[2], bf[3], z);
+          for (int t = 0; t < NT; ++t) mma8<BF16>(s[t], a0, a1, mb[32 * t]);
         }
+      }
+      // maxima of this warp's columns (a warp of padded columns only: a finite stand-in)
+      float m0 = -1e30f, m1 = -1e30f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        m0 = max3(m0, s[t][0], s[t][1]);
+        m1 = max3(m1, s[t][2], s[t][3]);
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(~0u, m0, o));
+        m1 = fmaxf(m1, __shfl_xor_sync(~0u, m1, o));
+      }
+      const float2 cc = both(c1), n0 = both(-m0 * c1), n1 = both(-m1 * c1);
+      float2 l0 = both(0.f), l1 = both(0.f);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 x0 = __ffma2_rn(two(s[t], 0), cc, n0), x1 = __ffma2_rn(two(s[t], 1), cc, n1);
+        const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
+        l0 = __fadd2_rn(l0, p0);
+        l1 = __fadd2_rn(l1, p1);
+        put(s[t], 0, p0);
+        put(s[t], 1, p1);
+      }
+      // dp = do v^T
+      float d[NT][4];
+      float g0 = 1.f, g1 = 1.f;
+      {
+        uint32_t a[R::KS][4];
+        ldsm_x4(gs + a_off, a[0]);
+        if constexpr (HD == 32) ldsm_x4(gs + a_off1, a[1]);
+        if constexpr (!BF16) {  // power-of-two scale of ds, from the row's largest |do|
+          __half2 h0 = __float2half2_rn(0.f), h1 = h0;
+#pragma unroll
+          for (int q = 0; q < R::KS; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __half2 v = __habs2(*reinterpret_cast<const __half2*>(&a[q][e]));
+              if (e & 1) h1 = __hmax2(h1, v);
+              else h0 = __hmax2(h0, v);
+            }
+          float am0 = __half2float(__hmax(__low2half(h0), __high2half(h0)));
+          float am1 = __half2float(__hmax(__low2half(h1), __high2half(h1)));
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
+            am1 = fmaxf(am1, __shfl_xor_sync(~0u, am1, o));
+          }
+          g0 = grad_scale(am0);
+          g1 = grad_scale(am1);
+          if (cg == 0) {  // the row group's, for the columns kernel
+            am0 = fmaxf(am0, am1);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
+            if (lane == 0)
+              p.amax[((long long)(share + k * p.S) * p.H + h) * ((p.N + 15) / 16) + rb * kRG + rg] =
+                  am0;
+          }
+        }
+        const float z[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (HD == 16) {
+#pragma unroll
+          for (int t = 0; t < NT; t += 2) {
+            uint32_t bf[4];
+            ldsm_x4(vs + b_off + uint32_t(8 * t * R::BYTES), bf);
+            mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
+            if (t + 1 < NT) mma16<BF16>(d[t + 1], a[0], bf[2], bf[3], z);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            uint32_t bf[4];
+            ldsm_x4(vs + b_off + uint32_t(8 * t * R::BYTES), bf);
+            mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
+            mma16<BF16>(d[t], a[1], bf[2], bf[3], d[t]);
+          }
+        }
+      }
+      float2 e0 = both(0.f), e1 = both(0.f);  // sums of p dp
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        e0 = __ffma2_rn(two(s[t], 0), two(d[t], 0), e0);
+        e1 = __ffma2_rn(two(s[t], 1), two(d[t], 1), e1);
+      }
+      // (sum of exponentials, sum of p dp) of the two rows
+      float2 q0 = make_float2(l0.x + l0.y, e0.x + e0.y), q1 = make_float2(l1.x + l1.y, e1.x + e1.y);
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        q0 = __fadd2_rn(q0, make_float2(__shfl_xor_sync(~0u, q0.x, o), __shfl_xor_sync(~0u, q0.y, o)));
+        q1 = __fadd2_rn(q1, make_float2(__shfl_xor_sync(~0u, q1.x, o), __shfl_xor_sync(~0u, q1.y, o)));
+      }
+      float r0 = 1.f, r1 = 1.f;  // this warp's exponentials relative to the row's
+      if constexpr (CG > 1) {
+        float4* x = ex + (k & 1) * CG * kBR + rg * 16;
+        if (t4 == 0) {
+          x[cg * kBR + g] = make_float4(m0, q0.x, q0.y, 0.f);
+          x[cg * kBR + g + 8] = make_float4(m1, q1.x, q1.y, 0.f);
+        }
+        bar_sync(1 + rg, 32 * CG);
+        if (k > 0) join(k - 1);
+        // every warp of the row adds the same parts in the same order
+        const float own0 = m0, own1 = m1;
+        float4 y0[CG], y1[CG];
+#pragma unroll
+        for (int c = 0; c < CG; ++c) {
+          y0[c] = x[c * kBR + g];
+          y1[c] = x[c * kBR + g + 8];
+          m0 = fmaxf(m0, y0[c].x);
+          m1 = fmaxf(m1, y1[c].x);
+        }
+        q0 = q1 = both(0.f);
+#pragma unroll
+        for (int c = 0; c < CG; ++c) {
+          q0 = __ffma2_rn(make_float2(y0[c].y, y0[c].z), both(ex2((y0[c].x - m0) * c1)), q0);
+          q1 = __ffma2_rn(make_float2(y1[c].y, y1[c].z), both(ex2((y1[c].x - m1) * c1)), q1);
+        }
+        r0 = ex2((own0 - m0) * c1);
+        r1 = ex2((own1 - m1) * c1);
       } else {
+        __syncwarp();
+        if (k > 0) join(k - 1);
+      }
+      const float inv0 = rcp(q0.x), inv1 = rcp(q1.x);
+      const float del0 = q0.y * inv0, del1 = q1.y * inv1;
+      if (cg == 0 && t4 == 0) {  // statistics for the columns kernel
+        float2* to = p.stats + ((long long)(share + k * p.S) * p.H + h) * p.NS;
+        // (row N of an odd N is copied along by the columns kernel: its p has to be finite)
+        const float2 zero = make_float2(0.f, 0.f);
+        if (i0 < p.NS) to[i0] = i0 < p.N ? make_float2(fmaf(m0, c1, __log2f(q0.x)), del0) : zero;
+        if (i1 < p.NS) to[i1] = i1 < p.N ? make_float2(fmaf(m1, c1, __log2f(q1.x)), del1) : zero;
+      }
+      // ds = p (dp - delta), in place of dp; times the row's power of two in fp16
+      {
+        const float2 v0 = both(r0 * inv0 * g0), v1 = both(r1 * inv1 * g1);
+        const float2 w0 = both(-del0 * v0.x), w1 = both(-del1 * v1.x);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          uint32_t bf[4];
-          ldsm_x4(vs + col0 + uint32_t(8 * t * PITCH) + b_off, bf);
-          mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
-          mma16<BF16>(d[t], a[1], bf[2], bf[3], d[t]);
+          put(d[t], 0, __fmul2_rn(two(s[t], 0), __ffma2_rn(two(d[t], 0), v0, w0)));
+          put(d[t], 1, __fmul2_rn(two(s[t], 1), __ffma2_rn(two(d[t], 1), v1, w1)));
         }
       }
-    }
-    float e0 = 0.f, e1 = 0.f;  // sum of p dp, before the division by the row sum
+      // dbias += ds
+      tmem_wait_st();  // the previous window's sums are written
+      tm_ld<NT * 4>(tm_sum, s[0]);
+      // dq = ds k, ds rounded to the element type: the rounding errors of a row's keys are
+      // independent, so they add up like one rounding of dq itself
+      float acc[HD / 8][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      e0 = fmaf(s[t][0], d[t][0], e0);
-      e0 = fmaf(s[t][1], d[t][1], e0);
-      e1 = fmaf(s[t][2], d[t][2], e1);
-      e1 = fmaf(s[t][3], d[t][3], e1);
-    }
+      for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      l0 += __shfl_xor_sync(~0u, l0, o);
-      l1 += __shfl_xor_sync(~0u, l1, o);
-      e0 += __shfl_xor_sync(~0u, e0, o);
-      e1 += __shfl_xor_sync(~0u, e1, o);
-    }
-    if constexpr (CG > 1) {
-      if (t4 == 0) {
-        ex_sum[lr0 * CG + cg] = l0;
-        ex_sum[lr1 * CG + cg] = l1;
-        ex_dp[lr0 * CG + cg] = e0;
-        ex_dp[lr1 * CG + cg] = e1;
-      }
-      bar_sync(1 + rg, 32 * CG);
-      l0 = l1 = e0 = e1 = 0.f;  // every warp of the row adds the same partials in the same order
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
-      for (int c = 0; c < CG; ++c) {
-        l0 += ex_sum[lr0 * CG + c];
-        l1 += ex_sum[lr1 * CG + c];
-        e0 += ex_dp[lr0 * CG + c];
-        e1 += ex_dp[lr1 * CG + c];
-      }
-    }
-    const float inv0 = 1.f / l0, inv1 = 1.f / l1;
-    const float del0 = e0 * inv0, del1 = e1 * inv1;
-    if (cg == 0 && t4 == 0) {  // statistics for the columns kernel
-      const long long at = ((long long)b * p.H + h) * p.N;
-      if (i0 < p.N) p.stats[at + i0] = make_float2(fmaf(m0, c1, log2f(l0)), del0);
-      if (i1 < p.N) p.stats[at + i1] = make_float2(fmaf(m1, c1, log2f(l1)), del1);
-      if constexpr (!BF16) {
-        if (i0 < p.N) p.amax[at + i0] = am0;
-        if (i1 < p.N) p.amax[at + i1] = am1;
-      }
-    }
-    // ds = p (dp - delta), in place of dp
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      d[t][0] = (d[t][0] - del0) * (s[t][0] * inv0);
-      d[t][1] = (d[t][1] - del0) * (s[t][1] * inv0);
-      d[t][2] = (d[t][2] - del1) * (s[t][2] * inv1);
-      d[t][3] = (d[t][3] - del1) * (s[t][3] * inv1);
-    }
-    // dbias += ds
-    tmem_wait_st();  // the previous window's sums are written
-#pragma unroll
-    for (int t = 0; t < NT; ++t) tm_ld4(tm_sum + 4 * t, s[t]);
-    tm_wait<NT>(s);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][e] += d[t][e];
-      tm_st4(tm_sum + 4 * t, s[t]);
-    }
-    // dq = ds k, ds rounded to the element type (scaled as above): the rounding errors of a
-    // row's keys are independent, so they add up like one rounding of dq itself
-    float acc[HD / 8][4];
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; t += 2) {
-      uint32_t a[4];
-      a[0] = pack2<BF16>(d[t][0] * g0, d[t][1] * g0);
-      a[1] = pack2<BF16>(d[t][2] * g1, d[t][3] * g1);
-      if (t + 1 < NT) {
-        a[2] = pack2<BF16>(d[t + 1][0] * g0, d[t + 1][1] * g0);
-        a[3] = pack2<BF16>(d[t + 1][2] * g1, d[t + 1][3] * g1);
-      }
-#pragma unroll
-      for (int n = 0; n < HD / 16; ++n) {
-        uint32_t bf[4];  // past the last tile: as above
-        ldsm_x4_t(ks + col0 + uint32_t(8 * t * PITCH) + bt_off + 32 * n, bf);
+      for (int t = 0; t < NT; t += 2) {
+        uint32_t a[4];
+        a[0] = pack2<BF16>(d[t][0], d[t][1]);
+        a[1] = pack2<BF16>(d[t][2], d[t][3]);
         if (t + 1 < NT) {
-          mma16<BF16>(acc[2 * n], a, bf[0], bf[1], acc[2 * n]);
-          mma16<BF16>(acc[2 * n + 1], a, bf[2], bf[3], acc[2 * n + 1]);
-        } else {
-          mma8<BF16>(acc[2 * n], a[0], a[1], bf[0]);
-          mma8<BF16>(acc[2 * n + 1], a[0], a[1], bf[2]);
+          a[2] = pack2<BF16>(d[t + 1][0], d[t + 1][1]);
+          a[3] = pack2<BF16>(d[t + 1][2], d[t + 1][3]);
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+          uint32_t bf[4];  // past the last tile: as above
+          ldsm_x4_t(ks + (n ? bt_off1 : bt_off) + uint32_t(8 * t * R::BYTES), bf);
+          if (t + 1 < NT) {
+            mma16<BF16>(acc[2 * n], a, bf[0], bf[1], acc[2 * n]);
+            mma16<BF16>(acc[2 * n + 1], a, bf[2], bf[3], acc[2 * n + 1]);
+          } else {
+            mma8<BF16>(acc[2 * n], a[0], a[1], bf[0]);
+            mma8<BF16>(acc[2 * n + 1], a[0], a[1], bf[2]);
+          }
         }
       }
-    }
-    const float f0 = BF16 ? p.scale : p.scale / g0, f1 = BF16 ? p.scale : p.scale / g1;
-    float* mine = red + (rg * CG + cg) * 16 * HD;
+      const float u0 = inverse_scale(g0), u1 = inverse_scale(g1);
+      tm_wait<NT>(s);
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-      *reinterpret_cast<float2*>(mine + g * HD + 8 * n + 2 * t4) =
-          make_float2(acc[n][0] * f0, acc[n][1] * f0);
-      *reinterpret_cast<float2*>(mine + (g + 8) * HD + 8 * n + 2 * t4) =
-          make_float2(acc[n][2] * f1, acc[n][3] * f1);
-    }
-    bar_sync(1 + rg, 32 * CG);
-    const float* all = red + rg * CG * 16 * HD;
-    for (int o = cg * 32 + lane; o < 16 * HD / 2; o += 32 * CG) {
-      const int r = o / (HD / 2), c = (o % (HD / 2)) * 2;
-      float2 v = *reinterpret_cast<const float2*>(all + r * HD + c);
-#pragma unroll
-      for (int k = 1; k < CG; ++k) {
-        const float2 w = *reinterpret_cast<const float2*>(all + k * 16 * HD + r * HD + c);
-        v.x += w.x;
-        v.y += w.y;
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (BF16) {
+          put(s[t], 0, __fadd2_rn(two(s[t], 0), two(d[t], 0)));
+          put(s[t], 1, __fadd2_rn(two(s[t], 1), two(d[t], 1)));
+        } else {
+          put(s[t], 0, __ffma2_rn(two(d[t], 0), both(u0), two(s[t], 0)));
+          put(s[t], 1, __ffma2_rn(two(d[t], 1), both(u1), two(s[t], 1)));
+        }
       }
-      const int i = row0 + rg * 16 + r;
-      if (i < p.N)
-        *reinterpret_cast<uint32_t*>(p.dqkv + ((long long)b * p.N + i) * tok + h * HD + c) =
-            pack2<BF16>(v.x, v.y);
+      tm_st<NT * 4>(tm_sum, s[0]);
+      if (release_stage<STAGES>(tail, k, count, warps)) issue(k + STAGES);
+      // this warp's part of dq, joined behind the next window's barrier
+      const float h0 = p.scale * u0, h1 = p.scale * u1;
+      float* mine = red + ((k & 1) * S::WARPS + warp) * 16 * PITCH + g * PITCH + 2 * t4;
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) {
+        *reinterpret_cast<float2*>(mine + 8 * n) = make_float2(acc[n][0] * h0, acc[n][1] * h0);
+        *reinterpret_cast<float2*>(mine + 8 * PITCH + 8 * n) =
+            make_float2(acc[n][2] * h1, acc[n][3] * h1);
+      }
     }
-  }
-
-  if (live) {  // the head's dbias of this share of the windows
+    if (count > 0) {
+      bar_sync(1 + rg, 32 * CG);
+      join(count - 1);
+    }
+    // the head's dbias of this share of the windows
     tmem_wait_st();
     float* out = p.dbias + ((long long)share * p.H + h) * p.N * p.N;
-#pragma unroll 1
-    for (int t = 0; t < NT; ++t) {
-      float v[1][4];
-      tm_ld4(tm_sum + 4 * t, v[0]);
-      tm_wait<1>(v);
+    float v[NT][4];
+    tm_ld<NT * 4>(tm_sum, v[0]);
+    tm_wait<NT>(v);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = e < 2 ? i0 : i1, j = jb + 8 * t + (e & 1);
-        if (i < p.N && j < p.N) out[(long long)i * p.N + j] = v[0][e];
+        if (i < p.N && j < p.N) out[(long long)i * p.N + j] = v[t][e];
       }
-    }
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0) finish_ring<STAGES>(tail);
   if (warp == 0) {
+    __syncwarp();
     tc_fence_after();
-    tmem_dealloc(*tm_slot, S::TM_COLS);
+    tmem_dealloc(tail->tm_slot, S::TM_COLS);
   }
 }
 
 // --------------------------------------------------------------------- columns kernel
-// The same tiles transposed: rows are 64 keys, columns all queries; p and ds come from the
-// statistics, are rounded and multiplied by do and q at once, two tiles at a time.
+// A warp's rows are 16 keys, its columns all queries: p and ds come from the statistics, are
+// rounded and multiplied by do and q at once, two tiles of 8 queries at a time.
 template <class S, bool BF16>
-__global__ void __launch_bounds__(S::THREADS, S::MINB) grad_cols_kernel(const GradParams p) {
-  constexpr int NT = S::NT, HD = S::HD, CG = S::CG, PITCH = S::PITCH;
-  extern __shared__ __align__(16) uint8_t smem[];
-  float2* stat_s = reinterpret_cast<float2*>(smem + 2 * S::STAGE);      // [2][NPAD]
-  float* amax_s = reinterpret_cast<float*>(stat_s + 2 * S::NPAD);       // [2][NPAD]
-  float* red = amax_s + 2 * S::NPAD;                                    // [2][warp][16][HD]
-  uint8_t* code = reinterpret_cast<uint8_t*>(red) + S::RED_COLS;        // [NPAD]
+__global__ void __launch_bounds__(S::THREADS, S::MINB)
+grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
+  constexpr int NT = S::NT, HD = S::HD, STAGES = S::STAGES, TT = S::TT;
+  using R = Rows<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint32_t* mask_s = reinterpret_cast<uint32_t*>(smem + STAGES * S::STAGE);  // [NPAD][4]
+  Tail* tail = reinterpret_cast<Tail*>(mask_s + S::NPAD * 4);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rg = warp / CG, cg = warp % CG;
   const int g = lane >> 2, t4 = lane & 3;
   int blk = blockIdx.x;
   const int share = blk % p.S;
   blk /= p.S;
   const int rb = blk % p.RB, h = blk / p.RB;
-  const int row0 = rb * kBR;
-  const int rows = min(kBR, p.N - row0);
-  const bool live = rg * 16 < rows;
-  const int k0 = row0 + rg * 16 + g, k1 = k0 + 8;  // this thread's two keys
-  const int ib = cg * S::WC + 2 * t4;              // its first query; tile t adds 8 t
-  const float inv_scale = 1.f / p.scale;
-  const float c1 = p.scale * kLog2e;
-  const float pen = -100.f * inv_scale;
+  const int row0 = rb * S::BR;
+  const int rows = min(S::BR, p.N - row0);
+  const bool live = warp * 16 < rows;
+  const uint32_t warps = uint32_t((rows + 15) / 16);
+  const int count = (p.B - share + p.S - 1) / p.S;
+  const int k0 = row0 + warp * 16 + g, k1 = k0 + 8;  // this thread's two keys
+  const int groups = (p.N + 15) / 16;
+  const uint32_t stat_bytes = uint32_t(p.NS) * 8u;
 
-  // zero past the window's rows: Q, dO, K, V and the statistics
-  for (int i = tid * 16; i < 2 * S::STAGE + 2 * S::NPAD * 12; i += S::THREADS * 16)
-    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
-  if (p.analytic)
-    for (int i = tid; i < S::NPAD; i += S::THREADS)
-      code[i] = i < p.N ? uint8_t(side_code(p, i)) : uint8_t(0);
-  __syncthreads();
-
-  float bias[NT][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int k = e < 2 ? k0 : k1, i = ib + 8 * t + (e & 1);
-      bias[t][e] = i < p.N ? bias_start<BF16>(p, h, i, k, inv_scale) : -INFINITY;
-    }
-
-  const long long tok = 3LL * p.H * HD;
-  auto fetch = [&](int b, int st) {
-    const uint32_t base = smem_u32(smem) + uint32_t(st * S::STAGE);
-    const uint16_t* w = p.qkv + (long long)b * p.N * tok + h * HD;
-    copy_rows<HD, PITCH>(base, w, tok, p.N, tid, S::THREADS);
-    copy_rows<HD, PITCH>(base + S::COLS_BYTES, p.dout + (long long)b * p.N * p.H * HD + h * HD,
-                         p.H * HD, p.N, tid, S::THREADS);
-    copy_rows<HD, PITCH>(base + 2 * S::COLS_BYTES, w + p.H * HD + row0 * tok, tok, rows, tid,
-                         S::THREADS);
-    copy_rows<HD, PITCH>(base + 2 * S::COLS_BYTES + S::ROWS_BYTES, w + 2 * p.H * HD + row0 * tok,
-                         tok, rows, tid, S::THREADS);
-    const long long at = ((long long)b * p.H + h) * p.N;
-    for (int i = tid; i < p.N; i += S::THREADS) {
-      cp8(smem_u32(stat_s + st * S::NPAD + i), p.stats + at + i);
-      if constexpr (!BF16) cp4(smem_u32(amax_s + st * S::NPAD + i), p.amax + at + i);
-    }
-    cp_commit();
+  auto issue = [&](int k) {
+    const int st = k % STAGES, b = share + k * p.S;
+    uint8_t* base = smem + st * S::STAGE;
+    uint64_t* full = &tail->full[st];
+    if (p.analytic) tail->last[st] = last_axes(p, b);
+    tail->issued = k + 1;
+    mbar_arrive_expect_tx(full, 2 * S::COLS + 2 * S::ROWS + stat_bytes);
+    load_rows<HD, S::NPAD>(base, &maps.q_cols, full, 0, h, b);
+    load_rows<HD, S::NPAD>(base + S::COLS, &maps.o_cols, full, 0, h, b);
+    load_rows<HD, S::BR>(base + 2 * S::COLS, &maps.k_rows, full, row0, h, b);
+    load_rows<HD, S::BR>(base + 2 * S::COLS + S::ROWS, &maps.v_rows, full, row0, h, b);
+    bulk_load(base + 2 * S::COLS + 2 * S::ROWS, p.stats + ((long long)b * p.H + h) * p.NS,
+              stat_bytes, full);
   };
+  // the statistics of padded queries are not copied: 0 (read as p = 2^-inf)
+  for (int i = tid; i < STAGES * S::NPAD; i += S::THREADS)
+    *reinterpret_cast<float2*>(smem + (i / S::NPAD) * S::STAGE + 2 * S::COLS + 2 * S::ROWS +
+                               (i % S::NPAD) * 8) = make_float2(0.f, 0.f);
+  uint32_t f0 = 0, f1 = 0;
+  if (p.analytic) {
+    for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
+      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4, p.scale) : 0u;
+    f0 = k0 < p.N ? row_feature<BF16>(side_code(p, k0), t4) : 0u;
+    f1 = k1 < p.N ? row_feature<BF16>(side_code(p, k1), t4) : 0u;
+  }
+  if (warp == 0) {
+    tmem_alloc(&tail->tm_slot, S::TM_COLS);
+    tmem_relinquish();
+  }
+  if (tid == 0) init_tail(tail);
+  fence_proxy_async_shared();  // the zeroed statistics, before the copies over them
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0)
+    for (int k = 0; k < STAGES && k < count; ++k) issue(k);
+  const uint32_t tm_bias =
+      tail->tm_slot + (uint32_t(32 * (warp & 3)) << 16) + uint32_t((warp >> 2) * 4 * TT);
 
-  const uint32_t a_off = uint32_t((lane & 15) * PITCH + (lane >> 4) * 16);
-  const uint32_t b_off = HD == 16 ? uint32_t(((lane & 7) + (lane >> 4) * 8) * PITCH +
-                                             ((lane >> 3) & 1) * 16)
-                                  : uint32_t((lane & 7) * PITCH + (lane >> 3) * 16);
-  const uint32_t bt_off = uint32_t((lane & 15) * PITCH + (lane >> 4) * 16);
-
-  int st = 0;
-  if (share < p.B) fetch(share, 0);
-  for (int b = share; b < p.B; b += p.S, st ^= 1) {
-    cp_wait_all();
-    __syncthreads();
-    if (b + p.S < p.B) fetch(b + p.S, st ^ 1);
-    if (!live) continue;
-    const uint32_t qs = smem_u32(smem) + uint32_t(st * S::STAGE);
-    const uint32_t gs = qs + S::COLS_BYTES;
-    const uint32_t ks = gs + S::COLS_BYTES + uint32_t(rg * 16 * PITCH);
-    const uint32_t vs = ks + S::ROWS_BYTES;
-    const uint32_t col0 = uint32_t(cg * S::WC * PITCH);
-    const float2* stat = stat_s + st * S::NPAD;
-
-    // one power-of-two scale of ds for the window (fp16): its sum over the queries goes
-    // through one accumulator
-    float gscale = 1.f;
-    if constexpr (!BF16) {
-      float m = 0.f;
-      for (int i = lane; i < S::NPAD; i += 32) m = fmaxf(m, amax_s[st * S::NPAD + i]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-      gscale = grad_scale(m);
-    }
-    uint32_t last = 0;
-    if (p.analytic) last = last_axes(p, b);
-    const uint32_t r0 = last && k0 < p.N ? code[k0] : 0u, r1 = last && k1 < p.N ? code[k1] : 0u;
-
-    uint32_t ka[S::KS][4], va[S::KS][4];
-#pragma unroll
-    for (int k = 0; k < S::KS; ++k) {
-      ldsm_x4(ks + a_off + 32 * k, ka[k]);
-      ldsm_x4(vs + a_off + 32 * k, va[k]);
-    }
-    float dk[HD / 8][4], dv[HD / 8][4];
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
-
-#pragma unroll
-    for (int t = 0; t < NT; t += 2) {
-      constexpr float z[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t pa[4], da[4];
-      uint32_t bq[4], bg[4];
-      if constexpr (HD == 16) {
-        ldsm_x4(qs + col0 + uint32_t(8 * t * PITCH) + b_off, bq);
-        ldsm_x4(gs + col0 + uint32_t(8 * t * PITCH) + b_off, bg);
+  if (live) {
+    float rest[2][4];  // the start values of the tiles past TT
+    {
+      constexpr int PART = TT % 8 == 0 ? 8 : TT % 6 == 0 ? 6 : 4;
+      static_assert(TT % PART == 0, "tiles per round of gathers");
+#pragma unroll 1
+      for (int t = 0; t < TT; t += PART) {
+        float v[PART][4];
+        start_values<PART, BF16, true>(p, h, k0, 8 * t + 2 * t4, v);
+        tm_st<4 * PART>(tm_bias + 4 * t, v[0]);
       }
+      if constexpr (TT < NT) start_values<2, BF16, true>(p, h, k0, 8 * TT + 2 * t4, rest);
+      tmem_wait_st();
+    }
+    const int width = p.H * HD, tok = 3 * width;
+    const float2 cc = both(p.scale * kLog2e);
+    const uint32_t a_off = R::at(warp * 16 + (lane & 15), lane >> 4);
+    const uint32_t a_off1 = HD == 32 ? R::at(warp * 16 + (lane & 15), (lane >> 4) + 2) : 0u;
+    const uint32_t b_off = HD == 16 ? R::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1)
+                                    : R::at(lane & 7, lane >> 3);
+    const uint32_t bt_off = R::at(lane & 15, lane >> 4);
+    const uint32_t bt_off1 = HD == 32 ? R::at(lane & 15, (lane >> 4) + 2) : 0u;
+    const float* amax = p.amax + ((long long)share * p.H + h) * groups + lane;
+    const long long amax_step = (long long)p.S * p.H * groups;
+    float am = 0.f;  // the next window's, fetched one window ahead
+    if constexpr (!BF16) am = lane < groups ? __ldg(amax) : 0.f;
+
+#pragma unroll 1
+    for (int k = 0; k < count; ++k) {
+      // one power-of-two scale of ds for the window (fp16): its sum over the queries goes
+      // through one accumulator
+      float gscale = 1.f;
+      if constexpr (!BF16) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (t + u >= NT) break;
-        float s[4], d[4];
+        for (int o = 16; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(~0u, am, o));
+        gscale = grad_scale(am);
+        am = lane < groups && k + 1 < count ? __ldg(amax + (k + 1) * amax_step) : 0.f;
+      }
+      float nb[2][4];  // start values of the next pair of tiles
+      wait_stage<STAGES>(tail, k);
+      tm_ld<8>(tm_bias, nb[0]);
+      const uint32_t qs = smem_u32(smem) + uint32_t((k % STAGES) * S::STAGE);
+      const uint32_t gs = qs + S::COLS, ks = gs + S::COLS, vs = ks + S::ROWS;
+      const float2* stat = reinterpret_cast<const float2*>(
+          smem + (k % STAGES) * S::STAGE + 2 * S::COLS + 2 * S::ROWS) + 2 * t4;
+      uint32_t last = 0;
+      if (p.analytic) last = tail->last[k % STAGES];
+      const bool on = (last >> t4) & 1u;
+      const uint32_t a0 = on ? f0 : 0u, a1 = on ? f1 : 0u;
+      const uint32_t* mb = mask_s + g * 4 + t4;
+
+      uint32_t ka[R::KS][4], va[R::KS][4];
+      ldsm_x4(ks + a_off, ka[0]);
+      ldsm_x4(vs + a_off, va[0]);
+      if constexpr (HD == 32) {
+        ldsm_x4(ks + a_off1, ka[1]);
+        ldsm_x4(vs + a_off1, va[1]);
+      }
+      float dk[HD / 8][4], dv[HD / 8][4];
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
+
+#pragma unroll
+      for (int t = 0; t < NT; t += 2) {
+        constexpr float z[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t at = uint32_t(8 * t * R::BYTES);
+        uint32_t pa[4], da[4];
+        float s[2][4], d[2][4];
+        if (t < TT) tm_wait<2>(nb);
         if constexpr (HD == 16) {
-          mma16<BF16>(s, ka[0], bq[2 * u], bq[2 * u + 1], bias[t + u]);
-          mma16<BF16>(d, va[0], bg[2 * u], bg[2 * u + 1], z);
+          uint32_t bq[4], bg[4];
+          ldsm_x4(qs + b_off + at, bq);
+          ldsm_x4(gs + b_off + at, bg);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mma16<BF16>(s[u], ka[0], bq[2 * u], bq[2 * u + 1], t < TT ? nb[u] : rest[u]);
+            mma16<BF16>(d[u], va[0], bg[2 * u], bg[2 * u + 1], z);
+          }
         } else {
-          ldsm_x4(qs + col0 + uint32_t(8 * (t + u) * PITCH) + b_off, bq);
-          ldsm_x4(gs + col0 + uint32_t(8 * (t + u) * PITCH) + b_off, bg);
-          mma16<BF16>(s, ka[0], bq[0], bq[1], bias[t + u]);
-          mma16<BF16>(s, ka[1], bq[2], bq[3], s);
-          mma16<BF16>(d, va[0], bg[0], bg[1], z);
-          mma16<BF16>(d, va[1], bg[2], bg[3], d);
-        }
-        const int i = ib + 8 * (t + u);
-        if (last) {
-          const uint32_t c0 = code[i], c1_ = code[i + 1];
-          if ((r0 ^ c0) & last) s[0] += pen;
-          if ((r0 ^ c1_) & last) s[1] += pen;
-          if ((r1 ^ c0) & last) s[2] += pen;
-          if ((r1 ^ c1_) & last) s[3] += pen;
-        }
-        const float4 x = *reinterpret_cast<const float4*>(stat + i);  // two queries' statistics
-        float q[4];
-        q[0] = ex2(fmaf(s[0], c1, -x.x));
-        q[1] = ex2(fmaf(s[1], c1, -x.z));
-        q[2] = ex2(fmaf(s[2], c1, -x.x));
-        q[3] = ex2(fmaf(s[3], c1, -x.z));
-        d[0] = (d[0] - x.y) * q[0];
-        d[1] = (d[1] - x.w) * q[1];
-        d[2] = (d[2] - x.y) * q[2];
-        d[3] = (d[3] - x.w) * q[3];
-        if constexpr (!BF16) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[e] *= gscale;
+          for (int u = 0; u < 2; ++u) {
+            uint32_t bq[4], bg[4];
+            ldsm_x4(qs + b_off + at + uint32_t(8 * u * R::BYTES), bq);
+            ldsm_x4(gs + b_off + at + uint32_t(8 * u * R::BYTES), bg);
+            mma16<BF16>(s[u], ka[0], bq[0], bq[1], t < TT ? nb[u] : rest[u]);
+            mma16<BF16>(s[u], ka[1], bq[2], bq[3], s[u]);
+            mma16<BF16>(d[u], va[0], bg[0], bg[1], z);
+            mma16<BF16>(d[u], va[1], bg[2], bg[3], d[u]);
+          }
         }
-        pa[2 * u] = pack2<BF16>(q[0], q[1]);
-        pa[2 * u + 1] = pack2<BF16>(q[2], q[3]);
-        da[2 * u] = pack2<BF16>(d[0], d[1]);
-        da[2 * u + 1] = pack2<BF16>(d[2], d[3]);
-      }
+        if (t + 2 < TT) tm_ld<8>(tm_bias + 4 * (t + 2), nb[0]);
+        if (last != 0) {
 #pragma unroll
-      for (int n = 0; n < HD / 16; ++n) {
-        uint32_t tq[4], tg[4];
-        ldsm_x4_t(gs + col0 + uint32_t(8 * t * PITCH) + bt_off + 32 * n, tg);
-        ldsm_x4_t(qs + col0 + uint32_t(8 * t * PITCH) + bt_off + 32 * n, tq);
-        if (t + 1 < NT) {
+          for (int u = 0; u < 2; ++u) mma8<BF16>(s[u], a0, a1, mb[32 * (t + u)]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float4 x =  // two queries' statistics
+              *reinterpret_cast<const float4*>(stat + 8 * (t + u));
+          const float2 lse = make_float2(-x.x, -x.z), del = make_float2(-x.y, -x.w);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float2 y = __ffma2_rn(two(s[u], r), cc, lse);
+            const float2 q = make_float2(ex2(y.x), ex2(y.y));
+            float2 ds = __fmul2_rn(__fadd2_rn(two(d[u], r), del), q);
+            if constexpr (!BF16) ds = __fmul2_rn(ds, both(gscale));
+            pa[2 * u + r] = pack2<BF16>(q.x, q.y);
+            da[2 * u + r] = pack2<BF16>(ds.x, ds.y);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+          uint32_t tq[4], tg[4];
+          ldsm_x4_t(gs + (n ? bt_off1 : bt_off) + at, tg);
+          ldsm_x4_t(qs + (n ? bt_off1 : bt_off) + at, tq);
           mma16<BF16>(dv[2 * n], pa, tg[0], tg[1], dv[2 * n]);
           mma16<BF16>(dv[2 * n + 1], pa, tg[2], tg[3], dv[2 * n + 1]);
           mma16<BF16>(dk[2 * n], da, tq[0], tq[1], dk[2 * n]);
           mma16<BF16>(dk[2 * n + 1], da, tq[2], tq[3], dk[2 * n + 1]);
-        } else {
-          mma8<BF16>(dv[2 * n], pa[0], pa[1], tg[0]);
-          mma8<BF16>(dv[2 * n + 1], pa[0], pa[1], tg[2]);
-          mma8<BF16>(dk[2 * n], da[0], da[1], tq[0]);
-          mma8<BF16>(dk[2 * n + 1], da[0], da[1], tq[2]);
+        }
+      }
+      if (release_stage<STAGES>(tail, k, count, warps)) issue(k + STAGES);
+      const float f = BF16 ? p.scale : p.scale * inverse_scale(gscale);
+      uint16_t* to = p.dqkv + ((long long)(share + k * p.S) * p.N + k0) * tok + width + h * HD + 2 * t4;
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) {
+        if (k0 < p.N) {
+          *reinterpret_cast<uint32_t*>(to + 8 * n) = pack2<BF16>(dk[n][0] * f, dk[n][1] * f);
+          *reinterpret_cast<uint32_t*>(to + width + 8 * n) = pack2<BF16>(dv[n][0], dv[n][1]);
+        }
+        if (k1 < p.N) {
+          *reinterpret_cast<uint32_t*>(to + 8 * tok + 8 * n) = pack2<BF16>(dk[n][2] * f, dk[n][3] * f);
+          *reinterpret_cast<uint32_t*>(to + 8 * tok + width + 8 * n) = pack2<BF16>(dv[n][2], dv[n][3]);
         }
       }
     }
-    const float f = BF16 ? p.scale : p.scale / gscale;
-    float* mk = red + (rg * CG + cg) * 16 * HD;
-    float* mv = mk + S::WARPS * 16 * HD;
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-      const int o0 = g * HD + 8 * n + 2 * t4, o1 = (g + 8) * HD + 8 * n + 2 * t4;
-      *reinterpret_cast<float2*>(mk + o0) = make_float2(dk[n][0] * f, dk[n][1] * f);
-      *reinterpret_cast<float2*>(mk + o1) = make_float2(dk[n][2] * f, dk[n][3] * f);
-      *reinterpret_cast<float2*>(mv + o0) = make_float2(dv[n][0], dv[n][1]);
-      *reinterpret_cast<float2*>(mv + o1) = make_float2(dv[n][2], dv[n][3]);
-    }
-    bar_sync(1 + rg, 32 * CG);
-    for (int o = cg * 32 + lane; o < 16 * HD; o += 32 * CG) {
-      const int w = o / (8 * HD), r = (o / (HD / 2)) % 16, c = (o % (HD / 2)) * 2;
-      const float* all = red + w * S::WARPS * 16 * HD + rg * CG * 16 * HD + r * HD + c;
-      float2 v = *reinterpret_cast<const float2*>(all);
-#pragma unroll
-      for (int k = 1; k < CG; ++k) {
-        const float2 a = *reinterpret_cast<const float2*>(all + k * 16 * HD);
-        v.x += a.x;
-        v.y += a.y;
-      }
-      const int i = row0 + rg * 16 + r;
-      if (i < p.N)
-        *reinterpret_cast<uint32_t*>(p.dqkv + ((long long)b * p.N + i) * tok +
-                                     (long long)(1 + w) * p.H * HD + h * HD + c) =
-            pack2<BF16>(v.x, v.y);
-    }
   }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0) finish_ring<STAGES>(tail);
+  if (warp == 0) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tail->tm_slot, S::TM_COLS);
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// 4D map {head_dim, N, H, B} over one part of the tokens (`tok` elements per token), in boxes of
+// `rows` rows; rows past N are zero-filled.
+int make_map(CUtensorMap* map, const void* base, const AttnGradArgs& a, int64_t tok, int rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return set_error(kErrCuda, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[4] = {cuuint64_t(a.head_dim), cuuint64_t(a.N), cuuint64_t(a.H),
+                              cuuint64_t(a.B)};
+  const cuuint64_t strides[3] = {cuuint64_t(tok) * 2, cuuint64_t(a.head_dim) * 2,
+                                 cuuint64_t(tok) * cuuint64_t(a.N) * 2};
+  const cuuint32_t box[4] = {cuuint32_t(a.head_dim), cuuint32_t(rows), 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = enc(
+      map, a.dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      a.head_dim == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(kErrInvalid, "cuTensorMapEncodeTiled rejected a tensor");
+  return kOk;
+}
+
+int make_maps(Maps* m, const AttnGradArgs& a, int cols, int rows) {
+  const int64_t width = a.H * a.head_dim;
+  const uint16_t* q = static_cast<const uint16_t*>(a.qkv);
+  const struct {
+    CUtensorMap *c, *r;
+    const void* base;
+    int64_t tok;
+  } parts[4] = {{&m->q_cols, &m->q_rows, q, 3 * width},
+                {&m->k_cols, &m->k_rows, q + width, 3 * width},
+                {&m->v_cols, &m->v_rows, q + 2 * width, 3 * width},
+                {&m->o_cols, &m->o_rows, a.grad_out, width}};
+  for (const auto& t : parts) {
+    if (int e = make_map(t.c, t.base, a, t.tok, box_rows(cols))) return e;
+    if (int e = make_map(t.r, t.base, a, t.tok, box_rows(rows))) return e;
+  }
+  return kOk;
 }
 
 int sm_count() {
@@ -820,62 +1092,93 @@ int sm_count() {
   return sms > 0 ? sms : 148;
 }
 
-template <class S, bool BF16>
-int launch_grad(const GradParams& p, cudaStream_t stream) {
+template <class K>
+int set_smem(K kernel, int bytes) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? kOk : set_cuda_error(e, "attention gradient smem attribute");
+}
+
+// Row blocks and shares of a kernel with `rows` rows per CTA and `per_sm` CTAs per SM: as many
+// shares as keep the SMs' CTA slots busy with one CTA per (head, row block, share), at most one
+// per window.
+void split(GradParams* p, int rows, int per_sm) {
+  p->RB = (p->N + rows - 1) / rows;
+  const int64_t s = int64_t(sm_count()) * per_sm / (int64_t(p->H) * p->RB);
+  p->S = int(s < 1 ? 1 : s > p->B ? p->B : s);
+}
+
+template <int NPAD, int HD, bool BF16>
+int launch_grad(GradParams p, const AttnGradArgs& a, cudaStream_t stream) {
+  using RS = RowsShape<NPAD, HD>;
+  using CS = ColsShape<NPAD, HD>;
   static bool configured[64] = {false};  // per device
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(grad_rows_kernel<S, BF16>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         S::SMEM_ROWS);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(grad_cols_kernel<S, BF16>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_COLS);
-    if (e != cudaSuccess) return set_cuda_error(e, "attention gradient smem attribute");
+    if (int e = set_smem(grad_rows_kernel<RS, BF16>, RS::SMEM)) return e;
+    if (int e = set_smem(grad_cols_kernel<CS, BF16>, CS::SMEM)) return e;
     if (dev < 64) configured[dev] = true;
   }
-  const unsigned blocks = unsigned(p.H) * unsigned(p.RB) * unsigned(p.S);
-  grad_rows_kernel<S, BF16><<<blocks, S::THREADS, S::SMEM_ROWS, stream>>>(p);
+  Maps maps;
+  if (int e = make_maps(&maps, a, NPAD, kBR)) return e;
+  p.RB = (p.N + kBR - 1) / kBR;
+  p.S = int(a.shares);
+  grad_rows_kernel<RS, BF16>
+      <<<unsigned(p.H) * unsigned(p.RB) * unsigned(p.S), RS::THREADS, RS::SMEM, stream>>>(maps, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "attention gradient (rows) launch");
-  grad_cols_kernel<S, BF16><<<blocks, S::THREADS, S::SMEM_COLS, stream>>>(p);
+  if (int r = make_maps(&maps, a, NPAD, CS::BR)) return r;
+  split(&p, CS::BR, CS::MINB);
+  grad_cols_kernel<CS, BF16>
+      <<<unsigned(p.H) * unsigned(p.RB) * unsigned(p.S), CS::THREADS, CS::SMEM, stream>>>(maps, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "attention gradient (columns) launch");
   return kOk;
 }
 
 template <int HD, bool BF16>
-int dispatch_npad(const GradParams& p, cudaStream_t stream) {
-  if (p.N <= 64) return launch_grad<Shape<64, HD>, BF16>(p, stream);
-  if (p.N <= 128) return launch_grad<Shape<128, HD>, BF16>(p, stream);
-  if (p.N <= 224) return launch_grad<Shape<224, HD>, BF16>(p, stream);
-  return launch_grad<Shape<352, HD>, BF16>(p, stream);
+int dispatch_npad(const GradParams& p, const AttnGradArgs& a, cudaStream_t stream) {
+  if (p.N <= 64) return launch_grad<64, HD, BF16>(p, a, stream);
+  if (p.N <= 128) return launch_grad<128, HD, BF16>(p, a, stream);
+  if (p.N <= 224) return launch_grad<224, HD, BF16>(p, a, stream);
+  return launch_grad<352, HD, BF16>(p, a, stream);
 }
 
 }  // namespace
 
-bool attention_grad_tensor_path(int dtype, int64_t N, int64_t head_dim) {
-  return dtype != kF32 && (head_dim == 16 || head_dim == 32) && N >= 1 && N <= 352;
+// (H: a window's offsets fit 32 bits)
+bool attention_grad_tensor_path(int dtype, int64_t H, int64_t N, int64_t head_dim) {
+  return dtype != kF32 && (head_dim == 16 || head_dim == 32) && N >= 1 && N <= 352 && H <= 4096;
 }
 
-// Shares the windows are split into: as many as keep every SM's CTA slots busy with one CTA
-// per (head, row block, share), at most one per window.
+// Shares of the windows of the rows kernel, each with its own part of the bias gradient.
 int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N) {
-  const int64_t per_sm = N <= 64 ? 4 : N <= 128 ? 2 : 1;
-  const int64_t blocks = H * ((N + kBR - 1) / kBR);
-  const int64_t s = int64_t(sm_count()) * per_sm / blocks;
-  return s < 1 ? 1 : s > B ? (B > 0 ? B : 1) : s;
+  GradParams p{};
+  p.B = int(B > 0 ? B : 1);
+  p.H = int(H);
+  p.N = int(N);
+  split(&p, kBR, N <= 64 ? 4 : N <= 128 ? 2 : 1);  // RowsShape::MINB
+  return p.S;
+}
+
+int read_attention_grad_error(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_grad_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_grad_error, &zero, sizeof(int));
+  }
+  return v;
 }
 
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   GradParams p{};
-  p.qkv = static_cast<const uint16_t*>(a.qkv);
-  p.dout = static_cast<const uint16_t*>(a.grad_out);
   p.dqkv = static_cast<uint16_t*>(a.grad_qkv);
   p.dbias = a.grad_bias;
   p.stats = reinterpret_cast<float2*>(a.stats);
-  p.amax = a.stats + 2 * a.B * a.H * a.N;
+  p.NS = int(a.N + (a.N & 1));
+  p.amax = a.stats + 2 * a.B * a.H * p.NS;
   p.table = a.table;
   p.pairs = a.pairs;
   p.table_f32 = a.table_f32 ? 1 : 0;
@@ -892,13 +1195,11 @@ int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   p.B = int(a.B);
   p.H = int(a.H);
   p.N = int(a.N);
-  p.RB = int((a.N + kBR - 1) / kBR);
-  p.S = int(a.shares);
   p.scale = a.scale;
   const bool bf16 = a.dtype == kBF16;
   if (a.head_dim == 32)
-    return bf16 ? dispatch_npad<32, true>(p, stream) : dispatch_npad<32, false>(p, stream);
-  return bf16 ? dispatch_npad<16, true>(p, stream) : dispatch_npad<16, false>(p, stream);
+    return bf16 ? dispatch_npad<32, true>(p, a, stream) : dispatch_npad<32, false>(p, a, stream);
+  return bf16 ? dispatch_npad<16, true>(p, a, stream) : dispatch_npad<16, false>(p, a, stream);
 }
 
 }  // namespace crumpet

@@ -6,16 +6,17 @@
 // Both move one value per (head, pair) and compute next to nothing, so memory traffic and, at
 // a Swin window's size (343 x 343 pairs), launch latency bound them.
 //
-// Forward: a CTA takes one head and a run of pairs.  The head's column of the table goes to
-// shared memory first (2197 rows of a 7x7x7 window are 8.8 KB): neighbouring pairs have
-// neighbouring buckets, so gathers from the transposed column meet few bank conflicts, where
-// gathers from the [T, H] table would touch a 32-byte sector each.
+// Forward: a thread takes one pair (two neighbouring ones where the output's type has 16 bits,
+// so its stores have 4 bytes) and a 16-byte vector of heads, which lie next to each other in the
+// table: one gather per 4 or 8 heads, and every store of a warp is contiguous.
 //
 // Gradient: no atomics, so the sum's order never changes.  The caller sorted the pairs by
 // bucket once (`order`) and cut every bucket into items of a bounded number of pairs; one
-// warp sums one (item, head), in a fixed order, in fp32.  The warps of a CTA take neighbouring
-// items of one head, whose pairs are neighbours in memory, so the sectors that one gather
-// opens serve the others from L1.  Buckets of several items are finished by a second kernel.
+// warp sums an item in a fixed order, in fp32, for kUnit heads (or, of a gradient in several
+// slabs, for kUnit slabs of one head) at a time: a pair's place is read once for all of them and
+// the gathers, which are all latency, go out together.  The warps of a CTA take neighbouring
+// items, whose pairs are neighbours in memory, so the sectors that one gather opens serve the
+// others from L1.  Buckets of several items are finished by a second kernel.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -24,8 +25,7 @@ namespace crumpet {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 8;                  // pairs per thread of the forward kernel
-constexpr int kTableSmem = 48 * 1024;          // largest table column kept in shared memory
+constexpr int kUnit = 8;  // heads (or slabs) that a warp gathers together
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
@@ -48,31 +48,33 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-template <typename T, typename O, bool SMEM>
+// V heads (16 bytes of the table, or one) of PP neighbouring pairs per thread
+template <typename T, typename O, int V, int PP>
 __global__ void __launch_bounds__(kThreads)
-bias_gather_kernel(O* bias, const T* table, const int* pairs, long long npairs, int rows, int H) {
-  extern __shared__ float column[];
-  const int h = blockIdx.y;
-  if constexpr (SMEM) {
-    for (int t = threadIdx.x; t < rows; t += kThreads)
-      column[t] = to_float(table[(long long)t * H + h]);
-    __syncthreads();
-  }
-  O* out = bias + h * npairs;
-  const long long step = (long long)kThreads * kPerThread;
-  for (long long base = blockIdx.x * step; base < npairs; base += gridDim.x * step) {
-    int t[kPerThread];
+bias_gather_kernel(O* bias, const T* table, const int* pairs, long long npairs, int H) {
+  struct alignas(V * sizeof(T)) Heads {
+    T v[V];
+  };
+  struct alignas(PP * sizeof(O)) Out {
+    O v[PP];
+  };
+  struct alignas(PP * 4) Pairs {
+    int v[PP];
+  };
+  const long long i = (blockIdx.x * (long long)kThreads + threadIdx.x) * PP;
+  if (i >= npairs) return;
+  const int h = blockIdx.y * V;
+  const Pairs at = *reinterpret_cast<const Pairs*>(pairs + i);
+  Heads w[PP];
 #pragma unroll
-    for (int u = 0; u < kPerThread; ++u) {
-      const long long i = base + u * kThreads + threadIdx.x;
-      t[u] = i < npairs ? __ldg(pairs + i) : 0;
-    }
+  for (int u = 0; u < PP; ++u)
+    w[u] = *reinterpret_cast<const Heads*>(table + (long long)at.v[u] * H + h);
 #pragma unroll
-    for (int u = 0; u < kPerThread; ++u) {
-      const long long i = base + u * kThreads + threadIdx.x;
-      if (i < npairs)
-        out[i] = from_float<O>(SMEM ? column[t[u]] : to_float(table[(long long)t[u] * H + h]));
-    }
+  for (int k = 0; k < V; ++k) {
+    Out o;
+#pragma unroll
+    for (int u = 0; u < PP; ++u) o.v[u] = from_float<O>(to_float(w[u].v[k]));
+    *reinterpret_cast<Out*>(bias + (h + k) * npairs + i) = o;
   }
 }
 
@@ -84,28 +86,42 @@ struct GradBuckets {
   int H;
 };
 
-// One warp per (item, head).  An item whose bucket is whole writes the table's gradient,
-// the others their part of it: partial[item, h].
-template <typename G, typename O>
+// One warp per item and kUnit heads (SLABS: per item and head, kUnit slabs at a time).  An item
+// whose bucket is whole writes the table's gradient, the others their part: partial[item, h].
+template <typename G, typename O, bool SLABS>
 __global__ void __launch_bounds__(kThreads)
 bias_grad_kernel(O* grad_table, float* partial, const G* grad, int slabs, GradBuckets b) {
   const int lane = threadIdx.x & 31;
   const long long item = blockIdx.x * (long long)(kThreads / 32) + (threadIdx.x >> 5);
-  const int h = blockIdx.y;
   if (item >= b.n_items) return;
+  const int h = SLABS ? blockIdx.y : blockIdx.y * kUnit;
   const int bucket = b.items[3 * item], begin = b.items[3 * item + 1], end = b.items[3 * item + 2];
-  const long long slab = b.npairs * b.H;
-  const G* src = grad + h * b.npairs;
-  float sum = 0.f;
-  for (int e = begin + lane; e < end; e += 32) {
-    const long long at = b.order[e];
-    for (int s = 0; s < slabs; ++s) sum += to_float(src[s * slab + at]);
+  const long long step = SLABS ? b.npairs * b.H : b.npairs;  // from unit to unit
+  const int units = SLABS ? slabs : min(kUnit, b.H - h);
+  float sum[kUnit] = {};
+  for (int u0 = 0; u0 < units; u0 += kUnit) {
+    const G* src = grad + h * b.npairs + u0 * step;
+#pragma unroll 2
+    for (int e = begin + lane; e < end; e += 32) {
+      const G* from = src + b.order[e];
+#pragma unroll
+      for (int u = 0; u < kUnit; ++u)
+        if (u0 + u < units) sum[u] += to_float(from[u * step]);
+    }
+  }
+  if constexpr (SLABS) {
+#pragma unroll
+    for (int u = 1; u < kUnit; ++u) sum[0] += sum[u];
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (lane != 0) return;
-  if (bucket >= 0) grad_table[(long long)bucket * b.H + h] = from_float<O>(sum);
-  else partial[item * b.H + h] = sum;
+  for (int u = 0; u < (SLABS ? 1 : kUnit); ++u) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[u] += __shfl_xor_sync(~0u, sum[u], o);
+    if (lane == u && u < (SLABS ? 1 : units)) {
+      if (bucket >= 0) grad_table[(long long)bucket * b.H + h + u] = from_float<O>(sum[u]);
+      else partial[item * b.H + h + u] = sum[u];
+    }
+  }
 }
 
 template <typename O>
@@ -123,38 +139,53 @@ bias_grad_join_kernel(O* grad_table, const float* partial, GradBuckets b) {
   if (lane == 0) grad_table[(long long)bucket * b.H + h] = from_float<O>(sum);
 }
 
+template <typename T, typename O, int V, int PP>
+void gather(void* bias, const void* table, const int* pairs, int64_t npairs, int64_t H,
+            cudaStream_t stream) {
+  const int64_t per = int64_t(kThreads) * PP;
+  bias_gather_kernel<T, O, V, PP><<<dim3(unsigned((npairs + per - 1) / per), unsigned(H / V)),
+                                    kThreads, 0, stream>>>(
+      static_cast<O*>(bias), static_cast<const T*>(table), pairs, npairs, int(H));
+}
+
 template <typename T, typename O>
-int launch_gather(void* bias, const void* table, const int* pairs, int64_t npairs, int64_t rows,
-                  int64_t H, cudaStream_t stream) {
-  const int64_t step = int64_t(kThreads) * kPerThread;
-  const int64_t want = (npairs + step - 1) / step;
-  const dim3 grid(unsigned(want < 0x7fffffff ? want : 0x7fffffff), unsigned(H));
-  if (rows * 4 <= kTableSmem)
-    bias_gather_kernel<T, O, true><<<grid, kThreads, size_t(rows) * 4, stream>>>(
-        static_cast<O*>(bias), static_cast<const T*>(table), pairs, npairs, int(rows), int(H));
-  else
-    bias_gather_kernel<T, O, false><<<grid, kThreads, 0, stream>>>(
-        static_cast<O*>(bias), static_cast<const T*>(table), pairs, npairs, int(rows), int(H));
+int launch_gather(void* bias, const void* table, const int* pairs, int64_t npairs, int64_t H,
+                  cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T), PP = 4 / sizeof(O);
+  const auto aligned = [](const void* p, uintptr_t n) {
+    return reinterpret_cast<uintptr_t>(p) % n == 0;
+  };
+  const bool heads = H % V == 0 && aligned(table, 16);
+  const bool two = npairs % PP == 0 && aligned(bias, 4) && aligned(pairs, 4 * PP);
+  if (heads && two) gather<T, O, V, PP>(bias, table, pairs, npairs, H, stream);
+  else if (heads) gather<T, O, V, 1>(bias, table, pairs, npairs, H, stream);
+  else if (two) gather<T, O, 1, PP>(bias, table, pairs, npairs, H, stream);
+  else gather<T, O, 1, 1>(bias, table, pairs, npairs, H, stream);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "relative position bias launch");
 }
 
 template <typename T>
 int gather_out(void* bias, int out_dtype, const void* table, const int* pairs, int64_t npairs,
-               int64_t rows, int64_t H, cudaStream_t stream) {
-  if (out_dtype == kF32) return launch_gather<T, float>(bias, table, pairs, npairs, rows, H, stream);
+               int64_t H, cudaStream_t stream) {
+  if (out_dtype == kF32) return launch_gather<T, float>(bias, table, pairs, npairs, H, stream);
   if (out_dtype == kF16)
-    return launch_gather<T, __half>(bias, table, pairs, npairs, rows, H, stream);
-  return launch_gather<T, __nv_bfloat16>(bias, table, pairs, npairs, rows, H, stream);
+    return launch_gather<T, __half>(bias, table, pairs, npairs, H, stream);
+  return launch_gather<T, __nv_bfloat16>(bias, table, pairs, npairs, H, stream);
 }
 
 template <typename G, typename O>
 int launch_grad(const BiasGradArgs& a, cudaStream_t stream) {
   GradBuckets b{a.order, a.items, a.multi, a.n_items, a.n_multi, a.npairs, int(a.H)};
   const int per = kThreads / 32;
-  bias_grad_kernel<G, O><<<dim3(unsigned((a.n_items + per - 1) / per), unsigned(a.H)), kThreads, 0,
-                           stream>>>(static_cast<O*>(a.grad_table), a.partial,
-                                     static_cast<const G*>(a.grad), int(a.slabs), b);
+  const unsigned blocks = unsigned((a.n_items + per - 1) / per);
+  if (a.slabs > 1)
+    bias_grad_kernel<G, O, true><<<dim3(blocks, unsigned(a.H)), kThreads, 0, stream>>>(
+        static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), int(a.slabs), b);
+  else
+    bias_grad_kernel<G, O, false>
+        <<<dim3(blocks, unsigned((a.H + kUnit - 1) / kUnit)), kThreads, 0, stream>>>(
+            static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), 1, b);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "relative position bias gradient launch");
   if (a.n_multi > 0) {
@@ -176,13 +207,12 @@ int grad_out(const BiasGradArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
-                                  const int* pairs, int64_t npairs, int64_t rows, int64_t H,
-                                  cudaStream_t stream) {
+                                  const int* pairs, int64_t npairs, int64_t H, cudaStream_t stream) {
   if (table_dtype == kF32)
-    return gather_out<float>(bias, out_dtype, table, pairs, npairs, rows, H, stream);
+    return gather_out<float>(bias, out_dtype, table, pairs, npairs, H, stream);
   if (table_dtype == kF16)
-    return gather_out<__half>(bias, out_dtype, table, pairs, npairs, rows, H, stream);
-  return gather_out<__nv_bfloat16>(bias, out_dtype, table, pairs, npairs, rows, H, stream);
+    return gather_out<__half>(bias, out_dtype, table, pairs, npairs, H, stream);
+  return gather_out<__nv_bfloat16>(bias, out_dtype, table, pairs, npairs, H, stream);
 }
 
 int launch_relative_position_bias_grad(const BiasGradArgs& a, cudaStream_t stream) {

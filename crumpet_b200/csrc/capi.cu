@@ -443,7 +443,7 @@ int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
     return set_error(kErrInvalid, "relative position bias: table_rows, npairs or H out of range");
   if (!bias || !table || !pairs) return set_error(kErrInvalid, "null tensor pointer");
   return launch_relative_position_bias(bias, out_dtype, table, table_dtype, pairs, npairs,
-                                       table_rows, H, static_cast<cudaStream_t>(stream));
+                                       H, static_cast<cudaStream_t>(stream));
 }
 
 int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, int64_t H,
@@ -481,7 +481,7 @@ int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, i
 int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N, int64_t head_dim,
                                                  int dtype) {
   if (B < 0 || H < 1 || N < 1) return 0;
-  return attention_grad_tensor_path(dtype, N, head_dim) ? attention_grad_shares(B, H, N)
+  return attention_grad_tensor_path(dtype, H, N, head_dim) ? attention_grad_shares(B, H, N)
                                                         : attention_grad_shares_simt(B, H, N);
 }
 
@@ -512,7 +512,7 @@ int crumpet_swin_window_attention_qkv_backward(
       if (ss[a] < 0 || ss[a] >= ws[a])
         return set_error(kErrInvalid, "analytic mask shift must satisfy 0 <= shift < window");
   }
-  const bool sized = attention_grad_tensor_path(dtype, N, head_dim);
+  const bool sized = attention_grad_tensor_path(dtype, H, N, head_dim);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(grad_qkv) |
                          reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(qkv);
   if (shares < 1 || shares > 0xffff || shares > (B > 0 ? B : 1))
@@ -528,8 +528,8 @@ int crumpet_swin_window_attention_qkv_backward(
   if (!grad_qkv || !stats || !grad_out || !qkv || !bias_table || !pairs)
     return set_error(kErrInvalid, "null tensor pointer");
   if (table_rows < 1) return set_error(kErrInvalid, "relative position bias table has no rows");
-  if (reinterpret_cast<uintptr_t>(stats) & 7u)
-    return set_error(kErrInvalid, "stats must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(stats) & 15u)
+    return set_error(kErrInvalid, "stats must be 16-byte aligned");
   AttnGradArgs a{};
   a.grad_qkv = grad_qkv;
   a.grad_bias = grad_bias;

@@ -140,7 +140,7 @@ int launch_window_attention_simt(const AttnArgs& a, cudaStream_t stream);
 struct AttnGradArgs {
   void* grad_qkv;        // [B, N, 3, H, head_dim]
   float* grad_bias;      // [shares, H, N, N]
-  float* stats;          // [3, B, H, N] floats
+  float* stats;          // B * H * (3 N + 4) floats
   const void* grad_out;  // [B, N, H * head_dim]
   const void* qkv;       // [B, N, 3, H, head_dim]
   const void* table;     // [T, H]
@@ -151,17 +151,17 @@ struct AttnGradArgs {
   float scale;
   int dtype;
 };
-bool attention_grad_tensor_path(int dtype, int64_t N, int64_t head_dim);
+bool attention_grad_tensor_path(int dtype, int64_t H, int64_t N, int64_t head_dim);
 int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
 int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N);
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
+int read_attention_grad_error(bool clear);
 int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream);
 
 // Relative-position bias by buckets: bias[h, p] = table[pairs[p], h] and the table's gradient
 // from `slabs` parts of grad [H, npairs].
 int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
-                                  const int* pairs, int64_t npairs, int64_t rows, int64_t H,
-                                  cudaStream_t stream);
+                                  const int* pairs, int64_t npairs, int64_t H, cudaStream_t stream);
 struct BiasGradArgs {
   void* grad_table;  // [T, H]
   int table_dtype;

@@ -672,7 +672,7 @@ void swin_window_attention_qkv_backward(at::Tensor& grad_qkv, at::Tensor& grad_b
   TORCH_CHECK(grad_bias.scalar_type() == at::kFloat && grad_bias.dim() == 4 &&
                   grad_bias.size(1) == H && grad_bias.size(2) == N && grad_bias.size(3) == N,
               "grad_bias must be a float32 [shares, H, N, N] tensor");
-  check_f32(stats, 3 * B * H * N, "stats");
+  check_f32(stats, B * H * (3 * N + 4), "stats");
   TORCH_CHECK(num_windows.size() == 3 && window_size.size() == 3 && shift_size.size() == 3,
               "num_windows, window_size and shift_size take three values");
   same_device(qkv, grad_qkv, "grad_qkv");

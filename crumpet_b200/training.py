@@ -36,7 +36,7 @@ from .fused_attention import (_ATTN_DTYPES, attention_bias_tiles, head_dim_suppo
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 GROUP = 32  # neighbouring channels that share one scale of an 8-bit checkpoint
 MAX_CHANNELS = 4096  # of norm_gate_residual
-_ITEM = 1024  # most pairs of one bucket that one warp sums
+_ITEM = 512  # most pairs of one bucket that one warp sums
 
 
 def _require_cuda(what: str, *tensors) -> None:
@@ -231,7 +231,7 @@ def _attention_backward(grad_out, qkv, table, buckets, place):
         shares = int(_native.capi().crumpet_window_attention_backward_shares(B, H, N, D, code))
     grad_qkv = torch.empty_like(qkv)
     grad_bias = torch.empty((shares, H, N, N), dtype=torch.float32, device=qkv.device)
-    stats = torch.empty(3 * B * H * N, dtype=torch.float32, device=qkv.device)
+    stats = torch.empty(B * H * (3 * N + 4), dtype=torch.float32, device=qkv.device)
     token = _prof.kernel_begin("swin_window_attention_qkv_backward", lambda: {
         "bytes": 7 * B * H * N * D * qkv.element_size(), "flops": 10 * B * H * N * N * D,
         "exps": B * H * N * N})

@@ -414,7 +414,7 @@ CRUMPET_API int crumpet_relative_position_bias_backward(
  * grad_bias fp32 [shares, H, N, N], whose sum over the shares is the gradient of the bias
  * (pass it on to crumpet_relative_position_bias_backward with slabs = shares).  `shares` is
  * what crumpet_window_attention_backward_shares gives for these sizes; `stats` is fp32
- * scratch of 3 * B * H * N elements.  The bias is used as the table has it (the forward rounds
+ * scratch of B * H * (3 * N + 4) elements, 16-byte aligned.  The bias is used as the table has it (the forward rounds
  * it to dtype); the row statistics are taken again in fp32.  dtype, head_dim and N as for the
  * forward: F16 / BF16 with head_dim 16 or 32, N <= 352 and 16-byte aligned tensors run the
  * tensor-core kernels, every other call an fp32 SIMT kernel.
