@@ -31,6 +31,7 @@
 // depends on another CTA; sums have a fixed order, so results do not change from run to run.
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -52,7 +53,7 @@ constexpr int kSmemBudget = 227 * 1024 - 1024;  // per SM, less what the CTAs re
 struct GradParams {
   uint16_t* dqkv;        // [B, N, 3, H, HD]
   float* dbias;          // [S, H, N, N]
-  float2* stats;         // [B, H, NS]: (log2 of the row's sum of exponentials, delta)
+  float* stats;          // [B, H, NS / 2][4]: of two rows, -log2 of the sums of exponentials, -deltas
   float* amax;           // [B, H, groups of 16 rows]: their largest |do| (fp16 only)
   const void* table;     // [T, H]: fp32 (table_f32) or the element type
   const int* pairs;      // [N, N]: bucket of every (query, key) pair, in [0, T)
@@ -577,6 +578,62 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
           }
         }
       }
+      float g0 = 1.f, g1 = 1.f;
+      uint32_t ga[R::KS][4];
+      ldsm_x4(gs + a_off, ga[0]);
+      if constexpr (HD == 32) ldsm_x4(gs + a_off1, ga[1]);
+      if constexpr (!BF16) {  // power-of-two scale of ds, from the row's largest |do|
+        __half2 h0 = __float2half2_rn(0.f), h1 = h0;
+#pragma unroll
+        for (int q = 0; q < R::KS; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __half2 v = __habs2(*reinterpret_cast<const __half2*>(&ga[q][e]));
+            if (e & 1) h1 = __hmax2(h1, v);
+            else h0 = __hmax2(h0, v);
+          }
+        float am0 = __half2float(__hmax(__low2half(h0), __high2half(h0)));
+        float am1 = __half2float(__hmax(__low2half(h1), __high2half(h1)));
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
+          am1 = fmaxf(am1, __shfl_xor_sync(~0u, am1, o));
+        }
+        g0 = grad_scale(am0);
+        g1 = grad_scale(am1);
+        if (cg == 0) {  // the row group's, for the columns kernel
+          am0 = fmaxf(am0, am1);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
+          if (lane == 0)
+            p.amax[((long long)(share + k * p.S) * p.H + h) * ((p.N + 15) / 16) + rb * kRG + rg] =
+                am0;
+        }
+      }
+      // dp = do v^T of a pair of tiles, taken twice: for its sum with p, and again for ds once the
+      // row's statistics are known.  Keeping it instead (44 registers more) left the scheduler
+      // nothing to overlap with.
+      float d[2][2][4];
+      auto dp_pair = [&](int t) {
+        const float z[4] = {0.f, 0.f, 0.f, 0.f};
+        float(&dd)[2][4] = d[(t >> 1) & 1];
+        if constexpr (HD == 16) {
+          uint32_t bf[4];  // past the last tile: rows of the next warp or of Q, not used
+          ldsm_x4(vs + b_off + uint32_t(8 * t * R::BYTES), bf);
+          mma16<BF16>(dd[0], ga[0], bf[0], bf[1], z);
+          if (t + 1 < NT) mma16<BF16>(dd[1], ga[0], bf[2], bf[3], z);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (t + u >= NT) break;
+            uint32_t bf[4];
+            ldsm_x4(vs + b_off + uint32_t(8 * (t + u) * R::BYTES), bf);
+            mma16<BF16>(dd[u], ga[0], bf[0], bf[1], z);
+            mma16<BF16>(dd[u], ga[1], bf[2], bf[3], dd[u]);
+          }
+        }
+      };
+      dp_pair(0);
       if (p.analytic) {
         const uint32_t last = tail->last[k % STAGES];
         if (last != 0) {
@@ -600,75 +657,20 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
         m1 = fmaxf(m1, __shfl_xor_sync(~0u, m1, o));
       }
       const float2 cc = both(c1), n0 = both(-m0 * c1), n1 = both(-m1 * c1);
-      float2 l0 = both(0.f), l1 = both(0.f);
+      float2 l0 = both(0.f), l1 = both(0.f);  // sums of exponentials
+      float2 e0 = both(0.f), e1 = both(0.f);  // sums of p dp
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        if (t % 2 == 0 && t + 2 < NT) dp_pair(t + 2);
+        const float(&dt)[4] = d[(t >> 1) & 1][t & 1];
         const float2 x0 = __ffma2_rn(two(s[t], 0), cc, n0), x1 = __ffma2_rn(two(s[t], 1), cc, n1);
         const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
         l0 = __fadd2_rn(l0, p0);
         l1 = __fadd2_rn(l1, p1);
+        e0 = __ffma2_rn(p0, two(dt, 0), e0);
+        e1 = __ffma2_rn(p1, two(dt, 1), e1);
         put(s[t], 0, p0);
         put(s[t], 1, p1);
-      }
-      // dp = do v^T
-      float d[NT][4];
-      float g0 = 1.f, g1 = 1.f;
-      {
-        uint32_t a[R::KS][4];
-        ldsm_x4(gs + a_off, a[0]);
-        if constexpr (HD == 32) ldsm_x4(gs + a_off1, a[1]);
-        if constexpr (!BF16) {  // power-of-two scale of ds, from the row's largest |do|
-          __half2 h0 = __float2half2_rn(0.f), h1 = h0;
-#pragma unroll
-          for (int q = 0; q < R::KS; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2 v = __habs2(*reinterpret_cast<const __half2*>(&a[q][e]));
-              if (e & 1) h1 = __hmax2(h1, v);
-              else h0 = __hmax2(h0, v);
-            }
-          float am0 = __half2float(__hmax(__low2half(h0), __high2half(h0)));
-          float am1 = __half2float(__hmax(__low2half(h1), __high2half(h1)));
-#pragma unroll
-          for (int o = 1; o < 4; o <<= 1) {
-            am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
-            am1 = fmaxf(am1, __shfl_xor_sync(~0u, am1, o));
-          }
-          g0 = grad_scale(am0);
-          g1 = grad_scale(am1);
-          if (cg == 0) {  // the row group's, for the columns kernel
-            am0 = fmaxf(am0, am1);
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) am0 = fmaxf(am0, __shfl_xor_sync(~0u, am0, o));
-            if (lane == 0)
-              p.amax[((long long)(share + k * p.S) * p.H + h) * ((p.N + 15) / 16) + rb * kRG + rg] =
-                  am0;
-          }
-        }
-        const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (HD == 16) {
-#pragma unroll
-          for (int t = 0; t < NT; t += 2) {
-            uint32_t bf[4];
-            ldsm_x4(vs + b_off + uint32_t(8 * t * R::BYTES), bf);
-            mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
-            if (t + 1 < NT) mma16<BF16>(d[t + 1], a[0], bf[2], bf[3], z);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            uint32_t bf[4];
-            ldsm_x4(vs + b_off + uint32_t(8 * t * R::BYTES), bf);
-            mma16<BF16>(d[t], a[0], bf[0], bf[1], z);
-            mma16<BF16>(d[t], a[1], bf[2], bf[3], d[t]);
-          }
-        }
-      }
-      float2 e0 = both(0.f), e1 = both(0.f);  // sums of p dp
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        e0 = __ffma2_rn(two(s[t], 0), two(d[t], 0), e0);
-        e1 = __ffma2_rn(two(s[t], 1), two(d[t], 1), e1);
       }
       // (sum of exponentials, sum of p dp) of the two rows
       float2 q0 = make_float2(l0.x + l0.y, e0.x + e0.y), q1 = make_float2(l1.x + l1.y, e1.x + e1.y);
@@ -677,6 +679,8 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
         q0 = __fadd2_rn(q0, make_float2(__shfl_xor_sync(~0u, q0.x, o), __shfl_xor_sync(~0u, q0.y, o)));
         q1 = __fadd2_rn(q1, make_float2(__shfl_xor_sync(~0u, q1.x, o), __shfl_xor_sync(~0u, q1.y, o)));
       }
+      dp_pair(0);       // for ds, while the row's warps meet
+      tmem_wait_st();   // the previous window's dbias is written
       float r0 = 1.f, r1 = 1.f;  // this warp's exponentials relative to the row's
       if constexpr (CG > 1) {
         float4* x = ex + (k & 1) * CG * kBR + rg * 16;
@@ -711,27 +715,22 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
       const float inv0 = rcp(q0.x), inv1 = rcp(q1.x);
       const float del0 = q0.y * inv0, del1 = q1.y * inv1;
       if (cg == 0 && t4 == 0) {  // statistics for the columns kernel
-        float2* to = p.stats + ((long long)(share + k * p.S) * p.H + h) * p.NS;
-        // (row N of an odd N is copied along by the columns kernel: its p has to be finite)
-        const float2 zero = make_float2(0.f, 0.f);
-        if (i0 < p.NS) to[i0] = i0 < p.N ? make_float2(fmaf(m0, c1, __log2f(q0.x)), del0) : zero;
-        if (i1 < p.NS) to[i1] = i1 < p.N ? make_float2(fmaf(m1, c1, __log2f(q1.x)), del1) : zero;
+        float* to = p.stats + ((long long)(share + k * p.S) * p.H + h) * p.NS * 2;
+        auto keep = [&](int i, float m, float2 q, float del) {
+          if (i >= p.NS) return;
+          // (row N of an odd N is copied along by the columns kernel: its p has to be finite)
+          to[(i >> 1) * 4 + (i & 1)] = i < p.N ? -fmaf(m, c1, __log2f(q.x)) : 0.f;
+          to[(i >> 1) * 4 + (i & 1) + 2] = i < p.N ? -del : 0.f;
+        };
+        keep(i0, m0, q0, del0);
+        keep(i1, m1, q1, del1);
       }
-      // ds = p (dp - delta), in place of dp; times the row's power of two in fp16
-      {
-        const float2 v0 = both(r0 * inv0 * g0), v1 = both(r1 * inv1 * g1);
-        const float2 w0 = both(-del0 * v0.x), w1 = both(-del1 * v1.x);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          put(d[t], 0, __fmul2_rn(two(s[t], 0), __ffma2_rn(two(d[t], 0), v0, w0)));
-          put(d[t], 1, __fmul2_rn(two(s[t], 1), __ffma2_rn(two(d[t], 1), v1, w1)));
-        }
-      }
-      // dbias += ds
-      tmem_wait_st();  // the previous window's sums are written
-      tm_ld<NT * 4>(tm_sum, s[0]);
-      // dq = ds k, ds rounded to the element type: the rounding errors of a row's keys are
-      // independent, so they add up like one rounding of dq itself
+      // ds = p (dp - delta), times the row's power of two in fp16; dbias += ds; dq += ds k with ds
+      // rounded to the element type: the rounding errors of a row's keys are independent, so they
+      // add up like one rounding of dq itself
+      const float2 v0 = both(r0 * inv0 * g0), v1 = both(r1 * inv1 * g1);
+      const float2 w0 = both(-del0 * v0.x), w1 = both(-del1 * v1.x);
+      const float u0 = inverse_scale(g0), u1 = inverse_scale(g1);
       float acc[HD / 8][4];
 #pragma unroll
       for (int n = 0; n < HD / 8; ++n)
@@ -739,39 +738,53 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < NT; t += 2) {
+        constexpr int kLast = NT - 1;
+        const bool pair = t < kLast;
+        float sum[2][4];
+        if (pair) tm_ld<8>(tm_sum + 4 * t, sum[0]);
+        else tm_ld<4>(tm_sum + 4 * t, sum[0]);
+        uint32_t bf[HD / 16][4];  // past the last tile: as above
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n)
+          ldsm_x4_t(ks + (n ? bt_off1 : bt_off) + uint32_t(8 * t * R::BYTES), bf[n]);
+        if (t + 2 < NT) dp_pair(t + 2);
+        float ds[2][4];
         uint32_t a[4];
-        a[0] = pack2<BF16>(d[t][0], d[t][1]);
-        a[1] = pack2<BF16>(d[t][2], d[t][3]);
-        if (t + 1 < NT) {
-          a[2] = pack2<BF16>(d[t + 1][0], d[t + 1][1]);
-          a[3] = pack2<BF16>(d[t + 1][2], d[t + 1][3]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (t + u >= NT) break;
+          const float(&dt)[4] = d[(t >> 1) & 1][u];
+          put(ds[u], 0, __fmul2_rn(two(s[t + u], 0), __ffma2_rn(two(dt, 0), v0, w0)));
+          put(ds[u], 1, __fmul2_rn(two(s[t + u], 1), __ffma2_rn(two(dt, 1), v1, w1)));
+          a[2 * u] = pack2<BF16>(ds[u][0], ds[u][1]);
+          a[2 * u + 1] = pack2<BF16>(ds[u][2], ds[u][3]);
         }
 #pragma unroll
         for (int n = 0; n < HD / 16; ++n) {
-          uint32_t bf[4];  // past the last tile: as above
-          ldsm_x4_t(ks + (n ? bt_off1 : bt_off) + uint32_t(8 * t * R::BYTES), bf);
-          if (t + 1 < NT) {
-            mma16<BF16>(acc[2 * n], a, bf[0], bf[1], acc[2 * n]);
-            mma16<BF16>(acc[2 * n + 1], a, bf[2], bf[3], acc[2 * n + 1]);
+          if (pair) {
+            mma16<BF16>(acc[2 * n], a, bf[n][0], bf[n][1], acc[2 * n]);
+            mma16<BF16>(acc[2 * n + 1], a, bf[n][2], bf[n][3], acc[2 * n + 1]);
           } else {
-            mma8<BF16>(acc[2 * n], a[0], a[1], bf[0]);
-            mma8<BF16>(acc[2 * n + 1], a[0], a[1], bf[2]);
+            mma8<BF16>(acc[2 * n], a[0], a[1], bf[n][0]);
+            mma8<BF16>(acc[2 * n + 1], a[0], a[1], bf[n][2]);
           }
         }
-      }
-      const float u0 = inverse_scale(g0), u1 = inverse_scale(g1);
-      tm_wait<NT>(s);
+        if (pair) tm_wait<2>(sum);
+        else tm_wait<1>(reinterpret_cast<float(&)[1][4]>(sum));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (BF16) {
-          put(s[t], 0, __fadd2_rn(two(s[t], 0), two(d[t], 0)));
-          put(s[t], 1, __fadd2_rn(two(s[t], 1), two(d[t], 1)));
-        } else {
-          put(s[t], 0, __ffma2_rn(two(d[t], 0), both(u0), two(s[t], 0)));
-          put(s[t], 1, __ffma2_rn(two(d[t], 1), both(u1), two(s[t], 1)));
+        for (int u = 0; u < 2; ++u) {
+          if (t + u >= NT) break;
+          if constexpr (BF16) {
+            put(sum[u], 0, __fadd2_rn(two(sum[u], 0), two(ds[u], 0)));
+            put(sum[u], 1, __fadd2_rn(two(sum[u], 1), two(ds[u], 1)));
+          } else {
+            put(sum[u], 0, __ffma2_rn(two(ds[u], 0), both(u0), two(sum[u], 0)));
+            put(sum[u], 1, __ffma2_rn(two(ds[u], 1), both(u1), two(sum[u], 1)));
+          }
         }
+        if (pair) tm_st<8>(tm_sum + 4 * t, sum[0]);
+        else tm_st<4>(tm_sum + 4 * t, sum[0]);
       }
-      tm_st<NT * 4>(tm_sum, s[0]);
       if (release_stage<STAGES>(tail, k, count, warps)) issue(k + STAGES);
       // this warp's part of dq, joined behind the next window's barrier
       const float h0 = p.scale * u0, h1 = p.scale * u1;
@@ -851,7 +864,7 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
     load_rows<HD, S::NPAD>(base + S::COLS, &maps.o_cols, full, 0, h, b);
     load_rows<HD, S::BR>(base + 2 * S::COLS, &maps.k_rows, full, row0, h, b);
     load_rows<HD, S::BR>(base + 2 * S::COLS + S::ROWS, &maps.v_rows, full, row0, h, b);
-    bulk_load(base + 2 * S::COLS + 2 * S::ROWS, p.stats + ((long long)b * p.H + h) * p.NS,
+    bulk_load(base + 2 * S::COLS + 2 * S::ROWS, p.stats + ((long long)b * p.H + h) * p.NS * 2,
               stat_bytes, full);
   };
   // the statistics of padded queries are not copied: 0 (read as p = 2^-inf)
@@ -943,12 +956,13 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
 
-#pragma unroll
-      for (int t = 0; t < NT; t += 2) {
+      // The scores and dp of a pair of tiles, one pair ahead of what is made of them
+      float s[2][2][4], d[2][2][4];
+      auto products = [&](auto masked, int t) {
         constexpr float z[4] = {0.f, 0.f, 0.f, 0.f};
         const uint32_t at = uint32_t(8 * t * R::BYTES);
-        uint32_t pa[4], da[4];
-        float s[2][4], d[2][4];
+        float(&sp)[2][4] = s[(t >> 1) & 1];
+        float(&dp)[2][4] = d[(t >> 1) & 1];
         if (t < TT) tm_wait<2>(nb);
         if constexpr (HD == 16) {
           uint32_t bq[4], bg[4];
@@ -956,8 +970,8 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
           ldsm_x4(gs + b_off + at, bg);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            mma16<BF16>(s[u], ka[0], bq[2 * u], bq[2 * u + 1], t < TT ? nb[u] : rest[u]);
-            mma16<BF16>(d[u], va[0], bg[2 * u], bg[2 * u + 1], z);
+            mma16<BF16>(sp[u], ka[0], bq[2 * u], bq[2 * u + 1], t < TT ? nb[u] : rest[u]);
+            mma16<BF16>(dp[u], va[0], bg[2 * u], bg[2 * u + 1], z);
           }
         } else {
 #pragma unroll
@@ -965,43 +979,58 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
             uint32_t bq[4], bg[4];
             ldsm_x4(qs + b_off + at + uint32_t(8 * u * R::BYTES), bq);
             ldsm_x4(gs + b_off + at + uint32_t(8 * u * R::BYTES), bg);
-            mma16<BF16>(s[u], ka[0], bq[0], bq[1], t < TT ? nb[u] : rest[u]);
-            mma16<BF16>(s[u], ka[1], bq[2], bq[3], s[u]);
-            mma16<BF16>(d[u], va[0], bg[0], bg[1], z);
-            mma16<BF16>(d[u], va[1], bg[2], bg[3], d[u]);
+            mma16<BF16>(sp[u], ka[0], bq[0], bq[1], t < TT ? nb[u] : rest[u]);
+            mma16<BF16>(dp[u], va[0], bg[0], bg[1], z);
+            mma16<BF16>(sp[u], ka[1], bq[2], bq[3], sp[u]);
+            mma16<BF16>(dp[u], va[1], bg[2], bg[3], dp[u]);
           }
         }
         if (t + 2 < TT) tm_ld<8>(tm_bias + 4 * (t + 2), nb[0]);
-        if (last != 0) {
+        if constexpr (decltype(masked)::value) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) mma8<BF16>(s[u], a0, a1, mb[32 * (t + u)]);
+          for (int u = 0; u < 2; ++u) mma8<BF16>(sp[u], a0, a1, mb[32 * (t + u)]);
         }
+      };
+      auto sweep = [&](auto masked) {
+        products(masked, 0);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float4 x =  // two queries' statistics
-              *reinterpret_cast<const float4*>(stat + 8 * (t + u));
-          const float2 lse = make_float2(-x.x, -x.z), del = make_float2(-x.y, -x.w);
+        for (int t = 0; t < NT; t += 2) {
+          const uint32_t at = uint32_t(8 * t * R::BYTES);
+          uint32_t tq[HD / 16][4], tg[HD / 16][4];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float2 y = __ffma2_rn(two(s[u], r), cc, lse);
-            const float2 q = make_float2(ex2(y.x), ex2(y.y));
-            float2 ds = __fmul2_rn(__fadd2_rn(two(d[u], r), del), q);
-            if constexpr (!BF16) ds = __fmul2_rn(ds, both(gscale));
-            pa[2 * u + r] = pack2<BF16>(q.x, q.y);
-            da[2 * u + r] = pack2<BF16>(ds.x, ds.y);
+          for (int n = 0; n < HD / 16; ++n) {
+            ldsm_x4_t(gs + (n ? bt_off1 : bt_off) + at, tg[n]);
+            ldsm_x4_t(qs + (n ? bt_off1 : bt_off) + at, tq[n]);
+          }
+          if (t + 2 < NT) products(masked, t + 2);
+          uint32_t pa[4], da[4];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // two queries' statistics: (-lse, -lse, -delta, -delta)
+            const float4 x = *reinterpret_cast<const float4*>(stat + 8 * (t + u));
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float2 y =
+                  __ffma2_rn(two(s[(t >> 1) & 1][u], r), cc, make_float2(x.x, x.y));
+              const float2 q = make_float2(ex2(y.x), ex2(y.y));
+              float2 ds = __fmul2_rn(
+                  __fadd2_rn(two(d[(t >> 1) & 1][u], r), make_float2(x.z, x.w)), q);
+              if constexpr (!BF16) ds = __fmul2_rn(ds, both(gscale));
+              pa[2 * u + r] = pack2<BF16>(q.x, q.y);
+              da[2 * u + r] = pack2<BF16>(ds.x, ds.y);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < HD / 16; ++n) {
+            mma16<BF16>(dv[2 * n], pa, tg[n][0], tg[n][1], dv[2 * n]);
+            mma16<BF16>(dv[2 * n + 1], pa, tg[n][2], tg[n][3], dv[2 * n + 1]);
+            mma16<BF16>(dk[2 * n], da, tq[n][0], tq[n][1], dk[2 * n]);
+            mma16<BF16>(dk[2 * n + 1], da, tq[n][2], tq[n][3], dk[2 * n + 1]);
           }
         }
-#pragma unroll
-        for (int n = 0; n < HD / 16; ++n) {
-          uint32_t tq[4], tg[4];
-          ldsm_x4_t(gs + (n ? bt_off1 : bt_off) + at, tg);
-          ldsm_x4_t(qs + (n ? bt_off1 : bt_off) + at, tq);
-          mma16<BF16>(dv[2 * n], pa, tg[0], tg[1], dv[2 * n]);
-          mma16<BF16>(dv[2 * n + 1], pa, tg[2], tg[3], dv[2 * n + 1]);
-          mma16<BF16>(dk[2 * n], da, tq[0], tq[1], dk[2 * n]);
-          mma16<BF16>(dk[2 * n + 1], da, tq[2], tq[3], dk[2 * n + 1]);
-        }
-      }
+      };
+      if (last != 0) sweep(std::true_type{});
+      else sweep(std::false_type{});
       if (release_stage<STAGES>(tail, k, count, warps)) issue(k + STAGES);
       const float f = BF16 ? p.scale : p.scale * inverse_scale(gscale);
       uint16_t* to = p.dqkv + ((long long)(share + k * p.S) * p.N + k0) * tok + width + h * HD + 2 * t4;
@@ -1176,7 +1205,7 @@ int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   GradParams p{};
   p.dqkv = static_cast<uint16_t*>(a.grad_qkv);
   p.dbias = a.grad_bias;
-  p.stats = reinterpret_cast<float2*>(a.stats);
+  p.stats = a.stats;
   p.NS = int(a.N + (a.N & 1));
   p.amax = a.stats + 2 * a.B * a.H * p.NS;
   p.table = a.table;
