@@ -439,8 +439,10 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* map, 
     tma_load_4d(dst + r * HD * 2, map, full, 0, row0 + r, h, b);
 }
 
-struct Maps {  // q, k, v and do, in boxes of a window's (cols) and of a CTA's (rows) tokens
-  CUtensorMap q_cols, k_cols, v_cols, o_cols, q_rows, k_rows, v_rows, o_rows;
+// The tensors that a kernel loads: two in boxes of all the window's tokens, two of the CTA's rows
+// (rows kernel: k, v and q, do; columns kernel: q, do and k, v).
+struct Maps {
+  CUtensorMap cols0, cols1, rows0, rows1;
 };
 
 // ------------------------------------------------------------------------ rows kernel
@@ -480,10 +482,10 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
     if (p.analytic) tail->last[st] = last_axes(p, b);
     tail->issued = k + 1;
     mbar_arrive_expect_tx(full, S::STAGE);
-    load_rows<HD, S::NPAD>(base, &maps.k_cols, full, 0, h, b);
-    load_rows<HD, S::NPAD>(base + S::COLS, &maps.v_cols, full, 0, h, b);
-    load_rows<HD, kBR>(base + 2 * S::COLS, &maps.q_rows, full, row0, h, b);
-    load_rows<HD, kBR>(base + 2 * S::COLS + S::ROWS, &maps.o_rows, full, row0, h, b);
+    load_rows<HD, S::NPAD>(base, &maps.cols0, full, 0, h, b);
+    load_rows<HD, S::NPAD>(base + S::COLS, &maps.cols1, full, 0, h, b);
+    load_rows<HD, kBR>(base + 2 * S::COLS, &maps.rows0, full, row0, h, b);
+    load_rows<HD, kBR>(base + 2 * S::COLS + S::ROWS, &maps.rows1, full, row0, h, b);
   };
   if (tid == 0) {
     init_tail(tail);
@@ -860,10 +862,10 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
     if (p.analytic) tail->last[st] = last_axes(p, b);
     tail->issued = k + 1;
     mbar_arrive_expect_tx(full, 2 * S::COLS + 2 * S::ROWS + stat_bytes);
-    load_rows<HD, S::NPAD>(base, &maps.q_cols, full, 0, h, b);
-    load_rows<HD, S::NPAD>(base + S::COLS, &maps.o_cols, full, 0, h, b);
-    load_rows<HD, S::BR>(base + 2 * S::COLS, &maps.k_rows, full, row0, h, b);
-    load_rows<HD, S::BR>(base + 2 * S::COLS + S::ROWS, &maps.v_rows, full, row0, h, b);
+    load_rows<HD, S::NPAD>(base, &maps.cols0, full, 0, h, b);
+    load_rows<HD, S::NPAD>(base + S::COLS, &maps.cols1, full, 0, h, b);
+    load_rows<HD, S::BR>(base + 2 * S::COLS, &maps.rows0, full, row0, h, b);
+    load_rows<HD, S::BR>(base + 2 * S::COLS + S::ROWS, &maps.rows1, full, row0, h, b);
     bulk_load(base + 2 * S::COLS + 2 * S::ROWS, p.stats + ((long long)b * p.H + h) * p.NS * 2,
               stat_bytes, full);
   };
@@ -895,8 +897,8 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
   if (live) {
     float rest[2][4];  // the start values of the tiles past TT
     {
-      constexpr int PART = TT % 8 == 0 ? 8 : TT % 6 == 0 ? 6 : 4;
-      static_assert(TT % PART == 0, "tiles per round of gathers");
+      constexpr int PART = TT == 42 ? 14 : TT == 28 ? 7 : 8;  // tiles per round of gathers
+      static_assert(TT % PART == 0, "whole rounds");
 #pragma unroll 1
       for (int t = 0; t < TT; t += PART) {
         float v[PART][4];
@@ -1096,22 +1098,19 @@ int make_map(CUtensorMap* map, const void* base, const AttnGradArgs& a, int64_t 
   return kOk;
 }
 
-int make_maps(Maps* m, const AttnGradArgs& a, int cols, int rows) {
+int make_maps(Maps* m, const AttnGradArgs& a, bool of_rows_kernel, int cols, int rows) {
   const int64_t width = a.H * a.head_dim;
   const uint16_t* q = static_cast<const uint16_t*>(a.qkv);
-  const struct {
-    CUtensorMap *c, *r;
-    const void* base;
-    int64_t tok;
-  } parts[4] = {{&m->q_cols, &m->q_rows, q, 3 * width},
-                {&m->k_cols, &m->k_rows, q + width, 3 * width},
-                {&m->v_cols, &m->v_rows, q + 2 * width, 3 * width},
-                {&m->o_cols, &m->o_rows, a.grad_out, width}};
-  for (const auto& t : parts) {
-    if (int e = make_map(t.c, t.base, a, t.tok, box_rows(cols))) return e;
-    if (int e = make_map(t.r, t.base, a, t.tok, box_rows(rows))) return e;
-  }
-  return kOk;
+  CUtensorMap* const qo[2] = {of_rows_kernel ? &m->rows0 : &m->cols0,
+                              of_rows_kernel ? &m->rows1 : &m->cols1};
+  CUtensorMap* const kv[2] = {of_rows_kernel ? &m->cols0 : &m->rows0,
+                              of_rows_kernel ? &m->cols1 : &m->rows1};
+  const int qo_box = box_rows(of_rows_kernel ? rows : cols);
+  const int kv_box = box_rows(of_rows_kernel ? cols : rows);
+  if (int e = make_map(qo[0], q, a, 3 * width, qo_box)) return e;
+  if (int e = make_map(qo[1], a.grad_out, a, width, qo_box)) return e;
+  if (int e = make_map(kv[0], q + width, a, 3 * width, kv_box)) return e;
+  return make_map(kv[1], q + 2 * width, a, 3 * width, kv_box);
 }
 
 int sm_count() {
@@ -1150,14 +1149,14 @@ int launch_grad(GradParams p, const AttnGradArgs& a, cudaStream_t stream) {
     if (dev < 64) configured[dev] = true;
   }
   Maps maps;
-  if (int e = make_maps(&maps, a, NPAD, kBR)) return e;
+  if (int e = make_maps(&maps, a, true, NPAD, kBR)) return e;
   p.RB = (p.N + kBR - 1) / kBR;
   p.S = int(a.shares);
   grad_rows_kernel<RS, BF16>
       <<<unsigned(p.H) * unsigned(p.RB) * unsigned(p.S), RS::THREADS, RS::SMEM, stream>>>(maps, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "attention gradient (rows) launch");
-  if (int r = make_maps(&maps, a, NPAD, CS::BR)) return r;
+  if (int r = make_maps(&maps, a, false, NPAD, CS::BR)) return r;
   split(&p, CS::BR, CS::MINB);
   grad_cols_kernel<CS, BF16>
       <<<unsigned(p.H) * unsigned(p.RB) * unsigned(p.S), CS::THREADS, CS::SMEM, stream>>>(maps, p);

@@ -21,6 +21,7 @@ change from run to run (no atomics).  CUDA tensors only, as elsewhere in the pac
 
 from __future__ import annotations
 
+import functools
 import sys
 import types
 from typing import NamedTuple, Sequence
@@ -30,8 +31,8 @@ import torch.nn.functional as F
 
 from . import _ops as _native
 from . import profiling as _prof
-from .fused_attention import (_ATTN_DTYPES, attention_bias_tiles, head_dim_supported,
-                              swin_window_attention_qkv, tensor_core_attention)
+from .fused_attention import (_ATTN_DTYPES, head_dim_supported, swin_window_attention_qkv,
+                              tensor_core_attention)
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 GROUP = 32  # neighbouring channels that share one scale of an 8-bit checkpoint
@@ -46,7 +47,31 @@ def _require_cuda(what: str, *tensors) -> None:
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+# Sizes that the library works out from a call's shapes and the device's SM count; asked once
+# for each, since the call and the switch to the device cost more than a small launch.
+@functools.lru_cache(maxsize=1024)
+def _shares(B: int, H: int, N: int, D: int, dtype: torch.dtype, device: int) -> int:
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    with torch.cuda.device(device):
+        return int(_native.capi().crumpet_window_attention_backward_shares(B, H, N, D, code))
+
+
+@functools.lru_cache(maxsize=1024)
+def _partials(rows: int, C: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return int(_native.capi().crumpet_norm_gate_residual_backward_partials(rows, C))
+
+
+@functools.lru_cache(maxsize=1024)
+def _tile_bytes(H: int, N: int) -> int:
+    return int(_native.capi().crumpet_attention_bias_tiles_bytes(H, N))
 
 
 # ------------------------------------------------------------------ relative-position bias
@@ -97,16 +122,17 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
 
 
 def _check_table(table: torch.Tensor, buckets: RelativePositionBuckets) -> int:
-    if table.ndim != 2 or int(table.shape[0]) != buckets.num_buckets:
+    if table.ndim != 2 or table.shape[0] != buckets.num_buckets:
         raise ValueError(f"table must have shape [{buckets.num_buckets}, heads]")
     if table.dtype not in _DTYPES:
         raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
-    return int(table.shape[1])
+    return table.shape[1]
 
 
 def _bias_forward(table, buckets, dtype):
-    heads = int(table.shape[1])
-    bias = torch.empty((heads, *buckets.pairs.shape), dtype=dtype, device=table.device)
+    if table.requires_grad:
+        table = table.detach()
+    bias = torch.empty((table.shape[1], *buckets.pairs.shape), dtype=dtype, device=table.device)
     token = _prof.kernel_begin("relative_position_bias", lambda: {
         "bytes": bias.numel() * bias.element_size() + buckets.pairs.numel() * 4})
     _native.require().relative_position_bias(bias, table.contiguous(), buckets.pairs)
@@ -163,7 +189,7 @@ def relative_position_bias_backward(grad_bias: torch.Tensor, buckets: RelativePo
     """Gradient of the table, ``[num_buckets, heads]`` in ``dtype`` (default: ``grad_bias``'s),
     from the gradient ``[heads, rows, cols]`` of the bias: per bucket the fp32 sum over its
     pairs, rounded once."""
-    if grad_bias.ndim != 3 or tuple(grad_bias.shape[1:]) != tuple(buckets.pairs.shape):
+    if grad_bias.ndim != 3 or grad_bias.shape[1:] != buckets.pairs.shape:
         raise ValueError(f"grad_bias must have shape [heads, {', '.join(map(str, buckets.pairs.shape))}]")
     dtype = grad_bias.dtype if dtype is None else dtype
     if grad_bias.dtype not in _DTYPES or dtype not in _DTYPES:
@@ -173,31 +199,36 @@ def relative_position_bias_backward(grad_bias: torch.Tensor, buckets: RelativePo
 
 
 # ------------------------------------------------------------------------- window attention
+def _triple(value):
+    return value if type(value) is tuple and len(value) == 3 else tuple(map(int, value))
+
+
 def _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale):
     if qkv.ndim != 5 or qkv.shape[2] != 3:
         raise ValueError("qkv must have shape [B, N, 3, H, head_dim]")
-    B, N, _, H, D = (int(s) for s in qkv.shape)
+    B, N, _, H, D = qkv.shape
     if qkv.dtype not in _ATTN_DTYPES:
         raise TypeError("window attention supports torch.float32, torch.float16 and torch.bfloat16")
     if not head_dim_supported(D):
         raise ValueError("window attention requires a power-of-two head_dim between 16 and 256")
     if _check_table(table, buckets) != H:
         raise ValueError(f"table must have shape [{buckets.num_buckets}, {H}]")
-    if tuple(buckets.pairs.shape) != (N, N):
+    if buckets.pairs.shape != (N, N):
         raise ValueError(f"buckets must be made of an index [{N}, {N}] (index[:n, :n] of a "
                          "clamped window)")
-    num_windows, shift_size = tuple(map(int, num_windows)), tuple(map(int, shift_size))
-    window_size = (N, 1, 1) if window_size is None else tuple(map(int, window_size))
+    num_windows, shift_size = _triple(num_windows), _triple(shift_size)
+    window_size = (N, 1, 1) if window_size is None else _triple(window_size)
     if not len(num_windows) == len(window_size) == len(shift_size) == 3:
         raise ValueError("num_windows, window_size and shift_size must contain exactly three values")
     if min(num_windows) < 1 or min(window_size) < 1:
         raise ValueError("num_windows and window_size values must be positive")
     if window_size[0] * window_size[1] * window_size[2] != N:
         raise ValueError(f"window_size must hold N = {N} tokens")
-    if any(not 0 <= s < w for s, w in zip(shift_size, window_size)):
-        raise ValueError("shift_size must satisfy 0 <= shift < window_size")
-    if any(shift_size) and B % (num_windows[0] * num_windows[1] * num_windows[2]):
-        raise ValueError("B must be a multiple of the number of windows")
+    if shift_size != (0, 0, 0):
+        if any(not 0 <= s < w for s, w in zip(shift_size, window_size)):
+            raise ValueError("shift_size must satisfy 0 <= shift < window_size")
+        if B % (num_windows[0] * num_windows[1] * num_windows[2]):
+            raise ValueError("B must be a multiple of the number of windows")
     scale = 1.0 / (D ** 0.5) if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError("window attention requires a finite scale > 0")
@@ -206,29 +237,39 @@ def _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, 
 
 
 def _attention_table(table, dtype):
-    table = table.detach()
+    if table.requires_grad:
+        table = table.detach()
     return (table if table.dtype in (torch.float32, dtype) else table.float()).contiguous()
 
 
 def _attention_forward(qkv, table, buckets, place):
     num_windows, window_size, shift_size, scale = place
     qkv = qkv.contiguous()
-    N, D = int(qkv.shape[1]), int(qkv.shape[4])
-    tiles = None
-    if tensor_core_attention(qkv.dtype, N, D) and qkv.numel() and qkv.data_ptr() % 16 == 0:
-        # the table changes every step, so its operands are built every step
-        tiles = attention_bias_tiles(table, buckets.index, N, scale, qkv.dtype)
-    return swin_window_attention_qkv(qkv, _attention_table(table, qkv.dtype), buckets.index,
-                                     num_windows, window_size, shift_size, scale, bias_tiles=tiles)
+    B, N, _, H, D = qkv.shape
+    table = _attention_table(table, qkv.dtype)
+    if not (tensor_core_attention(qkv.dtype, N, D) and B and qkv.data_ptr() % 16 == 0):
+        return swin_window_attention_qkv(qkv, table, buckets.index, num_windows, window_size,
+                                         shift_size, scale)
+    # the table changes every step, so its operands are built every step
+    ops = _native.require()
+    tiles = torch.empty(_tile_bytes(H, N), dtype=torch.uint8, device=qkv.device)
+    out = torch.empty((B, N, H * D), dtype=qkv.dtype, device=qkv.device)
+    ops.attention_bias_tiles(tiles, table, buckets.index, N, scale, qkv.dtype)
+    _prof.count("attention_bias_tiles")
+    token = _prof.kernel_begin("swin_window_attention_qkv", lambda: {
+        "bytes": 4 * B * H * N * D * qkv.element_size(), "flops": 4 * B * H * N * N * D,
+        "exps": B * H * N * N})
+    ops.swin_window_attention_qkv_tiles(out, qkv, tiles, num_windows, window_size, shift_size, scale)
+    _prof.count("swin_window_attention_qkv")
+    _prof.kernel_end(token)
+    return out
 
 
 def _attention_backward(grad_out, qkv, table, buckets, place):
     num_windows, window_size, shift_size, scale = place
     qkv, grad_out = qkv.contiguous(), grad_out.contiguous()
-    B, N, _, H, D = (int(s) for s in qkv.shape)
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[qkv.dtype]
-    with torch.cuda.device(qkv.device):
-        shares = int(_native.capi().crumpet_window_attention_backward_shares(B, H, N, D, code))
+    B, N, _, H, D = qkv.shape
+    shares = _shares(B, H, N, D, qkv.dtype, qkv.get_device())
     grad_qkv = torch.empty_like(qkv)
     grad_bias = torch.empty((shares, H, N, N), dtype=torch.float32, device=qkv.device)
     stats = torch.empty(B * H * (3 * N + 4), dtype=torch.float32, device=qkv.device)
@@ -288,8 +329,8 @@ def swin_window_attention_backward(
     [B, N, H * head_dim]`` and the forward's own arguments, in the dtypes of ``qkv`` and
     ``table``."""
     place = _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale)
-    B, N, _, H, D = (int(s) for s in qkv.shape)
-    if tuple(grad_out.shape) != (B, N, H * D) or grad_out.dtype != qkv.dtype:
+    B, N, _, H, D = qkv.shape
+    if grad_out.shape != (B, N, H * D) or grad_out.dtype != qkv.dtype:
         raise ValueError(f"grad_out must have shape {(B, N, H * D)} and the dtype of qkv")
     _require_cuda("window attention", grad_out)
     return _attention_backward(grad_out, qkv, table, buckets, place)
@@ -311,9 +352,13 @@ class NormGateGrads(NamedTuple):
 def _vector(t, n, device, what):
     if t is None:
         return None
-    if tuple(t.shape) != (n,) or not t.is_floating_point():
+    if t.shape != (n,) or not t.is_floating_point():
         raise ValueError(f"{what} must be a floating-point tensor of shape ({n},)")
-    return t.detach().to(device=device, dtype=torch.float32).contiguous()
+    if t.requires_grad:
+        t = t.detach()
+    if t.dtype is not torch.float32 or t.device != device:
+        t = t.to(device=device, dtype=torch.float32)
+    return t.contiguous()
 
 
 def _check_norm_gate(branch, stream, gate, row_scale, post_norm, pre_norm, eps):
@@ -322,26 +367,30 @@ def _check_norm_gate(branch, stream, gate, row_scale, post_norm, pre_norm, eps):
     if branch.dtype not in _DTYPES or stream.dtype not in (branch.dtype, torch.float32):
         raise TypeError("norm_gate_residual takes float32, float16 or bfloat16 branches and a "
                         "residual stream in float32 or the branch's dtype")
-    C = int(branch.shape[-1])
+    C = branch.shape[-1]
     if not 1 <= C <= MAX_CHANNELS:
         raise ValueError(f"norm_gate_residual needs 1 to {MAX_CHANNELS} channels")
     if not eps > 0:
         raise ValueError("eps must be positive")
-    for name, norm in (("post_norm", post_norm), ("pre_norm", pre_norm)):
-        if norm is not None and len(norm) != 2:
-            raise ValueError(f"{name} must be a (weight, bias) pair")
-    rows = branch.numel() // C
-    if row_scale is not None and (row_scale.ndim != 1 or not row_scale.numel()
-                                  or rows % row_scale.numel()):
-        raise ValueError("row_scale must be one value per sample, the rows a multiple of it")
     _require_cuda("norm_gate_residual", branch, stream)
     dev = branch.device
-    post = post_norm or (None, None)
-    pre = pre_norm or (None, None)
-    return (_vector(gate, C, dev, "gate"),
-            None if row_scale is None else _vector(row_scale, row_scale.numel(), dev, "row_scale"),
-            _vector(post[0], C, dev, "post_norm weight"), _vector(post[1], C, dev, "post_norm bias"),
-            _vector(pre[0], C, dev, "pre_norm weight"), _vector(pre[1], C, dev, "pre_norm bias"))
+    post_w = post_b = pre_w = pre_b = None
+    if post_norm is not None:
+        if len(post_norm) != 2:
+            raise ValueError("post_norm must be a (weight, bias) pair")
+        post_w = _vector(post_norm[0], C, dev, "post_norm weight")
+        post_b = _vector(post_norm[1], C, dev, "post_norm bias")
+    if pre_norm is not None:
+        if len(pre_norm) != 2:
+            raise ValueError("pre_norm must be a (weight, bias) pair")
+        pre_w = _vector(pre_norm[0], C, dev, "pre_norm weight")
+        pre_b = _vector(pre_norm[1], C, dev, "pre_norm bias")
+    if row_scale is not None:
+        samples = row_scale.numel()
+        if row_scale.ndim != 1 or not samples or branch.numel() // C % samples:
+            raise ValueError("row_scale must be one value per sample, the rows a multiple of it")
+        row_scale = _vector(row_scale, samples, dev, "row_scale")
+    return _vector(gate, C, dev, "gate"), row_scale, post_w, post_b, pre_w, pre_b
 
 
 def _norm_gate_forward(branch, residual, params, eps):
@@ -361,15 +410,15 @@ def _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps):
     gate, row_scale, post_w, post_b, pre_w, _ = params
     branch, out, grad_out = branch.contiguous(), out.contiguous(), grad_out.contiguous()
     grad_normed = None if pre_w is None else grad_normed.contiguous()
-    C = int(branch.shape[-1])
+    C = branch.shape[-1]
     grad_residual, grad_branch = torch.empty_like(out), torch.empty_like(branch)
     sums = partial = None
+    columns = (None,) * 5
     if gate is not None or post_w is not None or pre_w is not None:
-        with torch.cuda.device(branch.device):
-            n = int(_native.capi().crumpet_norm_gate_residual_backward_partials(
-                branch.numel() // C, C))
         sums = torch.empty((5, C), dtype=torch.float32, device=branch.device)
-        partial = torch.empty(n, dtype=torch.float32, device=branch.device)
+        partial = torch.empty(_partials(branch.numel() // C, C, branch.get_device()),
+                              dtype=torch.float32, device=branch.device)
+        columns = sums.unbind(0)
     token = _prof.kernel_begin("norm_gate_residual_backward", lambda: {
         "bytes": sum(t.numel() * t.element_size() for t in (
             grad_out, grad_normed, out if pre_w is not None else None,
@@ -380,9 +429,9 @@ def _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps):
         row_scale, post_w, post_b, pre_w, float(eps))
     _prof.count("norm_gate_residual_backward")
     _prof.kernel_end(token)
-    given = (gate, post_w, post_w, pre_w, pre_w)
-    return NormGateGrads(grad_residual, grad_branch,
-                         *(None if g is None else sums[i] for i, g in enumerate(given)))
+    return NormGateGrads(grad_residual, grad_branch, None if gate is None else columns[0],
+                         *((None, None) if post_w is None else columns[1:3]),
+                         *((None, None) if pre_w is None else columns[3:5]))
 
 
 class _NormGate(torch.autograd.Function):
