@@ -53,11 +53,13 @@ struct alignas(16) Pack8 {
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  Pack8<T> w;
+__device__ __forceinline__ void load8(const T* p, Pack8<T>& w) {
 #pragma unroll
   for (int k = 0; k < int(sizeof(w)) / 16; ++k)
     reinterpret_cast<uint4*>(&w)[k] = ldg_stream(reinterpret_cast<const uint4*>(p) + k);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Pack8<T>& w, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_f32(w.v[i]);
 }
@@ -71,19 +73,51 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     stg(reinterpret_cast<uint4*>(p) + k, reinterpret_cast<const uint4*>(&w)[k]);
 }
 
-// F(x), and exp(-x^2 / 2) in *e
-__device__ __forceinline__ float normal_cdf(float x, float* e) {
-  const float z = fabsf(x) * 0.70710678118654752f;
-  float t, ex;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, z, 1.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ex) : "f"(z * z * -1.4426950408889634f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  q = 0.5f * q * t * ex;  // F(-|x|)
-  *e = ex;
-  return x < 0.f ? q : 1.f - q;
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// max(x, 0), NaN for NaN
+__device__ __forceinline__ float relu(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// F(-|x|) of two values, and exp(-x^2 / 2) in *e; the packed arithmetic takes two per instruction
+__device__ __forceinline__ float2 lower_tail(float2 a, float2* e) {
+  // a = |x|: 1 + 0.3275911 a / sqrt 2, and -a^2 / 2 in powers of two
+  const float2 d = __ffma2_rn(a, both(0.23164189f), both(1.f));
+  const float2 y = __fmul2_rn(__fmul2_rn(a, a), both(-0.72134752044448170f));
+  float2 t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(d.y));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e->x) : "f"(y.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e->y) : "f"(y.y));
+  // half the formula's coefficients: F(-a) = erfc / 2
+  float2 q = __ffma2_rn(both(0.5307027145f), t, both(-0.7265760135f));
+  q = __ffma2_rn(q, t, both(0.7107068705f));
+  q = __ffma2_rn(q, t, both(-0.142248368f));
+  q = __ffma2_rn(q, t, both(0.127414796f));
+  return __fmul2_rn(__fmul2_rn(q, t), *e);
+}
+// gelu(x) = x F(x) = max(x, 0) - |x| F(-|x|): one expression for both signs, exact in the tails.
+// |x| is taken as finite, so infinities give inf and 0; NaN gives NaN through max(x, 0).
+__device__ __forceinline__ float2 gelu(float2 x) {
+  constexpr float kMax = 3.402823466e38f;
+  const float2 a = make_float2(fminf(fabsf(x.x), kMax), fminf(fabsf(x.y), kMax));
+  float2 e;
+  const float2 q = lower_tail(a, &e);
+  return __ffma2_rn(make_float2(-a.x, -a.y), q, make_float2(relu(x.x), relu(x.y)));
+}
+// gelu and its slope F(x) + x f(x) of finite x or NaN: with r = |x| f - F(-|x|) the slope is 1 + r, and -r for
+// negative x
+__device__ __forceinline__ float2 gelu_slope(float2 x, float2* y) {
+  const float2 a = make_float2(fabsf(x.x), fabsf(x.y));
+  float2 e;
+  const float2 q = lower_tail(a, &e);
+  *y = __ffma2_rn(make_float2(-a.x, -a.y), q, make_float2(relu(x.x), relu(x.y)));
+  const float2 r = __ffma2_rn(__fmul2_rn(a, both(0.39894228040143268f)), e,
+                              make_float2(-q.x, -q.y));
+  const float2 s = make_float2(copysignf(1.f, x.x), copysignf(1.f, x.y));
+  return __ffma2_rn(r, s, __ffma2_rn(s, both(0.5f), both(0.5f)));
 }
 
 // Scale byte of a group from the bits of its largest magnitude.
@@ -99,11 +133,31 @@ __device__ __forceinline__ float code_inverse(uint32_t code) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// q of one value: 0 in a group with an infinity or NaN (its inverse step is 0; the product of
-// 0 and an infinity, NaN, converts to 0)
-__device__ __forceinline__ int quantise(float x, float inv) { return __float2int_rn(x * inv); }
+// Rounding to whole numbers by adding 1.5 * 2^23: the sum's low byte is q in two's complement.
+// In a group with an infinity or NaN (code 255) q is 0.
+constexpr float kRound = 12582912.f;
+__device__ __forceinline__ uint32_t quantise4(const float* x, float inv, uint32_t code) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(x[i], inv, kRound));
+  const uint32_t w = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040),
+                                 0x5410);
+  return code == 255u ? 0u : w;
+}
+__device__ __forceinline__ int quantise(float x, float inv, uint32_t code) {
+  return code == 255u ? 0 : int(int8_t(__float_as_uint(fmaf(x, inv, kRound)) & 0xffu));
+}
+// u of four values of a word: a byte with its sign bit flipped, under the exponent of 2^23, is
+// 2^23 + 128 + q
+__device__ __forceinline__ void restore4(uint32_t w, float s, float* x) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440u + i)) - 8388736.f) * s;
+}
 
 struct Rows {
+  bool whole;           // rows of whole groups: group g holds elements [32 g, 32 g + 32)
   long long groups;     // rows x groups per row
   uint32_t per_row;     // groups per row
   DivMod32 div;         // by per_row (row and group from a 32-bit group number)
@@ -121,24 +175,48 @@ __device__ __forceinline__ void place(const Rows& r, long long grp, long long* r
   *first = int(grp - q * r.per_row) * kGroup;
 }
 
+// Where the 8 channels of part `part` of a group lie
+struct Place {
+  long long at;
+  bool in_group, in;
+};
+__device__ __forceinline__ Place find_part(const Rows& r, long long grp, int part) {
+  Place q;
+  q.in_group = grp < r.groups;
+  if (r.whole) {
+    q.in = q.in_group;
+    q.at = grp * kGroup + part * 8;
+    return q;
+  }
+  long long row = 0;
+  int c = 0;
+  if (q.in_group) place(r, grp, &row, &c);
+  c += part * 8;
+  q.in = q.in_group && c < r.C;
+  q.at = row * r.C + c;
+  return q;
+}
+
 // C a multiple of 8 and 16-byte aligned tensors: four lanes per group
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 gelu_keep_kernel(T* y, int8_t* kept, uint8_t* scales, const T* x, Rows r) {
   const int part = threadIdx.x & 3;
   const long long step = (long long)gridDim.x * (kThreads / 4);
+  auto find = [&](long long grp) { return find_part(r, grp, part); };
+  long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
+  // the next group's load is in flight through this one's arithmetic
+  Place q = find(grp);
+  Pack8<T> ahead = {};
+  if (q.in) load8(x + q.at, ahead);
   // whole warps take part in the shuffles: the bound is rounded up to a warp's 8 groups
-  for (long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
-       grp - (grp & 7) < r.groups; grp += step) {
-    long long row = 0;
-    int c = 0;
-    const bool in_group = grp < r.groups;
-    if (in_group) place(r, grp, &row, &c);
-    c += part * 8;
-    const bool in = in_group && c < r.C;
-    const long long at = row * r.C + c;
+  for (; grp - (grp & 7) < r.groups; grp += step) {
+    const long long at = q.at;
+    const bool in_group = q.in_group, in = q.in;
     float v[8] = {};
-    if (in) load8(x + at, v);
+    if (in) unpack8(ahead, v);
+    q = find(grp + step);
+    if (q.in) load8(x + q.at, ahead);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
@@ -148,14 +226,14 @@ gelu_keep_kernel(T* y, int8_t* kept, uint8_t* scales, const T* x, Rows r) {
     if (in_group && part == 0) scales[grp] = uint8_t(code);
     if (!in) continue;
     const float inv = code_inverse(code);
-    uint32_t w[2] = {0, 0};
+    stg(reinterpret_cast<uint2*>(kept + at),
+        make_uint2(quantise4(v, inv, code), quantise4(v + 4, inv, code)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i >> 2] |= (uint32_t(quantise(v[i], inv)) & 0xffu) << (8 * (i & 3));
-    stg(reinterpret_cast<uint2*>(kept + at), make_uint2(w[0], w[1]));
-    float e;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= normal_cdf(v[i], &e);
+    for (int i = 0; i < 8; i += 2) {
+      const float2 f = gelu(make_float2(v[i], v[i + 1]));
+      v[i] = f.x;
+      v[i + 1] = f.y;
+    }
     store8(y + at, v);
   }
 }
@@ -177,9 +255,8 @@ gelu_keep_any_kernel(T* y, int8_t* kept, uint8_t* scales, const T* x, Rows r) {
     const uint32_t code = scale_code(__reduce_max_sync(~0u, abs_bits(v)));
     if (lane == 0) scales[grp] = uint8_t(code);
     if (c < r.C) {
-      kept[at] = int8_t(quantise(v, code_inverse(code)));
-      float e;
-      y[at] = from_f32<T>(v * normal_cdf(v, &e));
+      kept[at] = int8_t(quantise(v, code_inverse(code), code));
+      y[at] = from_f32<T>(gelu(both(v)).x);
     }
   }
 }
@@ -191,29 +268,45 @@ kept_use_kernel(T* grad_x, T* again, const T* grad_y, const int8_t* kept, const 
                 Rows r) {
   const int part = threadIdx.x & 3;
   const long long step = (long long)gridDim.x * (kThreads / 4);
-  for (long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
-       grp < r.groups; grp += step) {
-    long long row;
-    int c;
-    place(r, grp, &row, &c);
-    c += part * 8;
-    if (c >= r.C) continue;
-    const long long at = row * r.C + c;
-    const uint2 w = ldg_stream(reinterpret_cast<const uint2*>(kept + at));
-    float g[8];
-    if constexpr (GRAD) load8(grad_y + at, g);
-    const float s = code_step(__ldg(scales + grp));
+  struct Part {
+    Pack8<T> g;
+    uint2 w;
+    uint32_t code;
+  };
+  auto load = [&](const Place& q, long long grp, Part& d) {
+    if (!q.in) return;
+    d.w = ldg_stream(reinterpret_cast<const uint2*>(kept + q.at));
+    if constexpr (GRAD) load8(grad_y + q.at, d.g);
+    d.code = __ldg(scales + grp);
+  };
+  long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
+  // the next group's loads are in flight through this one's arithmetic
+  Place q = find_part(r, grp, part);
+  Part ahead = {};
+  load(q, grp, ahead);
+  for (; grp < r.groups; grp += step) {
+    const Part now = ahead;
+    const Place here = q;
+    q = find_part(r, grp + step, part);
+    load(q, grp + step, ahead);
+    if (!here.in) continue;
+    const long long at = here.at;
+    const uint2 w = now.w;
+    const float s = code_step(now.code);
     float a[8];
+    restore4(w.x, s, a);
+    restore4(w.y, s, a + 4);
+    float g[8];
+    if constexpr (GRAD) {
+      unpack8(now.g, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = s * float(int8_t((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
-      if constexpr (GRAD) {
-        float e;
-        const float f = normal_cdf(x, &e);
-        g[i] *= fmaf(x * 0.39894228040143268f, e, f);
-        a[i] = x * f;
-      } else {
-        a[i] = x;
+      for (int i = 0; i < 8; i += 2) {
+        float2 y;
+        const float2 slope = gelu_slope(make_float2(a[i], a[i + 1]), &y);
+        g[i] *= slope.x;
+        g[i + 1] *= slope.y;
+        a[i] = y.x;
+        a[i + 1] = y.y;
       }
     }
     if constexpr (GRAD) store8(grad_x + at, g);
@@ -237,10 +330,10 @@ kept_use_any_kernel(T* grad_x, T* again, const T* grad_y, const int8_t* kept,
     const long long at = row * r.C + c;
     const float x = code_step(__ldg(scales + grp)) * float(kept[at]);
     if constexpr (GRAD) {
-      float e;
-      const float f = normal_cdf(x, &e);
-      grad_x[at] = from_f32<T>(to_f32(grad_y[at]) * fmaf(x * 0.39894228040143268f, e, f));
-      again[at] = from_f32<T>(x * f);
+      float2 y;
+      const float slope = gelu_slope(both(x), &y).x;
+      grad_x[at] = from_f32<T>(to_f32(grad_y[at]) * slope);
+      again[at] = from_f32<T>(y.x);
     } else {
       again[at] = from_f32<T>(x);
     }
@@ -259,6 +352,7 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 Rows make_rows(int64_t M, int64_t C) {
   Rows r{};
   r.per_row = uint32_t((C + kGroup - 1) / kGroup);
+  r.whole = C % kGroup == 0;
   r.groups = M * int64_t(r.per_row);
   r.div = DivMod32::make(r.per_row);
   r.C = int(C);
@@ -267,7 +361,7 @@ Rows make_rows(int64_t M, int64_t C) {
 
 unsigned grid_for(int64_t groups, int per_block) {
   const int64_t want = (groups + per_block - 1) / per_block;
-  const int64_t most = int64_t(sm_count()) * 64;
+  const int64_t most = int64_t(sm_count()) * 16;
   return unsigned(want < most ? want : most);
 }
 

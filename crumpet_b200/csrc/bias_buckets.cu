@@ -17,6 +17,8 @@
 // the gathers, which are all latency, go out together.  The warps of a CTA take neighbouring
 // items, whose pairs are neighbours in memory, so the sectors that one gather opens serve the
 // others from L1.  Buckets of several items are finished by a second kernel.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -25,7 +27,8 @@ namespace crumpet {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnit = 8;  // heads (or slabs) that a warp gathers together
+constexpr int kUnit = 8;   // heads (or slabs) that a warp gathers together
+constexpr int kGradThreads = 512;  // 16 neighbouring items per CTA share the sectors in L1
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
@@ -89,26 +92,37 @@ struct GradBuckets {
 // One warp per item and kUnit heads (SLABS: per item and head, kUnit slabs at a time).  An item
 // whose bucket is whole writes the table's gradient, the others their part: partial[item, h].
 template <typename G, typename O, bool SLABS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kGradThreads)
 bias_grad_kernel(O* grad_table, float* partial, const G* grad, int slabs, GradBuckets b) {
   const int lane = threadIdx.x & 31;
-  const long long item = blockIdx.x * (long long)(kThreads / 32) + (threadIdx.x >> 5);
+  const long long item = blockIdx.x * (long long)(kGradThreads / 32) + (threadIdx.x >> 5);
   if (item >= b.n_items) return;
   const int h = SLABS ? blockIdx.y : blockIdx.y * kUnit;
   const int bucket = b.items[3 * item], begin = b.items[3 * item + 1], end = b.items[3 * item + 2];
   const long long step = SLABS ? b.npairs * b.H : b.npairs;  // from unit to unit
   const int units = SLABS ? slabs : min(kUnit, b.H - h);
   float sum[kUnit] = {};
-  for (int u0 = 0; u0 < units; u0 += kUnit) {
-    const G* src = grad + h * b.npairs + u0 * step;
-#pragma unroll 2
-    for (int e = begin + lane; e < end; e += 32) {
-      const G* from = src + b.order[e];
+  // N rounds of 32 pairs, all their places read at once
+  auto rounds = [&](auto n_tag, int e0) {
+    constexpr int n = decltype(n_tag)::value;
+    int at[n];
 #pragma unroll
-      for (int u = 0; u < kUnit; ++u)
-        if (u0 + u < units) sum[u] += to_float(from[u * step]);
+    for (int r = 0; r < n; ++r) at[r] = e0 + 32 * r < end ? b.order[e0 + 32 * r] : -1;
+    for (int u0 = 0; u0 < units; u0 += kUnit) {
+      const G* src = grad + h * b.npairs + u0 * step;
+#pragma unroll
+      for (int u = 0; u < kUnit; ++u) {
+        if (u0 + u >= units) break;
+#pragma unroll
+        for (int r = 0; r < n; ++r)
+          if (at[r] >= 0) sum[u] += to_float(__ldg(src + u * step + at[r]));
+      }
     }
-  }
+  };
+  int e = begin;
+  for (; end - e > 64; e += 256) rounds(std::integral_constant<int, 8>{}, e + lane);
+  if (end - e > 32) rounds(std::integral_constant<int, 2>{}, e + lane);
+  else if (end - e > 0) rounds(std::integral_constant<int, 1>{}, e + lane);
   if constexpr (SLABS) {
 #pragma unroll
     for (int u = 1; u < kUnit; ++u) sum[0] += sum[u];
@@ -178,13 +192,14 @@ template <typename G, typename O>
 int launch_grad(const BiasGradArgs& a, cudaStream_t stream) {
   GradBuckets b{a.order, a.items, a.multi, a.n_items, a.n_multi, a.npairs, int(a.H)};
   const int per = kThreads / 32;
-  const unsigned blocks = unsigned((a.n_items + per - 1) / per);
+  constexpr int items = kGradThreads / 32;
+  const unsigned blocks = unsigned((a.n_items + items - 1) / items);
   if (a.slabs > 1)
-    bias_grad_kernel<G, O, true><<<dim3(blocks, unsigned(a.H)), kThreads, 0, stream>>>(
+    bias_grad_kernel<G, O, true><<<dim3(blocks, unsigned(a.H)), kGradThreads, 0, stream>>>(
         static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), int(a.slabs), b);
   else
     bias_grad_kernel<G, O, false>
-        <<<dim3(blocks, unsigned((a.H + kUnit - 1) / kUnit)), kThreads, 0, stream>>>(
+        <<<dim3(blocks, unsigned((a.H + kUnit - 1) / kUnit)), kGradThreads, 0, stream>>>(
             static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), 1, b);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "relative position bias gradient launch");

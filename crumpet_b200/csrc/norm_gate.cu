@@ -46,6 +46,7 @@ struct Args {
   const float* pre_b;
   long long M;
   long long rows_per_sample;
+  DivMod32 by_sample;  // by rows_per_sample, for rows that fit 32 bits
   int C, P;
   float eps, inv_c;
 };
@@ -83,24 +84,18 @@ struct Lane {
   __device__ __forceinline__ int col(int k) const { return VEC ? 8 * lane + k : lane + k * P; }
   __device__ __forceinline__ bool has(int k) const { return VEC ? 8 * lane < C : col(k) < C; }
 
+  // the lane's values of a row as they are stored (0 past the row or the last channel)
   template <typename T>
-  __device__ __forceinline__ void load(const T* row, bool in, float (&x)[8]) const {
+  __device__ __forceinline__ void fetch(const T* row, bool in, Pack8<T>& w) const {
     if constexpr (VEC) {
-      Pack8<T> w;
-      if (in && has(0)) {
 #pragma unroll
-        for (int k = 0; k < int(sizeof(w)) / 16; ++k)
-          reinterpret_cast<uint4*>(&w)[k] =
-              ldg_stream(reinterpret_cast<const uint4*>(row + 8 * lane) + k);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = to_f32(w.v[k]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 0.f;
-      }
+      for (int k = 0; k < int(sizeof(w)) / 16; ++k)
+        reinterpret_cast<uint4*>(&w)[k] =
+            in && has(0) ? ldg_stream(reinterpret_cast<const uint4*>(row + 8 * lane) + k)
+                         : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = in && has(k) ? to_f32(row[col(k)]) : 0.f;
+      for (int k = 0; k < 8; ++k) w.v[k] = in && has(k) ? row[col(k)] : from_f32<T>(0.f);
     }
   }
   template <typename T>
@@ -136,6 +131,19 @@ struct Lane {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void unpack(const Pack8<T>& w, float (&x)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = to_f32(w.v[k]);
+}
+
+// The row's factor: 1, or its sample's.
+__device__ __forceinline__ float row_factor(const Args& a, long long row, bool in) {
+  if (a.row_scale == nullptr || !in) return 1.f;
+  return __ldg(a.row_scale + (a.M <= 0xffffffffLL ? (long long)a.by_sample.div(uint32_t(row))
+                                                  : row / a.rows_per_sample));
+}
+
 // Sums of two values over the P lanes of a row.  BLOCK: the row spans warps of the CTA, whose
 // parts meet in shared memory (every thread of the CTA takes part).
 template <bool BLOCK>
@@ -160,42 +168,64 @@ __device__ __forceinline__ float2 row_sum(float a, float b, int P, float2* sh) {
   return make_float2(a, b);
 }
 
-// x -> x^ = (x - mean) rstd; 0 in the lane's channels past C
-template <bool VEC, bool BLOCK>
-__device__ __forceinline__ float normalise(float (&x)[8], const Lane<VEC>& ln, const Args& a,
-                                           float2* sh) {
-  float s = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) s += x[k];
-  const float mean = row_sum<BLOCK>(s, 0.f, a.P, sh).x * a.inv_c;
-  float q = 0.f;
+// x -> x^ = (x - mean) rstd, 0 in the lane's channels past C, for one or two rows' values whose
+// sums go together; the rstds.  Two passes: the variance is of the centred values.
+template <bool VEC, bool BLOCK, bool TWO>
+__device__ __forceinline__ float2 normalise(float (&x)[8], float (&y)[8], const Lane<VEC>& ln,
+                                            const Args& a, float2* sh) {
+  float s = 0.f, t = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    x[k] = ln.has(k) ? x[k] - mean : 0.f;
-    q = fmaf(x[k], x[k], q);
+    s += x[k];
+    if constexpr (TWO) t += y[k];
   }
-  const float var = row_sum<BLOCK>(q, 0.f, a.P, sh).x * a.inv_c;
-  const float rstd = 1.f / sqrtf(var + a.eps);
+  const float2 mean = row_sum<BLOCK>(s, t, a.P, sh);
+  s = t = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] *= rstd;
+  for (int k = 0; k < 8; ++k) {
+    x[k] = ln.has(k) ? fmaf(-mean.x, a.inv_c, x[k]) : 0.f;
+    s = fmaf(x[k], x[k], s);
+    if constexpr (TWO) {
+      y[k] = ln.has(k) ? fmaf(-mean.y, a.inv_c, y[k]) : 0.f;
+      t = fmaf(y[k], y[k], t);
+    }
+  }
+  const float2 var = row_sum<BLOCK>(s, t, a.P, sh);
+  const float2 rstd = make_float2(1.f / sqrtf(fmaf(var.x, a.inv_c, a.eps)),
+                                  TWO ? 1.f / sqrtf(fmaf(var.y, a.inv_c, a.eps)) : 0.f);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    x[k] *= rstd.x;
+    if constexpr (TWO) y[k] *= rstd.y;
+  }
   return rstd;
 }
 
+// Both kernels fetch a row ahead: its loads are in flight through the sums and shuffles of the
+// row before.
 template <typename T, typename R, bool VEC, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_forward_kernel(const Args a) {
   __shared__ float2 sh[16];
   const int per_cta = blockDim.x / a.P;
   const Lane<VEC> ln{int(threadIdx.x) % a.P, a.P, a.C};
-  for (long long r0 = blockIdx.x * (long long)per_cta; r0 < a.M;
-       r0 += (long long)gridDim.x * per_cta) {
-    const long long row = r0 + threadIdx.x / a.P;
+  const long long step = (long long)gridDim.x * per_cta;
+  long long row = blockIdx.x * (long long)per_cta + threadIdx.x / a.P;
+  Pack8<T> yp;
+  Pack8<R> rp;
+  ln.fetch(static_cast<const T*>(a.branch) + row * a.C, row < a.M, yp);
+  ln.fetch(static_cast<const R*>(a.residual) + row * a.C, row < a.M, rp);
+  for (long long r0 = blockIdx.x * (long long)per_cta; r0 < a.M; r0 += step, row += step) {
     const bool in = row < a.M;
     float y[8], r[8], w[8], b[8];
-    ln.load(static_cast<const T*>(a.branch) + row * a.C, in, y);
-    ln.load(static_cast<const R*>(a.residual) + row * a.C, in, r);
-    const float s = a.row_scale && in ? __ldg(a.row_scale + row / a.rows_per_sample) : 1.f;
+    unpack(yp, y);
+    unpack(rp, r);
+    if (r0 + step < a.M) {
+      ln.fetch(static_cast<const T*>(a.branch) + (row + step) * a.C, row + step < a.M, yp);
+      ln.fetch(static_cast<const R*>(a.residual) + (row + step) * a.C, row + step < a.M, rp);
+    }
+    const float s = row_factor(a, row, in);
     if (a.post_w) {
-      normalise<VEC, BLOCK>(y, ln, a, sh);
+      normalise<VEC, BLOCK, false>(y, y, ln, a, sh);
       ln.param(a.post_w, w);
       ln.param(a.post_b, b);
 #pragma unroll
@@ -211,7 +241,7 @@ __global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_forward_ker
     for (int k = 0; k < 8; ++k) r[k] = to_f32(from_f32<R>(fmaf(y[k], s, r[k])));
     ln.store(static_cast<R*>(a.out) + row * a.C, in, r);
     if (a.pre_w) {
-      normalise<VEC, BLOCK>(r, ln, a, sh);
+      normalise<VEC, BLOCK, false>(r, r, ln, a, sh);
       ln.param(a.pre_w, w);
       ln.param(a.pre_b, b);
 #pragma unroll
@@ -221,28 +251,59 @@ __global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_forward_ker
   }
 }
 
+// What a lane reads of a row backward
+template <typename T, typename R, bool VEC>
+struct BackRow {
+  Pack8<R> t, x;  // grad_out, out
+  Pack8<T> g, y;  // grad_normed, branch
+  __device__ __forceinline__ void fetch(const Args& a, const Lane<VEC>& ln, long long row,
+                                        bool need_branch) {
+    const bool in = row < a.M;
+    const long long at = row * a.C;
+    ln.fetch(static_cast<const R*>(a.grad_out) + at, in, t);
+    if (a.pre_w) {
+      ln.fetch(static_cast<const R*>(a.out) + at, in, x);
+      ln.fetch(static_cast<const T*>(a.grad_normed) + at, in, g);
+    }
+    if (need_branch) ln.fetch(static_cast<const T*>(a.branch) + at, in, y);
+  }
+};
+
 template <typename T, typename R, bool VEC, bool BLOCK, bool POST>
-__global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_backward_kernel(const Args a) {
+__global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256, BLOCK ? 1 : 2)
+norm_gate_backward_kernel(const Args a) {
   __shared__ float2 sh[16];
   __shared__ float cols[kMaxLanes * 8];
   const int per_cta = blockDim.x / a.P;
   const Lane<VEC> ln{int(threadIdx.x) % a.P, a.P, a.C};
   const bool need_branch = POST || a.gate != nullptr;
+  const long long step = (long long)gridDim.x * per_cta;
+  long long row = blockIdx.x * (long long)per_cta + threadIdx.x / a.P;
   float sum[kSums][8] = {};
-  for (long long r0 = blockIdx.x * (long long)per_cta; r0 < a.M;
-       r0 += (long long)gridDim.x * per_cta) {
-    const long long row = r0 + threadIdx.x / a.P;
+  BackRow<T, R, VEC> ahead;
+  ahead.fetch(a, ln, row, need_branch);
+  for (long long r0 = blockIdx.x * (long long)per_cta; r0 < a.M; r0 += step, row += step) {
     const bool in = row < a.M;
-    float t[8], x[8], g[8], y[8], w[8], b[8];
-    ln.load(static_cast<const R*>(a.grad_out) + row * a.C, in, t);
+    float t[8], x[8], g[8], y[8], w[8];
+    unpack(ahead.t, t);
     if (a.pre_w) {
-      ln.load(static_cast<const R*>(a.out) + row * a.C, in, x);
-      ln.load(static_cast<const T*>(a.grad_normed) + row * a.C, in, g);
+      unpack(ahead.x, x);
+      unpack(ahead.g, g);
     }
-    if (need_branch) ln.load(static_cast<const T*>(a.branch) + row * a.C, in, y);
-    const float s = a.row_scale && in ? __ldg(a.row_scale + row / a.rows_per_sample) : 1.f;
+    if (need_branch) unpack(ahead.y, y);
+    if (r0 + step < a.M) ahead.fetch(a, ln, row + step, need_branch);
+    const float s = row_factor(a, row, in);
+    float2 rstd = make_float2(0.f, 0.f);  // of out and of branch
+    if constexpr (POST) {
+      if (a.pre_w) {
+        rstd = normalise<VEC, BLOCK, true>(x, y, ln, a, sh);
+      } else {
+        rstd.y = normalise<VEC, BLOCK, false>(y, y, ln, a, sh).x;
+      }
+    } else if (a.pre_w) {
+      rstd = normalise<VEC, BLOCK, false>(x, x, ln, a, sh);
+    }
     if (a.pre_w) {
-      const float rstd = normalise<VEC, BLOCK>(x, ln, a, sh);
       ln.param(a.pre_w, w);
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -256,27 +317,28 @@ __global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_backward_ke
       const float2 m = row_sum<BLOCK>(s1, s2, a.P, sh);
       const float m1 = m.x * a.inv_c, m2 = m.y * a.inv_c;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = fmaf(g[k] - m1 - x[k] * m2, rstd, t[k]);
+      for (int k = 0; k < 8; ++k) t[k] = fmaf(g[k] - m1 - x[k] * m2, rstd.x, t[k]);
     }
     ln.store(static_cast<R*>(a.grad_residual) + row * a.C, in, t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) t[k] *= s;
-    float rstd = 0.f;
-    if constexpr (POST) {
-      rstd = normalise<VEC, BLOCK>(y, ln, a, sh);
-      ln.param(a.post_w, w);
-      ln.param(a.post_b, b);
-    }
     if (a.gate) {
       float q[8];
+      if constexpr (POST) {
+        ln.param(a.post_w, w);
+        ln.param(a.post_b, q);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[0][k] = fmaf(t[k], fmaf(y[k], w[k], q[k]), sum[0][k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[0][k] = fmaf(t[k], y[k], sum[0][k]);
+      }
       ln.param(a.gate, q);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        sum[0][k] = fmaf(t[k], POST ? fmaf(y[k], w[k], b[k]) : y[k], sum[0][k]);
-        t[k] *= q[k];
-      }
+      for (int k = 0; k < 8; ++k) t[k] *= q[k];
     }
     if constexpr (POST) {
+      ln.param(a.post_w, w);
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -289,7 +351,7 @@ __global__ void __launch_bounds__(BLOCK ? kMaxLanes : 256) norm_gate_backward_ke
       const float2 m = row_sum<BLOCK>(s1, s2, a.P, sh);
       const float m1 = m.x * a.inv_c, m2 = m.y * a.inv_c;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = (t[k] - m1 - y[k] * m2) * rstd;
+      for (int k = 0; k < 8; ++k) t[k] = (t[k] - m1 - y[k] * m2) * rstd.y;
     }
     ln.store(static_cast<T*>(a.grad_branch) + row * a.C, in, t);
   }
@@ -388,6 +450,7 @@ Args make_args(const NormGateArgs& n) {
   a.pre_b = n.pre_b;
   a.M = n.M;
   a.rows_per_sample = n.samples > 0 ? n.M / n.samples : 1;
+  if (a.rows_per_sample <= 0xffffffffLL) a.by_sample = DivMod32::make(uint32_t(a.rows_per_sample));
   a.C = int(n.C);
   a.P = lanes_for(n.C);
   a.eps = n.eps;
@@ -400,7 +463,7 @@ int forward(const NormGateArgs& n, cudaStream_t stream) {
   const Args a = make_args(n);
   const int threads = threads_for(a.P);
   const int64_t tiles = (a.M + threads / a.P - 1) / (threads / a.P);
-  const int64_t most = int64_t(sm_count()) * 64;
+  const int64_t most = int64_t(sm_count()) * 8;
   const unsigned grid = unsigned(tiles < most ? tiles : most);
   const bool vec = a.C % 8 == 0 && aligned16(a.branch) && aligned16(a.residual) &&
                    aligned16(a.out) && aligned16(a.normed) && aligned16(a.gate) &&

@@ -37,7 +37,7 @@ from .fused_attention import (_ATTN_DTYPES, head_dim_supported, swin_window_atte
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 GROUP = 32  # neighbouring channels that share one scale of an 8-bit checkpoint
 MAX_CHANNELS = 4096  # of norm_gate_residual
-_ITEM = 512  # most pairs of one bucket that one warp sums
+_ITEM = 512  # most pairs of one bucket that one warp sums (half of it where buckets are longer)
 
 
 def _require_cuda(what: str, *tensors) -> None:
@@ -107,12 +107,15 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
     order = torch.sort(flat, stable=True).indices
     count = torch.bincount(flat, minlength=num_buckets)
     begin = torch.cumsum(count, 0) - count
-    parts = torch.clamp((count + _ITEM - 1) // _ITEM, min=1)  # an empty bucket has one item too
+    # a 7x7x7 window's buckets (up to 343 pairs) are one item each, so nothing is to be joined;
+    # long buckets are cut finer, for more warps
+    size = _ITEM if int(count.max()) <= _ITEM else _ITEM // 2
+    parts = torch.clamp((count + size - 1) // size, min=1)  # an empty bucket has one item too
     bucket = torch.repeat_interleave(torch.arange(num_buckets, device=index.device), parts)
     first = torch.cumsum(parts, 0) - parts
     part = torch.arange(bucket.numel(), device=index.device) - first[bucket]
-    lo = begin[bucket] + part * _ITEM
-    hi = torch.minimum(lo + _ITEM, (begin + count)[bucket])
+    lo = begin[bucket] + part * size
+    hi = torch.minimum(lo + size, (begin + count)[bucket])
     several = parts > 1
     items = torch.stack((torch.where(several[bucket], -1, bucket), lo, hi), 1)
     which = torch.nonzero(several).reshape(-1)

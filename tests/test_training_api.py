@@ -38,7 +38,7 @@ def test_bucket_plan():
     _check_plan(torch.randint(0, 7, (31, 17), generator=g), 7)
     _check_plan(torch.randint(0, 50, (3, 5), generator=g), 60)  # empty buckets
     plan = _check_plan(torch.zeros((60, 60), dtype=torch.int32), 2)  # one long bucket, one empty
-    assert plan.multi.tolist() == [[0, 0, -(-3600 // training._ITEM)]]
+    assert plan.multi.tolist() == [[0, 0, -(-3600 // (training._ITEM // 2))]]
     _check_plan(torch.zeros((0, 3), dtype=torch.long), 2)
     index = torch.arange(12).view(3, 4)
     plan = _check_plan(index[:, :2], 12)  # a slice, as of a clamped window

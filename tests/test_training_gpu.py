@@ -565,6 +565,16 @@ def test_gelu_checkpoint_overflow_reads_back_as_nan(bad, c):
     assert torch.equal(grad_x.isnan(), hit) and torch.equal(again.isnan(), hit)
 
 
+def test_gelu_of_infinities():
+    """The limits: inf and 0 (torch's product gives NaN for -inf); NaN stays NaN."""
+    inf, nan = float("inf"), float("nan")
+    for c in (32, 31):
+        x = torch.zeros(1, c, device="cuda")
+        x[0, :3] = torch.tensor([inf, -inf, nan])
+        y, _ = crumpet.gelu_checkpoint(x)
+        assert y[0, 0] == inf and y[0, 1] == 0 and y[0, 2].isnan() and not y[0, 3:].any()
+
+
 def test_gelu_checkpoint_against_differences():
     """grad_x is the slope of gelu at the kept input: differences in 64 bits at 2^-10, an error
     of h^2 f'''/6 below 1e-6."""
