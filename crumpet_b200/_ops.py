@@ -140,7 +140,7 @@ def capi() -> ctypes.CDLL:
         lib.crumpet_relative_position_bias.argtypes = [vp, i32, vp, i32, i64, i64, vp, i64, vp]
         lib.crumpet_relative_position_bias.restype = i32
         lib.crumpet_relative_position_bias_backward.argtypes = [
-            vp, i32, i64, vp, i32, i64, vp, i64, vp, i64, vp, i64, vp, vp]
+            vp, i32, i64, vp, i32, vp, i64, vp, i64, vp, i64, vp, vp]
         lib.crumpet_relative_position_bias_backward.restype = i32
         lib.crumpet_window_attention_backward_shares.argtypes = [i64] * 4 + [i32]
         lib.crumpet_window_attention_backward_shares.restype = i64

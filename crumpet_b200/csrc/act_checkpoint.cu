@@ -268,37 +268,21 @@ kept_use_kernel(T* grad_x, T* again, const T* grad_y, const int8_t* kept, const 
                 Rows r) {
   const int part = threadIdx.x & 3;
   const long long step = (long long)gridDim.x * (kThreads / 4);
-  struct Part {
-    Pack8<T> g;
-    uint2 w;
-    uint32_t code;
-  };
-  auto load = [&](const Place& q, long long grp, Part& d) {
-    if (!q.in) return;
-    d.w = ldg_stream(reinterpret_cast<const uint2*>(kept + q.at));
-    if constexpr (GRAD) load8(grad_y + q.at, d.g);
-    d.code = __ldg(scales + grp);
-  };
-  long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
-  // the next group's loads are in flight through this one's arithmetic
-  Place q = find_part(r, grp, part);
-  Part ahead = {};
-  load(q, grp, ahead);
-  for (; grp < r.groups; grp += step) {
-    const Part now = ahead;
-    const Place here = q;
-    q = find_part(r, grp + step, part);
-    load(q, grp + step, ahead);
-    if (!here.in) continue;
-    const long long at = here.at;
-    const uint2 w = now.w;
-    const float s = code_step(now.code);
+  for (long long grp = blockIdx.x * (long long)(kThreads / 4) + (threadIdx.x >> 2);
+       grp < r.groups; grp += step) {
+    const Place q = find_part(r, grp, part);
+    if (!q.in) continue;
+    const long long at = q.at;
+    const uint2 w = ldg_stream(reinterpret_cast<const uint2*>(kept + at));
+    Pack8<T> gw;
+    if constexpr (GRAD) load8(grad_y + at, gw);
+    const float s = code_step(__ldg(scales + grp));
     float a[8];
     restore4(w.x, s, a);
     restore4(w.y, s, a + 4);
     float g[8];
     if constexpr (GRAD) {
-      unpack8(now.g, g);
+      unpack8(gw, g);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         float2 y;
@@ -359,9 +343,9 @@ Rows make_rows(int64_t M, int64_t C) {
   return r;
 }
 
-unsigned grid_for(int64_t groups, int per_block) {
+unsigned grid_for(int64_t groups, int per_block, int per_sm) {
   const int64_t want = (groups + per_block - 1) / per_block;
-  const int64_t most = int64_t(sm_count()) * 16;
+  const int64_t most = int64_t(sm_count()) * per_sm;
   return unsigned(want < most ? want : most);
 }
 
@@ -370,10 +354,10 @@ int keep(void* y, int8_t* kept, uint8_t* scales, const void* x, int64_t M, int64
          cudaStream_t stream) {
   const Rows r = make_rows(M, C);
   if (C % 8 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(kept, 8))
-    gelu_keep_kernel<T><<<grid_for(r.groups, kThreads / 4), kThreads, 0, stream>>>(
+    gelu_keep_kernel<T><<<grid_for(r.groups, kThreads / 4, 16), kThreads, 0, stream>>>(
         static_cast<T*>(y), kept, scales, static_cast<const T*>(x), r);
   else
-    gelu_keep_any_kernel<T><<<grid_for(r.groups, kThreads / 32), kThreads, 0, stream>>>(
+    gelu_keep_any_kernel<T><<<grid_for(r.groups, kThreads / 32, 64), kThreads, 0, stream>>>(
         static_cast<T*>(y), kept, scales, static_cast<const T*>(x), r);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "gelu checkpoint launch");
@@ -385,11 +369,11 @@ int use(void* grad_x, void* again, const void* grad_y, const int8_t* kept, const
   const Rows r = make_rows(M, C);
   if (C % 8 == 0 && aligned(grad_x, 16) && aligned(again, 16) && aligned(grad_y, 16) &&
       aligned(kept, 8))
-    kept_use_kernel<T, GRAD><<<grid_for(r.groups, kThreads / 4), kThreads, 0, stream>>>(
+    kept_use_kernel<T, GRAD><<<grid_for(r.groups, kThreads / 4, 64), kThreads, 0, stream>>>(
         static_cast<T*>(grad_x), static_cast<T*>(again), static_cast<const T*>(grad_y), kept,
         scales, r);
   else
-    kept_use_any_kernel<T, GRAD><<<grid_for(r.groups, kThreads / 32), kThreads, 0, stream>>>(
+    kept_use_any_kernel<T, GRAD><<<grid_for(r.groups, kThreads / 32, 64), kThreads, 0, stream>>>(
         static_cast<T*>(grad_x), static_cast<T*>(again), static_cast<const T*>(grad_y), kept,
         scales, r);
   const cudaError_t e = cudaGetLastError();

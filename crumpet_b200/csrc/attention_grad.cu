@@ -1113,6 +1113,22 @@ int make_maps(Maps* m, const AttnGradArgs& a, bool of_rows_kernel, int cols, int
   return make_map(kv[1], q + 2 * width, a, 3 * width, kv_box);
 }
 
+// parts[0][i] = sum over s of parts[s][i]: 64 elements per CTA, four threads each taking a quarter
+// of the parts (8 loads in flight), joined in a fixed order.
+__global__ void __launch_bounds__(256) sum_shares_kernel(float* parts, int shares, long long n) {
+  __shared__ float quarter[3][64];
+  const int x = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const long long i = blockIdx.x * 64LL + x;
+  float sum = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (int s = q; s < shares; s += 4) sum += parts[s * n + i];
+  }
+  if (q > 0) quarter[q - 1][x] = sum;
+  __syncthreads();
+  if (q == 0 && i < n) parts[i] = sum + quarter[0][x] + quarter[1][x] + quarter[2][x];
+}
+
 int sm_count() {
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
@@ -1188,6 +1204,13 @@ int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N) {
   p.N = int(N);
   split(&p, kBR, N <= 64 ? 4 : N <= 128 ? 2 : 1);  // RowsShape::MINB
   return p.S;
+}
+
+int launch_sum_shares(float* parts, int64_t shares, int64_t n, cudaStream_t stream) {
+  if (shares <= 1 || n == 0) return kOk;
+  sum_shares_kernel<<<unsigned((n + 63) / 64), 256, 0, stream>>>(parts, int(shares), n);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? kOk : set_cuda_error(e, "attention gradient sum launch");
 }
 
 int read_attention_grad_error(bool clear) {

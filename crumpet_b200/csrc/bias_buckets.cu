@@ -12,9 +12,8 @@
 //
 // Gradient: no atomics, so the sum's order never changes.  The caller sorted the pairs by
 // bucket once (`order`) and cut every bucket into items of a bounded number of pairs; one
-// warp sums an item in a fixed order, in fp32, for kUnit heads (or, of a gradient in several
-// slabs, for kUnit slabs of one head) at a time: a pair's place is read once for all of them and
-// the gathers, which are all latency, go out together.  The warps of a CTA take neighbouring
+// warp sums an item in a fixed order, in fp32, for kUnit heads at a time: a pair's place is read
+// once for all of them and the gathers, which are all latency, go out together.  The warps of a CTA take neighbouring
 // items, whose pairs are neighbours in memory, so the sectors that one gather opens serve the
 // others from L1.  Buckets of several items are finished by a second kernel.
 #include <type_traits>
@@ -27,7 +26,8 @@ namespace crumpet {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnit = 8;   // heads (or slabs) that a warp gathers together
+constexpr int kUnit = 4;   // heads that a warp gathers together
+constexpr int kJoinThreads = 1024;
 constexpr int kGradThreads = 512;  // 16 neighbouring items per CTA share the sectors in L1
 
 template <typename T>
@@ -89,68 +89,69 @@ struct GradBuckets {
   int H;
 };
 
-// One warp per item and kUnit heads (SLABS: per item and head, kUnit slabs at a time).  An item
-// whose bucket is whole writes the table's gradient, the others their part: partial[item, h].
-template <typename G, typename O, bool SLABS>
-__global__ void __launch_bounds__(kGradThreads)
-bias_grad_kernel(O* grad_table, float* partial, const G* grad, int slabs, GradBuckets b) {
+// One warp per item and kUnit heads.  An item whose bucket is whole writes the table's gradient,
+// the others their part: partial[item, h].
+template <typename G, typename O>
+__global__ void __launch_bounds__(kGradThreads, 4)
+bias_grad_kernel(O* grad_table, float* partial, const G* grad, GradBuckets b) {
   const int lane = threadIdx.x & 31;
   const long long item = blockIdx.x * (long long)(kGradThreads / 32) + (threadIdx.x >> 5);
   if (item >= b.n_items) return;
-  const int h = SLABS ? blockIdx.y : blockIdx.y * kUnit;
+  const int h = blockIdx.y * kUnit;
   const int bucket = b.items[3 * item], begin = b.items[3 * item + 1], end = b.items[3 * item + 2];
-  const long long step = SLABS ? b.npairs * b.H : b.npairs;  // from unit to unit
-  const int units = SLABS ? slabs : min(kUnit, b.H - h);
+  const int units = min(kUnit, b.H - h);
+  const G* src = grad + h * b.npairs;
   float sum[kUnit] = {};
-  // N rounds of 32 pairs, all their places read at once
+  // n rounds of 32 pairs, all their places read at once
   auto rounds = [&](auto n_tag, int e0) {
     constexpr int n = decltype(n_tag)::value;
     int at[n];
 #pragma unroll
-    for (int r = 0; r < n; ++r) at[r] = e0 + 32 * r < end ? b.order[e0 + 32 * r] : -1;
-    for (int u0 = 0; u0 < units; u0 += kUnit) {
-      const G* src = grad + h * b.npairs + u0 * step;
+    for (int r = 0; r < n; ++r) at[r] = e0 + 32 * r < end ? __ldg(b.order + e0 + 32 * r) : -1;
 #pragma unroll
-      for (int u = 0; u < kUnit; ++u) {
-        if (u0 + u >= units) break;
+    for (int u = 0; u < kUnit; ++u) {
+      if (u >= units) break;
 #pragma unroll
-        for (int r = 0; r < n; ++r)
-          if (at[r] >= 0) sum[u] += to_float(__ldg(src + u * step + at[r]));
-      }
+      for (int r = 0; r < n; ++r)
+        if (at[r] >= 0) sum[u] += to_float(__ldg(src + u * b.npairs + at[r]));
     }
   };
   int e = begin;
-  for (; end - e > 64; e += 256) rounds(std::integral_constant<int, 8>{}, e + lane);
+  for (; end - e > 64; e += 128) rounds(std::integral_constant<int, 4>{}, e + lane);
   if (end - e > 32) rounds(std::integral_constant<int, 2>{}, e + lane);
   else if (end - e > 0) rounds(std::integral_constant<int, 1>{}, e + lane);
-  if constexpr (SLABS) {
 #pragma unroll
-    for (int u = 1; u < kUnit; ++u) sum[0] += sum[u];
-  }
-#pragma unroll
-  for (int u = 0; u < (SLABS ? 1 : kUnit); ++u) {
+  for (int u = 0; u < kUnit; ++u) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum[u] += __shfl_xor_sync(~0u, sum[u], o);
-    if (lane == u && u < (SLABS ? 1 : units)) {
+    if (lane == u && u < units) {
       if (bucket >= 0) grad_table[(long long)bucket * b.H + h + u] = from_float<O>(sum[u]);
       else partial[item * b.H + h + u] = sum[u];
     }
   }
 }
 
+// One CTA per bucket of several items and 32 heads: a lane per head, the items dealt to the warps.
 template <typename O>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kJoinThreads)
 bias_grad_join_kernel(O* grad_table, const float* partial, GradBuckets b) {
-  const int lane = threadIdx.x & 31;
-  const long long k = blockIdx.x * (long long)(kThreads / 32) + (threadIdx.x >> 5);
-  const int h = blockIdx.y;
-  if (k >= b.n_multi) return;
+  __shared__ float part[kJoinThreads / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long k = blockIdx.x;
+  const int h = blockIdx.y * 32 + lane;
   const int bucket = b.multi[3 * k], first = b.multi[3 * k + 1], last = b.multi[3 * k + 2];
   float sum = 0.f;
-  for (int i = first + lane; i < last; i += 32) sum += partial[(long long)i * b.H + h];
+  if (h < b.H) {
+#pragma unroll 8
+    for (int i = first + warp; i < last; i += kJoinThreads / 32)
+      sum += __ldg(partial + (long long)i * b.H + h);
+  }
+  part[warp][lane] = sum;
+  __syncthreads();
+  if (warp != 0 || h >= b.H) return;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (lane == 0) grad_table[(long long)bucket * b.H + h] = from_float<O>(sum);
+  for (int w = 1; w < kJoinThreads / 32; ++w) sum += part[w][lane];
+  grad_table[(long long)bucket * b.H + h] = from_float<O>(sum);
 }
 
 template <typename T, typename O, int V, int PP>
@@ -191,21 +192,16 @@ int gather_out(void* bias, int out_dtype, const void* table, const int* pairs, i
 template <typename G, typename O>
 int launch_grad(const BiasGradArgs& a, cudaStream_t stream) {
   GradBuckets b{a.order, a.items, a.multi, a.n_items, a.n_multi, a.npairs, int(a.H)};
-  const int per = kThreads / 32;
   constexpr int items = kGradThreads / 32;
-  const unsigned blocks = unsigned((a.n_items + items - 1) / items);
-  if (a.slabs > 1)
-    bias_grad_kernel<G, O, true><<<dim3(blocks, unsigned(a.H)), kGradThreads, 0, stream>>>(
-        static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), int(a.slabs), b);
-  else
-    bias_grad_kernel<G, O, false>
-        <<<dim3(blocks, unsigned((a.H + kUnit - 1) / kUnit)), kGradThreads, 0, stream>>>(
-            static_cast<O*>(a.grad_table), a.partial, static_cast<const G*>(a.grad), 1, b);
+  bias_grad_kernel<G, O><<<dim3(unsigned((a.n_items + items - 1) / items),
+                                unsigned((a.H + kUnit - 1) / kUnit)),
+                           kGradThreads, 0, stream>>>(static_cast<O*>(a.grad_table), a.partial,
+                                                      static_cast<const G*>(a.grad), b);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "relative position bias gradient launch");
   if (a.n_multi > 0) {
-    bias_grad_join_kernel<O><<<dim3(unsigned((a.n_multi + per - 1) / per), unsigned(a.H)),
-                               kThreads, 0, stream>>>(static_cast<O*>(a.grad_table), a.partial, b);
+    bias_grad_join_kernel<O><<<dim3(unsigned(a.n_multi), unsigned((a.H + 31) / 32)), kJoinThreads,
+                               0, stream>>>(static_cast<O*>(a.grad_table), a.partial, b);
     e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(e, "relative position bias gradient join launch");
   }

@@ -447,8 +447,7 @@ int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
 }
 
 int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, int64_t H,
-                                            const void* grad, int grad_dtype, int64_t slabs,
-                                            const int* order, int64_t npairs, const int* items,
+                                            const void* grad, int grad_dtype, const int* order, int64_t npairs, const int* items,
                                             int64_t n_items, const int* multi, int64_t n_multi,
                                             float* partial, void* stream) {
   if (int e = check_dtype(table_dtype)) return e;
@@ -456,8 +455,9 @@ int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, i
   if (H < 0 || npairs < 0 || n_items < 0 || n_multi < 0)
     return set_error(kErrInvalid, "H, npairs, n_items and n_multi must be non-negative");
   if (H == 0 || n_items == 0) return kOk;
-  if (npairs > 0x7fffffff || H > 0xffff || n_items > 0x7fffffff || slabs < 0 || slabs > 0x7fffffff)
-    return set_error(kErrInvalid, "relative position bias: npairs, H, items or slabs out of range");
+  if (npairs > 0x7fffffff || H > 0xffff || n_items > 0x7fffffff ||
+      n_multi > 0x7fffffff)
+    return set_error(kErrInvalid, "relative position bias: npairs, H or items out of range");
   if (!grad_table || !items || (npairs > 0 && (!grad || !order)) ||
       (n_multi > 0 && (!multi || !partial)))
     return set_error(kErrInvalid, "null tensor pointer");
@@ -466,7 +466,6 @@ int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, i
   a.table_dtype = table_dtype;
   a.grad = grad;
   a.grad_dtype = grad_dtype;
-  a.slabs = slabs;
   a.npairs = npairs;
   a.H = H;
   a.order = order;
@@ -521,7 +520,7 @@ int crumpet_swin_window_attention_qkv_backward(
     return set_error(kErrInvalid, "too many windows x heads for one launch");
   if (!grad_bias) return set_error(kErrInvalid, "null tensor pointer");
   if (B == 0) {  // no window: no gradient of the bias
-    const cudaError_t e = cudaMemsetAsync(grad_bias, 0, size_t(shares * H * N * N) * sizeof(float),
+    const cudaError_t e = cudaMemsetAsync(grad_bias, 0, size_t(H * N * N) * sizeof(float),
                                           static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? kOk : set_cuda_error(e, "window attention backward memset");
   }
@@ -555,8 +554,10 @@ int crumpet_swin_window_attention_qkv_backward(
   a.shares = shares;
   a.scale = scale;
   a.dtype = dtype;
-  if (sized && (bits & 15u) == 0) return launch_attention_grad(a, static_cast<cudaStream_t>(stream));
-  return launch_attention_grad_simt(a, static_cast<cudaStream_t>(stream));
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  const bool tensor = sized && (bits & 15u) == 0;
+  if (int e = tensor ? launch_attention_grad(a, on) : launch_attention_grad_simt(a, on)) return e;
+  return launch_sum_shares(grad_bias, shares, H * N * N, on);
 }
 
 namespace {

@@ -135,8 +135,9 @@ int launch_window_attention_static_tiles(const AttnArgs& a, cudaStream_t stream)
 bool simt_attention_head_dim(int64_t head_dim);
 int launch_window_attention_simt(const AttnArgs& a, cudaStream_t stream);
 
-// Gradient of the packed-qkv window attention.  `grad_bias` receives `shares` parts of the
-// bias gradient, each [H, N, N] summed over the windows of that share; `stats` is scratch.
+// Gradient of the packed-qkv window attention.  `grad_bias` has room for `shares` parts of the
+// bias gradient, each [H, N, N] over the windows of that share; their sum is left in the first
+// (launch_sum_shares).  `stats` is scratch.
 struct AttnGradArgs {
   void* grad_qkv;        // [B, N, 3, H, head_dim]
   float* grad_bias;      // [shares, H, N, N]
@@ -156,18 +157,20 @@ int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
 int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N);
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
 int read_attention_grad_error(bool clear);
+// parts[0] = sum of parts[0 .. shares - 1], each of n floats
+int launch_sum_shares(float* parts, int64_t shares, int64_t n, cudaStream_t stream);
 int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream);
 
 // Relative-position bias by buckets: bias[h, p] = table[pairs[p], h] and the table's gradient
-// from `slabs` parts of grad [H, npairs].
+// from grad [H, npairs].
 int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
                                   const int* pairs, int64_t npairs, int64_t H, cudaStream_t stream);
 struct BiasGradArgs {
   void* grad_table;  // [T, H]
   int table_dtype;
-  const void* grad;  // [slabs, H, npairs]
+  const void* grad;  // [H, npairs]
   int grad_dtype;
-  int64_t slabs, npairs, H;
+  int64_t npairs, H;
   const int* order;  // [npairs] pairs sorted by bucket
   const int* items;  // [n_items][3]: bucket (-1: one of several items), begin, end
   const int* multi;  // [n_multi][3]: bucket of several items, first item, last item + 1

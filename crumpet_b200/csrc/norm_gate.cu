@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(1024) norm_gate_columns_kernel(Sums out, const
   const int c = blockIdx.x * 32 + tx;
   float s = 0.f;
   if (c < C)
+#pragma unroll 8
     for (int r = ty; r < ctas; r += 32) s += partial[((long long)q * ctas + r) * C + c];
   part[ty][tx] = s;
   __syncthreads();

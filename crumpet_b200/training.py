@@ -145,7 +145,7 @@ def _bias_forward(table, buckets, dtype):
 
 
 def _table_gradient(grad, heads, buckets, dtype):
-    """[buckets, heads] from grad [slabs *, heads, rows, cols]."""
+    """[buckets, heads] from grad [heads, rows, cols]."""
     grad_table = torch.empty((buckets.num_buckets, heads), dtype=dtype, device=grad.device)
     partial = None
     if buckets.multi.shape[0]:
@@ -284,7 +284,7 @@ def _attention_backward(grad_out, qkv, table, buckets, place):
         buckets.pairs, num_windows, window_size, shift_size, scale)
     _prof.count("swin_window_attention_qkv_backward")
     _prof.kernel_end(token)
-    return grad_qkv, _table_gradient(grad_bias, H, buckets, table.dtype)
+    return grad_qkv, _table_gradient(grad_bias[0], H, buckets, table.dtype)
 
 
 class _WindowAttention(torch.autograd.Function):

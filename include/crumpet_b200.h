@@ -396,14 +396,14 @@ CRUMPET_API int crumpet_roi_argmax(uint8_t* labels, float* logits, const float* 
  * (`order`, int32 [npairs]) and cut into items: int32 triples (bucket, begin, end) into order,
  * in the order of the buckets, every bucket (an empty one too) with one item at least.  A
  * bucket of several items is written as -1 in them and listed in `multi`, int32 triples
- * (bucket, first item, last item + 1); then `partial` is fp32 scratch [n_items, H].  grad is
- * the sum of `slabs` tensors [H, npairs], one after another.  Sums are fp32 in a fixed order.
+ * (bucket, first item, last item + 1); then `partial` is fp32 scratch [n_items, H].  Sums are
+ * fp32 in a fixed order.
  */
 CRUMPET_API int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
                                                int table_dtype, int64_t table_rows, int64_t H,
                                                const int* pairs, int64_t npairs, void* stream);
 CRUMPET_API int crumpet_relative_position_bias_backward(
-    void* grad_table, int table_dtype, int64_t H, const void* grad, int grad_dtype, int64_t slabs,
+    void* grad_table, int table_dtype, int64_t H, const void* grad, int grad_dtype,
     const int* order, int64_t npairs, const int* items, int64_t n_items, const int* multi,
     int64_t n_multi, float* partial, void* stream);
 
@@ -411,8 +411,8 @@ CRUMPET_API int crumpet_relative_position_bias_backward(
  * Gradient of crumpet_swin_window_attention_qkv: from grad_out [B, N, H * head_dim] and the
  * forward's qkv, table and geometry (arguments as there; pairs int32 [N, N] holds the buckets
  * index[:N, :N], every value in [0, table_rows)), writes grad_qkv [B, N, 3, H, head_dim] and
- * grad_bias fp32 [shares, H, N, N], whose sum over the shares is the gradient of the bias
- * (pass it on to crumpet_relative_position_bias_backward with slabs = shares).  `shares` is
+ * into the first [H, N, N] of grad_bias, fp32 [shares, H, N, N], the gradient of the bias (to
+ * pass on to crumpet_relative_position_bias_backward); the rest of it is scratch.  `shares` is
  * what crumpet_window_attention_backward_shares gives for these sizes; `stats` is fp32
  * scratch of B * H * (3 * N + 4) elements, 16-byte aligned.  The bias is used as the table has it (the forward rounds
  * it to dtype); the row statistics are taken again in fp32.  dtype, head_dim and N as for the

@@ -88,9 +88,9 @@ def test_c_abi_refuses_bad_arguments_without_touching_the_device():
     rejects(lib.crumpet_relative_position_bias(f, 0, f, 7, 5, 2, f, 9, null), 1, "float32")
     rejects(lib.crumpet_relative_position_bias(f, 0, f, 0, 0, 2, f, 9, null), 1, "table_rows")
     assert lib.crumpet_relative_position_bias(null, 0, null, 0, 5, 2, null, 0, null) == 0
-    rejects(lib.crumpet_relative_position_bias_backward(f, 0, 2, f, 0, 1, f, 9, null, 3, null, 0,
+    rejects(lib.crumpet_relative_position_bias_backward(f, 0, 2, f, 0, f, 9, null, 3, null, 0,
                                                         null, null), 1, "null")
-    rejects(lib.crumpet_relative_position_bias_backward(f, 0, 2, f, 0, 1, f, 9, f, 3, f, 1, null,
+    rejects(lib.crumpet_relative_position_bias_backward(f, 0, 2, f, 0, f, 9, f, 3, f, 1, null,
                                                         null), 1, "null")
 
     def backward(shares=1, ws=(7, 7, 7), ss=(0, 0, 0), dtype=2, B=2, H=3, N=343, d=16, scale=0.25,
