@@ -55,14 +55,6 @@ _OP_NAMES = (
     "patch_merge_norm_3d",
     "proj_out_norm_3d",
     "window_linear",
-    "relative_position_bias",
-    "relative_position_bias_backward",
-    "swin_window_attention_qkv_backward",
-    "norm_gate_residual",
-    "norm_gate_residual_backward",
-    "gelu_checkpoint",
-    "gelu_checkpoint_backward",
-    "restore_activation",
 )
 
 
@@ -84,6 +76,13 @@ def _register_fake_impls() -> None:
             register(f"crumpet_ops::{name}")(noop)
         except (RuntimeError, AttributeError, ValueError):
             pass  # already registered (a second package import in the same process)
+    from .training import FAKE_IMPLS  # the ops that return new tensors: their shapes
+
+    for name, fake in FAKE_IMPLS.items():
+        try:
+            register(f"crumpet_ops::{name}")(fake)
+        except (RuntimeError, AttributeError, ValueError):
+            pass
 
 
 _native.on_load(_register_fake_impls)

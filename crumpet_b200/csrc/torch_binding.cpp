@@ -4,9 +4,9 @@
 // (torch-ext/torch_binding.cpp:9-39), CUDA implementations only, plus
 // fused_swin_attention, which the reference exposes only as a Python/Triton
 // function (torch-ext/crumpet/fused_attention.py:149-226), and ops without a reference
-// counterpart.  Every impl checks
-// the tensors, takes the current stream and calls the C ABI in
-// libcrumpet_b200.so; ops never allocate (outputs are preallocated `Tensor!`).
+// counterpart.  Every impl checks the tensors, takes the current stream and calls the C ABI in
+// libcrumpet_b200.so; ops never allocate (outputs are preallocated `Tensor!`) but for the
+// training operators, which return new tensors.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -584,233 +584,361 @@ void roi_normalize(at::Tensor& logits, const at::Tensor& acc, const at::Tensor& 
 }
 
 // ---- training operators -------------------------------------------------------------
+//
+// These return new tensors (and take their scratch from the caching allocator): a training step
+// makes thousands of such calls, and checks and allocations cost several times as much in
+// Python.  Bad shapes and values raise ValueError, bad types TypeError.
 
-void check_int32(const at::Tensor& t, const char* name) {
-  check_cuda_contig(t, name);
-  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be an int32 tensor");
-}
+int64_t rows_of(const at::Tensor& t) { return t.numel() / t.size(-1); }
 
-void check_f32(const at::Tensor& t, int64_t n, const char* name) {
-  check_cuda_contig(t, name);
-  TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == n, name,
-              " must be a float32 tensor of ", n, " elements");
-}
-
-// The float32 [n] vector of an optional tensor, or null.
-float* optional_f32(const at::Tensor& ref, const c10::optional<at::Tensor>& t, int64_t n,
-                    const char* name) {
-  if (!t.has_value() || !t->defined()) return nullptr;
-  check_f32(*t, n, name);
-  same_device(ref, *t, name);
-  return t->data_ptr<float>();
-}
-
-void relative_position_bias(at::Tensor& bias, const at::Tensor& table, const at::Tensor& pairs) {
-  check_cuda_contig(bias, "bias");
-  check_cuda_contig(table, "table");
-  check_int32(pairs, "pairs");
-  TORCH_CHECK(table.dim() == 2, "table must be [buckets, heads]");
-  TORCH_CHECK(bias.numel() == pairs.numel() * table.size(1), "bias must be [heads, pairs]");
-  same_device(bias, table, "table");
-  same_device(bias, pairs, "pairs");
-  const c10::cuda::CUDAGuard guard(bias.device());
-  check_rc(crumpet_relative_position_bias(bias.data_ptr(), dtype_code(bias), table.data_ptr(),
-                                          dtype_code(table), table.size(0), table.size(1),
-                                          pairs.data_ptr<int>(), pairs.numel(), cur_stream(bias)));
-}
-
-void relative_position_bias_backward(at::Tensor& grad_table, const at::Tensor& grad,
-                                     const at::Tensor& order, const at::Tensor& items,
-                                     const at::Tensor& multi,
-                                     const c10::optional<at::Tensor>& partial) {
-  check_cuda_contig(grad_table, "grad_table");
-  check_cuda_contig(grad, "grad");
-  check_int32(order, "order");
-  check_int32(items, "items");
-  check_int32(multi, "multi");
-  TORCH_CHECK(grad_table.dim() == 2, "grad_table must be [buckets, heads]");
-  TORCH_CHECK(items.dim() == 2 && items.size(1) == 3 && multi.dim() == 2 && multi.size(1) == 3,
-              "items and multi must be [n, 3]");
-  const int64_t H = grad_table.size(1), pairs = order.numel();
-  TORCH_CHECK(grad.numel() == H * pairs, "grad must be [heads, pairs]");
-  same_device(grad_table, grad, "grad");
-  same_device(grad_table, order, "order");
-  same_device(grad_table, items, "items");
-  same_device(grad_table, multi, "multi");
-  float* part = optional_f32(grad_table, partial, items.size(0) * H, "partial");
-  const c10::cuda::CUDAGuard guard(grad_table.device());
-  check_rc(crumpet_relative_position_bias_backward(
-      grad_table.data_ptr(), dtype_code(grad_table), H, grad.data_ptr(), dtype_code(grad),
-      order.data_ptr<int>(), pairs, items.data_ptr<int>(), items.size(0), multi.data_ptr<int>(), multi.size(0), part,
-      cur_stream(grad_table)));
-}
-
-void swin_window_attention_qkv_backward(at::Tensor& grad_qkv, at::Tensor& grad_bias,
-                                        at::Tensor& stats, const at::Tensor& grad_out,
-                                        const at::Tensor& qkv, const at::Tensor& table,
-                                        const at::Tensor& pairs, at::IntArrayRef num_windows,
-                                        at::IntArrayRef window_size, at::IntArrayRef shift_size,
-                                        double scale) {
-  check_cuda_contig(grad_qkv, "grad_qkv");
-  check_cuda_contig(grad_out, "grad_out");
-  check_cuda_contig(qkv, "qkv");
-  check_cuda_contig(table, "table");
-  check_int32(pairs, "pairs");
-  TORCH_CHECK(qkv.dim() == 5 && qkv.size(2) == 3, "qkv must have shape [B, N, 3, H, head_dim]");
-  const int64_t B = qkv.size(0), N = qkv.size(1), H = qkv.size(3), Dh = qkv.size(4);
-  TORCH_CHECK(grad_qkv.sizes() == qkv.sizes() && grad_qkv.scalar_type() == qkv.scalar_type(),
-              "grad_qkv must have the shape and dtype of qkv");
-  TORCH_CHECK(grad_out.numel() == B * N * H * Dh && grad_out.scalar_type() == qkv.scalar_type(),
-              "grad_out must be [B, N, H * head_dim] in the dtype of qkv");
-  TORCH_CHECK(table.dim() == 2 && table.size(1) == H, "table must be [buckets, H]");
-  TORCH_CHECK(table.scalar_type() == at::kFloat || table.scalar_type() == qkv.scalar_type(),
-              "table must be float32 or of the dtype of qkv");
-  TORCH_CHECK(pairs.numel() == N * N, "pairs must be [N, N]");
-  check_cuda_contig(grad_bias, "grad_bias");
-  TORCH_CHECK(grad_bias.scalar_type() == at::kFloat && grad_bias.dim() == 4 &&
-                  grad_bias.size(1) == H && grad_bias.size(2) == N && grad_bias.size(3) == N,
-              "grad_bias must be a float32 [shares, H, N, N] tensor");
-  check_f32(stats, B * H * (3 * N + 4), "stats");
-  TORCH_CHECK(num_windows.size() == 3 && window_size.size() == 3 && shift_size.size() == 3,
-              "num_windows, window_size and shift_size take three values");
-  same_device(qkv, grad_qkv, "grad_qkv");
-  same_device(qkv, grad_bias, "grad_bias");
-  same_device(qkv, stats, "stats");
-  same_device(qkv, grad_out, "grad_out");
-  same_device(qkv, table, "table");
-  same_device(qkv, pairs, "pairs");
-  const c10::cuda::CUDAGuard guard(qkv.device());
-  check_rc(crumpet_swin_window_attention_qkv_backward(
-      grad_qkv.data_ptr(), grad_bias.data_ptr<float>(), stats.data_ptr<float>(),
-      grad_out.data_ptr(), qkv.data_ptr(), table.data_ptr(),
-      table.scalar_type() == at::kFloat ? 1 : 0, table.size(0), pairs.data_ptr<int>(),
-      grad_bias.size(0), num_windows[0], num_windows[1], num_windows[2], window_size[0],
-      window_size[1], window_size[2], shift_size[0], shift_size[1], shift_size[2],
-      dtype_code(qkv), B, H, N, Dh, static_cast<float>(scale), cur_stream(qkv)));
-}
-
-// Rows of `t` must be a contiguous [M, C] (any leading dims) of the dtype of `like`.
-void check_rows(const at::Tensor& ref, const at::Tensor& t, const at::Tensor& like,
-                const char* name) {
-  check_cuda_contig(t, name);
+void check_cuda(const at::Tensor& ref, const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   same_device(ref, t, name);
-  TORCH_CHECK(t.sizes() == ref.sizes() && t.scalar_type() == like.scalar_type(), name,
-              " must have the shape of branch and its stream's dtype");
 }
 
-void norm_gate_residual(at::Tensor& out, const c10::optional<at::Tensor>& normed,
-                        const at::Tensor& branch, const at::Tensor& residual,
-                        const c10::optional<at::Tensor>& gate,
-                        const c10::optional<at::Tensor>& row_scale,
-                        const c10::optional<at::Tensor>& post_w,
-                        const c10::optional<at::Tensor>& post_b,
-                        const c10::optional<at::Tensor>& pre_w,
-                        const c10::optional<at::Tensor>& pre_b, double eps) {
-  check_cuda_contig(branch, "branch");
-  TORCH_CHECK(branch.dim() >= 1, "branch must be [..., C]");
-  const int64_t C = branch.size(-1), M = C ? branch.numel() / C : 0;
-  check_rows(branch, residual, residual, "residual");
-  check_rows(branch, out, residual, "out");
-  void* normed_ptr = nullptr;
-  if (normed.has_value() && normed->defined()) {
-    check_rows(branch, *normed, branch, "normed");
-    normed_ptr = normed->data_ptr();
+void check_int32(const at::Tensor& ref, const at::Tensor& t, const char* name) {
+  check_cuda(ref, t, name);
+  TORCH_CHECK(t.is_contiguous() && t.scalar_type() == at::kInt, name,
+              " must be a contiguous int32 tensor");
+}
+
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// An optional parameter vector as a contiguous float32 [n] tensor (undefined if absent).
+at::Tensor vector_of(const at::Tensor& ref, const OptTensor& t, int64_t n, const char* name) {
+  if (!given(t)) return at::Tensor();
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n && t->is_floating_point(), name,
+                    " must be a floating-point tensor of shape (", n, ",)");
+  const at::Tensor v = t->device() == ref.device() && t->scalar_type() == at::kFloat
+                           ? *t
+                           : t->to(ref.device(), at::kFloat);
+  return v.contiguous();
+}
+
+const float* f32(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+at::Tensor f32_like(const at::Tensor& ref, at::IntArrayRef shape) {
+  return at::empty(shape, ref.options().dtype(at::kFloat));
+}
+
+at::Tensor relative_position_bias(const at::Tensor& table, const at::Tensor& pairs,
+                                  at::ScalarType dtype) {
+  check_int32(table, pairs, "pairs");
+  TORCH_CHECK_VALUE(table.dim() == 2 && pairs.dim() == 2, "table must be [buckets, heads]");
+  const c10::cuda::CUDAGuard guard(table.device());
+  const at::Tensor from = table.contiguous();
+  at::Tensor bias = at::empty({table.size(1), pairs.size(0), pairs.size(1)},
+                              table.options().dtype(dtype));
+  check_rc(crumpet_relative_position_bias(bias.data_ptr(), dtype_code(bias), from.data_ptr(),
+                                          dtype_code(from), table.size(0), table.size(1),
+                                          pairs.const_data_ptr<int>(), pairs.numel(),
+                                          cur_stream(bias)));
+  return bias;
+}
+
+// The table's gradient from grad [heads, pairs] (contiguous)
+at::Tensor table_gradient(const void* grad, const at::Tensor& ref, int grad_code, int64_t H,
+                          const at::Tensor& order, const at::Tensor& items,
+                          const at::Tensor& multi, int64_t buckets, at::ScalarType dtype) {
+  check_int32(ref, order, "order");
+  check_int32(ref, items, "items");
+  check_int32(ref, multi, "multi");
+  at::Tensor table = at::empty({buckets, H}, ref.options().dtype(dtype));
+  at::Tensor partial;
+  if (multi.size(0) > 0) partial = f32_like(ref, {items.size(0) * H});
+  check_rc(crumpet_relative_position_bias_backward(
+      table.data_ptr(), dtype_code(table), H, grad, grad_code, order.const_data_ptr<int>(),
+      order.numel(), items.const_data_ptr<int>(), items.size(0), multi.const_data_ptr<int>(),
+      multi.size(0), partial.defined() ? partial.data_ptr<float>() : nullptr, cur_stream(ref)));
+  return table;
+}
+
+at::Tensor relative_position_bias_backward(const at::Tensor& grad, const at::Tensor& order,
+                                           const at::Tensor& items, const at::Tensor& multi,
+                                           int64_t buckets, at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(grad.dim() == 3 && grad.size(1) * grad.size(2) == order.numel(),
+                    "grad_bias must have shape [heads, rows, cols] of the index");
+  const c10::cuda::CUDAGuard guard(grad.device());
+  const at::Tensor g = grad.contiguous();
+  return table_gradient(g.data_ptr(), g, dtype_code(g), g.size(0), order, items, multi, buckets,
+                        dtype);
+}
+
+// The table in float32 or qkv's dtype, contiguous
+at::Tensor attention_table(const at::Tensor& table, const at::Tensor& qkv) {
+  return (table.scalar_type() == at::kFloat || table.scalar_type() == qkv.scalar_type()
+              ? table
+              : table.to(at::kFloat))
+      .contiguous();
+}
+
+struct Place {
+  int64_t nw[3], ws[3], ss[3];
+};
+
+// Shapes and window geometry of the attention's forward and backward
+Place check_attention(const at::Tensor& qkv, const at::Tensor& table, const at::Tensor& index,
+                      at::IntArrayRef num_windows, at::IntArrayRef window_size,
+                      at::IntArrayRef shift_size, double scale) {
+  TORCH_CHECK_VALUE(qkv.dim() == 5 && qkv.size(2) == 3, "qkv must have shape [B, N, 3, H, head_dim]");
+  const int64_t B = qkv.size(0), N = qkv.size(1), H = qkv.size(3), Dh = qkv.size(4);
+  dtype_code(qkv);
+  TORCH_CHECK_VALUE(Dh == 16 || Dh == 32 || Dh == 64 || Dh == 128 || Dh == 256,
+                    "window attention requires a power-of-two head_dim between 16 and 256");
+  dtype_code(table);
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) == H, "table must have shape [num_buckets, ",
+                    H, "]");
+  check_cuda(qkv, table, "table");
+  check_cuda(qkv, index, "index");
+  TORCH_CHECK_VALUE(index.dim() == 2 && index.size(0) == N && index.size(1) == N,
+                    "buckets must be made of an index [", N, ", ", N,
+                    "] (index[:n, :n] of a clamped window)");
+  TORCH_CHECK_VALUE(num_windows.size() == 3 && window_size.size() == 3 && shift_size.size() == 3,
+                    "num_windows, window_size and shift_size must contain exactly three values");
+  Place p;
+  int64_t windows = 1, volume = 1;
+  bool shifted = false;
+  for (int a = 0; a < 3; ++a) {
+    p.nw[a] = num_windows[a];
+    p.ws[a] = window_size[a];
+    p.ss[a] = shift_size[a];
+    TORCH_CHECK_VALUE(p.nw[a] >= 1 && p.ws[a] >= 1,
+                      "num_windows and window_size values must be positive");
+    TORCH_CHECK_VALUE(p.ss[a] >= 0 && p.ss[a] < p.ws[a],
+                      "shift_size must satisfy 0 <= shift < window_size");
+    windows *= p.nw[a];
+    volume *= p.ws[a];
+    shifted = shifted || p.ss[a] != 0;
   }
-  const int64_t samples = row_scale.has_value() && row_scale->defined() ? row_scale->numel() : 1;
+  TORCH_CHECK_VALUE(volume == N, "window_size must hold N = ", N, " tokens");
+  TORCH_CHECK_VALUE(!shifted || B % windows == 0, "B must be a multiple of the number of windows");
+  TORCH_CHECK_VALUE(scale > 0 && scale < 1e30, "window attention requires a finite scale > 0");
+  return p;
+}
+
+at::Tensor swin_window_attention_train(const at::Tensor& qkv, const at::Tensor& table,
+                                       const at::Tensor& index, at::IntArrayRef num_windows,
+                                       at::IntArrayRef window_size, at::IntArrayRef shift_size,
+                                       double scale) {
+  const Place p = check_attention(qkv, table, index, num_windows, window_size, shift_size, scale);
+  TORCH_CHECK(index.is_contiguous() && index.scalar_type() == at::kLong,
+              "index must be a contiguous int64 tensor");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  const at::Tensor x = qkv.contiguous(), t = attention_table(table, x);
+  const int64_t B = x.size(0), N = x.size(1), H = x.size(3), Dh = x.size(4);
+  at::Tensor out = at::empty({B, N, H * Dh}, x.options());
+  const int code = dtype_code(x), t32 = t.scalar_type() == at::kFloat ? 1 : 0;
+  const float s = static_cast<float>(scale);
+  void* const stream = cur_stream(x);
+  // The tensor-core kernel's domain.  The table changes every step, so its bias operands are
+  // built every step.
+  const bool tiles_apply = code != CRUMPET_DTYPE_F32 && (Dh == 16 || Dh == 32) && N <= 352 &&
+                           B > 0 && reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
+  if (tiles_apply) {
+    at::Tensor tiles =
+        at::empty({crumpet_attention_bias_tiles_bytes(H, N)}, x.options().dtype(at::kByte));
+    check_rc(crumpet_attention_bias_tiles(tiles.data_ptr(), t.data_ptr(), t32, t.size(0),
+                                          index.const_data_ptr<int64_t>(), N, code, H, N, s,
+                                          stream));
+    check_rc(crumpet_swin_window_attention_qkv_tiles(
+        out.data_ptr(), x.data_ptr(), tiles.data_ptr(), p.nw[0], p.nw[1], p.nw[2], p.ws[0],
+        p.ws[1], p.ws[2], p.ss[0], p.ss[1], p.ss[2], code, B, H, N, Dh, s, stream));
+  } else {
+    check_rc(crumpet_swin_window_attention_qkv(
+        out.data_ptr(), x.data_ptr(), t.data_ptr(), t32, t.size(0),
+        index.const_data_ptr<int64_t>(), N, p.nw[0], p.nw[1], p.nw[2], p.ws[0], p.ws[1], p.ws[2],
+        p.ss[0], p.ss[1], p.ss[2], code, B, H, N, Dh, s, stream));
+  }
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> swin_window_attention_backward(
+    const at::Tensor& grad_out, const at::Tensor& qkv, const at::Tensor& table,
+    const at::Tensor& pairs, const at::Tensor& order, const at::Tensor& items,
+    const at::Tensor& multi, at::IntArrayRef num_windows, at::IntArrayRef window_size,
+    at::IntArrayRef shift_size, double scale) {
+  const Place p = check_attention(qkv, table, pairs, num_windows, window_size, shift_size, scale);
+  check_int32(qkv, pairs, "pairs");
+  check_cuda(qkv, grad_out, "grad_out");
+  const int64_t B = qkv.size(0), N = qkv.size(1), H = qkv.size(3), Dh = qkv.size(4);
+  TORCH_CHECK_VALUE(grad_out.dim() == 3 && grad_out.size(0) == B && grad_out.size(1) == N &&
+                        grad_out.size(2) == H * Dh && grad_out.scalar_type() == qkv.scalar_type(),
+                    "grad_out must have shape [B, N, H * head_dim] and the dtype of qkv");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  const at::Tensor x = qkv.contiguous(), g = grad_out.contiguous(), t = attention_table(table, x);
+  const int code = dtype_code(x);
+  const int64_t shares = crumpet_window_attention_backward_shares(B, H, N, Dh, code);
+  at::Tensor grad_qkv = at::empty(x.sizes(), x.options());
+  at::Tensor grad_bias = f32_like(x, {shares, H, N, N});
+  at::Tensor stats = f32_like(x, {B * H * (3 * N + 4)});
+  check_rc(crumpet_swin_window_attention_qkv_backward(
+      grad_qkv.data_ptr(), grad_bias.data_ptr<float>(), stats.data_ptr<float>(), g.data_ptr(),
+      x.data_ptr(), t.data_ptr(), t.scalar_type() == at::kFloat ? 1 : 0, t.size(0),
+      pairs.const_data_ptr<int>(), shares, p.nw[0], p.nw[1], p.nw[2], p.ws[0], p.ws[1], p.ws[2],
+      p.ss[0], p.ss[1], p.ss[2], code, B, H, N, Dh, static_cast<float>(scale), cur_stream(x)));
+  return {grad_qkv, table_gradient(grad_bias.data_ptr(), x, CRUMPET_DTYPE_F32, H, order, items,
+                                   multi, table.size(0), table.scalar_type())};
+}
+
+struct NormGate {
+  at::Tensor gate, row_scale, post_w, post_b, pre_w, pre_b;
+  int64_t M, C, samples;
+};
+
+NormGate check_norm_gate(const at::Tensor& branch, const at::Tensor& stream, const OptTensor& gate,
+                         const OptTensor& row_scale, const OptTensor& post_w,
+                         const OptTensor& post_b, const OptTensor& pre_w, const OptTensor& pre_b,
+                         double eps) {
+  TORCH_CHECK_VALUE(branch.dim() >= 1 && branch.sizes() == stream.sizes(),
+                    "branch and the residual stream must share a shape [..., C]");
+  dtype_code(branch);
+  TORCH_CHECK_TYPE(stream.scalar_type() == branch.scalar_type() ||
+                       stream.scalar_type() == at::kFloat,
+                   "norm_gate_residual takes float32, float16 or bfloat16 branches and a residual "
+                   "stream in float32 or the branch's dtype");
+  check_cuda(branch, stream, "the residual stream");
+  NormGate n;
+  n.C = branch.size(-1);
+  TORCH_CHECK_VALUE(n.C >= 1 && n.C <= 4096, "norm_gate_residual needs 1 to 4096 channels");
+  TORCH_CHECK_VALUE(eps > 0, "eps must be positive");
+  n.M = rows_of(branch);
+  n.samples = 1;
+  if (given(row_scale)) {
+    n.samples = row_scale->numel();
+    TORCH_CHECK_VALUE(row_scale->dim() == 1 && n.samples > 0 && n.M % n.samples == 0,
+                      "row_scale must be one value per sample, the rows a multiple of it");
+  }
+  n.row_scale = vector_of(branch, row_scale, n.samples, "row_scale");
+  n.gate = vector_of(branch, gate, n.C, "gate");
+  n.post_w = vector_of(branch, post_w, n.C, "post_norm weight");
+  n.post_b = vector_of(branch, post_b, n.C, "post_norm bias");
+  n.pre_w = vector_of(branch, pre_w, n.C, "pre_norm weight");
+  n.pre_b = vector_of(branch, pre_b, n.C, "pre_norm bias");
+  return n;
+}
+
+// [out] or [out, normed]
+std::vector<at::Tensor> norm_gate_residual(const at::Tensor& branch, const at::Tensor& residual,
+                                           const OptTensor& gate, const OptTensor& row_scale,
+                                           const OptTensor& post_w, const OptTensor& post_b,
+                                           const OptTensor& pre_w, const OptTensor& pre_b,
+                                           double eps) {
+  const NormGate n =
+      check_norm_gate(branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps);
   const c10::cuda::CUDAGuard guard(branch.device());
+  const at::Tensor x = branch.contiguous(), r = residual.contiguous();
+  std::vector<at::Tensor> res{at::empty(r.sizes(), r.options())};
+  if (n.pre_w.defined()) res.push_back(at::empty(x.sizes(), x.options()));
   check_rc(crumpet_norm_gate_residual(
-      out.data_ptr(), normed_ptr, branch.data_ptr(), residual.data_ptr(), dtype_code(branch),
-      dtype_code(residual), optional_f32(branch, gate, C, "gate"),
-      optional_f32(branch, row_scale, samples, "row_scale"), samples,
-      optional_f32(branch, post_w, C, "post weight"), optional_f32(branch, post_b, C, "post bias"),
-      optional_f32(branch, pre_w, C, "pre weight"), optional_f32(branch, pre_b, C, "pre bias"),
-      static_cast<float>(eps), M, C, cur_stream(branch)));
+      res[0].data_ptr(), n.pre_w.defined() ? res[1].data_ptr() : nullptr, x.data_ptr(),
+      r.data_ptr(), dtype_code(x), dtype_code(r), f32(n.gate), f32(n.row_scale), n.samples,
+      f32(n.post_w), f32(n.post_b), f32(n.pre_w), f32(n.pre_b), static_cast<float>(eps), n.M, n.C,
+      cur_stream(x)));
+  return res;
 }
 
-void norm_gate_residual_backward(at::Tensor& grad_residual, at::Tensor& grad_branch,
-                                 const c10::optional<at::Tensor>& sums,
-                                 const c10::optional<at::Tensor>& partial,
-                                 const at::Tensor& grad_out,
-                                 const c10::optional<at::Tensor>& grad_normed,
-                                 const at::Tensor& out, const at::Tensor& branch,
-                                 const c10::optional<at::Tensor>& gate,
-                                 const c10::optional<at::Tensor>& row_scale,
-                                 const c10::optional<at::Tensor>& post_w,
-                                 const c10::optional<at::Tensor>& post_b,
-                                 const c10::optional<at::Tensor>& pre_w, double eps) {
-  check_cuda_contig(branch, "branch");
-  TORCH_CHECK(branch.dim() >= 1, "branch must be [..., C]");
-  const int64_t C = branch.size(-1), M = C ? branch.numel() / C : 0;
-  check_rows(branch, grad_out, out, "grad_out");
-  check_rows(branch, out, out, "out");
-  check_rows(branch, grad_residual, out, "grad_residual");
-  check_rows(branch, grad_branch, branch, "grad_branch");
-  const void* gn = nullptr;
-  if (grad_normed.has_value() && grad_normed->defined()) {
-    check_rows(branch, *grad_normed, branch, "grad_normed");
-    gn = grad_normed->data_ptr();
-  }
-  float* part = optional_f32(branch, partial, crumpet_norm_gate_residual_backward_partials(M, C),
-                             "partial");
-  float* s = optional_f32(branch, sums, 5 * C, "sums");  // gate, post w, post b, pre w, pre b
-  float* at_[5];
-  for (int q = 0; q < 5; ++q) at_[q] = s ? s + q * C : nullptr;
-  const int64_t samples = row_scale.has_value() && row_scale->defined() ? row_scale->numel() : 1;
+// [grad_residual, grad_branch], then what is given of gate, post weight and bias, pre weight and
+// bias
+std::vector<at::Tensor> norm_gate_residual_backward(
+    const at::Tensor& grad_out, const OptTensor& grad_normed, const at::Tensor& out,
+    const at::Tensor& branch, const OptTensor& gate, const OptTensor& row_scale,
+    const OptTensor& post_w, const OptTensor& post_b, const OptTensor& pre_w, double eps) {
+  const NormGate n =
+      check_norm_gate(branch, out, gate, row_scale, post_w, post_b, pre_w, OptTensor(), eps);
+  TORCH_CHECK_VALUE(grad_out.sizes() == out.sizes() && grad_out.scalar_type() == out.scalar_type(),
+                    "grad_out must have the shape and dtype of out");
+  check_cuda(branch, grad_out, "grad_out");
+  TORCH_CHECK_VALUE(given(grad_normed) == n.pre_w.defined(),
+                    "grad_normed belongs to pre_norm: give both or neither");
   const c10::cuda::CUDAGuard guard(branch.device());
+  at::Tensor gn;
+  if (given(grad_normed)) {
+    TORCH_CHECK_VALUE(grad_normed->sizes() == branch.sizes() &&
+                          grad_normed->scalar_type() == branch.scalar_type(),
+                      "grad_normed must have the shape and dtype of branch");
+    check_cuda(branch, *grad_normed, "grad_normed");
+    gn = grad_normed->contiguous();
+  }
+  const at::Tensor x = branch.contiguous(), o = out.contiguous(), go = grad_out.contiguous();
+  std::vector<at::Tensor> res{at::empty(o.sizes(), o.options()), at::empty(x.sizes(), x.options())};
+  float* sums[5] = {};  // gate, post weight and bias, pre weight and bias
+  const bool has[5] = {n.gate.defined(), n.post_w.defined(), n.post_w.defined(),
+                       n.pre_w.defined(), n.pre_w.defined()};
+  for (int q = 0; q < 5; ++q) {
+    if (!has[q]) continue;
+    res.push_back(f32_like(x, {n.C}));
+    sums[q] = res.back().data_ptr<float>();
+  }
+  at::Tensor partial;
+  if (res.size() > 2)
+    partial = f32_like(x, {crumpet_norm_gate_residual_backward_partials(n.M, n.C)});
   check_rc(crumpet_norm_gate_residual_backward(
-      grad_residual.data_ptr(), grad_branch.data_ptr(), at_[0], at_[1], at_[2], at_[3], at_[4],
-      grad_out.data_ptr(), gn, out.data_ptr(), branch.data_ptr(), dtype_code(branch),
-      dtype_code(out), optional_f32(branch, gate, C, "gate"),
-      optional_f32(branch, row_scale, samples, "row_scale"), samples,
-      optional_f32(branch, post_w, C, "post weight"), optional_f32(branch, post_b, C, "post bias"),
-      optional_f32(branch, pre_w, C, "pre weight"), static_cast<float>(eps), part, M, C,
-      cur_stream(branch)));
+      res[0].data_ptr(), res[1].data_ptr(), sums[0], sums[1], sums[2], sums[3], sums[4],
+      go.data_ptr(), gn.defined() ? gn.data_ptr() : nullptr, o.data_ptr(), x.data_ptr(),
+      dtype_code(x), dtype_code(o), f32(n.gate), f32(n.row_scale), n.samples, f32(n.post_w),
+      f32(n.post_b), f32(n.pre_w), static_cast<float>(eps),
+      partial.defined() ? partial.data_ptr<float>() : nullptr, n.M, n.C, cur_stream(x)));
+  return res;
 }
 
-// int8 [.., C] and uint8 [.., ceil(C / 32)] of an activation [.., C]
-void check_kept(const at::Tensor& x, const at::Tensor& kept, const at::Tensor& scales) {
-  check_cuda_contig(x, "x");
-  check_cuda_contig(kept, "kept");
-  check_cuda_contig(scales, "scales");
-  same_device(x, kept, "kept");
-  same_device(x, scales, "scales");
-  TORCH_CHECK(x.dim() >= 1, "x must be [..., C]");
-  TORCH_CHECK(kept.scalar_type() == at::kChar && kept.numel() == x.numel(),
-              "kept must be an int8 tensor of x's elements");
-  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
-  TORCH_CHECK(scales.scalar_type() == at::kByte && scales.numel() == M * ((C + 31) / 32),
-              "scales must be a uint8 tensor of one element per 32 channels");
-}
-
-void gelu_checkpoint(at::Tensor& y, at::Tensor& kept, at::Tensor& scales, const at::Tensor& x) {
-  check_kept(x, kept, scales);
-  check_rows(x, y, x, "y");
-  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gelu_checkpoint(const at::Tensor& x) {
+  dtype_code(x);
+  TORCH_CHECK_VALUE(x.dim() >= 1, "x must be [..., C]");
   const c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor in = x.contiguous();
+  const int64_t C = in.size(-1), M = C ? in.numel() / C : 0;
+  at::Tensor y = at::empty(in.sizes(), in.options());
+  at::Tensor kept = at::empty(in.sizes(), in.options().dtype(at::kChar));
+  auto shape = in.sizes().vec();
+  shape.back() = (C + 31) / 32;
+  at::Tensor scales = at::empty(shape, in.options().dtype(at::kByte));
   check_rc(crumpet_gelu_checkpoint(y.data_ptr(), kept.data_ptr<int8_t>(),
-                                   scales.data_ptr<uint8_t>(), x.data_ptr(), dtype_code(x), M, C,
-                                   cur_stream(x)));
+                                   scales.data_ptr<uint8_t>(), in.data_ptr(), dtype_code(in), M, C,
+                                   cur_stream(in)));
+  return {y, kept, scales};
 }
 
-void gelu_checkpoint_backward(at::Tensor& grad_x, at::Tensor& again, const at::Tensor& grad_y,
-                              const at::Tensor& kept, const at::Tensor& scales) {
-  check_kept(grad_y, kept, scales);
-  check_rows(grad_y, grad_x, grad_y, "grad_x");
-  check_rows(grad_y, again, grad_y, "again");
-  const int64_t C = grad_y.size(-1), M = C ? grad_y.numel() / C : 0;
+// int8 [..., C] and uint8 [..., ceil(C / 32)]
+void check_kept(const at::Tensor& kept, const at::Tensor& scales) {
+  TORCH_CHECK(kept.is_cuda() && kept.is_contiguous() && kept.scalar_type() == at::kChar &&
+                  kept.dim() >= 1,
+              "kept must be a contiguous int8 CUDA tensor [..., C]");
+  same_device(kept, scales, "scales");
+  const int64_t C = kept.size(-1), M = C ? kept.numel() / C : 0;
+  TORCH_CHECK(scales.is_contiguous() && scales.scalar_type() == at::kByte &&
+                  scales.numel() == M * ((C + 31) / 32),
+              "scales must be a contiguous uint8 tensor of one element per 32 channels");
+}
+
+std::tuple<at::Tensor, at::Tensor> gelu_checkpoint_backward(const at::Tensor& grad_y,
+                                                            const at::Tensor& kept,
+                                                            const at::Tensor& scales) {
+  check_kept(kept, scales);
+  check_cuda(kept, grad_y, "grad_y");
+  TORCH_CHECK_VALUE(grad_y.sizes() == kept.sizes(),
+                    "grad_y must have the shape and dtype of the kept activation");
   const c10::cuda::CUDAGuard guard(grad_y.device());
+  const at::Tensor g = grad_y.contiguous();
+  const int64_t C = g.size(-1), M = C ? g.numel() / C : 0;
+  at::Tensor grad_x = at::empty(g.sizes(), g.options()), again = at::empty(g.sizes(), g.options());
   check_rc(crumpet_gelu_checkpoint_backward(
-      grad_x.data_ptr(), again.data_ptr(), grad_y.data_ptr(), kept.data_ptr<int8_t>(),
-      scales.data_ptr<uint8_t>(), dtype_code(grad_y), M, C, cur_stream(grad_y)));
+      grad_x.data_ptr(), again.data_ptr(), g.data_ptr(), kept.const_data_ptr<int8_t>(),
+      scales.const_data_ptr<uint8_t>(), dtype_code(g), M, C, cur_stream(g)));
+  return {grad_x, again};
 }
 
-void restore_activation(at::Tensor& x, const at::Tensor& kept, const at::Tensor& scales) {
-  check_kept(x, kept, scales);
-  const int64_t C = x.size(-1), M = C ? x.numel() / C : 0;
-  const c10::cuda::CUDAGuard guard(x.device());
-  check_rc(crumpet_restore_activation(x.data_ptr(), kept.data_ptr<int8_t>(),
-                                      scales.data_ptr<uint8_t>(), dtype_code(x), M, C,
+at::Tensor restore_activation(const at::Tensor& kept, const at::Tensor& scales,
+                              at::ScalarType dtype) {
+  check_kept(kept, scales);
+  const c10::cuda::CUDAGuard guard(kept.device());
+  const int64_t C = kept.size(-1), M = C ? kept.numel() / C : 0;
+  at::Tensor x = at::empty(kept.sizes(), kept.options().dtype(dtype));
+  check_rc(crumpet_restore_activation(x.data_ptr(), kept.const_data_ptr<int8_t>(),
+                                      scales.const_data_ptr<uint8_t>(), dtype_code(x), M, C,
                                       cur_stream(x)));
+  return x;
 }
 
 }  // namespace
@@ -887,34 +1015,44 @@ TORCH_LIBRARY(crumpet_ops, ops) {
       "roi_normalize(Tensor! logits, Tensor acc, Tensor count_d, Tensor count_h, "
       "Tensor count_w) -> ()",
       kTags);
-  ops.def("relative_position_bias(Tensor! bias, Tensor table, Tensor pairs) -> ()", kTags);
+  ops.def("relative_position_bias(Tensor table, Tensor pairs, ScalarType dtype) -> Tensor", kTags);
   ops.def(
-      "relative_position_bias_backward(Tensor! grad_table, Tensor grad, Tensor order, "
-      "Tensor items, Tensor multi, Tensor(a!)? partial) -> ()",
+      "relative_position_bias_backward(Tensor grad, Tensor order, Tensor items, Tensor multi, "
+      "int buckets, ScalarType dtype) -> Tensor",
       kTags);
   ops.def(
-      "swin_window_attention_qkv_backward(Tensor(a!) grad_qkv, Tensor(b!) grad_bias, "
-      "Tensor(c!) stats, Tensor grad_out, Tensor qkv, Tensor table, Tensor pairs, "
-      "int[] num_windows, int[] window_size, int[] shift_size, float scale) -> ()",
+      "swin_window_attention_train(Tensor qkv, Tensor table, Tensor index, int[] num_windows, "
+      "int[] window_size, int[] shift_size, float scale) -> Tensor",
       kTags);
   ops.def(
-      "norm_gate_residual(Tensor(a!) out, Tensor(b!)? normed, Tensor branch, Tensor residual, "
-      "Tensor? gate, Tensor? row_scale, Tensor? post_w, Tensor? post_b, Tensor? pre_w, "
-      "Tensor? pre_b, float eps) -> ()",
+      "swin_window_attention_backward(Tensor grad_out, Tensor qkv, Tensor table, Tensor pairs, "
+      "Tensor order, Tensor items, Tensor multi, int[] num_windows, int[] window_size, "
+      "int[] shift_size, float scale) -> (Tensor, Tensor)",
       kTags);
   ops.def(
-      "norm_gate_residual_backward(Tensor(a!) grad_residual, Tensor(b!) grad_branch, "
-      "Tensor(c!)? sums, Tensor(d!)? partial, Tensor grad_out, Tensor? grad_normed, Tensor out, "
+      "norm_gate_residual(Tensor branch, Tensor residual, Tensor? gate, Tensor? row_scale, "
+      "Tensor? post_w, Tensor? post_b, Tensor? pre_w, Tensor? pre_b, float eps) -> Tensor[]",
+      kTags);
+  ops.def(
+      "norm_gate_residual_backward(Tensor grad_out, Tensor? grad_normed, Tensor out, "
       "Tensor branch, Tensor? gate, Tensor? row_scale, Tensor? post_w, Tensor? post_b, "
-      "Tensor? pre_w, float eps) -> ()",
+      "Tensor? pre_w, float eps) -> Tensor[]",
       kTags);
+  ops.def("gelu_checkpoint(Tensor x) -> (Tensor, Tensor, Tensor)", kTags);
   ops.def(
-      "gelu_checkpoint(Tensor(a!) y, Tensor(b!) kept, Tensor(c!) scales, Tensor x) -> ()", kTags);
-  ops.def(
-      "gelu_checkpoint_backward(Tensor(a!) grad_x, Tensor(b!) again, Tensor grad_y, Tensor kept, "
-      "Tensor scales) -> ()",
+      "gelu_checkpoint_backward(Tensor grad_y, Tensor kept, Tensor scales) -> (Tensor, Tensor)",
       kTags);
-  ops.def("restore_activation(Tensor! x, Tensor kept, Tensor scales) -> ()", kTags);
+  ops.def("restore_activation(Tensor kept, Tensor scales, ScalarType dtype) -> Tensor", kTags);
+}
+
+// The training operators' gradients are crumpet_b200.training's autograd functions; called by
+// themselves they record nothing.
+TORCH_LIBRARY_IMPL(crumpet_ops, Autograd, ops) {
+  for (const char* name :
+       {"relative_position_bias", "relative_position_bias_backward", "swin_window_attention_train",
+        "swin_window_attention_backward", "norm_gate_residual", "norm_gate_residual_backward",
+        "gelu_checkpoint", "gelu_checkpoint_backward", "restore_activation"})
+    ops.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(crumpet_ops, CUDA, ops) {
@@ -940,7 +1078,8 @@ TORCH_LIBRARY_IMPL(crumpet_ops, CUDA, ops) {
   ops.impl("roi_normalize", &roi_normalize);
   ops.impl("relative_position_bias", &relative_position_bias);
   ops.impl("relative_position_bias_backward", &relative_position_bias_backward);
-  ops.impl("swin_window_attention_qkv_backward", &swin_window_attention_qkv_backward);
+  ops.impl("swin_window_attention_train", &swin_window_attention_train);
+  ops.impl("swin_window_attention_backward", &swin_window_attention_backward);
   ops.impl("norm_gate_residual", &norm_gate_residual);
   ops.impl("norm_gate_residual_backward", &norm_gate_residual_backward);
   ops.impl("gelu_checkpoint", &gelu_checkpoint);

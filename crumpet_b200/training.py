@@ -21,7 +21,6 @@ change from run to run (no atomics).  CUDA tensors only, as elsewhere in the pac
 
 from __future__ import annotations
 
-import functools
 import sys
 import types
 from typing import NamedTuple, Sequence
@@ -31,8 +30,7 @@ import torch.nn.functional as F
 
 from . import _ops as _native
 from . import profiling as _prof
-from .fused_attention import (_ATTN_DTYPES, head_dim_supported, swin_window_attention_qkv,
-                              tensor_core_attention)
+from .fused_attention import head_dim_supported
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 GROUP = 32  # neighbouring channels that share one scale of an 8-bit checkpoint
@@ -54,24 +52,19 @@ def _needs_grad(*tensors) -> bool:
     return False
 
 
-# Sizes that the library works out from a call's shapes and the device's SM count; asked once
-# for each, since the call and the switch to the device cost more than a small launch.
-@functools.lru_cache(maxsize=1024)
-def _shares(B: int, H: int, N: int, D: int, dtype: torch.dtype, device: int) -> int:
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
-    with torch.cuda.device(device):
-        return int(_native.capi().crumpet_window_attention_backward_shares(B, H, N, D, code))
+def _launch(name: str, work, *args):
+    """One call of a training op of the library (which checks its arguments and allocates what it
+    returns), counted, and timed while a timer is active; ``work`` gives its algorithmic work."""
+    op = getattr(_native.require(), name)
+    token = _prof.kernel_begin(name, work) if _prof._active else None
+    res = op(*args)
+    _prof.count(name)
+    _prof.kernel_end(token)
+    return res
 
 
-@functools.lru_cache(maxsize=1024)
-def _partials(rows: int, C: int, device: int) -> int:
-    with torch.cuda.device(device):
-        return int(_native.capi().crumpet_norm_gate_residual_backward_partials(rows, C))
-
-
-@functools.lru_cache(maxsize=1024)
-def _tile_bytes(H: int, N: int) -> int:
-    return int(_native.capi().crumpet_attention_bias_tiles_bytes(H, N))
+def _nbytes(*tensors) -> int:
+    return sum(t.numel() * t.element_size() for t in tensors if t is not None)
 
 
 # ------------------------------------------------------------------ relative-position bias
@@ -124,40 +117,17 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
                                    multi.int().contiguous(), num_buckets)
 
 
-def _check_table(table: torch.Tensor, buckets: RelativePositionBuckets) -> int:
+def _check_table(table: torch.Tensor, buckets: RelativePositionBuckets) -> None:
     if table.ndim != 2 or table.shape[0] != buckets.num_buckets:
         raise ValueError(f"table must have shape [{buckets.num_buckets}, heads]")
     if table.dtype not in _DTYPES:
         raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
-    return table.shape[1]
 
 
 def _bias_forward(table, buckets, dtype):
-    if table.requires_grad:
-        table = table.detach()
-    bias = torch.empty((table.shape[1], *buckets.pairs.shape), dtype=dtype, device=table.device)
-    token = _prof.kernel_begin("relative_position_bias", lambda: {
-        "bytes": bias.numel() * bias.element_size() + buckets.pairs.numel() * 4})
-    _native.require().relative_position_bias(bias, table.contiguous(), buckets.pairs)
-    _prof.count("relative_position_bias")
-    _prof.kernel_end(token)
-    return bias
-
-
-def _table_gradient(grad, heads, buckets, dtype):
-    """[buckets, heads] from grad [heads, rows, cols]."""
-    grad_table = torch.empty((buckets.num_buckets, heads), dtype=dtype, device=grad.device)
-    partial = None
-    if buckets.multi.shape[0]:
-        partial = torch.empty(buckets.items.shape[0] * heads, dtype=torch.float32,
-                              device=grad.device)
-    token = _prof.kernel_begin("relative_position_bias_backward", lambda: {
-        "bytes": grad.numel() * grad.element_size() + buckets.order.numel() * 4})
-    _native.require().relative_position_bias_backward(grad_table, grad, buckets.order,
-                                                      buckets.items, buckets.multi, partial)
-    _prof.count("relative_position_bias_backward")
-    _prof.kernel_end(token)
-    return grad_table
+    pairs = buckets.pairs
+    return _launch("relative_position_bias", lambda: {
+        "bytes": pairs.numel() * (table.shape[1] * dtype.itemsize + 4)}, table, pairs, dtype)
 
 
 class _Bias(torch.autograd.Function):
@@ -198,93 +168,39 @@ def relative_position_bias_backward(grad_bias: torch.Tensor, buckets: RelativePo
     if grad_bias.dtype not in _DTYPES or dtype not in _DTYPES:
         raise TypeError("CRUMPET supports torch.float32, torch.float16 and torch.bfloat16")
     _require_cuda("relative_position_bias_backward", grad_bias, buckets.order)
-    return _table_gradient(grad_bias.contiguous(), int(grad_bias.shape[0]), buckets, dtype)
+    return _launch("relative_position_bias_backward", lambda: {
+        "bytes": _nbytes(grad_bias, buckets.order)}, grad_bias, buckets.order, buckets.items,
+        buckets.multi, buckets.num_buckets, dtype)
 
 
 # ------------------------------------------------------------------------- window attention
-def _triple(value):
-    return value if type(value) is tuple and len(value) == 3 else tuple(map(int, value))
-
-
-def _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale):
-    if qkv.ndim != 5 or qkv.shape[2] != 3:
+def _place(qkv, table, buckets, num_windows, window_size, shift_size, scale):
+    """The arguments as the ops take them (which check the rest)."""
+    if qkv.ndim != 5:
         raise ValueError("qkv must have shape [B, N, 3, H, head_dim]")
-    B, N, _, H, D = qkv.shape
-    if qkv.dtype not in _ATTN_DTYPES:
-        raise TypeError("window attention supports torch.float32, torch.float16 and torch.bfloat16")
-    if not head_dim_supported(D):
-        raise ValueError("window attention requires a power-of-two head_dim between 16 and 256")
-    if _check_table(table, buckets) != H:
-        raise ValueError(f"table must have shape [{buckets.num_buckets}, {H}]")
-    if buckets.pairs.shape != (N, N):
-        raise ValueError(f"buckets must be made of an index [{N}, {N}] (index[:n, :n] of a "
-                         "clamped window)")
-    num_windows, shift_size = _triple(num_windows), _triple(shift_size)
-    window_size = (N, 1, 1) if window_size is None else _triple(window_size)
-    if not len(num_windows) == len(window_size) == len(shift_size) == 3:
-        raise ValueError("num_windows, window_size and shift_size must contain exactly three values")
-    if min(num_windows) < 1 or min(window_size) < 1:
-        raise ValueError("num_windows and window_size values must be positive")
-    if window_size[0] * window_size[1] * window_size[2] != N:
-        raise ValueError(f"window_size must hold N = {N} tokens")
-    if shift_size != (0, 0, 0):
-        if any(not 0 <= s < w for s, w in zip(shift_size, window_size)):
-            raise ValueError("shift_size must satisfy 0 <= shift < window_size")
-        if B % (num_windows[0] * num_windows[1] * num_windows[2]):
-            raise ValueError("B must be a multiple of the number of windows")
-    scale = 1.0 / (D ** 0.5) if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("window attention requires a finite scale > 0")
+    _check_table(table, buckets)
     _require_cuda("window attention", qkv, table, buckets.pairs)
+    if window_size is None:
+        window_size = (qkv.shape[1], 1, 1)
+    if scale is None:
+        scale = qkv.shape[4] ** -0.5
     return num_windows, window_size, shift_size, scale
 
 
-def _attention_table(table, dtype):
-    if table.requires_grad:
-        table = table.detach()
-    return (table if table.dtype in (torch.float32, dtype) else table.float()).contiguous()
+def _attention_work(qkv, tensors: int, products: int):
+    B, N, _, H, D = qkv.shape
+    return {"bytes": tensors * B * H * N * D * qkv.element_size(),
+            "flops": 2 * products * B * H * N * N * D, "exps": B * H * N * N}
 
 
 def _attention_forward(qkv, table, buckets, place):
-    num_windows, window_size, shift_size, scale = place
-    qkv = qkv.contiguous()
-    B, N, _, H, D = qkv.shape
-    table = _attention_table(table, qkv.dtype)
-    if not (tensor_core_attention(qkv.dtype, N, D) and B and qkv.data_ptr() % 16 == 0):
-        return swin_window_attention_qkv(qkv, table, buckets.index, num_windows, window_size,
-                                         shift_size, scale)
-    # the table changes every step, so its operands are built every step
-    ops = _native.require()
-    tiles = torch.empty(_tile_bytes(H, N), dtype=torch.uint8, device=qkv.device)
-    out = torch.empty((B, N, H * D), dtype=qkv.dtype, device=qkv.device)
-    ops.attention_bias_tiles(tiles, table, buckets.index, N, scale, qkv.dtype)
-    _prof.count("attention_bias_tiles")
-    token = _prof.kernel_begin("swin_window_attention_qkv", lambda: {
-        "bytes": 4 * B * H * N * D * qkv.element_size(), "flops": 4 * B * H * N * N * D,
-        "exps": B * H * N * N})
-    ops.swin_window_attention_qkv_tiles(out, qkv, tiles, num_windows, window_size, shift_size, scale)
-    _prof.count("swin_window_attention_qkv")
-    _prof.kernel_end(token)
-    return out
+    return _launch("swin_window_attention_train", lambda: _attention_work(qkv, 4, 2), qkv, table,
+                   buckets.index, *place)
 
 
 def _attention_backward(grad_out, qkv, table, buckets, place):
-    num_windows, window_size, shift_size, scale = place
-    qkv, grad_out = qkv.contiguous(), grad_out.contiguous()
-    B, N, _, H, D = qkv.shape
-    shares = _shares(B, H, N, D, qkv.dtype, qkv.get_device())
-    grad_qkv = torch.empty_like(qkv)
-    grad_bias = torch.empty((shares, H, N, N), dtype=torch.float32, device=qkv.device)
-    stats = torch.empty(B * H * (3 * N + 4), dtype=torch.float32, device=qkv.device)
-    token = _prof.kernel_begin("swin_window_attention_qkv_backward", lambda: {
-        "bytes": 7 * B * H * N * D * qkv.element_size(), "flops": 10 * B * H * N * N * D,
-        "exps": B * H * N * N})
-    _native.require().swin_window_attention_qkv_backward(
-        grad_qkv, grad_bias, stats, grad_out, qkv, _attention_table(table, qkv.dtype),
-        buckets.pairs, num_windows, window_size, shift_size, scale)
-    _prof.count("swin_window_attention_qkv_backward")
-    _prof.kernel_end(token)
-    return grad_qkv, _table_gradient(grad_bias[0], H, buckets, table.dtype)
+    return _launch("swin_window_attention_backward", lambda: _attention_work(qkv, 7, 5), grad_out,
+                   qkv, table, buckets.pairs, buckets.order, buckets.items, buckets.multi, *place)
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -312,7 +228,7 @@ def swin_window_attention_train(
     """:func:`~crumpet_b200.swin_window_attention_qkv` for training: the same result, from
     ``qkv [B, N, 3, H, head_dim]``, the bias ``table [num_buckets, H]`` and its ``buckets``
     (of the ``[N, N]`` index), differentiable in ``qkv`` and ``table``."""
-    place = _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale)
+    place = _place(qkv, table, buckets, num_windows, window_size, shift_size, scale)
     if _needs_grad(qkv, table):
         return _WindowAttention.apply(qkv, table, buckets, place)
     return _attention_forward(qkv, table, buckets, place)
@@ -331,10 +247,7 @@ def swin_window_attention_backward(
     """``(grad_qkv, grad_table)`` of :func:`swin_window_attention_train` from ``grad_out
     [B, N, H * head_dim]`` and the forward's own arguments, in the dtypes of ``qkv`` and
     ``table``."""
-    place = _check_attention(qkv, table, buckets, window_size, shift_size, num_windows, scale)
-    B, N, _, H, D = qkv.shape
-    if grad_out.shape != (B, N, H * D) or grad_out.dtype != qkv.dtype:
-        raise ValueError(f"grad_out must have shape {(B, N, H * D)} and the dtype of qkv")
+    place = _place(qkv, table, buckets, num_windows, window_size, shift_size, scale)
     _require_cuda("window attention", grad_out)
     return _attention_backward(grad_out, qkv, table, buckets, place)
 
@@ -352,112 +265,54 @@ class NormGateGrads(NamedTuple):
     pre_bias: torch.Tensor | None
 
 
-def _vector(t, n, device, what):
-    if t is None:
-        return None
-    if t.shape != (n,) or not t.is_floating_point():
-        raise ValueError(f"{what} must be a floating-point tensor of shape ({n},)")
-    if t.requires_grad:
-        t = t.detach()
-    if t.dtype is not torch.float32 or t.device != device:
-        t = t.to(device=device, dtype=torch.float32)
-    return t.contiguous()
+def _pair(norm, name):
+    if norm is None:
+        return None, None
+    if len(norm) != 2:
+        raise ValueError(f"{name} must be a (weight, bias) pair")
+    return norm
 
 
-def _check_norm_gate(branch, stream, gate, row_scale, post_norm, pre_norm, eps):
-    if branch.ndim < 1 or branch.shape != stream.shape:
-        raise ValueError("branch and the residual stream must share a shape [..., C]")
-    if branch.dtype not in _DTYPES or stream.dtype not in (branch.dtype, torch.float32):
-        raise TypeError("norm_gate_residual takes float32, float16 or bfloat16 branches and a "
-                        "residual stream in float32 or the branch's dtype")
-    C = branch.shape[-1]
-    if not 1 <= C <= MAX_CHANNELS:
-        raise ValueError(f"norm_gate_residual needs 1 to {MAX_CHANNELS} channels")
-    if not eps > 0:
-        raise ValueError("eps must be positive")
-    _require_cuda("norm_gate_residual", branch, stream)
-    dev = branch.device
-    post_w = post_b = pre_w = pre_b = None
-    if post_norm is not None:
-        if len(post_norm) != 2:
-            raise ValueError("post_norm must be a (weight, bias) pair")
-        post_w = _vector(post_norm[0], C, dev, "post_norm weight")
-        post_b = _vector(post_norm[1], C, dev, "post_norm bias")
-    if pre_norm is not None:
-        if len(pre_norm) != 2:
-            raise ValueError("pre_norm must be a (weight, bias) pair")
-        pre_w = _vector(pre_norm[0], C, dev, "pre_norm weight")
-        pre_b = _vector(pre_norm[1], C, dev, "pre_norm bias")
-    if row_scale is not None:
-        samples = row_scale.numel()
-        if row_scale.ndim != 1 or not samples or branch.numel() // C % samples:
-            raise ValueError("row_scale must be one value per sample, the rows a multiple of it")
-        row_scale = _vector(row_scale, samples, dev, "row_scale")
-    return _vector(gate, C, dev, "gate"), row_scale, post_w, post_b, pre_w, pre_b
+def _norm_gate_forward(branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps):
+    res = _launch("norm_gate_residual", lambda: {
+        "bytes": _nbytes(branch, residual, residual, branch if pre_w is not None else None)},
+        branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps)
+    return res if pre_w is not None else (res[0], None)
 
 
-def _norm_gate_forward(branch, residual, params, eps):
-    branch, residual = branch.contiguous(), residual.contiguous()
-    out = torch.empty_like(residual)
-    normed = None if params[4] is None else torch.empty_like(branch)
-    token = _prof.kernel_begin("norm_gate_residual", lambda: {
-        "bytes": sum(t.numel() * t.element_size() for t in (branch, residual, out, normed)
-                     if t is not None)})
-    _native.require().norm_gate_residual(out, normed, branch, residual, *params, float(eps))
-    _prof.count("norm_gate_residual")
-    _prof.kernel_end(token)
-    return out, normed
-
-
-def _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps):
-    gate, row_scale, post_w, post_b, pre_w, _ = params
-    branch, out, grad_out = branch.contiguous(), out.contiguous(), grad_out.contiguous()
-    grad_normed = None if pre_w is None else grad_normed.contiguous()
-    C = branch.shape[-1]
-    grad_residual, grad_branch = torch.empty_like(out), torch.empty_like(branch)
-    sums = partial = None
-    columns = (None,) * 5
-    if gate is not None or post_w is not None or pre_w is not None:
-        sums = torch.empty((5, C), dtype=torch.float32, device=branch.device)
-        partial = torch.empty(_partials(branch.numel() // C, C, branch.get_device()),
-                              dtype=torch.float32, device=branch.device)
-        columns = sums.unbind(0)
-    token = _prof.kernel_begin("norm_gate_residual_backward", lambda: {
-        "bytes": sum(t.numel() * t.element_size() for t in (
-            grad_out, grad_normed, out if pre_w is not None else None,
-            branch if gate is not None or post_w is not None else None, grad_residual,
-            grad_branch) if t is not None)})
-    _native.require().norm_gate_residual_backward(
-        grad_residual, grad_branch, sums, partial, grad_out, grad_normed, out, branch, gate,
-        row_scale, post_w, post_b, pre_w, float(eps))
-    _prof.count("norm_gate_residual_backward")
-    _prof.kernel_end(token)
-    return NormGateGrads(grad_residual, grad_branch, None if gate is None else columns[0],
-                         *((None, None) if post_w is None else columns[1:3]),
-                         *((None, None) if pre_w is None else columns[3:5]))
+def _norm_gate_backward(grad_out, grad_normed, out, branch, gate, row_scale, post_w, post_b, pre_w,
+                        eps):
+    res = _launch("norm_gate_residual_backward", lambda: {
+        "bytes": _nbytes(grad_out, grad_normed, out if pre_w is not None else None,
+                         branch if gate is not None or post_w is not None else None, out, branch)},
+        grad_out, grad_normed, out, branch, gate, row_scale, post_w, post_b, pre_w, eps)
+    sums = iter(res[2:])
+    return NormGateGrads(res[0], res[1], None if gate is None else next(sums),
+                         *((None, None) if post_w is None else (next(sums), next(sums))),
+                         *((None, None) if pre_w is None else (next(sums), next(sums))))
 
 
 class _NormGate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, branch, residual, gate, post_w, post_b, pre_w, pre_b, row_scale, params, eps):
-        out, normed = _norm_gate_forward(branch, residual, params, eps)
-        ctx.save_for_backward(branch if gate is not None or post_w is not None else None, out,
-                              *params)
+    def forward(ctx, branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps):
+        out, normed = _norm_gate_forward(branch, residual, gate, row_scale, post_w, post_b, pre_w,
+                                         pre_b, eps)
+        # branch is read again for the gate's and the post-norm's gradients alone
+        ctx.save_for_backward(branch if gate is not None or post_w is not None else None, out, gate,
+                              row_scale, post_w, post_b, pre_w)
         ctx.eps, ctx.branch_dtype = eps, branch.dtype
         ctx.dtypes = tuple(None if t is None else t.dtype
                            for t in (gate, post_w, post_b, pre_w, pre_b))
-        if normed is None:
-            return out
-        return out, normed
+        return out if normed is None else (out, normed)
 
     @staticmethod
     def backward(ctx, grad_out, grad_normed=None):
         branch, out, *params = ctx.saved_tensors
         if branch is None:  # not read
             branch = torch.empty_like(out, dtype=ctx.branch_dtype)
-        g = _norm_gate_backward(grad_out, grad_normed, out, branch, params, ctx.eps)
-        vectors = (None if t is None else t.to(dt) for t, dt in zip(g[2:], ctx.dtypes))
-        return (g.branch, g.residual, *vectors, None, None, None)
+        g = _norm_gate_backward(grad_out, grad_normed, out, branch, *params, ctx.eps)
+        gate, *norms = (None if t is None else t.to(dt) for t, dt in zip(g[2:], ctx.dtypes))
+        return g.branch, g.residual, gate, None, *norms, None
 
 
 def norm_gate_residual(
@@ -479,14 +334,15 @@ def norm_gate_residual(
     0 or 1 / keep; the leading dimensions are cut evenly).  Differentiable in all but
     ``row_scale``.  C at most 4096.
     """
+    post_w, post_b = _pair(post_norm, "post_norm")
+    pre_w, pre_b = _pair(pre_norm, "pre_norm")
     if branch.device.type == "meta":
-        return (torch.empty_like(residual), None if pre_norm is None else torch.empty_like(branch))
-    params = _check_norm_gate(branch, residual, gate, row_scale, post_norm, pre_norm, eps)
-    post, pre = post_norm or (None, None), pre_norm or (None, None)
-    if _needs_grad(branch, residual, gate, *post, *pre):
-        res = _NormGate.apply(branch, residual, gate, *post, *pre, row_scale, params, eps)
-        return res if pre_norm is not None else (res, None)
-    return _norm_gate_forward(branch, residual, params, eps)
+        return torch.empty_like(residual), None if pre_w is None else torch.empty_like(branch)
+    _require_cuda("norm_gate_residual", branch, residual)
+    if _needs_grad(branch, residual, gate, post_w, post_b, pre_w, pre_b):
+        res = _NormGate.apply(branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps)
+        return res if pre_w is not None else (res, None)
+    return _norm_gate_forward(branch, residual, gate, row_scale, post_w, post_b, pre_w, pre_b, eps)
 
 
 def norm_gate_residual_backward(
@@ -503,16 +359,11 @@ def norm_gate_residual_backward(
     """Gradients of :func:`norm_gate_residual` from those of its results, its own ``out`` and
     the forward's arguments; ``grad_normed`` is None without ``pre_norm``.  The norms' and the
     gate's gradients are float32."""
-    params = _check_norm_gate(branch, out, gate, row_scale, post_norm, pre_norm, eps)
-    if grad_out.shape != out.shape or grad_out.dtype != out.dtype:
-        raise ValueError("grad_out must have the shape and dtype of out")
-    if (grad_normed is None) != (pre_norm is None):
-        raise ValueError("grad_normed belongs to pre_norm: give both or neither")
-    if grad_normed is not None and (grad_normed.shape != branch.shape
-                                    or grad_normed.dtype != branch.dtype):
-        raise ValueError("grad_normed must have the shape and dtype of branch")
-    _require_cuda("norm_gate_residual", grad_out, grad_normed)
-    return _norm_gate_backward(grad_out, grad_normed, out, branch, params, eps)
+    post_w, post_b = _pair(post_norm, "post_norm")
+    pre_w, _ = _pair(pre_norm, "pre_norm")
+    _require_cuda("norm_gate_residual", branch, out, grad_out, grad_normed)
+    return _norm_gate_backward(grad_out, grad_normed, out, branch, gate, row_scale, post_w, post_b,
+                               pre_w, eps)
 
 
 # -------------------------------------------------------------- 8-bit activation checkpoints
@@ -530,22 +381,12 @@ def gelu_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, KeptActivation]:
     """``gelu(x)`` (exact, as ``torch.nn.GELU()``) and ``x`` in 8 bits for
     :func:`gelu_checkpoint_backward`.  Called outside autograd (:func:`checkpointed_mlp` is the
     differentiable form)."""
-    if x.ndim < 1 or x.dtype not in _DTYPES:
-        raise TypeError("gelu_checkpoint takes float32, float16 or bfloat16 tensors [..., C]")
     if _needs_grad(x):
         raise RuntimeError("gelu_checkpoint is not differentiable by itself; use "
                            "checkpointed_mlp, or call it under torch.no_grad()")
     _require_cuda("gelu_checkpoint", x)
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    kept = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], -(-x.shape[-1] // GROUP)), dtype=torch.uint8,
-                         device=x.device)
-    token = _prof.kernel_begin("gelu_checkpoint", lambda: {
-        "bytes": x.numel() * (2 * x.element_size() + 1) + scales.numel()})
-    _native.require().gelu_checkpoint(y, kept, scales, x)
-    _prof.count("gelu_checkpoint")
-    _prof.kernel_end(token)
+    y, kept, scales = _launch("gelu_checkpoint", lambda: {
+        "bytes": x.numel() * (2 * x.element_size() + 1 + 1 / GROUP)}, x)
     return y, KeptActivation(kept, scales, x.dtype)
 
 
@@ -553,26 +394,19 @@ def gelu_checkpoint_backward(grad_y: torch.Tensor, kept: KeptActivation
                              ) -> tuple[torch.Tensor, torch.Tensor]:
     """``(grad_x, again)`` from the gradient of ``y``: with ``u`` the kept input, ``grad_y *
     gelu'(u)`` and ``gelu(u)``, the input of the next Linear's weight gradient."""
-    if grad_y.shape != kept.kept.shape or grad_y.dtype != kept.dtype:
+    if grad_y.dtype != kept.dtype:
         raise ValueError("grad_y must have the shape and dtype of the kept activation")
     _require_cuda("gelu_checkpoint_backward", grad_y)
-    grad_y = grad_y.contiguous()
-    grad_x, again = torch.empty_like(grad_y), torch.empty_like(grad_y)
-    token = _prof.kernel_begin("gelu_checkpoint_backward", lambda: {
-        "bytes": grad_y.numel() * (3 * grad_y.element_size() + 1) + kept.scales.numel()})
-    _native.require().gelu_checkpoint_backward(grad_x, again, grad_y, kept.kept, kept.scales)
-    _prof.count("gelu_checkpoint_backward")
-    _prof.kernel_end(token)
-    return grad_x, again
+    return _launch("gelu_checkpoint_backward", lambda: {
+        "bytes": grad_y.numel() * (3 * grad_y.element_size() + 1 + 1 / GROUP)}, grad_y, kept.kept,
+        kept.scales)
 
 
 def restore_activation(kept: KeptActivation) -> torch.Tensor:
     """The kept activation in its own dtype."""
     _require_cuda("restore_activation", kept.kept)
-    x = torch.empty(kept.kept.shape, dtype=kept.dtype, device=kept.kept.device)
-    _native.require().restore_activation(x, kept.kept, kept.scales)
-    _prof.count("restore_activation")
-    return x
+    return _launch("restore_activation", lambda: {
+        "bytes": kept.kept.numel() * (1 + kept.dtype.itemsize)}, kept.kept, kept.scales, kept.dtype)
 
 
 class _Mlp(torch.autograd.Function):
@@ -768,6 +602,36 @@ def disable_training_kernels(model: torch.nn.Module) -> int:
             layer.__dict__["forward"] = eager
     return len(layers)
 
+
+def _fake_norm_gate_backward(grad_out, grad_normed, out, branch, gate, row_scale, post_w, post_b,
+                             pre_w, eps):
+    n = (gate is not None) + 2 * (post_w is not None) + 2 * (pre_w is not None)
+    vector = branch.new_empty(branch.shape[-1:], dtype=torch.float32)
+    return [torch.empty_like(out), torch.empty_like(branch),
+            *(torch.empty_like(vector) for _ in range(n))]
+
+
+# What the ops that return new tensors return, for tracing (shape and dtype only)
+FAKE_IMPLS = {
+    "relative_position_bias": lambda table, pairs, dtype: table.new_empty(
+        (table.shape[1], *pairs.shape), dtype=dtype),
+    "relative_position_bias_backward": lambda grad, order, items, multi, buckets, dtype:
+        grad.new_empty((buckets, grad.shape[0]), dtype=dtype),
+    "swin_window_attention_train": lambda qkv, table, index, nw, ws, ss, scale: qkv.new_empty(
+        (qkv.shape[0], qkv.shape[1], qkv.shape[3] * qkv.shape[4])),
+    "swin_window_attention_backward": lambda grad, qkv, table, pairs, order, items, multi, nw, ws,
+        ss, scale: (qkv.new_empty(qkv.shape), table.new_empty(table.shape)),
+    "norm_gate_residual": lambda branch, residual, gate, scale, post_w, post_b, pre_w, pre_b, eps:
+        [residual.new_empty(residual.shape)]
+        + ([] if pre_w is None else [branch.new_empty(branch.shape)]),
+    "norm_gate_residual_backward": _fake_norm_gate_backward,
+    "gelu_checkpoint": lambda x: (
+        x.new_empty(x.shape), x.new_empty(x.shape, dtype=torch.int8),
+        x.new_empty((*x.shape[:-1], -(-x.shape[-1] // GROUP)), dtype=torch.uint8)),
+    "gelu_checkpoint_backward": lambda grad, kept, scales: (grad.new_empty(grad.shape),
+                                                            grad.new_empty(grad.shape)),
+    "restore_activation": lambda kept, scales, dtype: kept.new_empty(kept.shape, dtype=dtype),
+}
 
 __all__ = [
     "RelativePositionBuckets", "relative_position_buckets", "relative_position_bias",

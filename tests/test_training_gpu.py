@@ -681,9 +681,9 @@ def test_stage_trains_as_the_eager_one(size, amp):
     layer.train()
     from crumpet_b200 import profiling
 
-    before = profiling.counters["swin_window_attention_qkv_backward"]
+    before = profiling.counters["swin_window_attention_backward"]
     out, got = _grads(layer, x, amp)
-    assert profiling.counters["swin_window_attention_qkv_backward"] == before + 2
+    assert profiling.counters["swin_window_attention_backward"] == before + 2
     tol = 2e-2 if amp is None else 6e-2
     assert rel(out, want_out) <= (1e-4 if amp is None else 2e-2)
     for name, w in want.items():
