@@ -147,6 +147,9 @@ def capi() -> ctypes.CDLL:
         lib.crumpet_swin_window_attention_qkv_backward.argtypes = (
             [vp] * 6 + [i32, i64, vp, i64] + [i64] * 9 + [i32] + [i64] * 4 + [f32, vp])
         lib.crumpet_swin_window_attention_qkv_backward.restype = i32
+        lib.crumpet_swin_window_attention_qkv_pairs.argtypes = (
+            [vp, vp, vp, i32, i64, vp] + [i64] * 9 + [i32] + [i64] * 4 + [f32, vp])
+        lib.crumpet_swin_window_attention_qkv_pairs.restype = i32
         lib.crumpet_norm_gate_residual.argtypes = (
             [vp] * 4 + [i32, i32, vp, vp, i64] + [vp] * 4 + [f32, i64, i64, vp])
         lib.crumpet_norm_gate_residual.restype = i32

@@ -1,16 +1,21 @@
 // crumpet_b200: gradient of the window attention for the inputs attention_grad.cu does not
 // take: float32 qkv, head dims 64 to 256, windows of more than 352 tokens, unaligned tensors.
 //
-// The formulas of attention_grad.cu in plain fp32 arithmetic, in three kernels that stream
-// tiles of the other side through shared memory (fp32, 32 tokens at a time):
+// The formulas of attention_grad.cu in plain fp32 arithmetic.  Tiles of 32 tokens of the other
+// side stream through shared memory (as fp32):
+//   * forward: one query row per lane group, online softmax (no gradient; the training forward of
+//              the same inputs);
 //   * rows:    one query row per lane group; a first sweep over the keys takes the row's
 //              statistics with an online softmax (maximum, sum, sum of p dp), a second dq;
 //   * columns: one key row per lane group, one sweep over the queries for dk and dv;
 //   * bias:    one 32 x 32 tile of (query, key) pairs of one head per CTA, summed over the
 //              windows of its share in registers.
-// A row belongs to TPR = max(1, D / 32) neighbouring lanes of E = D / TPR channels, whose
-// partial products are added with shuffles.  fp32 FMA work bounds it: 11 products of depth D
-// per score, three of them the repeated scores.
+// A row belongs to 4 lanes that share out the other side's tokens (head dims up to 32: each lane
+// keeps the row's channels in registers, so a product is free of shuffles, and four times the
+// threads hide the latency of small batches), or to D / 32 lanes of 32 channels each, whose
+// partial products are added with shuffles.  The bias (+ mask) of the CTA's rows is gathered
+// into shared memory once where it fits.  fp32 FMA work bounds it: 11 products of depth D per
+// score, three of them the repeated scores.
 #include <cmath>
 
 #include "common.cuh"
@@ -34,8 +39,10 @@ struct Params {
   const int* pairs;   // [N, N]
   int table_f32, analytic;
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
-  int B, H, N, QB, S;
+  int B, H, N, QB, S, bias_pitch;
+  int vec;            // every tensor on 16-byte boundaries: four channels per load
   float scale;
+  void* out;          // forward: [B, N, H, D]
 };
 
 template <typename T>
@@ -76,27 +83,42 @@ __device__ __forceinline__ uint32_t last_axes(const Params& p, int b) {
          (uint32_t(p.ssw != 0 && iw == p.nww - 1) << 2);
 }
 
-// bias (+ mask) of one pair times log2 e
+// Four consecutive channels as fp32
 template <typename T>
-__device__ __forceinline__ float extra(const Params& p, int h, int i, int j, uint32_t last) {
-  const long long t = p.pairs[(long long)i * p.N + j];
-  float v = p.table_f32 ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
-                        : load(static_cast<const T*>(p.table), t * p.H + h);
-  if (last != 0 && ((side_code(p, i) ^ side_code(p, j)) & last)) v += -100.f;
-  return v * kLog2e;
+__device__ __forceinline__ float4 load4(const Params& p, const T* at) {
+  if (p.vec) {
+    if constexpr (sizeof(T) == 4) {
+      return __ldg(reinterpret_cast<const float4*>(at));
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
+      const T* v = reinterpret_cast<const T*>(&w);
+      return make_float4(float(v[0]), float(v[1]), float(v[2]), float(v[3]));
+    }
+  }
+  return make_float4(load(at, 0), load(at, 1), load(at, 2), load(at, 3));
+}
+
+// bias of one bucket times log2 e
+template <typename T>
+__device__ __forceinline__ float bias_of(const Params& p, int h, long long t) {
+  return kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
+                               : load(static_cast<const T*>(p.table), t * p.H + h));
 }
 
 template <int D>
 struct Shape {
-  static constexpr int TPR = D >= 64 ? D / 32 : 1;
-  static constexpr int E = D / TPR;
-  static constexpr int R = kThreads / TPR;            // rows per CTA
-  static constexpr int SLICE = E + (TPR > 1 ? 4 : 0);  // slices of a row in different banks
+  static constexpr int KL = D <= 32 ? 4 : 1;            // lanes that share out the tokens
+  static constexpr int TPR = D <= 32 ? 1 : D / 32;      // lanes that share out the channels
+  static constexpr int LANES = KL * TPR;                // lanes per row
+  static constexpr int E = D / TPR;                     // channels per lane
+  static constexpr int R = kThreads / LANES;            // rows per CTA
+  static constexpr int SLICE = E + 4;  // slices (of a row, or of the KL rows read at once) in
+                                       // different banks
   static constexpr int ROW = TPR * SLICE;
-  static constexpr int PAD = kTile + 1;
-  static constexpr int SMEM = (2 * kTile * ROW + R * PAD) * 4 + kTile * 8;
+  static constexpr int STAGED = 2 * kTile * ROW * 4 + kTile * 8;  // bytes of a tile and statistics
   static_assert(E % 4 == 0 && E <= 32, "channels per lane");
 };
+constexpr int kBiasBytes = 64 * 1024;  // most shared memory for the bias of a CTA's rows
 
 template <typename S>
 __device__ __forceinline__ float dot(const float (&a)[S::E], const float* row) {
@@ -124,27 +146,45 @@ __device__ __forceinline__ void add(float (&a)[S::E], float w, const float* row)
     a[4 * e + 3] = fmaf(w, v.w, a[4 * e + 3]);
   }
 }
+// sums over the lanes that share out the tokens
+template <typename S>
+__device__ __forceinline__ float over_tokens(float v) {
+#pragma unroll
+  for (int o = 1; o < S::KL; o <<= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+template <typename S>
+__device__ __forceinline__ void over_tokens(float (&a)[S::E]) {
+#pragma unroll
+  for (int e = 0; e < S::E; ++e) a[e] = over_tokens<S>(a[e]);
+}
 
 // kTile token rows starting at j0 (zero past N) as fp32 into pitched shared memory
 template <typename T, int D>
-__device__ __forceinline__ void stage(float* dst, const T* src, long long stride, int j0, int N) {
+__device__ __forceinline__ void stage(const Params& p, float* dst, const T* src, long long stride,
+                                      int j0) {
   using S = Shape<D>;
-  for (int f = threadIdx.x; f < kTile * D; f += kThreads) {
-    const int j = f / D, d = f % D;
-    dst[j * S::ROW + (d / S::E) * S::SLICE + d % S::E] =
-        j0 + j < N ? load(src, (long long)(j0 + j) * stride + d) : 0.f;
+#pragma unroll 4
+  for (int f = threadIdx.x; f < kTile * (D / 4); f += kThreads) {
+    const int j = f / (D / 4), d = f % (D / 4) * 4;
+    *reinterpret_cast<float4*>(dst + j * S::ROW + (d / S::E) * S::SLICE + d % S::E) =
+        j0 + j < p.N ? load4(p, src + (j0 + j) * stride + d) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
-template <typename T, int D, bool COLS>
+enum Mode { kForward, kRows, kCols };
+
+template <typename T, int D, int MODE>
 __global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
   using S = Shape<D>;
+  constexpr bool COLS = MODE == kCols;
   extern __shared__ float4 smem4[];
   float* xs = reinterpret_cast<float*>(smem4);       // K (or Q) rows
   float* ys = xs + kTile * S::ROW;                   // V (or dO) rows
-  float* tile = ys + kTile * S::ROW;                 // bias + mask of rows x streamed tokens
-  float2* stat = reinterpret_cast<float2*>(tile + S::R * S::PAD + ((S::R * S::PAD) & 1));
-  const int tid = threadIdx.x, row = tid / S::TPR, part = tid % S::TPR;
+  float2* stat = reinterpret_cast<float2*>(ys + kTile * S::ROW);
+  float* tile = reinterpret_cast<float*>(stat + kTile);  // bias + mask [row][pitch]
+  const int tid = threadIdx.x, row = tid / S::LANES;
+  const int part = tid % S::TPR, first = tid % S::KL;  // channel slice, first token of a tile
   long long blk = blockIdx.x;
   const int qb = int(blk % p.QB);
   blk /= p.QB;
@@ -159,84 +199,148 @@ __global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
   const T* g = static_cast<const T*>(p.dout) + (long long)b * p.N * hd + h * D;
   float2* stats = p.stats + ((long long)b * p.H + h) * p.N;
 
-  // this row's own two vectors: q and do (rows), k and v (columns)
+  // this row's own vectors: q and do (rows), k and v (columns)
   float a0[S::E], a1[S::E];
+  auto own = [&](float (&x)[S::E], const T* at) {
 #pragma unroll
-  for (int e = 0; e < S::E; ++e) {
-    const long long d = part * S::E + e;
-    a0[e] = valid ? load(COLS ? k : q, i * tok + d) : 0.f;
-    a1[e] = !valid ? 0.f : COLS ? load(v, i * tok + d) : load(g, i * hd + d);
-  }
+    for (int e = 0; e < S::E; e += 4) {
+      const float4 w = valid ? load4(p, at + part * S::E + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[e] = w.x, x[e + 1] = w.y, x[e + 2] = w.z, x[e + 3] = w.w;
+    }
+  };
+  own(a0, (COLS ? k : q) + i * tok);
+  if constexpr (MODE == kRows) own(a1, g + i * hd);
+  if constexpr (COLS) own(a1, v + i * tok);
   const float c1 = p.scale * kLog2e;
+  // the bias (+ mask) of `cols` tokens from j0 on, for the CTA's rows: lanes along the keys, which
+  // neighbour in `pairs`, eight gathers in flight per thread
+  const int whole = p.bias_pitch;  // the pitch of all of it in shared memory, or 0: tile by tile
+  const int pitch = whole ? whole : kTile + 1;
+  const int warp = tid / 32, lane = tid % 32;
+  // roll-side codes of the CTA's rows and of the gathered tokens (windows at a seam only)
+  uint8_t* row_code = reinterpret_cast<uint8_t*>(tile + S::R * pitch);
+  uint8_t* tok_code = row_code + S::R;
+  auto gather = [&](int j0, int cols) {
+    if (last != 0) {
+      for (int f = tid; f < S::R + cols; f += kThreads) {
+        const int t = f < S::R ? r0 + f : j0 + f - S::R;
+        row_code[f] = t < p.N ? uint8_t(side_code(p, t)) : uint8_t(0);
+      }
+      __syncthreads();  // `last` is the CTA's
+    }
+    auto value = [&](int r, int j) {
+      const int gi = r0 + r, gj = j0 + j;
+      if (gj >= p.N) return -INFINITY;  // past the end: drops out of the softmax
+      if (gi >= p.N) return 0.f;
+      float x = bias_of<T>(p, h, p.pairs[(long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj)]);
+      if (last != 0 && ((row_code[r] ^ tok_code[j]) & last)) x += -100.f * kLog2e;
+      return x;
+    };
+    constexpr int WARPS = kThreads / 32;
+    if constexpr (COLS) {
+      for (int r = lane; r < S::R; r += 32)
+#pragma unroll 8
+        for (int j = warp; j < cols; j += WARPS) tile[r * pitch + j] = value(r, j);
+    } else {
+      for (int j = lane; j < cols; j += 32)
+#pragma unroll 8
+        for (int r = warp; r < S::R; r += WARPS) tile[r * pitch + j] = value(r, j);
+    }
+  };
+  if (whole) gather(0, (p.N + kTile - 1) / kTile * kTile);
   auto fetch = [&](int j0) {
     __syncthreads();  // the previous tile is no longer read
-    stage<T, D>(xs, COLS ? q : k, tok, j0, p.N);
-    stage<T, D>(ys, COLS ? g : v, COLS ? hd : tok, j0, p.N);
-    for (int f = tid; f < S::R * kTile; f += kThreads) {
-      // along the keys, which neighbour in `pairs`
-      const int r = COLS ? f % S::R : f / kTile, j = COLS ? f / S::R : f % kTile;
-      const int gi = r0 + r, gj = j0 + j;
-      float x = -INFINITY;  // past the end: drops out of the softmax
-      if (gj < p.N) x = gi < p.N ? extra<T>(p, h, COLS ? gj : gi, COLS ? gi : gj, last) : 0.f;
-      tile[r * S::PAD + j] = x;
-    }
+    stage<T, D>(p, xs, COLS ? q : k, tok, j0);
+    stage<T, D>(p, ys, COLS ? g : v, COLS ? hd : tok, j0);
+    if (!whole) gather(j0, kTile);
     if (COLS && tid < kTile) stat[tid] = j0 + tid < p.N ? stats[j0 + tid] : make_float2(0.f, 0.f);
     __syncthreads();
+    return tile + row * pitch + (whole ? j0 : 0);
   };
 
   if constexpr (!COLS) {
-    float m = -INFINITY, l = 0.f, dp = 0.f;
-    for (int j0 = 0; j0 < p.N; j0 += kTile) {
-      fetch(j0);
-      float s[kTile], mc = m;
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) {
-        s[j] = fmaf(dot<S>(a0, xs + j * S::ROW + part * S::SLICE), c1, tile[row * S::PAD + j]);
-        mc = fmaxf(mc, s[j]);
-      }
-      const float alpha = exp2f(m - mc);  // the first tile: 2^-inf = 0
-      l *= alpha;
-      dp *= alpha;
-      m = mc;
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) {
-        const float e = exp2f(s[j] - m);
-        l += e;
-        dp = fmaf(e, dot<S>(a1, ys + j * S::ROW + part * S::SLICE), dp);
-      }
-    }
-    const float lse = m + log2f(l), delta = dp / l;
-    if (valid && part == 0) stats[i] = make_float2(lse, delta);
+    // per lane: maximum, sum of exponentials, and the sum of p dp or (forward) of p v
+    float m = -1e30f, l = 0.f, dp = 0.f;
     float acc[S::E] = {};
     for (int j0 = 0; j0 < p.N; j0 += kTile) {
-      fetch(j0);
-#pragma unroll 4
-      for (int j = 0; j < kTile; ++j) {
-        const float* xr = xs + j * S::ROW + part * S::SLICE;
-        const float e = exp2f(fmaf(dot<S>(a0, xr), c1, tile[row * S::PAD + j]) - lse);
-        add<S>(acc, e * (dot<S>(a1, ys + j * S::ROW + part * S::SLICE) - delta), xr);
+      const float* bias = fetch(j0);
+      float s[kTile / S::KL], mc = m;
+#pragma unroll
+      for (int n = 0; n < kTile / S::KL; ++n) {
+        const int j = first + n * S::KL;
+        s[n] = fmaf(dot<S>(a0, xs + j * S::ROW + part * S::SLICE), c1, bias[j]);
+        mc = fmaxf(mc, s[n]);
+      }
+      const float alpha = exp2f(m - mc);
+      l *= alpha;
+      dp *= alpha;
+      if constexpr (MODE == kForward) {
+#pragma unroll
+        for (int e = 0; e < S::E; ++e) acc[e] *= alpha;
+      }
+      m = mc;
+#pragma unroll
+      for (int n = 0; n < kTile / S::KL; ++n) {
+        const float* yr = ys + (first + n * S::KL) * S::ROW + part * S::SLICE;
+        const float e = exp2f(s[n] - m);
+        l += e;
+        if constexpr (MODE == kForward) add<S>(acc, e, yr);
+        else dp = fmaf(e, dot<S>(a1, yr), dp);
       }
     }
-    if (!valid) return;
-    T* out = static_cast<T*>(p.dqkv) + ((long long)b * p.N + i) * tok + h * D + part * S::E;
+    float top = m;
 #pragma unroll
-    for (int e = 0; e < S::E; ++e) out[e] = store_as<T>(acc[e] * p.scale);
+    for (int o = 1; o < S::KL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const float f = exp2f(m - top);
+    l = over_tokens<S>(l * f);
+    if constexpr (MODE == kForward) {
+#pragma unroll
+      for (int e = 0; e < S::E; ++e) acc[e] *= f;
+      over_tokens<S>(acc);
+      if (!valid || first != 0) return;
+      T* out = static_cast<T*>(p.out) + ((long long)b * p.N + i) * hd + h * D + part * S::E;
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int e = 0; e < S::E; ++e) out[e] = store_as<T>(acc[e] * inv);
+    } else {
+      dp = over_tokens<S>(dp * f);
+      const float lse = top + log2f(l), delta = dp / l;
+      if (valid && part == 0 && first == 0) stats[i] = make_float2(lse, delta);
+      for (int j0 = 0; j0 < p.N; j0 += kTile) {
+        const float* bias = fetch(j0);
+#pragma unroll 4
+        for (int n = 0; n < kTile / S::KL; ++n) {
+          const int j = first + n * S::KL;
+          const float* xr = xs + j * S::ROW + part * S::SLICE;
+          const float e = exp2f(fmaf(dot<S>(a0, xr), c1, bias[j]) - lse);
+          add<S>(acc, e * (dot<S>(a1, ys + j * S::ROW + part * S::SLICE) - delta), xr);
+        }
+      }
+      over_tokens<S>(acc);
+      if (!valid || first != 0) return;
+      T* out = static_cast<T*>(p.dqkv) + ((long long)b * p.N + i) * tok + h * D + part * S::E;
+#pragma unroll
+      for (int e = 0; e < S::E; ++e) out[e] = store_as<T>(acc[e] * p.scale);
+    }
   } else {
     float dk[S::E] = {}, dv[S::E] = {};
     for (int j0 = 0; j0 < p.N; j0 += kTile) {
-      fetch(j0);
+      const float* bias = fetch(j0);
 #pragma unroll 4
-      for (int j = 0; j < kTile; ++j) {
+      for (int n = 0; n < kTile / S::KL; ++n) {
+        const int j = first + n * S::KL;
         const float* xr = xs + j * S::ROW + part * S::SLICE;
         const float* yr = ys + j * S::ROW + part * S::SLICE;
         const float2 st = stat[j];
-        const float e = exp2f(fmaf(dot<S>(a0, xr), c1, tile[row * S::PAD + j]) - st.x);
+        const float e = exp2f(fmaf(dot<S>(a0, xr), c1, bias[j]) - st.x);
         const float ds = e * (dot<S>(a1, yr) - st.y);
         add<S>(dv, e, yr);
         add<S>(dk, ds, xr);
       }
     }
-    if (!valid) return;
+    over_tokens<S>(dk);
+    over_tokens<S>(dv);
+    if (!valid || first != 0) return;
     T* out = static_cast<T*>(p.dqkv) + ((long long)b * p.N + i) * tok + hd + h * D + part * S::E;
 #pragma unroll
     for (int e = 0; e < S::E; ++e) {
@@ -246,12 +350,12 @@ __global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
   }
 }
 
-// dbias of one 32 x 32 tile of pairs of one head, over the windows of one share: a thread
-// keeps 8 pairs.  Channels pass through shared memory 32 at a time.
-template <typename T>
+// dbias of one 32 x 32 tile of pairs of one head, over the windows of one share.  A thread keeps
+// one key and 8 queries; CH channels at a time, the key's in registers, the queries' read from
+// shared memory by all threads at once.
+template <typename T, int CH>
 __global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p, int D) {
-  constexpr int CH = 32, P = CH + 1;
-  __shared__ float qs[kTile * P], gs[kTile * P], ks[kTile * P], vs[kTile * P];
+  __shared__ __align__(16) float qs[kTile * CH], gs[kTile * CH];
   const int tiles = (p.N + kTile - 1) / kTile;
   long long blk = blockIdx.x;
   const int share = int(blk % p.S);
@@ -259,17 +363,18 @@ __global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p
   const int jt = int(blk % tiles);
   blk /= tiles;
   const int it = int(blk % tiles), h = int(blk / tiles);
-  const int jj = threadIdx.x % kTile, j = jt * kTile + jj;
+  const int j = jt * kTile + threadIdx.x % kTile;
   const int ib = threadIdx.x / kTile * 8;  // this thread's 8 query rows
   const long long hd = (long long)p.H * D, tok = 3 * hd;
   const float c1 = p.scale * kLog2e;
-  float base[8], apart[8], sum[8];
+  float base[8], sum[8];
+  uint32_t apart[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int i = it * kTile + ib + u;
     const bool in = i < p.N && j < p.N;
-    base[u] = in ? extra<T>(p, h, i, j, 0u) : 0.f;
-    apart[u] = in && p.analytic ? float(side_code(p, i) ^ side_code(p, j)) : 0.f;
+    base[u] = in ? bias_of<T>(p, h, p.pairs[(long long)i * p.N + j]) : 0.f;
+    apart[u] = in && p.analytic ? side_code(p, i) ^ side_code(p, j) : 0u;
     sum[u] = 0.f;
   }
   for (int b = share; b < p.B; b += p.S) {
@@ -277,23 +382,38 @@ __global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p
     const T* g = static_cast<const T*>(p.dout) + (long long)b * p.N * hd + h * D;
     float s[8] = {}, d[8] = {};
     for (int c0 = 0; c0 < D; c0 += CH) {
-      const int w = min(CH, D - c0);
-      __syncthreads();
-      for (int f = threadIdx.x; f < kTile * CH; f += kThreads) {
-        const int r = f / CH, c = f % CH;
-        const int i = it * kTile + r, k = jt * kTile + r;
-        qs[r * P + c] = i < p.N && c < w ? load(q, i * tok + c0 + c) : 0.f;
-        gs[r * P + c] = i < p.N && c < w ? load(g, i * hd + c0 + c) : 0.f;
-        ks[r * P + c] = k < p.N && c < w ? load(q, k * tok + hd + c0 + c) : 0.f;
-        vs[r * P + c] = k < p.N && c < w ? load(q, k * tok + 2 * hd + c0 + c) : 0.f;
+      float kr[CH], vr[CH];
+      const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < CH; c += 4) {
+        const float4 x = j < p.N ? load4(p, q + j * tok + hd + c0 + c) : z;
+        const float4 y = j < p.N ? load4(p, q + j * tok + 2 * hd + c0 + c) : z;
+        kr[c] = x.x, kr[c + 1] = x.y, kr[c + 2] = x.z, kr[c + 3] = x.w;
+        vr[c] = y.x, vr[c + 1] = y.y, vr[c + 2] = y.z, vr[c + 3] = y.w;
       }
       __syncthreads();
-      for (int c = 0; c < w; ++c) {
-        const float kk = ks[jj * P + c], vv = vs[jj * P + c];
+#pragma unroll 2
+      for (int f = threadIdx.x; f < kTile * CH / 4; f += kThreads) {
+        const int i = it * kTile + f / (CH / 4), c = c0 + f % (CH / 4) * 4;
+        reinterpret_cast<float4*>(qs)[f] = i < p.N ? load4(p, q + i * tok + c) : z;
+        reinterpret_cast<float4*>(gs)[f] = i < p.N ? load4(p, g + i * hd + c) : z;
+      }
+      __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          s[u] = fmaf(qs[(ib + u) * P + c], kk, s[u]);
-          d[u] = fmaf(gs[(ib + u) * P + c], vv, d[u]);
+      for (int u = 0; u < 8; ++u) {
+        const float4* qr = reinterpret_cast<const float4*>(qs + (ib + u) * CH);
+        const float4* gr = reinterpret_cast<const float4*>(gs + (ib + u) * CH);
+#pragma unroll
+        for (int e = 0; e < CH / 4; ++e) {
+          const float4 x = qr[e], y = gr[e];
+          s[u] = fmaf(x.x, kr[4 * e], s[u]);
+          d[u] = fmaf(y.x, vr[4 * e], d[u]);
+          s[u] = fmaf(x.y, kr[4 * e + 1], s[u]);
+          d[u] = fmaf(y.y, vr[4 * e + 1], d[u]);
+          s[u] = fmaf(x.z, kr[4 * e + 2], s[u]);
+          d[u] = fmaf(y.z, vr[4 * e + 2], d[u]);
+          s[u] = fmaf(x.w, kr[4 * e + 3], s[u]);
+          d[u] = fmaf(y.w, vr[4 * e + 3], d[u]);
         }
       }
     }
@@ -305,7 +425,7 @@ __global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p
       if (i >= p.N || j >= p.N) continue;
       const float2 st = stats[i];
       float x = fmaf(s[u], c1, base[u]);
-      if (uint32_t(apart[u]) & last) x += -100.f * kLog2e;
+      if (apart[u] & last) x += -100.f * kLog2e;
       sum[u] += exp2f(x - st.x) * (d[u] - st.y);
     }
   }
@@ -317,8 +437,20 @@ __global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p
   }
 }
 
+template <class K>
+int start(K kernel, long long blocks, int smem, const Params& p, cudaStream_t stream) {
+  if (smem > 32 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return set_cuda_error(e, "attention (simt) smem attribute");
+  }
+  kernel<<<unsigned(blocks), kThreads, smem, stream>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? kOk : set_cuda_error(e, "attention (simt) launch");
+}
+
 template <typename T, int D>
-int launch(Params p, cudaStream_t stream) {
+int launch(Params p, bool forward, cudaStream_t stream) {
   using S = Shape<D>;
   p.QB = (p.N + S::R - 1) / S::R;
   const long long blocks = (long long)p.B * p.H * p.QB;
@@ -326,49 +458,39 @@ int launch(Params p, cudaStream_t stream) {
   const long long bias_blocks = tiles * tiles * p.H * p.S;
   if (blocks > 0x7fffffffLL || bias_blocks > 0x7fffffffLL)
     return set_error(kErrInvalid, "too many windows x heads for one launch");
-  auto rows = grad_simt_kernel<T, D, false>;
-  auto cols = grad_simt_kernel<T, D, true>;
-  constexpr int smem = S::SMEM + 16;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(rows, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(cols, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return set_cuda_error(e, "attention gradient (simt) smem attribute");
-  }
-  rows<<<unsigned(blocks), kThreads, smem, stream>>>(p);
-  cols<<<unsigned(blocks), kThreads, smem, stream>>>(p);
-  grad_bias_simt_kernel<T><<<unsigned(bias_blocks), kThreads, 0, stream>>>(p, D);
+  // an odd pitch: lanes of neighbouring rows read different banks
+  const int pitch = int(tiles) * kTile + 1;
+  p.bias_pitch = S::R * pitch * 4 <= kBiasBytes ? pitch : 0;
+  const int smem = S::STAGED + S::R * (p.bias_pitch ? pitch : kTile + 1) * 4 + S::R +
+                   (p.bias_pitch ? int(tiles) * kTile : kTile);
+  if (forward) return start(grad_simt_kernel<T, D, kForward>, blocks, smem, p, stream);
+  if (int e = start(grad_simt_kernel<T, D, kRows>, blocks, smem, p, stream)) return e;
+  if (int e = start(grad_simt_kernel<T, D, kCols>, blocks, smem, p, stream)) return e;
+  constexpr int CH = D < 32 ? D : 32;
+  grad_bias_simt_kernel<T, CH><<<unsigned(bias_blocks), kThreads, 0, stream>>>(p, D);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "attention gradient (simt) launch");
 }
 
 template <typename T>
-int dispatch(const Params& p, int head_dim, cudaStream_t stream) {
+int dispatch(const Params& p, int head_dim, bool forward, cudaStream_t stream) {
   switch (head_dim) {
-    case 16: return launch<T, 16>(p, stream);
-    case 32: return launch<T, 32>(p, stream);
-    case 64: return launch<T, 64>(p, stream);
-    case 128: return launch<T, 128>(p, stream);
-    default: return launch<T, 256>(p, stream);
+    case 16: return launch<T, 16>(p, forward, stream);
+    case 32: return launch<T, 32>(p, forward, stream);
+    case 64: return launch<T, 64>(p, forward, stream);
+    case 128: return launch<T, 128>(p, forward, stream);
+    default: return launch<T, 256>(p, forward, stream);
   }
 }
 
-}  // namespace
-
-// Shares of the windows for the bias kernel: enough CTAs for the GPU's SMs, eight per SM.
-int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N) {
-  const int64_t tiles = (N + kTile - 1) / kTile;
-  const int64_t s = 148 * 8 / (tiles * tiles * H);
-  return s < 1 ? 1 : s > B ? (B > 0 ? B : 1) : s > 16 ? 16 : s;
-}
-
-int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream) {
+int launch_any(const AttnGradArgs& a, void* out, bool forward, cudaStream_t stream) {
   Params p{};
   p.qkv = a.qkv;
   p.dout = a.grad_out;
   p.dqkv = a.grad_qkv;
   p.dbias = a.grad_bias;
   p.stats = reinterpret_cast<float2*>(a.stats);
+  p.out = out;
   p.table = a.table;
   p.pairs = a.pairs;
   p.table_f32 = a.table_f32 ? 1 : 0;
@@ -387,9 +509,27 @@ int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream) {
   p.N = int(a.N);
   p.S = int(a.shares);
   p.scale = a.scale;
-  if (a.dtype == kF32) return dispatch<float>(p, int(a.head_dim), stream);
-  if (a.dtype == kF16) return dispatch<__half>(p, int(a.head_dim), stream);
-  return dispatch<__nv_bfloat16>(p, int(a.head_dim), stream);
+  p.vec = ((reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.grad_out)) & 15u) == 0;
+  if (a.dtype == kF32) return dispatch<float>(p, int(a.head_dim), forward, stream);
+  if (a.dtype == kF16) return dispatch<__half>(p, int(a.head_dim), forward, stream);
+  return dispatch<__nv_bfloat16>(p, int(a.head_dim), forward, stream);
+}
+
+}  // namespace
+
+// Shares of the windows for the bias kernel: enough CTAs for the GPU's SMs, eight per SM.
+int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N) {
+  const int64_t tiles = (N + kTile - 1) / kTile;
+  const int64_t s = 148 * 8 / (tiles * tiles * H);
+  return s < 1 ? 1 : s > B ? (B > 0 ? B : 1) : s > 16 ? 16 : s;
+}
+
+int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream) {
+  return launch_any(a, nullptr, false, stream);
+}
+
+int launch_attention_train_simt(const AttnGradArgs& a, void* out, cudaStream_t stream) {
+  return launch_any(a, out, true, stream);
 }
 
 }  // namespace crumpet

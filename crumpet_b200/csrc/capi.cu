@@ -484,12 +484,14 @@ int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N
                                                         : attention_grad_shares_simt(B, H, N);
 }
 
-int crumpet_swin_window_attention_qkv_backward(
-    void* grad_qkv, float* grad_bias, float* stats, const void* grad_out, const void* qkv,
-    const void* bias_table, int table_f32, int64_t table_rows, const int* pairs, int64_t shares,
-    int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d, int64_t ws_h, int64_t ws_w,
-    int64_t ss_d, int64_t ss_h, int64_t ss_w, int dtype, int64_t B, int64_t H, int64_t N,
-    int64_t head_dim, float scale, void* stream) {
+}  // extern "C"
+
+namespace {
+
+// Checks of the packed-qkv attention by pairs, forward and backward
+int check_train_attention(int dtype, int64_t B, int64_t H, int64_t N, int64_t head_dim, float scale,
+                          int64_t table_rows, const int64_t* nw, const int64_t* ws,
+                          const int64_t* ss) {
   if (int e = check_dtype(dtype)) return e;
   if (!simt_attention_head_dim(head_dim))
     return set_error(kErrUnsupported,
@@ -499,63 +501,100 @@ int crumpet_swin_window_attention_qkv_backward(
     return set_error(kErrUnsupported, "window attention requires a finite scale > 0");
   if (B > 0x7fffffff || H > 0xffff || N > 46340)
     return set_error(kErrInvalid, "B, H or N too large");
-  const bool shifted = (ss_d | ss_h | ss_w) != 0;
-  if (shifted) {
-    const int64_t ws[3] = {ws_d, ws_h, ws_w}, ss[3] = {ss_d, ss_h, ss_w};
-    if (nw_d < 1 || nw_h < 1 || nw_w < 1 || ws_d < 1 || ws_h < 1 || ws_w < 1 ||
-        ws_d * ws_h * ws_w != N)
+  if (table_rows < 1) return set_error(kErrInvalid, "relative position bias table has no rows");
+  if ((ss[0] | ss[1] | ss[2]) == 0) return kOk;
+  int64_t windows = 1;
+  for (int a = 0; a < 3; ++a) {
+    if (nw[a] < 1 || ws[a] < 1 || ws[a] > N)
       return set_error(kErrInvalid, "analytic mask geometry does not match N");
-    if (nw_d > 0xffff || nw_h > 0xffff || nw_w > 0xffff || nw_d * nw_h * nw_w > 0x7fffffff)
-      return set_error(kErrInvalid, "too many windows per axis");
-    for (int a = 0; a < 3; ++a)
-      if (ss[a] < 0 || ss[a] >= ws[a])
-        return set_error(kErrInvalid, "analytic mask shift must satisfy 0 <= shift < window");
+    if (nw[a] > 0xffff) return set_error(kErrInvalid, "too many windows per axis");
+    if (ss[a] < 0 || ss[a] >= ws[a])
+      return set_error(kErrInvalid, "analytic mask shift must satisfy 0 <= shift < window");
+    windows *= nw[a];
   }
-  const bool sized = attention_grad_tensor_path(dtype, H, N, head_dim);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(grad_qkv) |
-                         reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(qkv);
+  if (ws[0] * ws[1] * ws[2] != N)
+    return set_error(kErrInvalid, "analytic mask geometry does not match N");
+  if (windows > 0x7fffffff) return set_error(kErrInvalid, "too many windows");
+  return kOk;
+}
+
+AttnGradArgs train_args(const void* qkv, const void* bias_table, int table_f32, const int* pairs,
+                        const int64_t* nw, const int64_t* ws, const int64_t* ss, int dtype,
+                        int64_t B, int64_t H, int64_t N, int64_t head_dim, float scale) {
+  AttnGradArgs a{};
+  a.qkv = qkv;
+  a.table = bias_table;
+  a.table_f32 = table_f32 != 0 || dtype == kF32;
+  a.pairs = pairs;
+  for (int x = 0; x < 3; ++x) {
+    a.nwin[x] = nw[x];
+    a.win[x] = ws[x];
+    a.shift[x] = ss[x];
+  }
+  a.B = B;
+  a.H = H;
+  a.N = N;
+  a.head_dim = head_dim;
+  a.shares = 1;
+  a.scale = scale;
+  a.dtype = dtype;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int crumpet_swin_window_attention_qkv_pairs(void* out, const void* qkv, const void* bias_table,
+                                            int table_f32, int64_t table_rows, const int* pairs,
+                                            int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d,
+                                            int64_t ws_h, int64_t ws_w, int64_t ss_d, int64_t ss_h,
+                                            int64_t ss_w, int dtype, int64_t B, int64_t H,
+                                            int64_t N, int64_t head_dim, float scale,
+                                            void* stream) {
+  const int64_t nw[3] = {nw_d, nw_h, nw_w}, ws[3] = {ws_d, ws_h, ws_w}, ss[3] = {ss_d, ss_h, ss_w};
+  if (int e = check_train_attention(dtype, B, H, N, head_dim, scale, table_rows, nw, ws, ss))
+    return e;
+  if (B == 0) return kOk;
+  if (!out || !qkv || !bias_table || !pairs) return set_error(kErrInvalid, "null tensor pointer");
+  const AttnGradArgs a = train_args(qkv, bias_table, table_f32, pairs, nw, ws, ss, dtype, B, H, N,
+                                    head_dim, scale);
+  return launch_attention_train_simt(a, out, static_cast<cudaStream_t>(stream));
+}
+
+int crumpet_swin_window_attention_qkv_backward(
+    void* grad_qkv, float* grad_bias, float* stats, const void* grad_out, const void* qkv,
+    const void* bias_table, int table_f32, int64_t table_rows, const int* pairs, int64_t shares,
+    int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d, int64_t ws_h, int64_t ws_w,
+    int64_t ss_d, int64_t ss_h, int64_t ss_w, int dtype, int64_t B, int64_t H, int64_t N,
+    int64_t head_dim, float scale, void* stream) {
+  const int64_t nw[3] = {nw_d, nw_h, nw_w}, ws[3] = {ws_d, ws_h, ws_w}, ss[3] = {ss_d, ss_h, ss_w};
+  if (int e = check_train_attention(dtype, B, H, N, head_dim, scale, table_rows, nw, ws, ss))
+    return e;
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
   if (shares < 1 || shares > 0xffff || shares > (B > 0 ? B : 1))
     return set_error(kErrInvalid, "shares must be between 1 and the number of windows");
   if (H * ((N + 63) / 64) * shares > 0x7fffffff)
     return set_error(kErrInvalid, "too many windows x heads for one launch");
   if (!grad_bias) return set_error(kErrInvalid, "null tensor pointer");
   if (B == 0) {  // no window: no gradient of the bias
-    const cudaError_t e = cudaMemsetAsync(grad_bias, 0, size_t(H * N * N) * sizeof(float),
-                                          static_cast<cudaStream_t>(stream));
+    const cudaError_t e = cudaMemsetAsync(grad_bias, 0, size_t(H * N * N) * sizeof(float), on);
     return e == cudaSuccess ? kOk : set_cuda_error(e, "window attention backward memset");
   }
   if (!grad_qkv || !stats || !grad_out || !qkv || !bias_table || !pairs)
     return set_error(kErrInvalid, "null tensor pointer");
-  if (table_rows < 1) return set_error(kErrInvalid, "relative position bias table has no rows");
   if (reinterpret_cast<uintptr_t>(stats) & 15u)
     return set_error(kErrInvalid, "stats must be 16-byte aligned");
-  AttnGradArgs a{};
+  AttnGradArgs a = train_args(qkv, bias_table, table_f32, pairs, nw, ws, ss, dtype, B, H, N,
+                              head_dim, scale);
   a.grad_qkv = grad_qkv;
   a.grad_bias = grad_bias;
   a.stats = stats;
   a.grad_out = grad_out;
-  a.qkv = qkv;
-  a.table = bias_table;
-  a.table_f32 = table_f32 != 0 || dtype == kF32;
-  a.pairs = pairs;
-  a.nwin[0] = nw_d;
-  a.nwin[1] = nw_h;
-  a.nwin[2] = nw_w;
-  a.win[0] = ws_d;
-  a.win[1] = ws_h;
-  a.win[2] = ws_w;
-  a.shift[0] = ss_d;
-  a.shift[1] = ss_h;
-  a.shift[2] = ss_w;
-  a.B = B;
-  a.H = H;
-  a.N = N;
-  a.head_dim = head_dim;
   a.shares = shares;
-  a.scale = scale;
-  a.dtype = dtype;
-  const cudaStream_t on = static_cast<cudaStream_t>(stream);
-  const bool tensor = sized && (bits & 15u) == 0;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(grad_qkv) |
+                         reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(qkv);
+  const bool tensor = attention_grad_tensor_path(dtype, H, N, head_dim) && (bits & 15u) == 0;
   if (int e = tensor ? launch_attention_grad(a, on) : launch_attention_grad_simt(a, on)) return e;
   return launch_sum_shares(grad_bias, shares, H * N * N, on);
 }

@@ -156,6 +156,7 @@ bool attention_grad_tensor_path(int dtype, int64_t H, int64_t N, int64_t head_di
 int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
 int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N);
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
+int launch_attention_train_simt(const AttnGradArgs& a, void* out, cudaStream_t stream);
 int read_attention_grad_error(bool clear);
 // parts[0] = sum of parts[0 .. shares - 1], each of n floats
 int launch_sum_shares(float* parts, int64_t shares, int64_t n, cudaStream_t stream);

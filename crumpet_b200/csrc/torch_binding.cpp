@@ -719,12 +719,15 @@ Place check_attention(const at::Tensor& qkv, const at::Tensor& table, const at::
 }
 
 at::Tensor swin_window_attention_train(const at::Tensor& qkv, const at::Tensor& table,
-                                       const at::Tensor& index, at::IntArrayRef num_windows,
+                                       const at::Tensor& index, const at::Tensor& pairs,
+                                       at::IntArrayRef num_windows,
                                        at::IntArrayRef window_size, at::IntArrayRef shift_size,
                                        double scale) {
   const Place p = check_attention(qkv, table, index, num_windows, window_size, shift_size, scale);
   TORCH_CHECK(index.is_contiguous() && index.scalar_type() == at::kLong,
               "index must be a contiguous int64 tensor");
+  check_int32(qkv, pairs, "pairs");
+  TORCH_CHECK(pairs.sizes() == index.sizes(), "pairs must be the index as int32");
   const c10::cuda::CUDAGuard guard(qkv.device());
   const at::Tensor x = qkv.contiguous(), t = attention_table(table, x);
   const int64_t B = x.size(0), N = x.size(1), H = x.size(3), Dh = x.size(4);
@@ -746,10 +749,10 @@ at::Tensor swin_window_attention_train(const at::Tensor& qkv, const at::Tensor& 
         out.data_ptr(), x.data_ptr(), tiles.data_ptr(), p.nw[0], p.nw[1], p.nw[2], p.ws[0],
         p.ws[1], p.ws[2], p.ss[0], p.ss[1], p.ss[2], code, B, H, N, Dh, s, stream));
   } else {
-    check_rc(crumpet_swin_window_attention_qkv(
-        out.data_ptr(), x.data_ptr(), t.data_ptr(), t32, t.size(0),
-        index.const_data_ptr<int64_t>(), N, p.nw[0], p.nw[1], p.nw[2], p.ws[0], p.ws[1], p.ws[2],
-        p.ss[0], p.ss[1], p.ss[2], code, B, H, N, Dh, s, stream));
+    check_rc(crumpet_swin_window_attention_qkv_pairs(
+        out.data_ptr(), x.data_ptr(), t.data_ptr(), t32, t.size(0), pairs.const_data_ptr<int>(),
+        p.nw[0], p.nw[1], p.nw[2], p.ws[0], p.ws[1], p.ws[2], p.ss[0], p.ss[1], p.ss[2], code, B,
+        H, N, Dh, s, stream));
   }
   return out;
 }
@@ -1021,8 +1024,8 @@ TORCH_LIBRARY(crumpet_ops, ops) {
       "int buckets, ScalarType dtype) -> Tensor",
       kTags);
   ops.def(
-      "swin_window_attention_train(Tensor qkv, Tensor table, Tensor index, int[] num_windows, "
-      "int[] window_size, int[] shift_size, float scale) -> Tensor",
+      "swin_window_attention_train(Tensor qkv, Tensor table, Tensor index, Tensor pairs, "
+      "int[] num_windows, int[] window_size, int[] shift_size, float scale) -> Tensor",
       kTags);
   ops.def(
       "swin_window_attention_backward(Tensor grad_out, Tensor qkv, Tensor table, Tensor pairs, "

@@ -195,7 +195,7 @@ def _attention_work(qkv, tensors: int, products: int):
 
 def _attention_forward(qkv, table, buckets, place):
     return _launch("swin_window_attention_train", lambda: _attention_work(qkv, 4, 2), qkv, table,
-                   buckets.index, *place)
+                   buckets.index, buckets.pairs, *place)
 
 
 def _attention_backward(grad_out, qkv, table, buckets, place):
@@ -617,7 +617,7 @@ FAKE_IMPLS = {
         (table.shape[1], *pairs.shape), dtype=dtype),
     "relative_position_bias_backward": lambda grad, order, items, multi, buckets, dtype:
         grad.new_empty((buckets, grad.shape[0]), dtype=dtype),
-    "swin_window_attention_train": lambda qkv, table, index, nw, ws, ss, scale: qkv.new_empty(
+    "swin_window_attention_train": lambda qkv, table, index, pairs, nw, ws, ss, scale: qkv.new_empty(
         (qkv.shape[0], qkv.shape[1], qkv.shape[3] * qkv.shape[4])),
     "swin_window_attention_backward": lambda grad, qkv, table, pairs, order, items, multi, nw, ws,
         ss, scale: (qkv.new_empty(qkv.shape), table.new_empty(table.shape)),

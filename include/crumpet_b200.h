@@ -408,6 +408,18 @@ CRUMPET_API int crumpet_relative_position_bias_backward(
     int64_t n_multi, float* partial, void* stream);
 
 /*
+ * crumpet_swin_window_attention_qkv in fp32 arithmetic for every input of its domain, with the
+ * buckets as checked int32 pairs [N, N] (as the gradient below takes them): the training forward
+ * of what the tensor-core kernel does not take.  Four lanes share a row's keys for head dims up
+ * to 32, so small batches fill the GPU.
+ */
+CRUMPET_API int crumpet_swin_window_attention_qkv_pairs(
+    void* out, const void* qkv, const void* bias_table, int table_f32, int64_t table_rows,
+    const int* pairs, int64_t nw_d, int64_t nw_h, int64_t nw_w, int64_t ws_d, int64_t ws_h,
+    int64_t ws_w, int64_t ss_d, int64_t ss_h, int64_t ss_w, int dtype, int64_t B, int64_t H,
+    int64_t N, int64_t head_dim, float scale, void* stream);
+
+/*
  * Gradient of crumpet_swin_window_attention_qkv: from grad_out [B, N, H * head_dim] and the
  * forward's qkv, table and geometry (arguments as there; pairs int32 [N, N] holds the buckets
  * index[:N, :N], every value in [0, table_rows)), writes grad_qkv [B, N, 3, H, head_dim] and
