@@ -174,8 +174,12 @@ __device__ __forceinline__ void stage(const Params& p, float* dst, const T* src,
 
 enum Mode { kForward, kRows, kCols };
 
+// Sixteen channels leave room for six CTAs on an SM, which hides more of the
+// gathers' latency: 38 against 48 us forward and 57 against 71 us for the rows
+// at 64 windows of 125 tokens and three heads. The columns hold two sums per
+// token and lose to the spills (67 against 56 us), so they keep the default.
 template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, D == 16 && MODE != kCols ? 6 : D == 16 ? 5 : 1) grad_simt_kernel(const Params p) {
   using S = Shape<D>;
   constexpr bool COLS = MODE == kCols;
   extern __shared__ float4 smem4[];
@@ -228,23 +232,32 @@ __global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
       }
       __syncthreads();  // `last` is the CTA's
     }
-    auto value = [&](int r, int j) {
-      const int gi = r0 + r, gj = j0 + j;
-      if (gj >= p.N) return -INFINITY;  // past the end: drops out of the softmax
-      if (gi >= p.N) return 0.f;
-      float x = bias_of<T>(p, h, p.pairs[(long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj)]);
-      if (last != 0 && ((row_code[r] ^ tok_code[j]) & last)) x += -100.f * kLog2e;
-      return x;
-    };
-    constexpr int WARPS = kThreads / 32;
-    if constexpr (COLS) {
-      for (int r = lane; r < S::R; r += 32)
-#pragma unroll 8
-        for (int j = warp; j < cols; j += WARPS) tile[r * pitch + j] = value(r, j);
-    } else {
-      for (int j = lane; j < cols; j += 32)
-#pragma unroll 8
-        for (int r = warp; r < S::R; r += WARPS) tile[r * pitch + j] = value(r, j);
+    // eight pairs at a time: their indices, then their table entries, so that both loads of eight
+    // are in flight (with clamped indices; what lies past the end is replaced afterwards)
+    constexpr int WARPS = kThreads / 32, BATCH = 8;
+    const int across = COLS ? S::R : cols, along = COLS ? cols : S::R;
+    for (int x = lane; x < across; x += 32) {
+      for (int y0 = warp; y0 < along; y0 += WARPS * BATCH) {
+        int bucket[BATCH];
+        float v[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int y = y0 + u * WARPS;
+          const int gi = min(r0 + (COLS ? x : y), p.N - 1), gj = min(j0 + (COLS ? y : x), p.N - 1);
+          bucket[u] = __ldg(p.pairs + (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj));
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) v[u] = bias_of<T>(p, h, bucket[u]);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int y = y0 + u * WARPS;
+          if (y >= along) continue;
+          const int r = COLS ? x : y, j = COLS ? y : x;
+          if (last != 0 && ((row_code[r] ^ tok_code[j]) & last)) v[u] += -100.f * kLog2e;
+          // past the end of the softmax a pair drops out; past the rows nothing is stored
+          tile[r * pitch + j] = j0 + j >= p.N ? -INFINITY : v[u];
+        }
+      }
     }
   };
   if (whole) gather(0, (p.N + kTile - 1) / kTile * kTile);
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) grad_simt_kernel(const Params p) {
 // one key and 8 queries; CH channels at a time, the key's in registers, the queries' read from
 // shared memory by all threads at once.
 template <typename T, int CH>
-__global__ void __launch_bounds__(kThreads) grad_bias_simt_kernel(const Params p, int D) {
+__global__ void __launch_bounds__(kThreads, CH == 16 ? 6 : 1) grad_bias_simt_kernel(const Params p, int D) {
   __shared__ __align__(16) float qs[kTile * CH], gs[kTile * CH];
   const int tiles = (p.N + kTile - 1) / kTile;
   long long blk = blockIdx.x;
