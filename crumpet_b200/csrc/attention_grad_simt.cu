@@ -14,8 +14,14 @@
 // keeps the row's channels in registers, so a product is free of shuffles, and four times the
 // threads hide the latency of small batches), or to D / 32 lanes of 32 channels each, whose
 // partial products are added with shuffles.  The bias (+ mask) of the CTA's rows is gathered
-// into shared memory once where it fits.  fp32 FMA work bounds it: 11 products of depth D per
-// score, three of them the repeated scores.
+// into shared memory once where it fits.
+//
+// Bound by: 11 products of depth D per score, three of them the repeated scores, fed from shared
+// memory, where a 16-byte load gives four multiply-adds per lane.  At 64 windows of 125 tokens,
+// three heads of 16 channels, fp32: 28 us forward, 48 us rows, 49 us columns, 33 us bias; the
+// loads from shared memory take 62 % and 69 % of their rate in the first two, FMA 20 %.  Two rows
+// per lane halve those loads but need twice the registers, and came out level (33, 50 us); a tile
+// loaded ahead into registers, too (28, 51, 49 us).
 #include <cmath>
 
 #include "common.cuh"
@@ -174,10 +180,9 @@ __device__ __forceinline__ void stage(const Params& p, float* dst, const T* src,
 
 enum Mode { kForward, kRows, kCols };
 
-// Sixteen channels leave room for six CTAs on an SM, which hides more of the
-// gathers' latency: 38 against 48 us forward and 57 against 71 us for the rows
-// at 64 windows of 125 tokens and three heads. The columns hold two sums per
-// token and lose to the spills (67 against 56 us), so they keep the default.
+// At 16 channels registers are held to six CTAs per SM (five for the columns, which keep two
+// sums per lane): 38 against 48 us forward and 57 against 71 us for the rows at 64 windows of 125
+// tokens and three heads, where the gathers' latency counts.  A limit at the wider shapes spills.
 template <typename T, int D, int MODE>
 __global__ void __launch_bounds__(kThreads, D == 16 && MODE != kCols ? 6 : D == 16 ? 5 : 1) grad_simt_kernel(const Params p) {
   using S = Shape<D>;
