@@ -27,6 +27,7 @@ from typing import NamedTuple, Sequence
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _ops as _native
 from . import profiling as _prof
@@ -137,6 +138,7 @@ class _Bias(torch.autograd.Function):
         return _bias_forward(table, buckets, dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         return relative_position_bias_backward(grad, ctx.buckets, ctx.dtype), None, None
 
@@ -211,6 +213,7 @@ class _WindowAttention(torch.autograd.Function):
         return _attention_forward(qkv, table, buckets, place)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         qkv, table = ctx.saved_tensors
         return (*_attention_backward(grad_out, qkv, table, ctx.buckets, ctx.place), None, None)
@@ -306,6 +309,7 @@ class _NormGate(torch.autograd.Function):
         return out if normed is None else (out, normed)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, grad_normed=None):
         branch, out, *params = ctx.saved_tensors
         if branch is None:  # not read
@@ -423,6 +427,7 @@ class _Mlp(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, w1, w2, kept, scales = ctx.saved_tensors
         with torch.autocast("cuda", enabled=False):

@@ -748,7 +748,58 @@ def test_whole_model_trains():
     assert crumpet.device_status() == 0
 
 
+def test_traced_shapes(monkeypatch):
+    """What tracing is told about each op's results is what the op returns."""
+    from crumpet_b200 import training
+
+    seen, launch = {}, training._launch
+
+    def record(name, work, *args):
+        res = launch(name, work, *args)
+        same = lambda t: [(r.shape, r.dtype) for r in (t if isinstance(t, (tuple, list)) else [t])]  # noqa: E731
+        assert same(training.FAKE_IMPLS[name](*args)) == same(res), name
+        seen[name] = True
+        return res
+
+    monkeypatch.setattr(training, "_launch", record)
+    w = torch.ones(48, device="cuda", dtype=F16)
+    x = torch.randn(6, 48, device="cuda", dtype=F16)
+    out, normed = crumpet.norm_gate_residual(x, x.float(), w, None, (w, w), (w, w))
+    crumpet.norm_gate_residual(x, x)
+    crumpet.norm_gate_residual_backward(out, normed, out, x, w, None, (w, w), (w, w))
+    crumpet.norm_gate_residual_backward(out, None, out, x)
+    y, kept = crumpet.gelu_checkpoint(x)
+    crumpet.gelu_checkpoint_backward(y, kept)
+    crumpet.restore_activation(kept)
+    b = crumpet.relative_position_buckets(window_index((2, 2, 2)), 27)
+    table = torch.randn(27, 3, device="cuda")
+    crumpet.relative_position_bias_backward(crumpet.relative_position_bias(table, b, BF16), b, F16)
+    qkv = torch.randn(2, 8, 3, 3, 16, device="cuda", dtype=F16)
+    place = (table, b, (1, 1, 1), (2, 2, 2))
+    o = crumpet.swin_window_attention_train(qkv, *place)
+    crumpet.swin_window_attention_backward(o, qkv, *place)
+    assert set(seen) == set(training.FAKE_IMPLS)
+
+
 # -------------------------------------------------------------------------------- C ABI
+def test_second_derivatives_are_refused():
+    """The gradients are not differentiable again: asked for, that is an error, not a wrong sum."""
+    x = torch.randn(4, 32, device="cuda", requires_grad=True)
+    table = torch.randn(27, 2, device="cuda", requires_grad=True)
+    qkv = torch.randn(1, 8, 3, 2, 16, device="cuda", requires_grad=True)
+    b = crumpet.relative_position_buckets(window_index((2, 2, 2)), 27)
+    w = torch.ones(32, device="cuda")
+    weight = torch.randn(32, 32, device="cuda", requires_grad=True)
+    for out, wrt in (
+            (crumpet.relative_position_bias(table, b), table),
+            (crumpet.swin_window_attention_train(qkv, table, b, window_size=(2, 2, 2)), qkv),
+            (crumpet.norm_gate_residual(x, x, pre_norm=(w, w))[1], x),
+            (crumpet.checkpointed_mlp(x, weight, None, weight, None), x)):
+        g, = torch.autograd.grad((out ** 2).sum(), wrt, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad((g ** 2).sum(), wrt)
+
+
 def test_c_abi():
     """The entry points called directly give what the Python functions give."""
     import ctypes
