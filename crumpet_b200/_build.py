@@ -28,9 +28,9 @@ EXT = PKG / "_C.so"
 
 CUDA_SOURCES = ["capi.cu", "partition.cu", "mask.cu", "attention.cu", "attention_simt.cu",
                 "norm_partition.cu", "sliding_window.cu", "proj_norm.cu", "linear.cu",
-                "attention_grad.cu", "attention_grad_simt.cu", "bias_buckets.cu",
-                "norm_gate.cu", "act_checkpoint.cu"]
-CUDA_HEADERS = ["common.cuh", "sm100.cuh", "kernels.h"]
+                "attention_grad.cu", "attention_grad_simt.cu", "attention_grad_tf32.cu",
+                "bias_buckets.cu", "norm_gate.cu", "act_checkpoint.cu"]
+CUDA_HEADERS = ["common.cuh", "sm100.cuh", "kernels.h", "attention_grad_f32.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,103 @@
+// Shared by the fp32 window attention kernels for training (attention_grad_simt.cu,
+// attention_grad_tf32.cu): their parameters, loads, bias and mask.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace crumpet {
+namespace grad_f32 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+enum Mode { kForward, kRows, kCols };
+
+struct Params {
+  const void* qkv;    // [B, N, 3, H, D]
+  const void* dout;   // [B, N, H, D]
+  void* dqkv;         // [B, N, 3, H, D]
+  float* dbias;       // [S, H, N, N]
+  float2* stats;      // [B, H, N]
+  const void* table;  // [T, H]
+  const int* pairs;   // [N, N]
+  int table_f32, analytic;
+  int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
+  int B, H, N, QB, S, bias_pitch;
+  int vec;            // every tensor on 16-byte boundaries: four channels per load
+  float scale;
+  void* out;          // forward: [B, N, H, D]
+};
+
+template <typename T>
+__device__ __forceinline__ float load(const T* p, long long i);
+template <>
+__device__ __forceinline__ float load<float>(const float* p, long long i) { return __ldg(p + i); }
+template <>
+__device__ __forceinline__ float load<__half>(const __half* p, long long i) {
+  return __half2float(__ldg(p + i));
+}
+template <>
+__device__ __forceinline__ float load<__nv_bfloat16>(const __nv_bfloat16* p, long long i) {
+  return __bfloat162float(__ldg(p + i));
+}
+template <typename T>
+__device__ __forceinline__ T store_as(float v);
+template <>
+__device__ __forceinline__ float store_as<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half store_as<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 store_as<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ uint32_t side_code(const Params& p, int t) {
+  const int lw = t % p.wsw, t2 = t / p.wsw;
+  const int lh = t2 % p.wsh, ld = t2 / p.wsh;
+  return uint32_t(ld >= p.wsd - p.ssd) | (uint32_t(lh >= p.wsh - p.ssh) << 1) |
+         (uint32_t(lw >= p.wsw - p.ssw) << 2);
+}
+__device__ __forceinline__ uint32_t last_axes(const Params& p, int b) {
+  if (!p.analytic) return 0;
+  const int wi = b % (p.nwd * p.nwh * p.nww);
+  const int iw = wi % p.nww, t = wi / p.nww;
+  const int ih = t % p.nwh, id = t / p.nwh;
+  return uint32_t(p.ssd != 0 && id == p.nwd - 1) | (uint32_t(p.ssh != 0 && ih == p.nwh - 1) << 1) |
+         (uint32_t(p.ssw != 0 && iw == p.nww - 1) << 2);
+}
+
+// Four consecutive channels as fp32
+template <typename T>
+__device__ __forceinline__ float4 load4(const Params& p, const T* at) {
+  if (p.vec) {
+    if constexpr (sizeof(T) == 4) {
+      return __ldg(reinterpret_cast<const float4*>(at));
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
+      const T* v = reinterpret_cast<const T*>(&w);
+      return make_float4(float(v[0]), float(v[1]), float(v[2]), float(v[3]));
+    }
+  }
+  return make_float4(load(at, 0), load(at, 1), load(at, 2), load(at, 3));
+}
+
+// bias of one bucket times log2 e
+template <typename T>
+__device__ __forceinline__ float bias_of(const Params& p, int h, long long t) {
+  return kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
+                               : load(static_cast<const T*>(p.table), t * p.H + h));
+}
+
+}  // namespace grad_f32
+
+// attention_grad_tf32.cu: fp32 tensors, head_dim 16 or 32
+inline bool attention_tf32(int dtype, int64_t head_dim) { return dtype == kF32 && head_dim <= 32; }
+int64_t attention_grad_shares_tf32(int64_t B, int64_t H, int64_t N);
+int launch_attention_tf32(const grad_f32::Params& p, int head_dim, bool forward,
+                          cudaStream_t stream);
+
+}  // namespace crumpet

@@ -24,6 +24,7 @@
 // loaded ahead into registers, too (28, 51, 49 us).
 #include <cmath>
 
+#include "attention_grad_f32.cuh"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -31,86 +32,10 @@ namespace crumpet {
 
 namespace {
 
+using namespace grad_f32;
+
 constexpr int kThreads = 128;
 constexpr int kTile = 32;  // tokens streamed at a time
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Params {
-  const void* qkv;    // [B, N, 3, H, D]
-  const void* dout;   // [B, N, H, D]
-  void* dqkv;         // [B, N, 3, H, D]
-  float* dbias;       // [S, H, N, N]
-  float2* stats;      // [B, H, N]
-  const void* table;  // [T, H]
-  const int* pairs;   // [N, N]
-  int table_f32, analytic;
-  int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
-  int B, H, N, QB, S, bias_pitch;
-  int vec;            // every tensor on 16-byte boundaries: four channels per load
-  float scale;
-  void* out;          // forward: [B, N, H, D]
-};
-
-template <typename T>
-__device__ __forceinline__ float load(const T* p, long long i);
-template <>
-__device__ __forceinline__ float load<float>(const float* p, long long i) { return __ldg(p + i); }
-template <>
-__device__ __forceinline__ float load<__half>(const __half* p, long long i) {
-  return __half2float(__ldg(p + i));
-}
-template <>
-__device__ __forceinline__ float load<__nv_bfloat16>(const __nv_bfloat16* p, long long i) {
-  return __bfloat162float(__ldg(p + i));
-}
-template <typename T>
-__device__ __forceinline__ T store_as(float v);
-template <>
-__device__ __forceinline__ float store_as<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half store_as<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 store_as<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
-__device__ __forceinline__ uint32_t side_code(const Params& p, int t) {
-  const int lw = t % p.wsw, t2 = t / p.wsw;
-  const int lh = t2 % p.wsh, ld = t2 / p.wsh;
-  return uint32_t(ld >= p.wsd - p.ssd) | (uint32_t(lh >= p.wsh - p.ssh) << 1) |
-         (uint32_t(lw >= p.wsw - p.ssw) << 2);
-}
-__device__ __forceinline__ uint32_t last_axes(const Params& p, int b) {
-  if (!p.analytic) return 0;
-  const int wi = b % (p.nwd * p.nwh * p.nww);
-  const int iw = wi % p.nww, t = wi / p.nww;
-  const int ih = t % p.nwh, id = t / p.nwh;
-  return uint32_t(p.ssd != 0 && id == p.nwd - 1) | (uint32_t(p.ssh != 0 && ih == p.nwh - 1) << 1) |
-         (uint32_t(p.ssw != 0 && iw == p.nww - 1) << 2);
-}
-
-// Four consecutive channels as fp32
-template <typename T>
-__device__ __forceinline__ float4 load4(const Params& p, const T* at) {
-  if (p.vec) {
-    if constexpr (sizeof(T) == 4) {
-      return __ldg(reinterpret_cast<const float4*>(at));
-    } else {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
-      const T* v = reinterpret_cast<const T*>(&w);
-      return make_float4(float(v[0]), float(v[1]), float(v[2]), float(v[3]));
-    }
-  }
-  return make_float4(load(at, 0), load(at, 1), load(at, 2), load(at, 3));
-}
-
-// bias of one bucket times log2 e
-template <typename T>
-__device__ __forceinline__ float bias_of(const Params& p, int h, long long t) {
-  return kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
-                               : load(static_cast<const T*>(p.table), t * p.H + h));
-}
-
 template <int D>
 struct Shape {
   static constexpr int KL = D <= 32 ? 4 : 1;            // lanes that share out the tokens
@@ -177,8 +102,6 @@ __device__ __forceinline__ void stage(const Params& p, float* dst, const T* src,
         j0 + j < p.N ? load4(p, src + (j0 + j) * stride + d) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
-
-enum Mode { kForward, kRows, kCols };
 
 // At 16 channels registers are held to six CTAs per SM (five for the columns, which keep two
 // sums per lane): 38 against 48 us forward and 57 against 71 us for the rows at 64 windows of 125
@@ -492,9 +415,11 @@ int launch(Params p, bool forward, cudaStream_t stream) {
 
 template <typename T>
 int dispatch(const Params& p, int head_dim, bool forward, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2) {  // fp32 at these head dims: attention_grad_tf32.cu
+    if (head_dim == 16) return launch<T, 16>(p, forward, stream);
+    if (head_dim == 32) return launch<T, 32>(p, forward, stream);
+  }
   switch (head_dim) {
-    case 16: return launch<T, 16>(p, forward, stream);
-    case 32: return launch<T, 32>(p, forward, stream);
     case 64: return launch<T, 64>(p, forward, stream);
     case 128: return launch<T, 128>(p, forward, stream);
     default: return launch<T, 256>(p, forward, stream);
@@ -527,7 +452,10 @@ int launch_any(const AttnGradArgs& a, void* out, bool forward, cudaStream_t stre
   p.N = int(a.N);
   p.S = int(a.shares);
   p.scale = a.scale;
-  p.vec = ((reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.grad_out)) & 15u) == 0;
+  p.vec = ((reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.grad_out) |
+            reinterpret_cast<uintptr_t>(a.grad_qkv) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  if (attention_tf32(a.dtype, a.head_dim))
+    return launch_attention_tf32(p, int(a.head_dim), forward, stream);
   if (a.dtype == kF32) return dispatch<float>(p, int(a.head_dim), forward, stream);
   if (a.dtype == kF16) return dispatch<__half>(p, int(a.head_dim), forward, stream);
   return dispatch<__nv_bfloat16>(p, int(a.head_dim), forward, stream);
@@ -536,7 +464,8 @@ int launch_any(const AttnGradArgs& a, void* out, bool forward, cudaStream_t stre
 }  // namespace
 
 // Shares of the windows for the bias kernel: enough CTAs for the GPU's SMs, eight per SM.
-int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N) {
+int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N, int64_t head_dim, int dtype) {
+  if (attention_tf32(dtype, head_dim)) return attention_grad_shares_tf32(B, H, N);
   const int64_t tiles = (N + kTile - 1) / kTile;
   const int64_t s = 148 * 8 / (tiles * tiles * H);
   return s < 1 ? 1 : s > B ? (B > 0 ? B : 1) : s > 16 ? 16 : s;

@@ -480,8 +480,9 @@ int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, i
 int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N, int64_t head_dim,
                                                  int dtype) {
   if (B < 0 || H < 1 || N < 1) return 0;
-  return attention_grad_tensor_path(dtype, H, N, head_dim) ? attention_grad_shares(B, H, N)
-                                                        : attention_grad_shares_simt(B, H, N);
+  return attention_grad_tensor_path(dtype, H, N, head_dim)
+             ? attention_grad_shares(B, H, N)
+             : attention_grad_shares_simt(B, H, N, head_dim, dtype);
 }
 
 }  // extern "C"

@@ -154,7 +154,7 @@ struct AttnGradArgs {
 };
 bool attention_grad_tensor_path(int dtype, int64_t H, int64_t N, int64_t head_dim);
 int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
-int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N);
+int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N, int64_t head_dim, int dtype);
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
 int launch_attention_train_simt(const AttnGradArgs& a, void* out, cudaStream_t stream);
 int read_attention_grad_error(bool clear);
