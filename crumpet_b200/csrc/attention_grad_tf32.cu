@@ -33,9 +33,13 @@ constexpr int kWarps = 4;            // most of a CTA
 constexpr int kTile = 64;            // tokens staged at a time
 constexpr int kBlock = 32;           // tokens whose scores a warp holds at a time
 constexpr int kTiles = kBlock / 8;   // in tiles of 8
-constexpr int kCtasPerSm = 4;        // that registers allow
-constexpr int kBiasBytes = 80 * 1024;  // most shared memory for the bias of a CTA's rows
 
+// 2^x by the hardware's approximation (2^-22 relative), which no range handling surrounds
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The two tf32 halves of x
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xffffe000u;
@@ -77,7 +81,11 @@ __device__ __forceinline__ void dot(float (&s)[4], const Left<D>& a, int c, floa
   }
 }
 template <int D>
-struct Pitch {
+struct Stage {
+  static constexpr int CTAS = D == 16 ? 4 : 2;  // per SM, that registers allow
+  // most shared memory for the bias of a CTA's rows beside that many CTAs' staged tokens
+  static constexpr int BIAS = D == 16 ? 34 * 1024 : 68 * 1024;
+  static constexpr int FLOATS = 2 * kTile * (D + 4) + 2 * kTile;  // x, y and statistics
   static constexpr int ROW = D + 4;  // floats from a staged token to the next: both ways of
                                      // reading it (below) find the lanes' words in other banks
 };
@@ -87,7 +95,7 @@ __device__ __forceinline__ void dot_staged(float (&s)[4], const Left<D>& a, cons
                                            int g, int t) {
 #pragma unroll
   for (int c = 0; c < D / 16; ++c)
-    dot<D>(s, a, c, *reinterpret_cast<const float4*>(rows + g * Pitch<D>::ROW + 16 * c + 4 * t));
+    dot<D>(s, a, c, *reinterpret_cast<const float4*>(rows + g * Stage<D>::ROW + 16 * c + 4 * t));
 }
 // acc += w (16 rows x 8 tokens, as the scores lie) x the 8 staged tokens' channels; acc[2c + k]
 // holds channels 16c + 4t + k and 16c + 4t + 2 + k of rows g and g + 8
@@ -99,11 +107,11 @@ __device__ __forceinline__ void add_staged(float (&acc)[D / 8][4], const float (
   split(w[2], hi[1], lo[1]);
   split(w[1], hi[2], lo[2]);
   split(w[3], hi[3], lo[3]);
-  const float* at = rows + 2 * t * Pitch<D>::ROW + 2 * g;
+  const float* at = rows + 2 * t * Stage<D>::ROW + 2 * g;
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) {
     const float2 x = *reinterpret_cast<const float2*>(at + 16 * c);
-    const float2 y = *reinterpret_cast<const float2*>(at + Pitch<D>::ROW + 16 * c);
+    const float2 y = *reinterpret_cast<const float2*>(at + Stage<D>::ROW + 16 * c);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float xk = k ? x.y : x.x, yk = k ? y.y : y.x;
@@ -120,6 +128,23 @@ __device__ __forceinline__ void add_staged(float (&acc)[D / 8][4], const float (
     }
   }
 }
+// n (4, or 0: zeros) floats from global to shared memory, asynchronously
+__device__ __forceinline__ void copy(const Params& p, float* to, const float* from, int n) {
+  const uint32_t at = uint32_t(__cvta_generic_to_shared(to));
+  if (p.vec) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(4 * n)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at + 4 * e),
+                   "l"(from + e), "r"(n) : "memory");
+  }
+}
+__device__ __forceinline__ void copy_pair(float* to, const float2* from, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::
+               "r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from), "r"(in ? 8 : 0) : "memory");
+}
 template <int D>
 __device__ __forceinline__ void join(float (&sum)[D / 8][4], const float (&part)[D / 8][4]) {
 #pragma unroll
@@ -132,14 +157,13 @@ __device__ __forceinline__ void join(float (&sum)[D / 8][4], const float (&part)
 // A CTA takes 16 rows per warp of one head and walks the windows of its share, so the bias of its
 // rows, gathered once, stays in shared memory where it fits.
 template <int D, int MODE>
-__global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf32_kernel(const Params p, int shares) {
+__global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(const Params p, int shares) {
   constexpr bool COLS = MODE == kCols;
-  constexpr int ROW = Pitch<D>::ROW;
+  constexpr int ROW = Stage<D>::ROW;
   extern __shared__ float4 smem4[];
-  float* xs = reinterpret_cast<float*>(smem4);         // staged K (or Q)
-  float* ys = xs + kTile * ROW;                        // staged V (or dO)
-  float2* stat = reinterpret_cast<float2*>(ys + kTile * ROW);  // the staged queries' (columns)
-  float* tile = reinterpret_cast<float*>(stat + kTile);        // bias of the CTA's rows
+  // two stages of K, V (rows) or Q, dO and their statistics (columns)
+  float* staged = reinterpret_cast<float*>(smem4);
+  float* tile = staged + 2 * Stage<D>::FLOATS;  // bias of the CTA's rows
   const int threads = blockDim.x, rows = threads / 2;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   int blk = blockIdx.x;
@@ -197,6 +221,47 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
       tok_code[j] = j < p.N ? uint8_t(side_code(p, j)) : uint8_t(0);
   }
 
+  // starts the copies of window b's tokens j0 on, zero past the last, as far as a warp reads them
+  auto issue = [&](int b, int j0, float* to) {
+    const float* x = static_cast<const float*>(p.qkv) + (long long)b * p.N * tok + h * D;
+    const float* y = x + 2 * hd;
+    if constexpr (COLS) y = static_cast<const float*>(p.dout) + (long long)b * p.N * hd + h * D;
+    if constexpr (!COLS) x += hd;
+    const long long ytok = COLS ? hd : tok;
+    const int count = min(kTile, (p.N - j0 + kBlock - 1) / kBlock * kBlock) * (D / 4);
+    for (int f = tid; f < count; f += threads) {
+      const int j = f / (D / 4), d = f % (D / 4) * 4, n = j0 + j < p.N ? 4 : 0;
+      const long long at = n ? j0 + j : 0;
+      copy(p, to + j * ROW + d, x + at * tok + d, n);
+      copy(p, to + (kTile + j) * ROW + d, y + at * ytok + d, n);
+    }
+    if constexpr (COLS) {
+      const float2* stats = p.stats + ((long long)b * p.H + h) * p.N;
+      for (int j = tid; j < kTile; j += threads)
+        copy_pair(to + 2 * kTile * ROW + 2 * j, stats + (j0 + j < p.N ? j0 + j : 0), j0 + j < p.N);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // Tokens in the order the warps need them: per window once, or (rows of more than one tile)
+  // twice.  wait() makes tile j0 of window b readable and starts on the one after it.
+  constexpr bool TWICE = MODE == kRows;
+  int stage = 1;
+  if (share < p.B) issue(share, 0, staged);
+  auto wait = [&](int b, int j0, bool again) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // all copies have arrived, and no warp reads the other stage any more
+    stage ^= 1;
+    float* other = staged + (stage ^ 1) * Stage<D>::FLOATS;
+    if (j0 + kTile < p.N) issue(b, j0 + kTile, other);
+    else if (TWICE && !again && p.N > kTile) issue(b, 0, other);
+    else if (b + shares < p.B) issue(b + shares, 0, other);
+    if (!whole) {
+      gather(j0);
+      __syncthreads();
+    }
+    return staged + stage * Stage<D>::FLOATS;
+  };
+
   for (int b = share; b < p.B; b += shares) {
     const uint32_t last = last_axes(p, b);
     const float* q = static_cast<const float*>(p.qkv) + (long long)b * p.N * tok + h * D;
@@ -220,26 +285,6 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
     if constexpr (MODE == kRows) own(a1, o, hd);
     if constexpr (COLS) own(a1, v, tok);
 
-    // tokens j0 on, zero past the last, as far as a warp reads them
-    auto fetch = [&](int j0) {
-      __syncthreads();  // the previous tile is no longer read
-      const int count = min(kTile, (p.N - j0 + kBlock - 1) / kBlock * kBlock) * (D / 4);
-#pragma unroll 4
-      for (int f = tid; f < count; f += threads) {
-        const int j = f / (D / 4), d = f % (D / 4) * 4;
-        const bool in = j0 + j < p.N;
-        const float* x = (COLS ? q : k) + (j0 + j) * tok + d;
-        const float* y = COLS ? o + (j0 + j) * hd + d : v + (j0 + j) * tok + d;
-        *reinterpret_cast<float4*>(xs + j * ROW + d) = in ? load4(p, x) : zero;
-        *reinterpret_cast<float4*>(ys + j * ROW + d) = in ? load4(p, y) : zero;
-      }
-      if (!whole) gather(j0);
-      if (COLS) {
-        for (int j = tid; j < kTile; j += threads)
-          stat[j] = j0 + j < p.N ? stats[j0 + j] : make_float2(0.f, 0.f);
-      }
-      __syncthreads();
-    };
     // bias + mask of 8 tokens from staged token f on, as the scores lie
     auto bias_at = [&](float (&x)[4], int j0, int f) {
       const int at = (whole ? j0 : 0) + f + 2 * t;
@@ -285,7 +330,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
       float m[2] = {-1e30f, -1e30f}, l[2] = {}, dp[2] = {};
       float acc[D / 8][4] = {};
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
-        fetch(j0);
+        const float* xs = wait(b, j0, false);
+        const float* ys = xs + kTile * ROW;
         if (!busy) continue;
         for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
           float s[kTiles][4], mc[2] = {m[0], m[1]};
@@ -304,7 +350,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
           for (int u = 0; u < 2; ++u) {
             mc[u] = fmaxf(mc[u], __shfl_xor_sync(~0u, mc[u], 1));
             mc[u] = fmaxf(mc[u], __shfl_xor_sync(~0u, mc[u], 2));
-            const float alpha = exp2f(m[u] - mc[u]);
+            const float alpha = ex2(m[u] - mc[u]);
             m[u] = mc[u];
             l[u] *= alpha;
             dp[u] *= alpha;
@@ -313,17 +359,17 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
               for (int c = 0; c < D / 8; ++c) acc[c][2 * u] *= alpha, acc[c][2 * u + 1] *= alpha;
             }
           }
-          float now[D / 8][4] = {};
+          float now[2][D / 8][4] = {};
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              s[n][e] = exp2f(s[n][e] - m[e / 2]);
+              s[n][e] = ex2(s[n][e] - m[e / 2]);
               l[e / 2] += s[n][e];
             }
             const float* y = ys + (f + 8 * n) * ROW;
             if constexpr (MODE == kForward) {
-              add_staged<D>(now, s[n], y, g, t);
+              add_staged<D>(now[n % 2], s[n], y, g, t);
             } else {
               float d[4] = {};
               dot_staged<D>(d, a1, y, g, t);
@@ -331,7 +377,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
               for (int e = 0; e < 4; ++e) dp[e / 2] = fmaf(s[n][e], d[e], dp[e / 2]);
             }
           }
-          if constexpr (MODE == kForward) join<D>(acc, now);
+          if constexpr (MODE == kForward) join<D>(acc, now[0]);
+            join<D>(acc, now[1]);
         }
       }
 #pragma unroll
@@ -350,10 +397,12 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
         if (t < 2 && i0 + 8 * t < p.N)
           stats[i0 + 8 * t] = t ? make_float2(lse[1], delta[1]) : make_float2(lse[0], delta[0]);
         for (int j0 = 0; j0 < p.N; j0 += kTile) {
-          if (p.N > kTile) fetch(j0);  // else all tokens are still there
+          // a single tile is still there
+          const float* xs = p.N > kTile ? wait(b, j0, true) : staged + stage * Stage<D>::FLOATS;
+          const float* ys = xs + kTile * ROW;
           if (!busy) continue;
           for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
-            float now[D / 8][4] = {};
+            float now[2][D / 8][4] = {};
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
               float x[4], y[4] = {}, d[4] = {};
@@ -362,10 +411,11 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
               dot_staged<D>(d, a1, ys + (f + 8 * n) * ROW, g, t);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                y[e] = exp2f(fmaf(y[e], c1, x[e]) - lse[e / 2]) * (d[e] - delta[e / 2]);
-              add_staged<D>(now, y, xs + (f + 8 * n) * ROW, g, t);
+                y[e] = ex2(fmaf(y[e], c1, x[e]) - lse[e / 2]) * (d[e] - delta[e / 2]);
+              add_staged<D>(now[n % 2], y, xs + (f + 8 * n) * ROW, g, t);
             }
-            join<D>(acc, now);
+            join<D>(acc, now[0]);
+            join<D>(acc, now[1]);
           }
         }
         put(acc, p.scale, p.scale, dqkv, tok);
@@ -373,7 +423,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
     } else {
       float dk[D / 8][4] = {}, dv[D / 8][4] = {};
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
-        fetch(j0);
+        const float* xs = wait(b, j0, false);
+        const float* ys = xs + kTile * ROW;
         if (!busy) continue;
         for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
           float pk[D / 8][4] = {}, pv[D / 8][4] = {};
@@ -381,12 +432,13 @@ __global__ void __launch_bounds__(32 * kWarps, D == 16 ? kCtasPerSm : 2) grad_tf
           for (int n = 0; n < kTiles; ++n) {
             float x[4], y[4] = {}, d[4] = {};
             bias_at(x, j0, f + 8 * n);
-            const float4 st = *reinterpret_cast<const float4*>(stat + f + 8 * n + 2 * t);
+            const float4 st = 
+                *reinterpret_cast<const float4*>(xs + 2 * kTile * ROW + 2 * (f + 8 * n + 2 * t));
             dot_staged<D>(y, a0, xs + (f + 8 * n) * ROW, g, t);
             dot_staged<D>(d, a1, ys + (f + 8 * n) * ROW, g, t);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              y[e] = exp2f(fmaf(y[e], c1, x[e]) - (e % 2 ? st.z : st.x));
+              y[e] = ex2(fmaf(y[e], c1, x[e]) - (e % 2 ? st.z : st.x));
               d[e] = y[e] * (d[e] - (e % 2 ? st.w : st.y));
             }
             add_staged<D>(pv, y, ys + (f + 8 * n) * ROW, g, t);
@@ -472,7 +524,7 @@ __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Param
       for (int e = 0; e < 4; ++e) {
         float x = fmaf(s[e], c1, base[n][e]);
         if (apart[n] & last & (0xffu << (8 * e))) x += -100.f * kLog2e;
-        sum[n][e] += exp2f(x - st[e / 2].x) * (d[e] - st[e / 2].y);
+        sum[n][e] += ex2(x - st[e / 2].x) * (d[e] - st[e / 2].y);
       }
     }
   }
@@ -494,15 +546,15 @@ int start(Params p, cudaStream_t stream) {
   p.QB = (p.N + rows - 1) / rows;
   // as many windows per CTA as leave the SMs one full round of CTAs
   const long long units = (long long)p.B * p.H * p.QB;
-  const long long round = 148LL * kCtasPerSm * kWarps / warps;
+  const long long round = 148LL * Stage<D>::CTAS * kWarps / warps;
   const long long per = (units + round - 1) / round;
   const long long shares = (p.B + per - 1) / per, blocks = shares * p.H * p.QB;
   if (blocks > 0x7fffffffLL)
     return set_error(kErrInvalid, "too many windows x heads for one launch");
   const int cols = (p.N + kBlock - 1) / kBlock * kBlock;
   const int bytes = (MODE == kCols ? cols * (rows + 4) : rows * (cols + 8)) * 4;
-  p.bias_pitch = bytes <= kBiasBytes ? cols : 0;
-  const int smem = 2 * kTile * Pitch<D>::ROW * 4 + kTile * 8 + (p.N + kTile - 1) / kTile * kTile +
+  p.bias_pitch = bytes <= Stage<D>::BIAS ? cols : 0;
+  const int smem = 2 * Stage<D>::FLOATS * 4 + (p.N + kTile - 1) / kTile * kTile +
                    (p.bias_pitch ? bytes
                                  : (MODE == kCols ? kTile * (rows + 4) : rows * (kTile + 8)) * 4);
   auto kernel = grad_tf32_kernel<D, MODE>;
