@@ -83,8 +83,6 @@ __device__ __forceinline__ void dot(float (&s)[4], const Left<D>& a, int c, floa
 template <int D>
 struct Stage {
   static constexpr int CTAS = D == 16 ? 4 : 2;  // per SM, that registers allow
-  // most shared memory for the bias of a CTA's rows beside that many CTAs' staged tokens
-  static constexpr int BIAS = D == 16 ? 34 * 1024 : 68 * 1024;
   static constexpr int FLOATS = 2 * kTile * (D + 4) + 2 * kTile;  // x, y and statistics
   static constexpr int ROW = D + 4;  // floats from a staged token to the next: both ways of
                                      // reading it (below) find the lanes' words in other banks
@@ -128,23 +126,6 @@ __device__ __forceinline__ void add_staged(float (&acc)[D / 8][4], const float (
     }
   }
 }
-// n (4, or 0: zeros) floats from global to shared memory, asynchronously
-__device__ __forceinline__ void copy(const Params& p, float* to, const float* from, int n) {
-  const uint32_t at = uint32_t(__cvta_generic_to_shared(to));
-  if (p.vec) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(4 * n)
-                 : "memory");
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at + 4 * e),
-                   "l"(from + e), "r"(n) : "memory");
-  }
-}
-__device__ __forceinline__ void copy_pair(float* to, const float2* from, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::
-               "r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from), "r"(in ? 8 : 0) : "memory");
-}
 template <int D>
 __device__ __forceinline__ void join(float (&sum)[D / 8][4], const float (&part)[D / 8][4]) {
 #pragma unroll
@@ -161,9 +142,10 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
   constexpr bool COLS = MODE == kCols;
   constexpr int ROW = Stage<D>::ROW;
   extern __shared__ float4 smem4[];
-  // two stages of K, V (rows) or Q, dO and their statistics (columns)
-  float* staged = reinterpret_cast<float*>(smem4);
-  float* tile = staged + 2 * Stage<D>::FLOATS;  // bias of the CTA's rows
+  float* xs = reinterpret_cast<float*>(smem4);                 // staged K (or Q)
+  float* ys = xs + kTile * ROW;                                // staged V (or dO)
+  float2* stat = reinterpret_cast<float2*>(ys + kTile * ROW);  // the staged queries' (columns)
+  float* tile = xs + Stage<D>::FLOATS;                         // bias of the CTA's rows
   const int threads = blockDim.x, rows = threads / 2;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   int blk = blockIdx.x;
@@ -221,47 +203,6 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
       tok_code[j] = j < p.N ? uint8_t(side_code(p, j)) : uint8_t(0);
   }
 
-  // starts the copies of window b's tokens j0 on, zero past the last, as far as a warp reads them
-  auto issue = [&](int b, int j0, float* to) {
-    const float* x = static_cast<const float*>(p.qkv) + (long long)b * p.N * tok + h * D;
-    const float* y = x + 2 * hd;
-    if constexpr (COLS) y = static_cast<const float*>(p.dout) + (long long)b * p.N * hd + h * D;
-    if constexpr (!COLS) x += hd;
-    const long long ytok = COLS ? hd : tok;
-    const int count = min(kTile, (p.N - j0 + kBlock - 1) / kBlock * kBlock) * (D / 4);
-    for (int f = tid; f < count; f += threads) {
-      const int j = f / (D / 4), d = f % (D / 4) * 4, n = j0 + j < p.N ? 4 : 0;
-      const long long at = n ? j0 + j : 0;
-      copy(p, to + j * ROW + d, x + at * tok + d, n);
-      copy(p, to + (kTile + j) * ROW + d, y + at * ytok + d, n);
-    }
-    if constexpr (COLS) {
-      const float2* stats = p.stats + ((long long)b * p.H + h) * p.N;
-      for (int j = tid; j < kTile; j += threads)
-        copy_pair(to + 2 * kTile * ROW + 2 * j, stats + (j0 + j < p.N ? j0 + j : 0), j0 + j < p.N);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  // Tokens in the order the warps need them: per window once, or (rows of more than one tile)
-  // twice.  wait() makes tile j0 of window b readable and starts on the one after it.
-  constexpr bool TWICE = MODE == kRows;
-  int stage = 1;
-  if (share < p.B) issue(share, 0, staged);
-  auto wait = [&](int b, int j0, bool again) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();  // all copies have arrived, and no warp reads the other stage any more
-    stage ^= 1;
-    float* other = staged + (stage ^ 1) * Stage<D>::FLOATS;
-    if (j0 + kTile < p.N) issue(b, j0 + kTile, other);
-    else if (TWICE && !again && p.N > kTile) issue(b, 0, other);
-    else if (b + shares < p.B) issue(b + shares, 0, other);
-    if (!whole) {
-      gather(j0);
-      __syncthreads();
-    }
-    return staged + stage * Stage<D>::FLOATS;
-  };
-
   for (int b = share; b < p.B; b += shares) {
     const uint32_t last = last_axes(p, b);
     const float* q = static_cast<const float*>(p.qkv) + (long long)b * p.N * tok + h * D;
@@ -285,6 +226,35 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
     if constexpr (MODE == kRows) own(a1, o, hd);
     if constexpr (COLS) own(a1, v, tok);
 
+    // stages tokens j0 on, zero past the last, as far as a warp reads them
+    auto fetch = [&](int j0) {
+      __syncthreads();  // the previous tile is no longer read
+      const int count = min(kTile, (p.N - j0 + kBlock - 1) / kBlock * kBlock) * (D / 4);
+      for (int f0 = tid; f0 < count; f0 += 2 * threads) {
+        float4 x[2], y[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int f = f0 + u * threads, j = j0 + f / (D / 4), d = f % (D / 4) * 4;
+          const bool in = f < count && j < p.N;
+          x[u] = in ? load4(p, (COLS ? q : k) + j * tok + d) : zero;
+          y[u] = in ? load4(p, COLS ? o + j * hd + d : v + j * tok + d) : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int f = f0 + u * threads;
+          if (f >= count) continue;
+          float* at = xs + f / (D / 4) * ROW + f % (D / 4) * 4;
+          *reinterpret_cast<float4*>(at) = x[u];
+          *reinterpret_cast<float4*>(at + kTile * ROW) = y[u];
+        }
+      }
+      if (!whole) gather(j0);
+      if (COLS) {
+        for (int j = tid; j < kTile; j += threads)
+          stat[j] = j0 + j < p.N ? stats[j0 + j] : make_float2(0.f, 0.f);
+      }
+      __syncthreads();
+    };
     // bias + mask of 8 tokens from staged token f on, as the scores lie
     auto bias_at = [&](float (&x)[4], int j0, int f) {
       const int at = (whole ? j0 : 0) + f + 2 * t;
@@ -330,8 +300,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
       float m[2] = {-1e30f, -1e30f}, l[2] = {}, dp[2] = {};
       float acc[D / 8][4] = {};
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
-        const float* xs = wait(b, j0, false);
-        const float* ys = xs + kTile * ROW;
+        fetch(j0);
         if (!busy) continue;
         for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
           float s[kTiles][4], mc[2] = {m[0], m[1]};
@@ -397,9 +366,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
         if (t < 2 && i0 + 8 * t < p.N)
           stats[i0 + 8 * t] = t ? make_float2(lse[1], delta[1]) : make_float2(lse[0], delta[0]);
         for (int j0 = 0; j0 < p.N; j0 += kTile) {
-          // a single tile is still there
-          const float* xs = p.N > kTile ? wait(b, j0, true) : staged + stage * Stage<D>::FLOATS;
-          const float* ys = xs + kTile * ROW;
+          if (p.N > kTile) fetch(j0);  // else all tokens are still there
           if (!busy) continue;
           for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
             float now[2][D / 8][4] = {};
@@ -423,8 +390,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
     } else {
       float dk[D / 8][4] = {}, dv[D / 8][4] = {};
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
-        const float* xs = wait(b, j0, false);
-        const float* ys = xs + kTile * ROW;
+        fetch(j0);
         if (!busy) continue;
         for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
           float pk[D / 8][4] = {}, pv[D / 8][4] = {};
@@ -432,8 +398,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
           for (int n = 0; n < kTiles; ++n) {
             float x[4], y[4] = {}, d[4] = {};
             bias_at(x, j0, f + 8 * n);
-            const float4 st = 
-                *reinterpret_cast<const float4*>(xs + 2 * kTile * ROW + 2 * (f + 8 * n + 2 * t));
+            const float4 st = *reinterpret_cast<const float4*>(stat + f + 8 * n + 2 * t);
             dot_staged<D>(y, a0, xs + (f + 8 * n) * ROW, g, t);
             dot_staged<D>(d, a1, ys + (f + 8 * n) * ROW, g, t);
 #pragma unroll
@@ -553,8 +518,11 @@ int start(Params p, cudaStream_t stream) {
     return set_error(kErrInvalid, "too many windows x heads for one launch");
   const int cols = (p.N + kBlock - 1) / kBlock * kBlock;
   const int bytes = (MODE == kCols ? cols * (rows + 4) : rows * (cols + 8)) * 4;
-  p.bias_pitch = bytes <= Stage<D>::BIAS ? cols : 0;
-  const int smem = 2 * Stage<D>::FLOATS * 4 + (p.N + kTile - 1) / kTile * kTile +
+  // the bias is kept whole as far as that leaves shared memory for the CTAs that registers allow;
+  // the rows, which read it twice per window, go to three of four
+  const int most = MODE == kRows || D > 16 ? 64 * 1024 : 45 * 1024;
+  p.bias_pitch = bytes <= most ? cols : 0;
+  const int smem = Stage<D>::FLOATS * 4 + (p.N + kTile - 1) / kTile * kTile +
                    (p.bias_pitch ? bytes
                                  : (MODE == kCols ? kTile * (rows + 4) : rows * (kTile + 8)) * 4);
   auto kernel = grad_tf32_kernel<D, MODE>;
