@@ -18,6 +18,7 @@
 //   * bias:    a warp keeps 16 x 32 pairs of one head and sums ds over the windows of its share;
 //              operands come straight from global memory, nothing is shared between warps.
 #include <cmath>
+#include <type_traits>
 
 #include "attention_grad_f32.cuh"
 #include "common.cuh"
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
   uint32_t row_code[2] = {};
   if (p.analytic) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) row_code[u] = i0 + 8 * u < p.N ? side_code(p, i0 + 8 * u) : 0u;
+    for (int u = 0; u < 2; ++u) row_code[u] = i0 + 8 * u < p.N ? side_code(p, i0 + 8 * u) * 0x0101u : 0u;
     const int all = (p.N + kTile - 1) / kTile * kTile;
     for (int j = tid; j < all; j += threads)
       tok_code[j] = j < p.N ? uint8_t(side_code(p, j)) : uint8_t(0);
@@ -255,6 +256,13 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
       }
       __syncthreads();
     };
+    // the staged tokens in blocks of four tiles of 8, or two where that is all there is
+    auto each_block = [&](int j0, auto&& block) {
+      for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
+        if (p.N - j0 - f > kBlock / 2) block(std::integral_constant<int, kTiles>{}, f);
+        else block(std::integral_constant<int, kTiles / 2>{}, f);
+      }
+    };
     // bias + mask of 8 tokens from staged token f on, as the scores lie
     auto bias_at = [&](float (&x)[4], int j0, int f) {
       const int at = (whole ? j0 : 0) + f + 2 * t;
@@ -268,9 +276,15 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
         x[0] = u.x, x[1] = u.y, x[2] = u8.x, x[3] = u8.y;
       }
       if (last != 0) {
+        // two tokens' codes against each row's, copied beside itself
+        const uint32_t two = *reinterpret_cast<const uint16_t*>(tok_code + j0 + f + 2 * t);
+        const uint32_t sides = last * 0x0101u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((row_code[e / 2] ^ tok_code[j0 + f + 2 * t + e % 2]) & last) x[e] += -100.f * kLog2e;
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t apart = (two ^ row_code[u]) & sides;
+          if (apart & 0xff) x[2 * u] += -100.f * kLog2e;
+          if (apart & 0xff00) x[2 * u + 1] += -100.f * kLog2e;
+        }
       }
     };
     // the sums' 4 channels from 16c + 4t on of row i0 + 8u, times its factor
@@ -302,10 +316,11 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
         fetch(j0);
         if (!busy) continue;
-        for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
-          float s[kTiles][4], mc[2] = {m[0], m[1]};
+        auto block = [&](auto tiles, int f) {
+          constexpr int TILES = decltype(tiles)::value;
+          float s[TILES][4], mc[2] = {m[0], m[1]};
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
+          for (int n = 0; n < TILES; ++n) {
             float x[4], y[4] = {};
             bias_at(x, j0, f + 8 * n);
             dot_staged<D>(y, a0, xs + (f + 8 * n) * ROW, g, t);
@@ -330,7 +345,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
           }
           float now[2][D / 8][4] = {};
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
+          for (int n = 0; n < TILES; ++n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               s[n][e] = ex2(s[n][e] - m[e / 2]);
@@ -348,7 +363,8 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
           }
           if constexpr (MODE == kForward) join<D>(acc, now[0]);
             join<D>(acc, now[1]);
-        }
+        };
+        each_block(j0, block);
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -368,10 +384,11 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
         for (int j0 = 0; j0 < p.N; j0 += kTile) {
           if (p.N > kTile) fetch(j0);  // else all tokens are still there
           if (!busy) continue;
-          for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
+          auto block = [&](auto tiles, int f) {
+            constexpr int TILES = decltype(tiles)::value;
             float now[2][D / 8][4] = {};
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n) {
+            for (int n = 0; n < TILES; ++n) {
               float x[4], y[4] = {}, d[4] = {};
               bias_at(x, j0, f + 8 * n);
               dot_staged<D>(y, a0, xs + (f + 8 * n) * ROW, g, t);
@@ -383,7 +400,8 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
             }
             join<D>(acc, now[0]);
             join<D>(acc, now[1]);
-          }
+          };
+          each_block(j0, block);
         }
         put(acc, p.scale, p.scale, dqkv, tok);
       }
@@ -392,10 +410,11 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
       for (int j0 = 0; j0 < p.N; j0 += kTile) {
         fetch(j0);
         if (!busy) continue;
-        for (int f = 0; f < kTile && j0 + f < p.N; f += kBlock) {
+        auto block = [&](auto tiles, int f) {
+          constexpr int TILES = decltype(tiles)::value;
           float pk[D / 8][4] = {}, pv[D / 8][4] = {};
 #pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
+          for (int n = 0; n < TILES; ++n) {
             float x[4], y[4] = {}, d[4] = {};
             bias_at(x, j0, f + 8 * n);
             const float4 st = *reinterpret_cast<const float4*>(stat + f + 8 * n + 2 * t);
@@ -411,7 +430,8 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
           }
           join<D>(dk, pk);
           join<D>(dv, pv);
-        }
+        };
+        each_block(j0, block);
       }
       put(dk, p.scale, p.scale, dqkv + hd, tok);
       put(dv, 1.f, 1.f, dqkv + 2 * hd, tok);
