@@ -166,21 +166,31 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
   const int held = whole ? p.bias_pitch : kTile;
   const int pitch = COLS ? rows + 4 : held + 8;
   auto gather = [&](int j0) {
-    // eight pairs at a time, their indices first, so that both loads of eight are in flight
+    // eight pairs at a time, so that their loads are in flight together (forward: the indices',
+    // then the table's; the gradient finds the bias laid out where its own gradient will go)
     constexpr int BATCH = 8;
     const int warps = threads / 32, across = COLS ? rows : held, along = COLS ? held : rows;
     for (int x = lane; x < across; x += 32) {
       for (int y0 = warp; y0 < along; y0 += warps * BATCH) {
-        int bucket[BATCH];
+        long long at[BATCH];
         float w[BATCH];
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
           const int y = y0 + u * warps;
           const int gi = min(r0 + (COLS ? x : y), p.N - 1), gj = min(j0 + (COLS ? y : x), p.N - 1);
-          bucket[u] = __ldg(p.pairs + (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj));
+          at[u] = (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj);
         }
+        if constexpr (MODE == kForward) {
+          int bucket[BATCH];
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u) w[u] = bias_of<float>(p, h, bucket[u]);
+          for (int u = 0; u < BATCH; ++u) bucket[u] = __ldg(p.pairs + at[u]);
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u) w[u] = bias_of<float>(p, h, bucket[u]);
+        } else {
+          const float* dense = p.dbias + (long long)h * p.N * p.N;
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u) w[u] = kLog2e * __ldg(dense + at[u]);
+        }
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
           const int y = y0 + u * warps;
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
 }
 
 // dbias of 16 queries x 32 keys of one head per warp, over the windows of one share
-template <int D>
+template <int D, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Params p,
                                                                   long long warps) {
   const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -455,6 +465,10 @@ __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Param
   const long long hd = (long long)p.H * D, tok = 3 * hd;
   const float c1 = p.scale * kLog2e;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto channels = [&](const float* at) {  // VEC: every tensor on 16-byte boundaries
+    if constexpr (VEC) return __ldg(reinterpret_cast<const float4*>(at));
+    else return make_float4(__ldg(at), __ldg(at + 1), __ldg(at + 2), __ldg(at + 3));
+  };
   float base[kTiles][4], sum[kTiles][4] = {};
   uint32_t apart[kTiles];  // of each of four pairs, the axes on whose other side they lie: 4 x 8 bits
   {
@@ -483,7 +497,22 @@ __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Param
     const float* o = static_cast<const float*>(p.dout) + (long long)b * p.N * hd + h * D + 4 * t;
     const float2* stats = p.stats + ((long long)b * p.H + h) * p.N;
     const uint32_t last = last_axes(p, b) * 0x01010101u;
-    Left<D> a0, a1;
+    // the loads of two tiles go out together, the first with those of the rows
+    constexpr int AHEAD = kTiles / 2;
+    float4 kv[AHEAD][2][D / 16];
+    auto fetch = [&](int n0) {
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const int j = jt + 8 * (n0 + n) + g;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const float* at = q + j * tok + hd + 16 * c;
+          kv[n][0][c] = j < p.N ? channels(at) : zero;
+          kv[n][1][c] = j < p.N ? channels(at + hd) : zero;
+        }
+      }
+    };
+    float4 own[2][2][D / 16];
     float2 st[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -491,19 +520,28 @@ __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Param
       st[u] = i < p.N ? __ldg(stats + i) : make_float2(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        a0.set(u, c, i < p.N ? load4(p, q + i * tok + 16 * c) : zero);
-        a1.set(u, c, i < p.N ? load4(p, o + i * hd + 16 * c) : zero);
+        own[0][u][c] = i < p.N ? channels(q + i * tok + 16 * c) : zero;
+        own[1][u][c] = i < p.N ? channels(o + i * hd + 16 * c) : zero;
+      }
+    }
+    fetch(0);
+    Left<D> a0, a1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        a0.set(u, c, own[0][u][c]);
+        a1.set(u, c, own[1][u][c]);
       }
     }
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      const int j = jt + 8 * n + g;
+      if (n > 0 && n % AHEAD == 0) fetch(n);
       float s[4] = {}, d[4] = {};
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        const float* at = q + j * tok + hd + 16 * c;
-        dot<D>(s, a0, c, j < p.N ? load4(p, at) : zero);
-        dot<D>(d, a1, c, j < p.N ? load4(p, at + hd) : zero);
+        dot<D>(s, a0, c, kv[n % AHEAD][0][c]);
+        dot<D>(d, a1, c, kv[n % AHEAD][1][c]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -559,6 +597,10 @@ int start(Params p, cudaStream_t stream) {
 template <int D>
 int launch(const Params& p, bool forward, cudaStream_t stream) {
   if (forward) return start<D, kForward>(p, stream);
+  // the bias as [H, N, N], in the place of its gradient: two kernels read it, once per CTA or more
+  if (int e = launch_relative_position_bias(p.dbias, kF32, p.table, kF32, p.pairs,
+                                            (long long)p.N * p.N, p.H, stream))
+    return e;
   if (int e = start<D, kRows>(p, stream)) return e;
   if (int e = start<D, kCols>(p, stream)) return e;
   const long long warps =
@@ -566,7 +608,10 @@ int launch(const Params& p, bool forward, cudaStream_t stream) {
   const long long blocks = (warps + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffffLL)
     return set_error(kErrInvalid, "too many windows x heads for one launch");
-  grad_bias_tf32_kernel<D><<<unsigned(blocks), 32 * kWarps, 0, stream>>>(p, warps);
+  if (p.vec)
+    grad_bias_tf32_kernel<D, true><<<unsigned(blocks), 32 * kWarps, 0, stream>>>(p, warps);
+  else
+    grad_bias_tf32_kernel<D, false><<<unsigned(blocks), 32 * kWarps, 0, stream>>>(p, warps);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "attention gradient (tf32) launch");
 }
