@@ -16,6 +16,10 @@
 //
 // HBM traffic bounds both kernels: 5 bytes per element forward and 7 backward in 16 bits.  Four
 // lanes share a group (8 elements each, 16-byte accesses).
+//
+// Measured: 442368 x 192 in bf16, 83 us forward (66 us of HBM time; issue slots 77 % busy) and
+// 105 us backward (92 us).  The forward loads a group ahead; the backward, which has more CTAs in
+// flight, lost by that (108 us).
 #include "common.cuh"
 #include "kernels.h"
 

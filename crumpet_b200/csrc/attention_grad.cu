@@ -18,8 +18,8 @@
 // share one after another, so what belongs to the head -- the bias, and the sum dbias -- stays
 // on the SM, in tensor memory, used here as a second register file:
 //   * rows kernel (64 query rows, all keys): row statistics, dq and dbias.  A warp holds a
-//     16 x WC tile of scores and of dp in registers (WC <= 88 keys), so each exponential is
-//     taken once; the CG warps of a row exchange (maximum, sum, sum of p dp) through shared
+//     16 x WC tile of scores in registers (WC <= 88 keys), so each exponential is taken once (dp,
+//     one product, twice); the CG warps of a row exchange (maximum, sum, sum of p dp) through shared
 //     memory at one barrier per window, behind which they also join the dq of the window
 //     before.  The bias goes from tensor memory straight into the accumulators of q k^T; dbias
 //     is read from it, added to and written back once per window (2 x 64 x 352 fp32).
@@ -29,6 +29,13 @@
 // refills it, so warps drift apart by up to a ring and no warp waits only to copy.  Waits for
 // the loads are bounded like the forward kernel's (2 s, then the device error word).  No wait
 // depends on another CTA; sums have a fixed order, so results do not change from run to run.
+//
+// Measured, three heads of 16 channels and 343 tokens: 1372 windows in bf16 rows 561 us, columns
+// 325 us (the exponentials alone 117 us each, with the padding); 343 windows in fp16 178 and 114
+// us, issue slots 42 % and 37 % busy: latency bounds both, in the rows kernel that of the exchange
+// between the warps of a row (its largest stall; one row group alone on an SM takes 348 of 571
+// us).  Measured and not kept in the rows kernel, against 571 us: dp held in registers as well (595
+// to 661 us), two windows' halves in flight (740 us, registers spill).
 #include <cmath>
 #include <mutex>
 #include <type_traits>

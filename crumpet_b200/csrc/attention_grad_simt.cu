@@ -1,5 +1,6 @@
-// crumpet_b200: gradient of the window attention for the inputs attention_grad.cu does not
-// take: float32 qkv, head dims 64 to 256, windows of more than 352 tokens, unaligned tensors.
+// crumpet_b200: window attention for training on the inputs that neither attention_grad.cu nor
+// attention_grad_tf32.cu takes: head dims 64 to 256, and in 16 bits windows of more than 352
+// tokens or unaligned tensors.
 //
 // The formulas of attention_grad.cu in plain fp32 arithmetic.  Tiles of 32 tokens of the other
 // side stream through shared memory (as fp32):
@@ -18,10 +19,11 @@
 //
 // Bound by: 11 products of depth D per score, three of them the repeated scores, fed from shared
 // memory, where a 16-byte load gives four multiply-adds per lane.  At 64 windows of 125 tokens,
-// three heads of 16 channels, fp32: 28 us forward, 48 us rows, 49 us columns, 33 us bias; the
+// three heads of 16 channels, as fp32: 28 us forward, 48 us rows, 49 us columns, 33 us bias; the
 // loads from shared memory take 62 % and 69 % of their rate in the first two, FMA 20 %.  Two rows
 // per lane halve those loads but need twice the registers, and came out level (33, 50 us); a tile
-// loaded ahead into registers, too (28, 51, 49 us).
+// loaded ahead into registers, too (28, 51, 49 us).  At 16 windows of 216 tokens, three heads of
+// 64 channels, fp32: 69 us forward, 129 us rows, 98 us columns, 92 us bias.
 #include <cmath>
 
 #include "attention_grad_f32.cuh"

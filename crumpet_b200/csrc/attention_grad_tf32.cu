@@ -17,6 +17,17 @@
 //   * columns: the transposed scores, one sweep over the queries for dk and dv;
 //   * bias:    a warp keeps 16 x 32 pairs of one head and sums ds over the windows of its share;
 //              operands come straight from global memory, nothing is shared between warps.
+//
+// What bounds it: instructions, not the tensor cores (8.5 cycles per product and SM quarter when
+// they are alone, 16 to 20 % busy here): splitting the staged operands, which every warp does for
+// itself, and the softmax.  The bias kernel reads 6 KB per 16 x 32 pairs and window from L2 (3.4
+// TB/s at 343 tokens).  At 64 windows of 125 tokens, three heads of 16 channels: forward 19 us,
+// rows 26 us, columns 21 us, bias 22 us (fp32 arithmetic of attention_grad_simt.cu: 28, 48, 49,
+// 33 us); of 343 tokens: 94, 179, 123 and 81 us, with 32 channels 188, 332, 195 and 110 us.
+// Measured and not kept, at 125 tokens: two warps per 16 rows that share out the tokens (96 us in
+// all, against 84 us before the third part was added to the sums' operands); tokens staged a tile
+// ahead by asynchronous copies (94 us, the same, and 285 against 202 us at 144 tokens, where the
+// second stage takes the place of the bias).
 #include <cmath>
 #include <type_traits>
 

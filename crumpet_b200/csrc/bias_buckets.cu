@@ -16,6 +16,11 @@
 // once for all of them and the gathers, which are all latency, go out together.  The warps of a CTA take neighbouring
 // items, whose pairs are neighbours in memory, so the sectors that one gather opens serve the
 // others from L1.  Buckets of several items are finished by a second kernel.
+//
+// Measured: 24 heads of a 7 x 7 x 7 window in fp32, both ways: 18 us, three launches' latency (its
+// 25 MB would take 3.8 us); 1024 x 1024 pairs in logarithmic buckets, 16 heads, bf16, both ways:
+// 26 us, 12 us of them HBM time, the gradient's gathers (84 % of the warps resident, nearly all
+// waiting for loads) the larger part.  Eight heads per warp were slower than four.
 #include <type_traits>
 
 #include "common.cuh"

@@ -18,6 +18,11 @@
 // neighbour each other (16-byte accesses) where C and the pointers allow, else lie P apart.
 // Column sums stay in registers over all rows of a lane, are joined per CTA and written as one
 // partial row per CTA, which a second kernel adds up in a fixed order: no atomics.
+//
+// Measured: forward of 110592 x 48 in bf16 12 us, 6.6 us of HBM time; backward of 442368 x 48, fp16
+// branch and fp32 stream, all sums, 102 us, 59 us of HBM time: the shuffles of the rows' sums keep
+// the load/store pipe 69 % busy and 128 registers hold it to 16 warps per SM.  A ring of
+// asynchronous copies in shared memory instead of the registers' row ahead took 120 us.
 #include "common.cuh"
 #include "kernels.h"
 
