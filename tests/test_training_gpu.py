@@ -131,6 +131,37 @@ def test_attention_fp32_kernels(case, dtype):
     check_attention(attention_case(*case, dtype, F32))
 
 
+# fp32 at head dims 16 and 32 multiplies in split products, each 2^-22 from the fp32 one on
+# average (2^-20 at most), like the exponential: the same tolerance
+@pytest.mark.parametrize("case", [
+    ((1, 3, 5), (8, 8, 8), (0, 1, 2), 2, 3, 16),    # one warp per CTA, two windows per CTA
+    ((2, 4, 4), (4, 4, 4), (1, 2, 2), 4, 2, 32),    # 32 tokens: a block
+    ((3, 11, 1), (2, 2, 1), (1, 5, 0), 1, 2, 16),   # 33: one past it
+    ((7, 7, 7), (1, 2, 2), (0, 3, 3), 1, 2, 32),    # bias by tiles
+    ((8, 8, 8), (2, 1, 1), (4, 0, 0), 1, 1, 16),    # 512
+], ids=str)
+def test_attention_fp32_split_products(case):
+    check_attention(attention_case(*case, F32, F32))
+
+
+@pytest.mark.parametrize("d", [16, 32])
+def test_attention_fp32_unaligned(d):
+    """Tensors off 16-byte boundaries give the same bits as aligned ones."""
+    c = attention_case((3, 5, 5), (2, 1, 1), (1, 0, 0), 1, 2, d, F32, F32)
+    buckets = crumpet.relative_position_buckets(c["index"], c["table"].shape[0])
+
+    def off(t):
+        return torch.empty(t.numel() + 1, device="cuda")[1:].view(t.shape).copy_(t)
+
+    a = (c["grad"], c["qkv"], c["table"], buckets)
+    u = (off(c["grad"]), off(c["qkv"]), c["table"], buckets)
+    for x, y in zip(crumpet.swin_window_attention_backward(*a, **c["place"]),
+                    crumpet.swin_window_attention_backward(*u, **c["place"])):
+        assert torch.equal(x, y)
+    assert torch.equal(crumpet.swin_window_attention_train(*a[1:], **c["place"]),
+                       crumpet.swin_window_attention_train(*u[1:], **c["place"]))
+
+
 def test_attention_one_token():
     """A window of one token: softmax of one score; only v has a gradient."""
     for dtype in (F32, BF16):
