@@ -229,8 +229,9 @@ def swin_window_attention_train(
     scale: float | None = None,
 ) -> torch.Tensor:
     """:func:`~crumpet_b200.swin_window_attention_qkv` for training: the same result (in
-    fp32 to rounding, about 1e-6), from ``qkv [B, N, 3, H, head_dim]``, the bias ``table [num_buckets, H]`` and its ``buckets``
-    (of the ``[N, N]`` index), differentiable in ``qkv`` and ``table``."""
+    fp32 to rounding, about 1e-6), from ``qkv [B, N, 3, H, head_dim]``, the bias ``table
+    [num_buckets, H]`` and its ``buckets`` (of the ``[N, N]`` index), differentiable in ``qkv`` and
+    ``table``."""
     place = _place(qkv, table, buckets, num_windows, window_size, shift_size, scale)
     if _needs_grad(qkv, table):
         return _WindowAttention.apply(qkv, table, buckets, place)

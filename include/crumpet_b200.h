@@ -410,8 +410,8 @@ CRUMPET_API int crumpet_relative_position_bias_backward(
 /*
  * crumpet_swin_window_attention_qkv in fp32 arithmetic for every input of its domain, with the
  * buckets as checked int32 pairs [N, N] (as the gradient below takes them): the training forward
- * of what the tensor-core kernel does not take.  Four lanes share a row's keys for head dims up
- * to 32, so small batches fill the GPU.
+ * of what the 16-bit tensor-core kernel does not take.  fp32 at head dims 16 and 32 multiplies in
+ * split tf32 products (2^-22 on average).
  */
 CRUMPET_API int crumpet_swin_window_attention_qkv_pairs(
     void* out, const void* qkv, const void* bias_table, int table_f32, int64_t table_rows,
