@@ -21,10 +21,10 @@
 //     of the (head, query tile), stored as elem(bias)/scale in shared memory,
 //     multiplied by a 16x16 identity (one exact product per sum).  So S holds
 //     q.k + bias/scale; padded key columns carry -30000 and drop out.
+//   * The analytic shifted-window mask is one more MMA: -100 / scale where the roll-side
+//     codes of query and key differ on a "last window" axis.
 //   * Softmax warps pull S into registers, add a dense mask (global loads, read
-//     only for windows flagged in `boundary`) or the analytic shifted-window mask
-//     (entries whose roll-side codes differ on a "last window" axis become -inf,
-//     the exact limit of the reference's -100), take the chunk maximum, and
+//     only for windows flagged in `boundary`), take the chunk maximum, and
 //     write P = 2^(x - m_ref) (x = S * scale * log2 e) as fp16/bf16 into one of
 //     two TMEM P buffers.  m_ref is a lazy row maximum: it moves only when a
 //     chunk exceeds it by more than 8 (P <= 2^8), and then O is rescaled in TMEM.
@@ -105,10 +105,11 @@ struct Cfg {
   // [16 keys][16] of 1.0: every PV MMA (K = 16 keys) reads its ones columns from this one
   // block (the content is the same for every key, so the swizzle does not matter)
   static constexpr int ONES_BYTES = 16 * kRowBytes;
-  // Shifted-window mask on the tensor cores: three query-feature tiles (one per axis,
-  // [128 rows x 16], UMMA A operand like the bias tile) and one key-feature tile
-  // ([NPAD keys x 16], UMMA B operand, K-major without swizzle).
-  static constexpr int MASKA_BYTES = 3 * (kBM / 8) * 128 * 2;
+  // Shifted-window mask on the tensor cores: seven query-feature tiles (one per set of
+  // masked axes, [128 rows x 8], UMMA A operand like the bias tile) and one key-feature
+  // tile ([NPAD keys x 16], UMMA B operand, K-major without swizzle).
+  static constexpr int MASKA_TILE = (kBM / 8) * 128;
+  static constexpr int MASKA_BYTES = 7 * MASKA_TILE;
   static constexpr int MASKB_BYTES = (NPAD / 8) * 128 * 2;
   // TMEM columns of one WG: S chunk (64), NPB P chunk buffers (32 packed each),
   // O_0 (16) + row sum (16) [+ O_1 (16) for head dim 32].
@@ -523,21 +524,17 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
     fence_mbar_init();
   }
   if constexpr (MASK == kMaskAnalytic) {
-    // Key features of the mask MMA, B[j][2a] = (1 - code_j,a) * pen, B[j][2a+1] = code_j,a * pen
-    // with pen = elem(-100 / scale); with the query features A_a[i][2a] = code_i,a,
-    // A_a[i][2a+1] = 1 - code_i,a of one axis a, sum_k A_a[i][k] B[j][k] is pen exactly when
-    // the two tokens sit on different sides of that axis' roll seam, else 0.  Padded keys
-    // get no features (the bias tile already drops them).  K-major without swizzle: element
-    // (j, k) at (k / 8) * (NPAD / 8) * 128 + (j / 8) * 128 + (j % 8) * 16 + (k % 8) * 2.
-    const uint16_t pen = f32_to_elem<BF16>(-100.f / p.scale);
+    // The mask MMA sums A[i][k] B[j][k] over the eight roll-side codes k: B[j] is 1 at key j's
+    // own code, A[i] is elem(-100 / scale) at the codes that differ from query i's on a masked
+    // axis.  So a pair gets the penalty once, whatever the number of axes it differs on.  Padded
+    // keys get no features (the bias tile already drops them), and the upper half of the MMA's
+    // depth none (below).  K-major without swizzle: element (j, k) at
+    // (k / 8) * (NPAD / 8) * 128 + (j / 8) * 128 + (j % 8) * 16 + (k % 8) * 2.
+    const uint16_t one = BF16 ? 0x3F80u : 0x3C00u;
     uint16_t* mb = reinterpret_cast<uint16_t*>(maskb_s);
     for (int e = threadIdx.x; e < NPAD * 16; e += kThreads) {
       const int j = e >> 4, k = e & 15;
-      uint16_t val = 0;
-      if (j < p.N && k < 6) {
-        const uint32_t bit = (token_code(p, j) >> (k >> 1)) & 1u;
-        val = ((k & 1) ? bit : 1u - bit) ? pen : uint16_t(0);
-      }
+      const uint16_t val = j < p.N && token_code(p, j) == uint32_t(k) ? one : uint16_t(0);
       mb[((k >> 3) * (NPAD / 8) * 128 + (j >> 3) * 128 + (j & 7) * 16 + (k & 7) * 2) / 2] = val;
     }
   }
@@ -721,17 +718,15 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
                 umma_ss(tS + uint32_t(16 * i), bdesc, ident_desc, idesc_bias, 1u);
               }
               if constexpr (MASK == kMaskAnalytic) {
-                // shifted-window mask: one MMA per masked axis adds the penalty where the
-                // query and key sit on different sides of that axis' roll seam
-                const uint64_t kf = smem_desc(maskb_addr + uint32_t(c * kCH / 8) * 128u,
-                                              (NPAD / 8) * 128, 128, kLayoutNone);
-#pragma unroll
-                for (int a = 0; a < 3; ++a) {
-                  if ((am >> a) & 1u) {
-                    const uint64_t qf = smem_desc(maska_addr + uint32_t(a) * (kBM / 8) * 256u,
-                                                  (kBM / 8) * 128, 128, kLayoutNone);
-                    umma_ss(tS, qf, kf, idesc_f16(kBM, width, BF16, false), 1u);
-                  }
+                // shifted-window mask: the query features of this window's masked axes.  The
+                // MMA's depth is 16: its upper half reads the next set's tile (after the last
+                // one, the key features), which the key features multiply by 0.
+                if (am != 0) {
+                  const uint64_t kf = smem_desc(maskb_addr + uint32_t(c * kCH / 8) * 128u,
+                                                (NPAD / 8) * 128, 128, kLayoutNone);
+                  const uint64_t qf = smem_desc(maska_addr + (am - 1) * uint32_t(C::MASKA_TILE),
+                                                C::MASKA_TILE, 128, kLayoutNone);
+                  umma_ss(tS, qf, kf, idesc_f16(kBM, width, BF16, false), 1u);
                 }
               }
               umma_commit(bar(w, kSF));
@@ -787,21 +782,19 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
         build_bias_tile<NPAD, BF16>(p, h, mt, tid_sm, kSmThreads, bias_s);
       }
       if constexpr (MASK == kMaskAnalytic) {
-        // Query features of the mask MMA for this query tile, one [128 x 16] tile per axis a:
-        // A_a[r][2a] = code_a(row), A_a[r][2a + 1] = 1 - code_a(row), 0 elsewhere and in rows
-        // past N; same core-matrix layout as the bias tile.
-        const uint16_t one = BF16 ? 0x3F80u : 0x3C00u;
+        // Query features of the mask MMA for this query tile, one [128 x 8] tile per set of
+        // masked axes (bits of 1 .. 7): A[r][k] = elem(-100 / scale) where code k and the row's
+        // differ on one of them.  Core matrices as in the bias tile, without a second column group.
+        const uint16_t pen = f32_to_elem<BF16>(-100.f / p.scale);
         uint16_t* ma = reinterpret_cast<uint16_t*>(maska_s);
-        for (int e = tid_sm; e < 3 * kBM * 16; e += kSmThreads) {
-          const int a = e / (kBM * 16), r = (e / 16) % kBM, k = e % 16;
+        for (int e = tid_sm; e < kBM * 8; e += kSmThreads) {
+          const int r = e / 8, k = e % 8;
           const int grow = mt * kBM + r;
-          uint16_t val = 0;
-          if (grow < p.N && (k >> 1) == a) {
-            const uint32_t bit = (token_code(p, grow) >> a) & 1u;
-            val = ((k & 1) ? 1u - bit : bit) ? one : uint16_t(0);
-          }
-          ma[(a * (kBM / 8) * 256 + (k >> 3) * (kBM / 8) * 128 + (r >> 3) * 128 + (r & 7) * 16 +
-              (k & 7) * 2) / 2] = val;
+          const uint32_t apart = grow < p.N ? token_code(p, grow) ^ uint32_t(k) : 0u;
+#pragma unroll
+          for (int axes = 1; axes < 8; ++axes)
+            ma[((axes - 1) * C::MASKA_TILE + (r >> 3) * 128 + (r & 7) * 16 + k * 2) / 2] =
+                (apart & axes) ? pen : uint16_t(0);
         }
       }
       fence_proxy_async_shared();  // bias / mask tiles -> tensor-core (async proxy) reads

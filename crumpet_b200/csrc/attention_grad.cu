@@ -351,19 +351,19 @@ __device__ __forceinline__ void start_values(const GradParams& p, int h, int row
     }
 }
 
-// Shifted-window mask as one more product of depth 8 in the windows that need it: per axis a
-// (of the lane's t4) a row token has the features (bit, 1 - bit) of its roll-side code and a
-// column token ((1 - bit) pen, bit pen), pen = elem(-100 / scale), so their product is pen where
-// the two tokens lie on different sides of the seam, else 0.  Element pairs as mma operands.
-template <bool BF16>
-__device__ __forceinline__ uint32_t row_feature(uint32_t code, int axis) {
-  const uint32_t one = BF16 ? 0x3F80u : 0x3C00u;
-  return axis > 2 ? 0u : (code >> axis) & 1u ? one : one << 16;
+// Shifted-window mask as one more product of depth 8 in the windows that need it, over the eight
+// roll-side codes: a column token has the feature 1 at its own code, a row token pen = elem(-100 /
+// scale) at the codes that differ from its own on one of the window's masked axes `last`, so a pair
+// gets pen once, on however many axes it differs.  Element pairs (codes 2 t4 and 2 t4 + 1) as mma
+// operands.
+__device__ __forceinline__ uint32_t row_feature(uint32_t pen, uint32_t code, uint32_t last, int t4) {
+  const uint32_t apart = (uint32_t(2 * t4) ^ code) & last;  // of code 2 t4; the other's bit 0 differs
+  return (apart ? pen : 0u) | ((apart ^ (last & 1u)) ? pen << 16 : 0u);
 }
 template <bool BF16>
-__device__ __forceinline__ uint32_t col_feature(uint32_t code, int axis, float scale) {
-  const uint32_t pen = pack2<BF16>(-100.f / scale, 0.f) & 0xffffu;
-  return axis > 2 ? 0u : (code >> axis) & 1u ? pen << 16 : pen;
+__device__ __forceinline__ uint32_t col_feature(uint32_t code, int t4) {
+  const uint32_t one = BF16 ? 0x3F80u : 0x3C00u;
+  return int(code >> 1) != t4 ? 0u : (code & 1u) ? one << 16 : one;
 }
 
 // 2^-(e + 4) for the exponent e of m: rows of do scaled by it have magnitudes below 1/8, so
@@ -498,12 +498,13 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
     init_tail(tail);
     for (int k = 0; k < STAGES && k < count; ++k) issue(k);
   }
-  uint32_t f0 = 0, f1 = 0;
+  uint32_t code0 = 0, code1 = 0, pen = 0;
   if (p.analytic) {
     for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
-      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4, p.scale) : 0u;
-    f0 = i0 < p.N ? row_feature<BF16>(side_code(p, i0), t4) : 0u;
-    f1 = i1 < p.N ? row_feature<BF16>(side_code(p, i1), t4) : 0u;
+      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4) : 0u;
+    code0 = i0 < p.N ? side_code(p, i0) : 0u;
+    code1 = i1 < p.N ? side_code(p, i1) : 0u;
+    pen = pack2<BF16>(-100.f / p.scale, 0.f) & 0xffffu;
   }
   if (warp == 0) {
     tmem_alloc(&tail->tm_slot, S::TM_COLS);
@@ -646,8 +647,7 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
       if (p.analytic) {
         const uint32_t last = tail->last[k % STAGES];
         if (last != 0) {
-          const bool on = (last >> t4) & 1u;
-          const uint32_t a0 = on ? f0 : 0u, a1 = on ? f1 : 0u;
+          const uint32_t a0 = row_feature(pen, code0, last, t4), a1 = row_feature(pen, code1, last, t4);
           const uint32_t* mb = mask_s + (cg * S::WC + g) * 4 + t4;
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma8<BF16>(s[t], a0, a1, mb[32 * t]);
@@ -880,12 +880,13 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
   for (int i = tid; i < STAGES * S::NPAD; i += S::THREADS)
     *reinterpret_cast<float2*>(smem + (i / S::NPAD) * S::STAGE + 2 * S::COLS + 2 * S::ROWS +
                                (i % S::NPAD) * 8) = make_float2(0.f, 0.f);
-  uint32_t f0 = 0, f1 = 0;
+  uint32_t code0 = 0, code1 = 0, pen = 0;
   if (p.analytic) {
     for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
-      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4, p.scale) : 0u;
-    f0 = k0 < p.N ? row_feature<BF16>(side_code(p, k0), t4) : 0u;
-    f1 = k1 < p.N ? row_feature<BF16>(side_code(p, k1), t4) : 0u;
+      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4) : 0u;
+    code0 = k0 < p.N ? side_code(p, k0) : 0u;
+    code1 = k1 < p.N ? side_code(p, k1) : 0u;
+    pen = pack2<BF16>(-100.f / p.scale, 0.f) & 0xffffu;
   }
   if (warp == 0) {
     tmem_alloc(&tail->tm_slot, S::TM_COLS);
@@ -948,8 +949,7 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
           smem + (k % STAGES) * S::STAGE + 2 * S::COLS + 2 * S::ROWS) + 2 * t4;
       uint32_t last = 0;
       if (p.analytic) last = tail->last[k % STAGES];
-      const bool on = (last >> t4) & 1u;
-      const uint32_t a0 = on ? f0 : 0u, a1 = on ? f1 : 0u;
+      const uint32_t a0 = row_feature(pen, code0, last, t4), a1 = row_feature(pen, code1, last, t4);
       const uint32_t* mb = mask_s + g * 4 + t4;
 
       uint32_t ka[R::KS][4], va[R::KS][4];

@@ -1,0 +1,43 @@
+"""Training operators at the edges of their domain: masks that outweigh the scores, extreme
+values, plans and calls that a program can get wrong."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import crumpet_b200 as crumpet
+from test_training_gpu import BF16, F16, F32, TOL, attention64, attention_case, rel
+
+pytestmark = pytest.mark.gpu
+
+
+def attention_both(c, grad=None, **place):
+    buckets = crumpet.relative_position_buckets(c["index"], c["table"].shape[0])
+    place = dict(c["place"], **place)
+    return (crumpet.swin_window_attention_train(c["qkv"], c["table"], buckets, **place),
+            *crumpet.swin_window_attention_backward(c["grad"] if grad is None else grad, c["qkv"],
+                                                    c["table"], buckets, **place))
+
+
+def attention_wide(c):
+    qkv = c["qkv"].double().requires_grad_(True)
+    table = c["table"].double().requires_grad_(True)
+    out = attention64(qkv, table, c["index"], c["mask"], c["scale"])
+    return (out.detach(), *torch.autograd.grad(out, (qkv, table), c["grad"].double()))
+
+
+# Scores reach 2^10: the product, its sums with bias and mask, and the row's log-sum-exp each
+# round them to 2^-14 or finer in fp32, so p and ds are off by at most 4 * 2^-14 (relative); 1e-3
+# on top of the tolerances of check_attention.  fp32: the split products' 2^-22 of 2^10, within it.
+@pytest.mark.parametrize("shift", [(2, 0, 0), (2, 2, 0), (0, 2, 2), (2, 2, 2)], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_attention_mask_is_added_once(dtype, shift):
+    """Scores several hundred apart: two tokens on different sides of one, two or three seams
+    have one -100 between them (16 channels: -100 / scale is exact in every type)."""
+    c = attention_case((4, 4, 4), (2, 2, 2), shift, 2, 2, 16, dtype, F32)
+    c["qkv"][:, :, :2] *= 10
+    got, want = attention_both(c), attention_wide(c)
+    for a, b, tol in zip(got, want, (1.5 * TOL[dtype], TOL[dtype], TOL[F32])):
+        assert torch.isfinite(a.float()).all()
+        assert rel(a, b) <= tol + 1e-3
