@@ -362,8 +362,8 @@ __device__ __forceinline__ uint32_t window_last_axes(const KParams& p, int b) {
 // to dst (shared or global memory) as the UMMA K-major no-swizzle operand image:
 // elem(elem(bias) / scale) -- rounded to the element type first, as the reference's
 // .to(dtype) -- at rows < N and columns < N; -30000 in padded key columns (their
-// scores drop out of the softmax: 2^(-30000 scale log2 e) is 0); 0 in padded query
-// rows.  Core matrix (row group rg, column group cg) at cg * (kBM / 8) * 128 + rg * 128.
+// scores drop out of the softmax: 30000 scale is at least 117 (kTensorMinScale)); 0 in
+// padded query rows.  Core matrix (row group rg, column group cg) at cg * (kBM / 8) * 128 + rg * 128.
 // Each item is 8 consecutive columns of one row (one 16-byte core-matrix row); two
 // items per thread are in flight.  Threads tid = 0 .. nthreads-1 share the work.
 template <int NPAD, bool BF16>
@@ -1157,11 +1157,11 @@ int launch_window_attention(const AttnArgs& a, cudaStream_t stream) {
       if (a.shift[i] < 0 || a.shift[i] >= a.win[i])
         return set_error(kErrInvalid, "analytic mask shift must satisfy 0 <= shift < window");
   }
-  // The tensor-core kernel: fp16 / bf16, head_dim 16 or 32, N <= 352, q/k/v/out on
-  // 16-byte boundaries with 16-byte row strides (TMA); everything else runs the
-  // fp32 SIMT kernel (attention_simt.cu).
+  // The tensor-core kernel: fp16 / bf16, head_dim 16 or 32, N <= 352, a scale by which bias,
+  // mask and padding can be divided (kTensorMinScale), q/k/v/out on 16-byte boundaries with
+  // 16-byte row strides (TMA); everything else runs the fp32 SIMT kernel (attention_simt.cu).
   const bool tensor_path =
-      a.dtype != kF32 && (a.head_dim == 16 || a.head_dim == 32) && a.N <= 352 &&
+      a.dtype != kF32 && a.scale >= kTensorMinScale && (a.head_dim == 16 || a.head_dim == 32) && a.N <= 352 &&
       aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out) &&
       (a.qkv_stride_n | a.qkv_stride_h | a.qkv_stride_b) % 8 == 0 &&
       (a.out_stride_n | a.out_stride_h | a.out_stride_b) % 8 == 0;
@@ -1169,7 +1169,7 @@ int launch_window_attention(const AttnArgs& a, cudaStream_t stream) {
     if (a.bias_tiles)
       return set_error(kErrUnsupported,
                        "prebuilt bias tiles apply to fp16 / bf16 head_dim 16 or 32 windows of at "
-                       "most 352 tokens with 16-byte aligned tensors");
+                       "most 352 tokens with 16-byte aligned tensors and a scale of at least 2^-8");
     return launch_window_attention_simt(a, stream);
   }
 

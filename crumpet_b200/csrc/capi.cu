@@ -14,6 +14,8 @@
 
 namespace crumpet {
 
+static_assert(kTensorMinScale == CRUMPET_TENSOR_MIN_SCALE, "as the header says");
+
 namespace {
 thread_local char g_last_error[512] = {0};
 }
@@ -595,7 +597,8 @@ int crumpet_swin_window_attention_qkv_backward(
   a.shares = shares;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(grad_qkv) |
                          reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(qkv);
-  const bool tensor = attention_grad_tensor_path(dtype, H, N, head_dim) && (bits & 15u) == 0;
+  const bool tensor = attention_grad_tensor_path(dtype, H, N, head_dim) && (bits & 15u) == 0 &&
+                      scale >= kTensorMinScale;
   if (int e = tensor ? launch_attention_grad(a, on) : launch_attention_grad_simt(a, on)) return e;
   return launch_sum_shares(grad_bias, shares, H * N * N, on);
 }

@@ -132,6 +132,8 @@ int launch_window_attention_static_tiles(const AttnArgs& a, cudaStream_t stream)
 // The fp32 SIMT attention kernel (attention_simt.cu) for what the tensor-core kernel does
 // not take: float32 q/k/v, head_dim 64..256, N > 384, unaligned operands.  Arguments are
 // validated by launch_window_attention, which dispatches here.
+// Least scale of the 16-bit tensor-core attention kernels, forward and gradient.
+constexpr float kTensorMinScale = 1.f / 256.f;  // CRUMPET_TENSOR_MIN_SCALE
 bool simt_attention_head_dim(int64_t head_dim);
 int launch_window_attention_simt(const AttnArgs& a, cudaStream_t stream);
 

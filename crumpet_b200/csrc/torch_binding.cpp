@@ -738,7 +738,8 @@ at::Tensor swin_window_attention_train(const at::Tensor& qkv, const at::Tensor& 
   // The tensor-core kernel's domain.  The table changes every step, so its bias operands are
   // built every step.
   const bool tiles_apply = code != CRUMPET_DTYPE_F32 && (Dh == 16 || Dh == 32) && N <= 352 &&
-                           B > 0 && reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
+                           B > 0 && s >= CRUMPET_TENSOR_MIN_SCALE &&
+                           reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
   if (tiles_apply) {
     at::Tensor tiles =
         at::empty({crumpet_attention_bias_tiles_bytes(H, N)}, x.options().dtype(at::kByte));

@@ -112,9 +112,12 @@ def fused_swin_attention(
     return out
 
 
-def tensor_core_attention(dtype: torch.dtype, N: int, head_dim: int) -> bool:
-    """Whether the tcgen05 kernel runs these windows (else the fp32 SIMT kernel)."""
-    return dtype in (torch.float16, torch.bfloat16) and head_dim in (16, 32) and 1 <= N <= 352
+def tensor_core_attention(dtype: torch.dtype, N: int, head_dim: int,
+                          scale: float | None = None) -> bool:
+    """Whether the tcgen05 kernel runs these windows (else the fp32 SIMT kernel).  It divides
+    bias and mask by the scale in 16 bits, so it takes scales of at least 2^-8."""
+    return (dtype in (torch.float16, torch.bfloat16) and head_dim in (16, 32) and 1 <= N <= 352
+            and (scale is None or scale >= 2.0 ** -8))
 
 
 def attention_bias_tiles(relative_position_bias_table: torch.Tensor,
@@ -195,7 +198,7 @@ def swin_window_attention_qkv(
             "flops": 4 * B * H * N * N * D,
             "exps": B * H * N * N,
         })
-    if bias_tiles is not None and tensor_core_attention(qkv.dtype, N, D):
+    if bias_tiles is not None and tensor_core_attention(qkv.dtype, N, D, float(scale)):
         ops.swin_window_attention_qkv_tiles(out, qkv.contiguous(), bias_tiles, list(num_windows),
                                             list(window_size), list(shift_size), float(scale))
     else:

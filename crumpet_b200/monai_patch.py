@@ -270,7 +270,7 @@ def _bias_tiles(attn, n: int, head_dim: int, dtype: torch.dtype):
     ``attention_bias_tiles``), cached on the module and rebuilt when the table or index
     tensor, its in-place version, n, the dtype or the scale changes; None where the
     tensor-core kernel does not run these windows (it then gathers the bias itself)."""
-    if not tensor_core_attention(dtype, n, head_dim):
+    if not tensor_core_attention(dtype, n, head_dim, float(attn.scale)):
         return None
     table, index = attn.relative_position_bias_table, attn.relative_position_index
     key = (table.data_ptr(), table._version, index.data_ptr(), index._version, n, dtype,

@@ -33,6 +33,12 @@ extern "C" {
 #define CRUMPET_DTYPE_F16 1
 #define CRUMPET_DTYPE_BF16 2
 
+/* Least scale of the 16-bit tensor-core attention kernels, 2^-8: they add bias, mask and the
+ * exclusion of padded keys to the scores divided by it, in the element type, which has to hold
+ * -100 / scale (fp16: up to 65504) and a padding of -30000 that outweighs it.  Calls with a
+ * smaller scale run the fp32 kernels (with prebuilt bias tiles: CRUMPET_ERR_UNSUPPORTED). */
+#define CRUMPET_TENSOR_MIN_SCALE 0.00390625f
+
 /* Status codes. */
 #define CRUMPET_OK 0
 #define CRUMPET_ERR_INVALID 1     /* bad shape, size, dtype or pointer */
@@ -428,8 +434,8 @@ CRUMPET_API int crumpet_swin_window_attention_qkv_pairs(
  * what crumpet_window_attention_backward_shares gives for these sizes; `stats` is fp32
  * scratch of B * H * (3 * N + 4) elements, 16-byte aligned.  The bias is used as the table has it (the forward rounds
  * it to dtype); the row statistics are taken again in fp32.  dtype, head_dim and N as for the
- * forward: F16 / BF16 with head_dim 16 or 32, N <= 352 and 16-byte aligned tensors run the
- * tensor-core kernels, every other call an fp32 SIMT kernel.
+ * forward: F16 / BF16 with head_dim 16 or 32, N <= 352, 16-byte aligned tensors and a scale of
+ * at least CRUMPET_TENSOR_MIN_SCALE run the tensor-core kernels, every other call fp32 ones.
  */
 CRUMPET_API int64_t crumpet_window_attention_backward_shares(int64_t B, int64_t H, int64_t N,
                                                              int64_t head_dim, int dtype);

@@ -41,3 +41,17 @@ def test_attention_mask_is_added_once(dtype, shift):
     for a, b, tol in zip(got, want, (1.5 * TOL[dtype], TOL[dtype], TOL[F32])):
         assert torch.isfinite(a.float()).all()
         assert rel(a, b) <= tol + 1e-3
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -8, 1e-3, 1e-5])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_attention_small_scales(dtype, scale):
+    """A scale too small for the mask and the padding to be divided by it in the element type
+    (27 tokens: padded keys).  Queries and keys are larger by as much: scores of a usual size."""
+    c = attention_case((3, 3, 3), (2, 2, 2), (1, 1, 1), 1, 2, 16, dtype, F32)
+    c["qkv"][:, :, :2] *= (0.25 / scale) ** 0.5
+    c["scale"] = scale
+    got, want = attention_both(c, scale=scale), attention_wide(c)
+    for a, b, tol in zip(got, want, (1.5 * TOL[dtype], TOL[dtype], TOL[F32])):
+        assert torch.isfinite(a.float()).all()
+        assert rel(a, b) <= tol
