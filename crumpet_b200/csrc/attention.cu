@@ -146,6 +146,7 @@ struct KParams {
   int mask_windows;
   // analytic mask: windows per axis and window / shift sizes of the token grid
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
+  uint32_t mask_pen, mask_one;  // its features' values (MaskPenalty)
   // output
   uint16_t* out;
   long long out_sb, out_sh, out_sn;
@@ -524,13 +525,13 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
     fence_mbar_init();
   }
   if constexpr (MASK == kMaskAnalytic) {
-    // The mask MMA sums A[i][k] B[j][k] over the eight roll-side codes k: B[j] is 1 at key j's
-    // own code, A[i] is elem(-100 / scale) at the codes that differ from query i's on a masked
-    // axis.  So a pair gets the penalty once, whatever the number of axes it differs on.  Padded
+    // The mask MMA sums A[i][k] B[j][k] over the eight roll-side codes k: B[j] is mask_one at
+    // key j's own code, A[i] is mask_pen at the codes that differ from query i's on a masked
+    // axis (their product is -100 / scale).  So a pair gets the penalty once, whatever the number of axes it differs on.  Padded
     // keys get no features (the bias tile already drops them), and the upper half of the MMA's
     // depth none (below).  K-major without swizzle: element (j, k) at
     // (k / 8) * (NPAD / 8) * 128 + (j / 8) * 128 + (j % 8) * 16 + (k % 8) * 2.
-    const uint16_t one = BF16 ? 0x3F80u : 0x3C00u;
+    const uint16_t one = uint16_t(p.mask_one);
     uint16_t* mb = reinterpret_cast<uint16_t*>(maskb_s);
     for (int e = threadIdx.x; e < NPAD * 16; e += kThreads) {
       const int j = e >> 4, k = e & 15;
@@ -783,9 +784,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tq,
       }
       if constexpr (MASK == kMaskAnalytic) {
         // Query features of the mask MMA for this query tile, one [128 x 8] tile per set of
-        // masked axes (bits of 1 .. 7): A[r][k] = elem(-100 / scale) where code k and the row's
+        // masked axes (bits of 1 .. 7): A[r][k] = mask_pen where code k and the row's
         // differ on one of them.  Core matrices as in the bias tile, without a second column group.
-        const uint16_t pen = f32_to_elem<BF16>(-100.f / p.scale);
+        const uint16_t pen = uint16_t(p.mask_pen);
         uint16_t* ma = reinterpret_cast<uint16_t*>(maska_s);
         for (int e = tid_sm; e < kBM * 8; e += kSmThreads) {
           const int r = e / 8, k = e % 8;
@@ -1205,6 +1206,11 @@ int launch_window_attention(const AttnArgs& a, cudaStream_t stream) {
   kp.wsd = int(a.win[0]);
   kp.wsh = int(a.win[1]);
   kp.wsw = int(a.win[2]);
+  if (a.analytic) {
+    const MaskPenalty m = mask_penalty(a.scale, a.dtype == kBF16);
+    kp.mask_pen = m.pen;
+    kp.mask_one = m.one;
+  }
   kp.ssd = int(a.shift[0]);
   kp.ssh = int(a.shift[1]);
   kp.ssw = int(a.shift[2]);

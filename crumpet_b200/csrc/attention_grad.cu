@@ -67,6 +67,7 @@ struct GradParams {
   int table_f32;
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
   int analytic;
+  uint32_t mask_pen, mask_one;  // the mask features' values (MaskPenalty)
   int B, H, N, NS;       // NS = N rounded up to 2: rows of stats start on 16 bytes
   int RB, S;             // row blocks, and shares that the windows are split into
   float scale;
@@ -352,17 +353,15 @@ __device__ __forceinline__ void start_values(const GradParams& p, int h, int row
 }
 
 // Shifted-window mask as one more product of depth 8 in the windows that need it, over the eight
-// roll-side codes: a column token has the feature 1 at its own code, a row token pen = elem(-100 /
-// scale) at the codes that differ from its own on one of the window's masked axes `last`, so a pair
-// gets pen once, on however many axes it differs.  Element pairs (codes 2 t4 and 2 t4 + 1) as mma
-// operands.
+// roll-side codes: a column token has the feature mask_one at its own code, a row token mask_pen at
+// the codes that differ from its own on one of the window's masked axes `last`, so a pair gets their
+// product -100 / scale once, on however many axes it differs.  Element pairs (codes 2 t4 and
+// 2 t4 + 1) as mma operands.
 __device__ __forceinline__ uint32_t row_feature(uint32_t pen, uint32_t code, uint32_t last, int t4) {
   const uint32_t apart = (uint32_t(2 * t4) ^ code) & last;  // of code 2 t4; the other's bit 0 differs
   return (apart ? pen : 0u) | ((apart ^ (last & 1u)) ? pen << 16 : 0u);
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t col_feature(uint32_t code, int t4) {
-  const uint32_t one = BF16 ? 0x3F80u : 0x3C00u;
+__device__ __forceinline__ uint32_t col_feature(uint32_t one, uint32_t code, int t4) {
   return int(code >> 1) != t4 ? 0u : (code & 1u) ? one << 16 : one;
 }
 
@@ -498,13 +497,13 @@ grad_rows_kernel(const __grid_constant__ Maps maps, const GradParams p) {
     init_tail(tail);
     for (int k = 0; k < STAGES && k < count; ++k) issue(k);
   }
-  uint32_t code0 = 0, code1 = 0, pen = 0;
+  uint32_t code0 = 0, code1 = 0;
+  const uint32_t pen = p.mask_pen;
   if (p.analytic) {
     for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
-      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4) : 0u;
+      mask_s[i] = i / 4 < p.N ? col_feature(p.mask_one, side_code(p, i / 4), i % 4) : 0u;
     code0 = i0 < p.N ? side_code(p, i0) : 0u;
     code1 = i1 < p.N ? side_code(p, i1) : 0u;
-    pen = pack2<BF16>(-100.f / p.scale, 0.f) & 0xffffu;
   }
   if (warp == 0) {
     tmem_alloc(&tail->tm_slot, S::TM_COLS);
@@ -880,13 +879,13 @@ grad_cols_kernel(const __grid_constant__ Maps maps, const GradParams p) {
   for (int i = tid; i < STAGES * S::NPAD; i += S::THREADS)
     *reinterpret_cast<float2*>(smem + (i / S::NPAD) * S::STAGE + 2 * S::COLS + 2 * S::ROWS +
                                (i % S::NPAD) * 8) = make_float2(0.f, 0.f);
-  uint32_t code0 = 0, code1 = 0, pen = 0;
+  uint32_t code0 = 0, code1 = 0;
+  const uint32_t pen = p.mask_pen;
   if (p.analytic) {
     for (int i = tid; i < S::NPAD * 4; i += S::THREADS)
-      mask_s[i] = i / 4 < p.N ? col_feature<BF16>(side_code(p, i / 4), i % 4) : 0u;
+      mask_s[i] = i / 4 < p.N ? col_feature(p.mask_one, side_code(p, i / 4), i % 4) : 0u;
     code0 = k0 < p.N ? side_code(p, k0) : 0u;
     code1 = k1 < p.N ? side_code(p, k1) : 0u;
-    pen = pack2<BF16>(-100.f / p.scale, 0.f) & 0xffffu;
   }
   if (warp == 0) {
     tmem_alloc(&tail->tm_slot, S::TM_COLS);
@@ -1241,6 +1240,11 @@ int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   p.pairs = a.pairs;
   p.table_f32 = a.table_f32 ? 1 : 0;
   p.analytic = (a.shift[0] | a.shift[1] | a.shift[2]) != 0;
+  if (p.analytic) {
+    const MaskPenalty m = mask_penalty(a.scale, a.dtype == kBF16);
+    p.mask_pen = m.pen;
+    p.mask_one = m.one;
+  }
   p.nwd = int(a.nwin[0]);
   p.nwh = int(a.nwin[1]);
   p.nww = int(a.nwin[2]);

@@ -5,6 +5,7 @@
 // cuda/attn_mask_3d.cu:143), launches on the caller's stream, never allocates
 // and never synchronises.  Failures return a non-zero status and leave a
 // message for crumpet_last_error().
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 
@@ -28,6 +29,30 @@ int set_error(int code, const char* msg) {
 int set_cuda_error(cudaError_t err, const char* where) {
   std::snprintf(g_last_error, sizeof(g_last_error), "%s: %s", where, cudaGetErrorString(err));
   return kErrCuda;
+}
+
+MaskPenalty mask_penalty(float scale, bool bf16) {
+  const auto bits = [&](double v) -> uint32_t {
+    return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(float(v)))
+                : __half_as_ushort(__float2half_rn(float(v)));
+  };
+  const auto value = [&](uint32_t b) -> double {
+    return bf16 ? __bfloat162float(__ushort_as_bfloat16(uint16_t(b)))
+                : __half2float(__ushort_as_half(uint16_t(b)));
+  };
+  const double want = -100.0 / double(scale);
+  MaskPenalty best{bits(want), bits(1.0)};
+  double least = std::fabs(value(best.pen) - want);
+  for (int i = 1; i < 128 && least > 0.0; ++i) {  // 1 + i / 128: a number of either type
+    const double one = 1.0 + i / 128.0;
+    const uint32_t pen = bits(want / one);
+    const double off = std::fabs(value(pen) * one - want);
+    if (off < least) {
+      least = off;
+      best = MaskPenalty{pen, bits(one)};
+    }
+  }
+  return best;
 }
 
 namespace {

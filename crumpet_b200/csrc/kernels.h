@@ -19,6 +19,15 @@ enum Status : int {
 int set_error(int code, const char* msg);
 int set_cuda_error(cudaError_t err, const char* where);
 
+// The shifted-window mask's penalty -100 / scale as a product of two numbers of the element type
+// (bits): `pen` in the row features of the mask product, `one` in the column features.  One such
+// number alone is off by up to 0.4 in the score (bf16 at scale 32^-1/2: 0.3); their product, of
+// twice the bits, by 0.01.  one is 1 where -100 / scale is exact.
+struct MaskPenalty {
+  uint32_t pen, one;
+};
+MaskPenalty mask_penalty(float scale, bool bf16);
+
 struct ShapeArgs {
   int64_t B, D, H, W, C;
   int64_t ws_d, ws_h, ws_w;

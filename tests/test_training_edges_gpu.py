@@ -55,3 +55,21 @@ def test_attention_small_scales(dtype, scale):
     for a, b, tol in zip(got, want, (1.5 * TOL[dtype], TOL[dtype], TOL[F32])):
         assert torch.isfinite(a.float()).all()
         assert rel(a, b) <= tol
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_attention_mask_is_100_at_32_channels(dtype):
+    """-100 / scale is not a number of the element type at scale 32^-1/2.  The mask's weight shows
+    where the scores make up for it: all queries are one vector, and keys on one side of the
+    seam score 100 (to rounding) above the others, so both sides weigh about the same for
+    queries of the other side.  A mask off by e changes the odds by exp(e); one 16-bit number
+    is off by 0.3 in bf16 and 0.03 in fp16, the product of two by at most 2^-7 and 2^-11."""
+    c = attention_case((2, 4, 4), (1, 2, 1), (0, 2, 0), 1, 1, 32, dtype, F32)
+    h = (torch.arange(32, device="cuda") // 4 % 4) >= 2  # the rolled side of the last window
+    c["qkv"][:, :, 0] = 4.0
+    c["qkv"][:, :, 1] = 0.0
+    c["qkv"][:, h, 1] = 4.4219  # 32 * 4 * 4.42 / sqrt 32 = 100.06
+    c["table"].zero_()
+    got, want = attention_both(c)[0], attention_wide(c)[0]
+    off = {BF16: 2.0 ** -7, F16: 2.0 ** -11}[dtype]
+    assert rel(got, want) <= TOL[dtype] + off
