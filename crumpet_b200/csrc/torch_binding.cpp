@@ -771,7 +771,13 @@ std::tuple<at::Tensor, at::Tensor> swin_window_attention_backward(
                         grad_out.size(2) == H * Dh && grad_out.scalar_type() == qkv.scalar_type(),
                     "grad_out must have shape [B, N, H * head_dim] and the dtype of qkv");
   const c10::cuda::CUDAGuard guard(qkv.device());
-  const at::Tensor x = qkv.contiguous(), g = grad_out.contiguous(), t = attention_table(table, x);
+  const at::Tensor x = qkv.contiguous(), t = attention_table(table, x);
+  const auto off_16_bytes = [](const at::Tensor& v) {
+    return reinterpret_cast<uintptr_t>(v.const_data_ptr()) % 16 != 0;
+  };
+  // the forward chose its kernel by qkv; a gradient off 16-byte boundaries does not change that
+  at::Tensor g = grad_out.contiguous();
+  if (off_16_bytes(g) && !off_16_bytes(x)) g = g.clone();
   const int code = dtype_code(x);
   const int64_t shares = crumpet_window_attention_backward_shares(B, H, N, Dh, code);
   at::Tensor grad_qkv = at::empty(x.sizes(), x.options());

@@ -73,3 +73,14 @@ def test_attention_mask_is_100_at_32_channels(dtype):
     got, want = attention_both(c)[0], attention_wide(c)[0]
     off = {BF16: 2.0 ** -7, F16: 2.0 ** -11}[dtype]
     assert rel(got, want) <= TOL[dtype] + off
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_attention_gradient_off_16_bytes(dtype):
+    """A gradient off 16-byte boundaries gives what an aligned one does: the kernels are those of
+    the forward's qkv."""
+    c = attention_case((3, 4, 5), (2, 1, 1), (1, 0, 0), 1, 2, 16, dtype, F32)
+    off = torch.empty(c["grad"].numel() + 1, dtype=dtype, device="cuda")[1:].view(c["grad"].shape)
+    off.copy_(c["grad"])
+    assert off.data_ptr() % 16
+    assert all(torch.equal(a, b) for a, b in zip(attention_both(c, grad=off), attention_both(c)))
