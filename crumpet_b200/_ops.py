@@ -142,6 +142,9 @@ def capi() -> ctypes.CDLL:
         lib.crumpet_relative_position_bias_backward.argtypes = [
             vp, i32, i64, vp, i32, vp, i64, vp, i64, vp, i64, vp, vp]
         lib.crumpet_relative_position_bias_backward.restype = i32
+        lib.crumpet_relative_position_bias_backward_rows.argtypes = [
+            vp, i32, i64, i64, vp, i32, vp, i64, vp, i64, vp, i64, vp, vp]
+        lib.crumpet_relative_position_bias_backward_rows.restype = i32
         lib.crumpet_window_attention_backward_shares.argtypes = [i64] * 4 + [i32]
         lib.crumpet_window_attention_backward_shares.restype = i64
         lib.crumpet_swin_window_attention_qkv_backward.argtypes = (

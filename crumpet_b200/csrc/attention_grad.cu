@@ -46,7 +46,7 @@
 
 namespace crumpet {
 
-static __device__ int g_grad_error;  // 1: a bounded wait of these kernels expired
+static __device__ int g_grad_error;  // 1: a bounded wait expired, 2: a bucket out of range
 
 namespace {
 
@@ -63,8 +63,8 @@ struct GradParams {
   float* stats;          // [B, H, NS / 2][4]: of two rows, -log2 of the sums of exponentials, -deltas
   float* amax;           // [B, H, groups of 16 rows]: their largest |do| (fp16 only)
   const void* table;     // [T, H]: fp32 (table_f32) or the element type
-  const int* pairs;      // [N, N]: bucket of every (query, key) pair, in [0, T)
-  int table_f32;
+  const int* pairs;      // [N, N]: bucket of every (query, key) pair
+  int table_f32, table_rows;  // a bucket outside [0, table_rows) is flagged and adds no bias
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
   int analytic;
   uint32_t mask_pen, mask_one;  // the mask features' values (MaskPenalty)
@@ -334,22 +334,26 @@ __device__ __forceinline__ void start_values(const GradParams& p, int h, int row
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = row0 + (e < 2 ? 0 : 8), c = col0 + 8 * t + (e & 1);
-      at[t][e] = r < p.N && c < p.N ? __ldg(p.pairs + (COLS ? c * p.N + r : r * p.N + c)) : -1;
+      at[t][e] = r < p.N && c < p.N ? __ldg(p.pairs + (COLS ? c * p.N + r : r * p.N + c)) : 0;
     }
+  bool bad = false;
   const float inv = 1.f / p.scale;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int c = col0 + 8 * t + (e & 1);
+      const int r = row0 + (e < 2 ? 0 : 8), c = col0 + 8 * t + (e & 1);
       float x = c < p.N ? 0.f : -INFINITY;
-      if (at[t][e] >= 0) {
+      const bool inside = unsigned(at[t][e]) < unsigned(p.table_rows);
+      bad = bad || !inside;
+      if (inside && r < p.N && c < p.N) {
         const long long i = (long long)at[t][e] * p.H + h;
         x = inv * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + i)
                                : elem_f32<BF16>(__ldg(static_cast<const uint16_t*>(p.table) + i)));
       }
       v[t][e] = x;
     }
+  if (bad) atomicOr(&g_grad_error, 2);
 }
 
 // Shifted-window mask as one more product of depth 8 in the windows that need it, over the eight
@@ -1229,6 +1233,20 @@ int read_attention_grad_error(bool clear) {
   return v;
 }
 
+int training_error_word(int** word) {
+  static std::mutex mu;
+  static void* at[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  void* p = e == cudaSuccess && dev < 64 ? at[dev] : nullptr;
+  if (e == cudaSuccess && p == nullptr) e = cudaGetSymbolAddress(&p, g_grad_error);
+  if (e != cudaSuccess) return set_cuda_error(e, "error word of the training kernels");
+  if (dev < 64) at[dev] = p;
+  *word = static_cast<int*>(p);
+  return kOk;
+}
+
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   GradParams p{};
   p.dqkv = static_cast<uint16_t*>(a.grad_qkv);
@@ -1239,6 +1257,7 @@ int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream) {
   p.table = a.table;
   p.pairs = a.pairs;
   p.table_f32 = a.table_f32 ? 1 : 0;
+  p.table_rows = int(a.table_rows);
   p.analytic = (a.shift[0] | a.shift[1] | a.shift[2]) != 0;
   if (p.analytic) {
     const MaskPenalty m = mask_penalty(a.scale, a.dtype == kBF16);

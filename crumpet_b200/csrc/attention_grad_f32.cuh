@@ -24,7 +24,8 @@ struct Params {
   float2* stats;      // [B, H, N]
   const void* table;  // [T, H]
   const int* pairs;   // [N, N]
-  int table_f32, analytic;
+  int table_f32, table_rows, analytic;
+  int* error;         // training_error_word
   int nwd, nwh, nww, wsd, wsh, wsw, ssd, ssh, ssw;
   int B, H, N, QB, S, bias_pitch;
   int vec;            // every tensor on 16-byte boundaries: four channels per load
@@ -85,11 +86,22 @@ __device__ __forceinline__ float4 load4(const Params& p, const T* at) {
   return make_float4(load(at, 0), load(at, 1), load(at, 2), load(at, 3));
 }
 
-// bias of one bucket times log2 e
+// A bucket read from `pairs`, and the largest one read
+__device__ __forceinline__ unsigned bucket_of(const Params& p, long long pair, unsigned& most) {
+  const unsigned t = unsigned(__ldg(p.pairs + pair));
+  most = max(most, t);
+  return t;
+}
+__device__ __forceinline__ void check_buckets(const Params& p, unsigned most) {
+  if (most >= unsigned(p.table_rows)) atomicOr(p.error, 2);
+}
+// bias of one bucket times log2 e; 0 (a clamped load's place) outside the table
 template <typename T>
-__device__ __forceinline__ float bias_of(const Params& p, int h, long long t) {
-  return kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + t * p.H + h)
-                               : load(static_cast<const T*>(p.table), t * p.H + h));
+__device__ __forceinline__ float bias_of(const Params& p, int h, unsigned t) {
+  const long long at = (long long)min(t, unsigned(p.table_rows) - 1) * p.H + h;
+  const float v = kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + at)
+                                        : load(static_cast<const T*>(p.table), at));
+  return t < unsigned(p.table_rows) ? v : 0.f;
 }
 
 }  // namespace grad_f32

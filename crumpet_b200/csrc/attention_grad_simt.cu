@@ -165,16 +165,17 @@ __global__ void __launch_bounds__(kThreads, D == 16 && MODE != kCols ? 6 : D == 
     // eight pairs at a time: their indices, then their table entries, so that both loads of eight
     // are in flight (with clamped indices; what lies past the end is replaced afterwards)
     constexpr int WARPS = kThreads / 32, BATCH = 8;
+    unsigned most = 0;
     const int across = COLS ? S::R : cols, along = COLS ? cols : S::R;
     for (int x = lane; x < across; x += 32) {
       for (int y0 = warp; y0 < along; y0 += WARPS * BATCH) {
-        int bucket[BATCH];
+        unsigned bucket[BATCH];
         float v[BATCH];
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
           const int y = y0 + u * WARPS;
           const int gi = min(r0 + (COLS ? x : y), p.N - 1), gj = min(j0 + (COLS ? y : x), p.N - 1);
-          bucket[u] = __ldg(p.pairs + (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj));
+          bucket[u] = bucket_of(p, (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj), most);
         }
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) v[u] = bias_of<T>(p, h, bucket[u]);
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, D == 16 && MODE != kCols ? 6 : D == 
         }
       }
     }
+    check_buckets(p, most);
   };
   if (whole) gather(0, (p.N + kTile - 1) / kTile * kTile);
   auto fetch = [&](int j0) {
@@ -312,14 +314,16 @@ __global__ void __launch_bounds__(kThreads, CH == 16 ? 6 : 1) grad_bias_simt_ker
   const float c1 = p.scale * kLog2e;
   float base[8], sum[8];
   uint32_t apart[8];
+  unsigned most = 0;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int i = it * kTile + ib + u;
     const bool in = i < p.N && j < p.N;
-    base[u] = in ? bias_of<T>(p, h, p.pairs[(long long)i * p.N + j]) : 0.f;
+    base[u] = in ? bias_of<T>(p, h, bucket_of(p, (long long)i * p.N + j, most)) : 0.f;
     apart[u] = in && p.analytic ? side_code(p, i) ^ side_code(p, j) : 0u;
     sum[u] = 0.f;
   }
+  check_buckets(p, most);
   for (int b = share; b < p.B; b += p.S) {
     const T* q = static_cast<const T*>(p.qkv) + (long long)b * p.N * tok + h * D;
     const T* g = static_cast<const T*>(p.dout) + (long long)b * p.N * hd + h * D;
@@ -439,6 +443,8 @@ int launch_any(const AttnGradArgs& a, void* out, bool forward, cudaStream_t stre
   p.table = a.table;
   p.pairs = a.pairs;
   p.table_f32 = a.table_f32 ? 1 : 0;
+  p.table_rows = int(a.table_rows);
+  if (int e = training_error_word(&p.error)) return e;
   p.analytic = (a.shift[0] | a.shift[1] | a.shift[2]) != 0;
   p.nwd = int(a.nwin[0]);
   p.nwh = int(a.nwin[1]);

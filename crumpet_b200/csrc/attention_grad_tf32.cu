@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
     // eight pairs at a time, so that their loads are in flight together (forward: the indices',
     // then the table's; the gradient finds the bias laid out where its own gradient will go)
     constexpr int BATCH = 8;
+    unsigned most = 0;
     const int warps = threads / 32, across = COLS ? rows : held, along = COLS ? held : rows;
     for (int x = lane; x < across; x += 32) {
       for (int y0 = warp; y0 < along; y0 += warps * BATCH) {
@@ -192,9 +193,9 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
           at[u] = (long long)(COLS ? gj : gi) * p.N + (COLS ? gi : gj);
         }
         if constexpr (MODE == kForward) {
-          int bucket[BATCH];
+          unsigned bucket[BATCH];
 #pragma unroll
-          for (int u = 0; u < BATCH; ++u) bucket[u] = __ldg(p.pairs + at[u]);
+          for (int u = 0; u < BATCH; ++u) bucket[u] = bucket_of(p, at[u], most);
 #pragma unroll
           for (int u = 0; u < BATCH; ++u) w[u] = bias_of<float>(p, h, bucket[u]);
         } else {
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
         }
       }
     }
+    if constexpr (MODE == kForward) check_buckets(p, most);
   };
   if (whole) gather(0);
   // roll-side codes: of this lane's rows, and of all tokens
@@ -483,14 +485,15 @@ __global__ void __launch_bounds__(32 * kWarps) grad_bias_tf32_kernel(const Param
   float base[kTiles][4], sum[kTiles][4] = {};
   uint32_t apart[kTiles];  // of each of four pairs, the axes on whose other side they lie: 4 x 8 bits
   {
-    int bucket[kTiles][4];
+    unsigned bucket[kTiles][4], most = 0;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        bucket[n][e] = __ldg(p.pairs + (long long)min(i0 + e / 2 * 8, p.N - 1) * p.N +
-                             min(jt + 8 * n + 2 * t + e % 2, p.N - 1));
+        bucket[n][e] = bucket_of(p, (long long)min(i0 + e / 2 * 8, p.N - 1) * p.N +
+                                        min(jt + 8 * n + 2 * t + e % 2, p.N - 1), most);
     }
+    check_buckets(p, most);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       apart[n] = 0;
@@ -609,7 +612,7 @@ template <int D>
 int launch(const Params& p, bool forward, cudaStream_t stream) {
   if (forward) return start<D, kForward>(p, stream);
   // the bias as [H, N, N], in the place of its gradient: two kernels read it, once per CTA or more
-  if (int e = launch_relative_position_bias(p.dbias, kF32, p.table, kF32, p.pairs,
+  if (int e = launch_relative_position_bias(p.dbias, kF32, p.table, kF32, p.table_rows, p.pairs,
                                             (long long)p.N * p.N, p.H, stream))
     return e;
   if (int e = start<D, kRows>(p, stream)) return e;

@@ -59,7 +59,8 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 // V heads (16 bytes of the table, or one) of PP neighbouring pairs per thread
 template <typename T, typename O, int V, int PP>
 __global__ void __launch_bounds__(kThreads)
-bias_gather_kernel(O* bias, const T* table, const int* pairs, long long npairs, int H) {
+bias_gather_kernel(O* bias, const T* table, unsigned rows, const int* pairs, long long npairs,
+                   int H, int* error) {
   struct alignas(V * sizeof(T)) Heads {
     T v[V];
   };
@@ -74,9 +75,19 @@ bias_gather_kernel(O* bias, const T* table, const int* pairs, long long npairs, 
   const int h = blockIdx.y * V;
   const Pairs at = *reinterpret_cast<const Pairs*>(pairs + i);
   Heads w[PP];
+  unsigned most = 0;
 #pragma unroll
-  for (int u = 0; u < PP; ++u)
-    w[u] = *reinterpret_cast<const Heads*>(table + (long long)at.v[u] * H + h);
+  for (int u = 0; u < PP; ++u) {
+    most = max(most, unsigned(at.v[u]));
+    w[u] = *reinterpret_cast<const Heads*>(
+        table + (long long)min(unsigned(at.v[u]), rows - 1) * H + h);
+  }
+  if (most >= rows) {  // a bucket outside the table: no bias
+    atomicOr(error, 2);
+#pragma unroll
+    for (int u = 0; u < PP; ++u)
+      if (unsigned(at.v[u]) >= rows) w[u] = Heads{};
+  }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     Out o;
@@ -90,8 +101,9 @@ struct GradBuckets {
   const int* order;      // [npairs] pairs sorted by bucket
   const int* items;      // [n_items][3]: bucket, begin, end (into order)
   const int* multi;      // [n_multi][3]: bucket, first item, last item + 1
-  long long n_items, n_multi, npairs;
+  long long n_items, n_multi, npairs, rows;  // rows of the table
   int H;
+  int* error;  // what points outside its tensor is flagged here and left out
 };
 
 // One warp per item and kUnit heads.  An item whose bucket is whole writes the table's gradient,
@@ -104,27 +116,38 @@ bias_grad_kernel(O* grad_table, float* partial, const G* grad, GradBuckets b) {
   if (item >= b.n_items) return;
   const int h = blockIdx.y * kUnit;
   const int bucket = b.items[3 * item], begin = b.items[3 * item + 1], end = b.items[3 * item + 2];
+  if (bucket >= b.rows || (bucket < 0 && partial == nullptr) || begin < 0 || end > b.npairs) {
+    atomicOr(b.error, 2);
+    return;  // the whole warp
+  }
   const int units = min(kUnit, b.H - h);
   const G* src = grad + h * b.npairs;
+  const unsigned npairs = unsigned(b.npairs);
+  unsigned most = 0;
   float sum[kUnit] = {};
   // n rounds of 32 pairs, all their places read at once
   auto rounds = [&](auto n_tag, int e0) {
     constexpr int n = decltype(n_tag)::value;
-    int at[n];
+    unsigned at[n];
 #pragma unroll
-    for (int r = 0; r < n; ++r) at[r] = e0 + 32 * r < end ? __ldg(b.order + e0 + 32 * r) : -1;
+    for (int r = 0; r < n; ++r) {
+      const bool in = e0 + 32 * r < end;
+      at[r] = in ? unsigned(__ldg(b.order + e0 + 32 * r)) : ~0u;
+      most = max(most, in ? at[r] : 0u);
+    }
 #pragma unroll
     for (int u = 0; u < kUnit; ++u) {
       if (u >= units) break;
 #pragma unroll
       for (int r = 0; r < n; ++r)
-        if (at[r] >= 0) sum[u] += to_float(__ldg(src + u * b.npairs + at[r]));
+        if (at[r] < npairs) sum[u] += to_float(__ldg(src + u * b.npairs + at[r]));
     }
   };
   int e = begin;
   for (; end - e > 64; e += 128) rounds(std::integral_constant<int, 4>{}, e + lane);
   if (end - e > 32) rounds(std::integral_constant<int, 2>{}, e + lane);
   else if (end - e > 0) rounds(std::integral_constant<int, 1>{}, e + lane);
+  if (most >= npairs && end > begin) atomicOr(b.error, 2);
 #pragma unroll
   for (int u = 0; u < kUnit; ++u) {
 #pragma unroll
@@ -145,6 +168,10 @@ bias_grad_join_kernel(O* grad_table, const float* partial, GradBuckets b) {
   const long long k = blockIdx.x;
   const int h = blockIdx.y * 32 + lane;
   const int bucket = b.multi[3 * k], first = b.multi[3 * k + 1], last = b.multi[3 * k + 2];
+  if (bucket < 0 || bucket >= b.rows || first < 0 || last > b.n_items) {
+    if (threadIdx.x == 0) atomicOr(b.error, 2);
+    return;  // the whole CTA
+  }
   float sum = 0.f;
   if (h < b.H) {
 #pragma unroll 8
@@ -160,43 +187,49 @@ bias_grad_join_kernel(O* grad_table, const float* partial, GradBuckets b) {
 }
 
 template <typename T, typename O, int V, int PP>
-void gather(void* bias, const void* table, const int* pairs, int64_t npairs, int64_t H,
-            cudaStream_t stream) {
+void gather(void* bias, const void* table, int64_t rows, const int* pairs, int64_t npairs, int64_t H,
+            int* error, cudaStream_t stream) {
   const int64_t per = int64_t(kThreads) * PP;
   bias_gather_kernel<T, O, V, PP><<<dim3(unsigned((npairs + per - 1) / per), unsigned(H / V)),
                                     kThreads, 0, stream>>>(
-      static_cast<O*>(bias), static_cast<const T*>(table), pairs, npairs, int(H));
+      static_cast<O*>(bias), static_cast<const T*>(table), unsigned(rows), pairs, npairs, int(H),
+      error);
 }
 
 template <typename T, typename O>
-int launch_gather(void* bias, const void* table, const int* pairs, int64_t npairs, int64_t H,
-                  cudaStream_t stream) {
+int launch_gather(void* bias, const void* table, int64_t rows, const int* pairs, int64_t npairs,
+                  int64_t H, cudaStream_t stream) {
+  int* error = nullptr;
+  if (int e = training_error_word(&error)) return e;
   constexpr int V = 16 / sizeof(T), PP = 4 / sizeof(O);
   const auto aligned = [](const void* p, uintptr_t n) {
     return reinterpret_cast<uintptr_t>(p) % n == 0;
   };
   const bool heads = H % V == 0 && aligned(table, 16);
   const bool two = npairs % PP == 0 && aligned(bias, 4) && aligned(pairs, 4 * PP);
-  if (heads && two) gather<T, O, V, PP>(bias, table, pairs, npairs, H, stream);
-  else if (heads) gather<T, O, V, 1>(bias, table, pairs, npairs, H, stream);
-  else if (two) gather<T, O, 1, PP>(bias, table, pairs, npairs, H, stream);
-  else gather<T, O, 1, 1>(bias, table, pairs, npairs, H, stream);
+  if (heads && two) gather<T, O, V, PP>(bias, table, rows, pairs, npairs, H, error, stream);
+  else if (heads) gather<T, O, V, 1>(bias, table, rows, pairs, npairs, H, error, stream);
+  else if (two) gather<T, O, 1, PP>(bias, table, rows, pairs, npairs, H, error, stream);
+  else gather<T, O, 1, 1>(bias, table, rows, pairs, npairs, H, error, stream);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "relative position bias launch");
 }
 
 template <typename T>
-int gather_out(void* bias, int out_dtype, const void* table, const int* pairs, int64_t npairs,
-               int64_t H, cudaStream_t stream) {
-  if (out_dtype == kF32) return launch_gather<T, float>(bias, table, pairs, npairs, H, stream);
+int gather_out(void* bias, int out_dtype, const void* table, int64_t rows, const int* pairs,
+               int64_t npairs, int64_t H, cudaStream_t stream) {
+  if (out_dtype == kF32)
+    return launch_gather<T, float>(bias, table, rows, pairs, npairs, H, stream);
   if (out_dtype == kF16)
-    return launch_gather<T, __half>(bias, table, pairs, npairs, H, stream);
-  return launch_gather<T, __nv_bfloat16>(bias, table, pairs, npairs, H, stream);
+    return launch_gather<T, __half>(bias, table, rows, pairs, npairs, H, stream);
+  return launch_gather<T, __nv_bfloat16>(bias, table, rows, pairs, npairs, H, stream);
 }
 
 template <typename G, typename O>
 int launch_grad(const BiasGradArgs& a, cudaStream_t stream) {
-  GradBuckets b{a.order, a.items, a.multi, a.n_items, a.n_multi, a.npairs, int(a.H)};
+  GradBuckets b{a.order, a.items, a.multi, a.n_items, a.n_multi, a.npairs, a.table_rows, int(a.H),
+                nullptr};
+  if (int e = training_error_word(&b.error)) return e;
   constexpr int items = kGradThreads / 32;
   bias_grad_kernel<G, O><<<dim3(unsigned((a.n_items + items - 1) / items),
                                 unsigned((a.H + kUnit - 1) / kUnit)),
@@ -223,12 +256,13 @@ int grad_out(const BiasGradArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
-                                  const int* pairs, int64_t npairs, int64_t H, cudaStream_t stream) {
+                                  int64_t table_rows, const int* pairs, int64_t npairs, int64_t H,
+                                  cudaStream_t stream) {
   if (table_dtype == kF32)
-    return gather_out<float>(bias, out_dtype, table, pairs, npairs, H, stream);
+    return gather_out<float>(bias, out_dtype, table, table_rows, pairs, npairs, H, stream);
   if (table_dtype == kF16)
-    return gather_out<__half>(bias, out_dtype, table, pairs, npairs, H, stream);
-  return gather_out<__nv_bfloat16>(bias, out_dtype, table, pairs, npairs, H, stream);
+    return gather_out<__half>(bias, out_dtype, table, table_rows, pairs, npairs, H, stream);
+  return gather_out<__nv_bfloat16>(bias, out_dtype, table, table_rows, pairs, npairs, H, stream);
 }
 
 int launch_relative_position_bias_grad(const BiasGradArgs& a, cudaStream_t stream) {

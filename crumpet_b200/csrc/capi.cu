@@ -469,21 +469,33 @@ int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
   if (table_rows < 1 || table_rows > 0x7fffffff || npairs > 0x7fffffff || H > 0xffff)
     return set_error(kErrInvalid, "relative position bias: table_rows, npairs or H out of range");
   if (!bias || !table || !pairs) return set_error(kErrInvalid, "null tensor pointer");
-  return launch_relative_position_bias(bias, out_dtype, table, table_dtype, pairs, npairs,
-                                       H, static_cast<cudaStream_t>(stream));
+  return launch_relative_position_bias(bias, out_dtype, table, table_dtype, table_rows, pairs,
+                                       npairs, H, static_cast<cudaStream_t>(stream));
 }
 
 int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, int64_t H,
-                                            const void* grad, int grad_dtype, const int* order, int64_t npairs, const int* items,
-                                            int64_t n_items, const int* multi, int64_t n_multi,
-                                            float* partial, void* stream) {
+                                            const void* grad, int grad_dtype, const int* order,
+                                            int64_t npairs, const int* items, int64_t n_items,
+                                            const int* multi, int64_t n_multi, float* partial,
+                                            void* stream) {
+  return crumpet_relative_position_bias_backward_rows(grad_table, table_dtype, 0x7fffffff, H, grad,
+                                                      grad_dtype, order, npairs, items, n_items,
+                                                      multi, n_multi, partial, stream);
+}
+
+int crumpet_relative_position_bias_backward_rows(void* grad_table, int table_dtype,
+                                                 int64_t table_rows, int64_t H, const void* grad,
+                                                 int grad_dtype, const int* order, int64_t npairs,
+                                                 const int* items, int64_t n_items,
+                                                 const int* multi, int64_t n_multi, float* partial,
+                                                 void* stream) {
   if (int e = check_dtype(table_dtype)) return e;
   if (int e = check_dtype(grad_dtype)) return e;
   if (H < 0 || npairs < 0 || n_items < 0 || n_multi < 0)
     return set_error(kErrInvalid, "H, npairs, n_items and n_multi must be non-negative");
   if (H == 0 || n_items == 0) return kOk;
-  if (npairs > 0x7fffffff || H > 0xffff || n_items > 0x7fffffff ||
-      n_multi > 0x7fffffff)
+  if (table_rows < 0 || table_rows > 0x7fffffff || npairs > 0x7fffffff || H > 0xffff ||
+      n_items > 0x7fffffff || n_multi > 0x7fffffff)
     return set_error(kErrInvalid, "relative position bias: npairs, H or items out of range");
   if (!grad_table || !items || (npairs > 0 && (!grad || !order)) ||
       (n_multi > 0 && (!multi || !partial)))
@@ -491,6 +503,7 @@ int crumpet_relative_position_bias_backward(void* grad_table, int table_dtype, i
   BiasGradArgs a{};
   a.grad_table = grad_table;
   a.table_dtype = table_dtype;
+  a.table_rows = table_rows;
   a.grad = grad;
   a.grad_dtype = grad_dtype;
   a.npairs = npairs;
@@ -530,6 +543,7 @@ int check_train_attention(int dtype, int64_t B, int64_t H, int64_t N, int64_t he
   if (B > 0x7fffffff || H > 0xffff || N > 46340)
     return set_error(kErrInvalid, "B, H or N too large");
   if (table_rows < 1) return set_error(kErrInvalid, "relative position bias table has no rows");
+  if (table_rows > 0x7fffffff) return set_error(kErrInvalid, "relative position bias table too large");
   if ((ss[0] | ss[1] | ss[2]) == 0) return kOk;
   int64_t windows = 1;
   for (int a = 0; a < 3; ++a) {
@@ -546,13 +560,14 @@ int check_train_attention(int dtype, int64_t B, int64_t H, int64_t N, int64_t he
   return kOk;
 }
 
-AttnGradArgs train_args(const void* qkv, const void* bias_table, int table_f32, const int* pairs,
-                        const int64_t* nw, const int64_t* ws, const int64_t* ss, int dtype,
+AttnGradArgs train_args(const void* qkv, const void* bias_table, int table_f32, int64_t table_rows,
+                        const int* pairs, const int64_t* nw, const int64_t* ws, const int64_t* ss, int dtype,
                         int64_t B, int64_t H, int64_t N, int64_t head_dim, float scale) {
   AttnGradArgs a{};
   a.qkv = qkv;
   a.table = bias_table;
   a.table_f32 = table_f32 != 0 || dtype == kF32;
+  a.table_rows = table_rows;
   a.pairs = pairs;
   for (int x = 0; x < 3; ++x) {
     a.nwin[x] = nw[x];
@@ -585,8 +600,8 @@ int crumpet_swin_window_attention_qkv_pairs(void* out, const void* qkv, const vo
     return e;
   if (B == 0) return kOk;
   if (!out || !qkv || !bias_table || !pairs) return set_error(kErrInvalid, "null tensor pointer");
-  const AttnGradArgs a = train_args(qkv, bias_table, table_f32, pairs, nw, ws, ss, dtype, B, H, N,
-                                    head_dim, scale);
+  const AttnGradArgs a = train_args(qkv, bias_table, table_f32, table_rows, pairs, nw, ws, ss, dtype,
+                                    B, H, N, head_dim, scale);
   return launch_attention_train_simt(a, out, static_cast<cudaStream_t>(stream));
 }
 
@@ -613,8 +628,8 @@ int crumpet_swin_window_attention_qkv_backward(
     return set_error(kErrInvalid, "null tensor pointer");
   if (reinterpret_cast<uintptr_t>(stats) & 15u)
     return set_error(kErrInvalid, "stats must be 16-byte aligned");
-  AttnGradArgs a = train_args(qkv, bias_table, table_f32, pairs, nw, ws, ss, dtype, B, H, N,
-                              head_dim, scale);
+  AttnGradArgs a = train_args(qkv, bias_table, table_f32, table_rows, pairs, nw, ws, ss, dtype, B, H,
+                              N, head_dim, scale);
   a.grad_qkv = grad_qkv;
   a.grad_bias = grad_bias;
   a.stats = stats;

@@ -157,7 +157,8 @@ struct AttnGradArgs {
   const void* qkv;       // [B, N, 3, H, head_dim]
   const void* table;     // [T, H]
   bool table_f32;
-  const int* pairs;      // [N, N] buckets in [0, T)
+  int64_t table_rows;    // T
+  const int* pairs;      // [N, N] buckets; outside [0, T): flagged, bias 0
   int64_t nwin[3], win[3], shift[3];
   int64_t B, H, N, head_dim, shares;
   float scale;
@@ -168,18 +169,23 @@ int64_t attention_grad_shares(int64_t B, int64_t H, int64_t N);
 int64_t attention_grad_shares_simt(int64_t B, int64_t H, int64_t N, int64_t head_dim, int dtype);
 int launch_attention_grad(const AttnGradArgs& a, cudaStream_t stream);
 int launch_attention_train_simt(const AttnGradArgs& a, void* out, cudaStream_t stream);
+// The training kernels' error word of the current device (1: a bounded wait expired, 2: a bucket or
+// a place in the sorted pairs out of range), and its address there.
 int read_attention_grad_error(bool clear);
+int training_error_word(int** word);
 // parts[0] = sum of parts[0 .. shares - 1], each of n floats
 int launch_sum_shares(float* parts, int64_t shares, int64_t n, cudaStream_t stream);
 int launch_attention_grad_simt(const AttnGradArgs& a, cudaStream_t stream);
 
 // Relative-position bias by buckets: bias[h, p] = table[pairs[p], h] and the table's gradient
-// from grad [H, npairs].
+// from grad [H, npairs].  What points outside its tensor is flagged in the error word and left out.
 int launch_relative_position_bias(void* bias, int out_dtype, const void* table, int table_dtype,
-                                  const int* pairs, int64_t npairs, int64_t H, cudaStream_t stream);
+                                  int64_t table_rows, const int* pairs, int64_t npairs, int64_t H,
+                                  cudaStream_t stream);
 struct BiasGradArgs {
   void* grad_table;  // [T, H]
   int table_dtype;
+  int64_t table_rows;  // T, where the caller says
   const void* grad;  // [H, npairs]
   int grad_dtype;
   int64_t npairs, H;

@@ -645,11 +645,13 @@ at::Tensor table_gradient(const void* grad, const at::Tensor& ref, int grad_code
   check_int32(ref, order, "order");
   check_int32(ref, items, "items");
   check_int32(ref, multi, "multi");
+  TORCH_CHECK_VALUE(items.dim() == 2 && items.size(1) == 3 && multi.dim() == 2 && multi.size(1) == 3,
+                    "items and multi must hold triples");
   at::Tensor table = at::empty({buckets, H}, ref.options().dtype(dtype));
   at::Tensor partial;
   if (multi.size(0) > 0) partial = f32_like(ref, {items.size(0) * H});
-  check_rc(crumpet_relative_position_bias_backward(
-      table.data_ptr(), dtype_code(table), H, grad, grad_code, order.const_data_ptr<int>(),
+  check_rc(crumpet_relative_position_bias_backward_rows(
+      table.data_ptr(), dtype_code(table), buckets, H, grad, grad_code, order.const_data_ptr<int>(),
       order.numel(), items.const_data_ptr<int>(), items.size(0), multi.const_data_ptr<int>(),
       multi.size(0), partial.defined() ? partial.data_ptr<float>() : nullptr, cur_stream(ref)));
   return table;
@@ -765,6 +767,7 @@ std::tuple<at::Tensor, at::Tensor> swin_window_attention_backward(
     at::IntArrayRef shift_size, double scale) {
   const Place p = check_attention(qkv, table, pairs, num_windows, window_size, shift_size, scale);
   check_int32(qkv, pairs, "pairs");
+  TORCH_CHECK_VALUE(order.numel() == pairs.numel(), "order must hold the pairs of the index");
   check_cuda(qkv, grad_out, "grad_out");
   const int64_t B = qkv.size(0), N = qkv.size(1), H = qkv.size(3), Dh = qkv.size(4);
   TORCH_CHECK_VALUE(grad_out.dim() == 3 && grad_out.size(0) == B && grad_out.size(1) == N &&

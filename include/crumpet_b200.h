@@ -397,13 +397,14 @@ CRUMPET_API int crumpet_roi_argmax(uint8_t* labels, float* logits, const float* 
  * Learned relative-position bias by buckets:
  *   bias[h, p] = table[pairs[p], h]             for H heads and npairs (query, key) pairs
  *   grad_table[t, h] = sum over pairs p of bucket t of grad[h, p]
- * table [table_rows, H] and bias [H, npairs] in their dtypes; pairs int32, every value in
- * [0, table_rows) (the caller has checked them).  The gradient wants the pairs sorted by bucket
+ * table [table_rows, H] and bias [H, npairs] in their dtypes; pairs int32, values in
+ * [0, table_rows).  The gradient wants the pairs sorted by bucket
  * (`order`, int32 [npairs]) and cut into items: int32 triples (bucket, begin, end) into order,
  * in the order of the buckets, every bucket (an empty one too) with one item at least.  A
  * bucket of several items is written as -1 in them and listed in `multi`, int32 triples
  * (bucket, first item, last item + 1); then `partial` is fp32 scratch [n_items, H].  Sums are
- * fp32 in a fixed order.
+ * fp32 in a fixed order.  A pair, or an entry of order, items or multi, that points outside its
+ * tensor sets bit 2 of the device error word (crumpet_device_status) and is left out (no bias).
  */
 CRUMPET_API int crumpet_relative_position_bias(void* bias, int out_dtype, const void* table,
                                                int table_dtype, int64_t table_rows, int64_t H,
@@ -412,10 +413,15 @@ CRUMPET_API int crumpet_relative_position_bias_backward(
     void* grad_table, int table_dtype, int64_t H, const void* grad, int grad_dtype,
     const int* order, int64_t npairs, const int* items, int64_t n_items, const int* multi,
     int64_t n_multi, float* partial, void* stream);
+/* The same for a grad_table known to have table_rows rows. */
+CRUMPET_API int crumpet_relative_position_bias_backward_rows(
+    void* grad_table, int table_dtype, int64_t table_rows, int64_t H, const void* grad,
+    int grad_dtype, const int* order, int64_t npairs, const int* items, int64_t n_items,
+    const int* multi, int64_t n_multi, float* partial, void* stream);
 
 /*
  * crumpet_swin_window_attention_qkv in fp32 arithmetic for every input of its domain, with the
- * buckets as checked int32 pairs [N, N] (as the gradient below takes them): the training forward
+ * buckets as int32 pairs [N, N] (as the gradient below takes them): the training forward
  * of what the 16-bit tensor-core kernel does not take.  fp32 at head dims 16 and 32 multiplies in
  * split tf32 products (2^-22 on average).
  */
@@ -428,7 +434,7 @@ CRUMPET_API int crumpet_swin_window_attention_qkv_pairs(
 /*
  * Gradient of crumpet_swin_window_attention_qkv: from grad_out [B, N, H * head_dim] and the
  * forward's qkv, table and geometry (arguments as there; pairs int32 [N, N] holds the buckets
- * index[:N, :N], every value in [0, table_rows)), writes grad_qkv [B, N, 3, H, head_dim] and
+ * index[:N, :N]; one outside [0, table_rows) is flagged as above and adds no bias), writes grad_qkv [B, N, 3, H, head_dim] and
  * into the first [H, N, N] of grad_bias, fp32 [shares, H, N, N], the gradient of the bias (to
  * pass on to crumpet_relative_position_bias_backward); the rest of it is scratch.  `shares` is
  * what crumpet_window_attention_backward_shares gives for these sizes; `stats` is fp32

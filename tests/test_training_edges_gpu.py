@@ -84,3 +84,95 @@ def test_attention_gradient_off_16_bytes(dtype):
     off.copy_(c["grad"])
     assert off.data_ptr() % 16
     assert all(torch.equal(a, b) for a, b in zip(attention_both(c, grad=off), attention_both(c)))
+
+
+BAD_BUCKETS = [
+    (BF16, 16, (4, 4, 4)),  # tensor cores
+    (F16, 32, (5, 5, 3)),
+    (F32, 16, (3, 4, 5)),   # split tf32 products
+    (F32, 64, (3, 3, 3)),   # fp32 arithmetic, bias held whole
+    (BF16, 128, (8, 8, 9)),  # and tile by tile
+]
+
+
+@pytest.mark.parametrize("dtype,d,win", BAD_BUCKETS, ids=str)
+def test_attention_buckets_outside_the_table(dtype, d, win):
+    """Buckets outside the table add no bias, in both directions, and are reported."""
+    c = attention_case(win, (1, 1, 1), (0, 0, 0), 2, 2, d, dtype, F32)
+    rows = c["table"].shape[0]
+    c["table"][-1] = 0
+    good = crumpet.relative_position_buckets(c["index"], rows)
+    last = good.pairs == 3
+    zero = good.pairs.masked_fill(last, rows - 1)
+    bad = good.pairs.masked_fill(last, rows)
+    bad[last & (torch.arange(last.shape[0], device="cuda") % 2 == 0)] = -1
+
+    def run(pairs):
+        plan = good._replace(pairs=pairs, index=pairs.long())
+        return (crumpet.swin_window_attention_train(c["qkv"], c["table"], plan, **c["place"]),
+                *crumpet.swin_window_attention_backward(c["grad"], c["qkv"], c["table"], plan,
+                                                        **c["place"]))
+
+    crumpet.device_status(clear=True)
+    want = run(zero)
+    assert crumpet.device_status() == 0
+    got = run(bad)
+    assert crumpet.device_status(clear=True) == 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("heads", [3, 8])
+def test_bias_buckets_outside_the_table(heads, dtype):
+    index = torch.arange(64 * 33, device="cuda").view(64, 33) % 40
+    plan = crumpet.relative_position_buckets(index, 40)
+    table = torch.randn(40, heads, device="cuda").to(dtype)
+    want = crumpet.relative_position_bias(table, plan)
+    pairs = plan.pairs.clone()
+    pairs[5, 7], pairs[63, 32], pairs[0, 0] = 40, -3, 2 ** 31 - 1
+    crumpet.device_status(clear=True)
+    got = crumpet.relative_position_bias(table, plan._replace(pairs=pairs))
+    assert crumpet.device_status(clear=True) == 2
+    out = pairs != plan.pairs
+    assert torch.equal(got, want.masked_fill(out, 0))
+
+
+def test_bias_gradient_of_a_plan_that_is_not_one():
+    """Places, items and joined buckets outside their tensors are reported and left out."""
+    index = torch.arange(64 * 33, device="cuda").view(64, 33) % 40
+    plan = crumpet.relative_position_buckets(index, 40)
+    grad = torch.randn(3, 64, 33, device="cuda")
+    want = crumpet.relative_position_bias_backward(grad, plan)
+    long = crumpet.relative_position_buckets(torch.zeros_like(index), 2)
+    assert len(long.multi)
+
+    def run(plan, field, at, value):
+        t = getattr(plan, field).clone()
+        t[at] = value
+        crumpet.device_status(clear=True)
+        res = crumpet.relative_position_bias_backward(grad, plan._replace(**{field: t}))
+        assert crumpet.device_status(clear=True) == 2
+        return res
+
+    place = int(plan.order[0])
+    got = run(plan, "order", 0, 64 * 33)
+    assert torch.equal(got[1:], want[1:])
+    left = index.new_tensor(place)
+    less = grad.view(3, -1).clone()
+    less[:, left] = 0
+    assert torch.equal(got, crumpet.relative_position_bias_backward(less.view_as(grad), plan))
+    run(plan, "order", 7, -1)
+    for at, value in (((39, 0), 40), ((39, 0), -1), ((2, 1), -5), ((39, 2), 64 * 33 + 1)):
+        got = run(plan, "items", at, value)
+        rows = torch.arange(40, device="cuda") != at[0]
+        assert torch.equal(got[rows], want[rows])
+    for at, value in (((0, 0), 2), ((0, 0), -1), ((0, 1), -1), ((0, 2), len(long.items) + 1)):
+        run(long, "multi", at, value)
+    with pytest.raises(ValueError, match="triples"):
+        crumpet.relative_position_bias_backward(grad, plan._replace(items=plan.items.view(-1)))
+    qkv = torch.randn(1, 64, 3, 3, 16, device="cuda")
+    square = crumpet.relative_position_buckets(index[:, :1].expand(64, 64), 40)
+    with pytest.raises(ValueError, match="order"):
+        crumpet.swin_window_attention_backward(
+            torch.randn(1, 64, 48, device="cuda"), qkv, torch.randn(40, 3, device="cuda"),
+            square._replace(order=square.order[:-1]))
