@@ -125,13 +125,14 @@ bias_grad_kernel(O* grad_table, float* partial, const G* grad, GradBuckets b) {
   const unsigned npairs = unsigned(b.npairs);
   unsigned most = 0;
   float sum[kUnit] = {};
-  // n rounds of 32 pairs, all their places read at once
-  auto rounds = [&](auto n_tag, int e0) {
+  // n rounds of 32 pairs, all their places read at once (counted unsigned: they run past `end`,
+  // which may be the last int)
+  auto rounds = [&](auto n_tag, unsigned e0) {
     constexpr int n = decltype(n_tag)::value;
     unsigned at[n];
 #pragma unroll
     for (int r = 0; r < n; ++r) {
-      const bool in = e0 + 32 * r < end;
+      const bool in = e0 + 32 * r < unsigned(end);
       at[r] = in ? unsigned(__ldg(b.order + e0 + 32 * r)) : ~0u;
       most = max(most, in ? at[r] : 0u);
     }
@@ -143,10 +144,10 @@ bias_grad_kernel(O* grad_table, float* partial, const G* grad, GradBuckets b) {
         if (at[r] < npairs) sum[u] += to_float(__ldg(src + u * b.npairs + at[r]));
     }
   };
-  int e = begin;
-  for (; end - e > 64; e += 128) rounds(std::integral_constant<int, 4>{}, e + lane);
-  if (end - e > 32) rounds(std::integral_constant<int, 2>{}, e + lane);
-  else if (end - e > 0) rounds(std::integral_constant<int, 1>{}, e + lane);
+  unsigned e = begin;
+  for (; int(end - e) > 64; e += 128) rounds(std::integral_constant<int, 4>{}, e + lane);
+  if (int(end - e) > 32) rounds(std::integral_constant<int, 2>{}, e + lane);
+  else if (int(end - e) > 0) rounds(std::integral_constant<int, 1>{}, e + lane);
   if (most >= npairs && end > begin) atomicOr(b.error, 2);
 #pragma unroll
   for (int u = 0; u < kUnit; ++u) {
@@ -175,7 +176,7 @@ bias_grad_join_kernel(O* grad_table, const float* partial, GradBuckets b) {
   float sum = 0.f;
   if (h < b.H) {
 #pragma unroll 8
-    for (int i = first + warp; i < last; i += kJoinThreads / 32)
+    for (unsigned i = first + warp; i < unsigned(last); i += kJoinThreads / 32)
       sum += __ldg(partial + (long long)i * b.H + h);
   }
   part[warp][lane] = sum;

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import crumpet_b200 as crumpet
+from crumpet_b200 import training
 from test_training_gpu import BF16, F16, F32, TOL, attention64, attention_case, rel
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +177,20 @@ def test_bias_gradient_of_a_plan_that_is_not_one():
         crumpet.swin_window_attention_backward(
             torch.randn(1, 64, 48, device="cuda"), qkv, torch.randn(40, 3, device="cuda"),
             square._replace(order=square.order[:-1]))
+
+
+@pytest.mark.parametrize("length", [20, 50, 100, 300])
+def test_bias_gradient_at_the_last_of_2_31_pairs(length):
+    """Items at the end of as many pairs as an int counts (13 GB)."""
+    n = 2 ** 31 - 1
+    order = torch.zeros(n, dtype=torch.int32, device="cuda")
+    grad = torch.zeros(1, 1, n, dtype=F16, device="cuda")
+    grad[0, 0, 0] = 1
+    order[-1], grad[0, 0, -1] = n - 1, 3
+    plan = training.RelativePositionBuckets(
+        index=None, pairs=torch.zeros((1, 1), dtype=torch.int32, device="cuda").expand(1, n),
+        order=order, items=torch.tensor([[0, n - length, n]], dtype=torch.int32, device="cuda"),
+        multi=torch.zeros((0, 3), dtype=torch.int32, device="cuda"), num_buckets=1)
+    crumpet.device_status(clear=True)
+    got = crumpet.relative_position_bias_backward(grad, plan)
+    assert float(got) == length + 2 and crumpet.device_status(clear=True) == 0
