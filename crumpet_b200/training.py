@@ -484,30 +484,62 @@ def _off(module) -> bool:
         or getattr(module, "p", None) == 0.0
 
 
+def _plain(module, kind) -> bool:
+    """Exactly a ``kind`` with the class's own forward: not a subclass (adapters,
+    parametrizations), not an instance whose forward was replaced."""
+    return type(module) is kind and "forward" not in module.__dict__
+
+
+def _hooked(module) -> bool:
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks)
+
+
 def _fits(norm, C: int) -> bool:
-    return (isinstance(norm, torch.nn.LayerNorm) and tuple(norm.normalized_shape) == (C,)
-            and norm.weight is not None and norm.bias is not None)
+    return (_plain(norm, torch.nn.LayerNorm) and tuple(norm.normalized_shape) == (C,)
+            and norm.weight is not None and norm.bias is not None and norm.eps > 0)
+
+
+def _known(blk) -> bool:
+    """Whether the block, its attention and its MLP are the Swin classes of its own module."""
+    swin = sys.modules[type(blk).__module__]
+    mlp = getattr(swin, "Mlp", getattr(swin, "MLPBlock", None))
+    return (_plain(blk, getattr(swin, "SwinTransformerBlock", None))
+            and _plain(blk.attn, getattr(swin, "WindowAttention", None)) and _plain(blk.mlp, mlp))
 
 
 def _block_trains(blk, C: int) -> bool:
-    """Whether the training kernels compute exactly what the block does."""
+    """Whether the training kernels compute exactly what the block does.  They call the block's
+    qkv and proj as modules and read the parameters of all others, so those have to be the plain
+    classes, and nothing may be hooked to them."""
+    if not _known(blk):
+        return False
     attn, mlp = blk.attn, blk.mlp
-    act = getattr(mlp, "fn", None)
     path = getattr(blk, "drop_path", None)
+    softmax = getattr(attn, "softmax", None)
     heads = int(attn.num_heads)
+    called = {id(m) for top in (attn.qkv, attn.proj) for m in top.modules()}
     return (C <= MAX_CHANNELS and _fits(blk.norm1, C) and _fits(blk.norm2, C)
             and C % heads == 0 and head_dim_supported(C // heads)
+            and (softmax is None or _plain(softmax, torch.nn.Softmax) and softmax.dim == -1)
             and _off(attn.attn_drop) and _off(attn.proj_drop)
-            and isinstance(act, torch.nn.GELU) and act.approximate == "none"
+            and _plain(mlp.linear1, torch.nn.Linear) and _plain(mlp.linear2, torch.nn.Linear)
+            and _plain(mlp.fn, torch.nn.GELU) and mlp.fn.approximate == "none"
             and _off(getattr(mlp, "drop1", None)) and _off(getattr(mlp, "drop2", None))
-            and (_off(path) or (hasattr(path, "drop_prob") and getattr(path, "scale_by_keep", True)))
-            and not getattr(blk, "use_checkpoint", False))
+            and (_off(path) or (type(path).__name__ == "DropPath" and hasattr(path, "drop_prob")
+                                and "forward" not in path.__dict__
+                                and getattr(path, "scale_by_keep", True)))
+            and not getattr(blk, "use_checkpoint", False)
+            and not torch.nn.modules.module._has_any_global_hook()
+            and not any(_hooked(m) for m in blk.modules() if id(m) not in called))
 
 
 def _path_scale(blk, samples: int, device) -> torch.Tensor | None:
-    """Drop path's factor per sample: 0, or 1 / keep with probability keep."""
-    drop = float(getattr(getattr(blk, "drop_path", None), "drop_prob", 0.0) or 0.0)
-    if drop == 0.0:
+    """Drop path's factor per sample: 0, or 1 / keep with probability keep; None where it is not
+    in training mode."""
+    path = getattr(blk, "drop_path", None)
+    drop = float(getattr(path, "drop_prob", 0.0) or 0.0)
+    if drop == 0.0 or not path.training:
         return None
     keep = 1.0 - drop
     kept = torch.rand(samples, device=device) < keep
@@ -588,8 +620,9 @@ def enable_training_kernels(model: torch.nn.Module) -> int:
     """Run the Swin stages (``BasicLayer`` of MONAI or of ``crumpet_b200.swin_unetr``) of
     ``model`` on the training operators while they are in training mode, on CUDA; returns how
     many.  A stage with what they do not compute (attention, projection or MLP dropout,
-    activation checkpointing, another activation or norm) keeps its own forward, and so does
-    eval mode.  Undone by :func:`disable_training_kernels`."""
+    activation checkpointing, another activation or norm, and in place of a block, its norms, its
+    MLP or the MLP's Linears anything but the plain class: adapters, parametrizations, pruning,
+    hooks) keeps its own forward, and so does eval mode.  Undone by :func:`disable_training_kernels`."""
     layers = _layers(model)
     for layer in layers:
         if _FORWARD_ATTR not in layer.__dict__:

@@ -1,0 +1,133 @@
+"""Training operators, what needs no GPU: which blocks the switch takes, how a switched model
+copies, and what the functions refuse."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import crumpet_b200 as crumpet
+from crumpet_b200 import swin_unetr, training
+
+
+def block():
+    return swin_unetr.SwinTransformerBlock(48, 3, (7, 7, 7), (0, 0, 0)).train()
+
+
+class Adapter(torch.nn.Linear):
+    """A Linear with a low-rank addition."""
+
+    def __init__(self, *a):
+        super().__init__(*a)
+        self.down = torch.nn.Parameter(torch.randn(2, self.in_features))
+        self.up = torch.nn.Parameter(torch.randn(self.out_features, 2))
+
+    def forward(self, x):
+        return super().forward(x) + x @ self.down.t() @ self.up.t()
+
+
+class Wrapped(torch.nn.Module):
+    """A Linear held by another module that shows its parameters."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    weight = property(lambda self: self.inner.weight)
+    bias = property(lambda self: self.inner.bias)
+
+    def forward(self, x):
+        return 2 * self.inner(x)
+
+
+class Norm(torch.nn.LayerNorm):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+class Double(torch.nn.Module):
+    def forward(self, weight):
+        return 2 * weight
+
+
+class Block(swin_unetr.SwinTransformerBlock):
+    def forward(self, x, mask_matrix):
+        return 2 * super().forward(x, mask_matrix)
+
+
+class Mlp(swin_unetr.MLPBlock):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+def prune(linear):
+    import torch.nn.utils.prune as prune
+
+    prune.l1_unstructured(linear, "weight", 0.5)
+
+
+CHANGES = {
+    "adapter": lambda b: setattr(b.mlp, "linear1", Adapter(48, 192)),
+    "wrapped": lambda b: setattr(b.mlp, "linear2", Wrapped(b.mlp.linear2)),
+    "weight norm": lambda b: torch.nn.utils.weight_norm(b.mlp.linear1),
+    "parametrized": lambda b: torch.nn.utils.parametrize.register_parametrization(
+        b.mlp.linear1, "weight", Double()),
+    "pruned": lambda b: prune(b.mlp.linear2),
+    "norm subclass": lambda b: setattr(b, "norm2", Norm(48)),
+    "first norm": lambda b: setattr(b, "norm1", Norm(48)),
+    "block subclass": lambda b: setattr(b, "__class__", Block),
+    "mlp subclass": lambda b: setattr(b.mlp, "__class__", Mlp),
+    "own forward": lambda b: setattr(b.mlp, "forward", lambda x: x),
+    "other softmax": lambda b: setattr(b.attn, "softmax", torch.nn.Softmax(-2)),
+    "hook": lambda b: b.mlp.linear2.register_forward_hook(lambda *a: None),
+    "pre-hook": lambda b: b.norm2.register_forward_pre_hook(lambda *a: None),
+    "hook on the block": lambda b: b.register_forward_hook(lambda *a: None),
+    "hook on the attention": lambda b: b.attn.register_forward_hook(lambda *a: None),
+    "gradient hook": lambda b: b.mlp.register_full_backward_hook(lambda *a: None),
+    "gradient pre-hook": lambda b: b.mlp.fn.register_full_backward_pre_hook(lambda *a: None),
+    "drop path subclass": lambda b: setattr(b, "drop_path", MyDropPath()),
+}
+
+
+class DropPath(torch.nn.Module):
+    drop_prob, scale_by_keep = 0.5, True
+
+
+class MyDropPath(DropPath):
+    def forward(self, x):
+        return -x
+
+
+@pytest.mark.parametrize("what", CHANGES)
+def test_blocks_of_other_modules_keep_their_forward(what):
+    """The kernels read these modules' parameters without calling them."""
+    b = block()
+    assert training._block_trains(b, 48)
+    CHANGES[what](b)
+    assert not training._block_trains(b, 48)
+
+
+def test_modules_that_are_called_may_be_any():
+    """qkv and proj are called as modules, their hooks run."""
+    b = block()
+    b.attn.qkv = Adapter(48, 144)
+    b.attn.proj.register_forward_hook(lambda *a: None)
+    b.drop_path = DropPath()
+    assert training._block_trains(b, 48)
+
+
+def test_global_hooks():
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    try:
+        assert not training._block_trains(block(), 48)
+    finally:
+        handle.remove()
+    assert training._block_trains(block(), 48)
+
+
+def test_drop_path_of_a_block_in_eval_mode():
+    b = block()
+    b.drop_path = DropPath()
+    assert training._path_scale(b, 4, "cpu") is not None
+    b.eval()
+    assert training._path_scale(b, 4, "cpu") is None
