@@ -22,7 +22,7 @@ change from run to run (no atomics).  CUDA tensors only, as elsewhere in the pac
 from __future__ import annotations
 
 import sys
-import types
+import weakref
 from typing import NamedTuple, Sequence
 
 import torch
@@ -460,18 +460,17 @@ def checkpointed_mlp(x: torch.Tensor, weight1: torch.Tensor, bias1: torch.Tensor
 
 
 # ------------------------------------------------------------------- a Swin stage in training
-_BUCKETS_ATTR = "_crumpet_buckets"
-_FORWARD_ATTR = "_crumpet_eager_forward"
+# per attention module: its index, the index's version, and {n: buckets}
+_buckets = weakref.WeakKeyDictionary()
 
 
 def _module_buckets(attn, n: int) -> RelativePositionBuckets:
     """The buckets of the module's own index for windows of n tokens, laid out on first use and
     again if the index tensor is replaced or written to."""
     index = attn.relative_position_index
-    kept = getattr(attn, _BUCKETS_ATTR, None)
+    kept = _buckets.get(attn)
     if kept is None or kept[0] is not index or kept[1] != index._version:
-        kept = (index, index._version, {})
-        object.__setattr__(attn, _BUCKETS_ATTR, kept)
+        kept = _buckets[attn] = (index, index._version, {})
     if n not in kept[2]:
         kept[2][n] = relative_position_buckets(index[:n, :n],
                                                attn.relative_position_bias_table.shape[0])
@@ -597,17 +596,48 @@ def _train_layer(layer, x, get_window_size):
     return x.permute(0, 4, 1, 2, 3).contiguous()
 
 
+def _stage_trains(layer, x) -> bool:
+    return (x.dim() == 5 and x.is_cuda and layer.training and x.dtype in _DTYPES
+            and all(_block_trains(blk, int(x.shape[1])) for blk in layer.blocks))
+
+
 def _layer_forward(layer, x):
-    eager = layer.__dict__[_FORWARD_ATTR]
-    swin = sys.modules[type(layer).__module__]
-    c = int(x.shape[1]) if x.dim() == 5 else 0
-    if (x.dim() != 5 or not x.is_cuda or not layer.training or x.dtype not in _DTYPES
-            or not all(_block_trains(blk, c) for blk in layer.blocks)):
-        return eager(x) if eager is not None else type(layer).forward(layer, x)
+    base = type(layer)._crumpet_stage
+    if not _stage_trains(layer, x):
+        return base.forward(layer, x)
     if torch.is_autocast_enabled("cuda") and x.dtype not in (torch.float32,
                                                             torch.get_autocast_dtype("cuda")):
         x = x.float()
-    return _train_layer(layer, x, swin.get_window_size)
+    return _train_layer(layer, x, sys.modules[base.__module__].get_window_size)
+
+
+# A switched stage is an instance of a subclass of its class.  Its forward is then the copy's own
+# in every copy of the module (nn.DataParallel's replicas, deepcopy, pickles), which a method kept
+# in the instance is not.
+_switched: dict = {}
+
+
+def _restore_stage(base):
+    layer = base.__new__(base)
+    layer.__class__ = _switched_class(base)
+    return layer
+
+
+def _switched_class(base):
+    """The subclass of stage class ``base`` on the training kernels."""
+    cls = _switched.get(base)
+    if cls is None:
+        cls = _switched[base] = type(base.__name__, (base,), {
+            "__module__": base.__module__, "__qualname__": base.__qualname__,
+            "__doc__": base.__doc__, "_crumpet_stage": base, "forward": _layer_forward,
+            # pickled as the class it is made from (its own has no name to be found by)
+            "__reduce_ex__": lambda self, protocol: (_restore_stage, (base,), self.__getstate__()),
+        })
+    return cls
+
+
+def _is_switched(module) -> bool:
+    return _switched.get(getattr(type(module), "_crumpet_stage", None)) is type(module)
 
 
 def _layers(model):
@@ -622,23 +652,21 @@ def enable_training_kernels(model: torch.nn.Module) -> int:
     many.  A stage with what they do not compute (attention, projection or MLP dropout,
     activation checkpointing, another activation or norm, and in place of a block, its norms, its
     MLP or the MLP's Linears anything but the plain class: adapters, parametrizations, pruning,
-    hooks) keeps its own forward, and so does eval mode.  Undone by :func:`disable_training_kernels`."""
-    layers = _layers(model)
+    hooks) keeps its own forward, and so does eval mode.  Copies of the
+    model (replicas, deepcopy, pickles) keep the switch; a file of a pickled model then needs this
+    package to load.  Undone by :func:`disable_training_kernels`."""
+    layers = [m for m in _layers(model) if "forward" not in m.__dict__]
     for layer in layers:
-        if _FORWARD_ATTR not in layer.__dict__:
-            layer.__dict__[_FORWARD_ATTR] = layer.__dict__.get("forward")
-            layer.__dict__["forward"] = types.MethodType(_layer_forward, layer)
+        if not _is_switched(layer):
+            layer.__class__ = _switched_class(type(layer))
     return len(layers)
 
 
 def disable_training_kernels(model: torch.nn.Module) -> int:
     """Undo :func:`enable_training_kernels`; returns how many stages it changed back."""
-    layers = [m for m in model.modules() if _FORWARD_ATTR in m.__dict__]
+    layers = [m for m in model.modules() if _is_switched(m)]
     for layer in layers:
-        eager = layer.__dict__.pop(_FORWARD_ATTR)
-        layer.__dict__.pop("forward", None)
-        if eager is not None:
-            layer.__dict__["forward"] = eager
+        layer.__class__ = type(layer)._crumpet_stage
     return len(layers)
 
 

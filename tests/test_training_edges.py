@@ -131,3 +131,89 @@ def test_drop_path_of_a_block_in_eval_mode():
     assert training._path_scale(b, 4, "cpu") is not None
     b.eval()
     assert training._path_scale(b, 4, "cpu") is None
+
+
+def stage():
+    return swin_unetr.BasicLayer(48, 2, 3, (4, 4, 4)).train()
+
+
+def copies(layer):
+    """Replicas, deep copies and pickles of a stage."""
+    import copy
+    import io
+    import pickle
+
+    file = io.BytesIO()
+    torch.save(layer, file)
+    file.seek(0)
+    return {"replica": layer._replicate_for_data_parallel(), "deepcopy": copy.deepcopy(layer),
+            "copy": copy.copy(layer), "pickle": pickle.loads(pickle.dumps(layer)),
+            "file": torch.load(file, weights_only=False)}
+
+
+def test_copies_of_a_switched_stage_are_their_own(monkeypatch):
+    layer = stage()
+    x = torch.randn(1, 48, 4, 8, 4)
+    want = layer(x)
+    assert crumpet.enable_training_kernels(layer) == 1
+    for name, other in copies(layer).items():
+        assert other is not layer and isinstance(other, swin_unetr.BasicLayer), name
+        assert torch.equal(other(x), want), name  # on the CPU: the copy's own forward
+        assert type(other) is type(layer), name
+    monkeypatch.setattr(training, "_stage_trains", lambda layer, x: True)
+    monkeypatch.setattr(training, "_train_layer", lambda layer, x, size: layer)
+    for name, other in copies(layer).items():
+        assert other(x) is other, name
+        assert crumpet.disable_training_kernels(other) == 1, name
+        assert type(other) is swin_unetr.BasicLayer and torch.equal(other(x), want), name
+    assert layer(x) is layer
+    assert repr(layer).startswith("BasicLayer(")
+
+
+def test_a_stage_switched_back_leaves_no_trace():
+    import pickle
+
+    layer = stage()
+    before = pickle.dumps(layer)
+    crumpet.enable_training_kernels(layer)
+    training._module_buckets(layer.blocks[0].attn, 64)
+    assert training._module_buckets(layer.blocks[0].attn, 64) \
+        is training._module_buckets(layer.blocks[0].attn, 64)
+    crumpet.disable_training_kernels(layer)
+    assert pickle.dumps(layer) == before
+
+
+def test_the_patch_and_the_switch_in_either_order():
+    x = torch.randn(1, 48, 8, 8, 8)
+    layer, other = stage(), stage()
+    other.load_state_dict(layer.state_dict())
+    want = layer(x)
+    crumpet.enable_training_kernels(layer)
+    assert crumpet.patch_monai_swin_unetr(swin_unetr)
+    try:
+        crumpet.enable_training_kernels(other)
+        for m in (layer, other):
+            assert type(m)._crumpet_stage.forward is swin_unetr.BasicLayer.forward
+    finally:
+        crumpet.unpatch_monai_swin_unetr()
+    assert torch.equal(layer(x), want) and torch.equal(other(x), want)
+
+
+def test_a_stage_with_its_own_forward_is_left_alone():
+    layer = stage()
+    layer.forward = lambda x: x + 1
+    assert crumpet.enable_training_kernels(layer) == 0
+    x = torch.zeros(1)
+    assert torch.equal(layer(x), x + 1)
+
+
+def test_buckets_follow_the_index():
+    """Laid out again for an index that was written to or replaced, and not kept with the module."""
+    attn = block().attn
+    first = training._module_buckets(attn, 343)
+    assert training._module_buckets(attn, 343) is first
+    attn.relative_position_index[0, 0] = 0
+    again = training._module_buckets(attn, 343)
+    assert again is not first and int(again.pairs[0, 0]) == 0
+    attn.relative_position_index = attn.relative_position_index.clone()
+    assert training._module_buckets(attn, 343) is not again
