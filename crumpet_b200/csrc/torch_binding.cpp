@@ -1059,13 +1059,28 @@ TORCH_LIBRARY(crumpet_ops, ops) {
 }
 
 // The training operators' gradients are crumpet_b200.training's autograd functions; called by
-// themselves they record nothing.
+// themselves the ops record nothing.  They have no forward-mode derivative: an argument with a
+// tangent (which the functions' reverse mode does not see) is refused rather than dropped.
+namespace {
+void refuse_tangents(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
+                     torch::jit::Stack* stack) {
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (!v.isTensor()) continue;
+    const at::Tensor& t = v.toTensor();
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                op.schema().name(), " has no forward-mode derivative");
+  }
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+}
+}  // namespace
+
 TORCH_LIBRARY_IMPL(crumpet_ops, Autograd, ops) {
   for (const char* name :
        {"relative_position_bias", "relative_position_bias_backward", "swin_window_attention_train",
         "swin_window_attention_backward", "norm_gate_residual", "norm_gate_residual_backward",
         "gelu_checkpoint", "gelu_checkpoint_backward", "restore_activation"})
-    ops.impl(name, torch::CppFunction::makeFallthrough());
+    ops.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_tangents>());
 }
 
 TORCH_LIBRARY_IMPL(crumpet_ops, CUDA, ops) {

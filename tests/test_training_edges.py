@@ -217,3 +217,41 @@ def test_buckets_follow_the_index():
     assert again is not first and int(again.pairs[0, 0]) == 0
     attn.relative_position_index = attn.relative_position_index.clone()
     assert training._module_buckets(attn, 343) is not again
+
+
+def dual_calls(device):
+    """Every operator on a tensor with a tangent that needs no gradient, and none recorded."""
+    from crumpet_b200 import _ops
+
+    ops = _ops.require()
+    plan = crumpet.relative_position_buckets(torch.zeros((8, 8), dtype=torch.long, device=device), 1)
+    d = lambda *s: torch.autograd.forward_ad.make_dual(  # noqa: E731
+        torch.ones(s, device=device), torch.ones(s, device=device))
+    x, qkv, table = d(4, 32), d(1, 8, 3, 2, 16), d(1, 2)
+    kept = torch.ones((4, 32), dtype=torch.int8, device=device)
+    scales = torch.ones((4, 1), dtype=torch.uint8, device=device)
+    place = [1, 1, 1], [2, 2, 2], [0, 0, 0], 0.25
+    yield lambda: ops.relative_position_bias(table, plan.pairs, torch.float32)
+    yield lambda: ops.relative_position_bias_backward(d(2, 8, 8), *plan[2:5], 1, torch.float32)
+    yield lambda: ops.swin_window_attention_train(qkv, table, *plan[:2], *place)
+    yield lambda: ops.swin_window_attention_train(qkv.detach(), table, *plan[:2], *place)
+    yield lambda: ops.swin_window_attention_backward(d(1, 8, 32), qkv, table, *plan[1:5], *place)
+    yield lambda: ops.norm_gate_residual(x, x, None, None, None, None, None, None, 1e-5)
+    yield lambda: ops.norm_gate_residual(torch.ones_like(x).detach(), torch.ones_like(x).detach(),
+                                         d(32), None, None, None, None, None, 1e-5)
+    yield lambda: ops.norm_gate_residual_backward(x, None, x, x, None, None, None, None, None, 1e-5)
+    yield lambda: ops.gelu_checkpoint(x)
+    yield lambda: ops.gelu_checkpoint_backward(x, kept, scales)
+
+
+def test_tangents_are_refused():
+    """A result without its tangent would be a derivative of zero."""
+    with torch.autograd.forward_ad.dual_level():
+        for i, call in enumerate(dual_calls("cpu")):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        from crumpet_b200 import _ops
+
+        torch.func.jvp(lambda x: _ops.require().gelu_checkpoint(x)[0], (torch.ones(2, 32),),
+                       (torch.ones(2, 32),))

@@ -194,3 +194,35 @@ def test_bias_gradient_at_the_last_of_2_31_pairs(length):
     crumpet.device_status(clear=True)
     got = crumpet.relative_position_bias_backward(grad, plan)
     assert float(got) == length + 2 and crumpet.device_status(clear=True) == 0
+
+
+def test_tangents_are_refused():
+    """Through the functions, from tensors that need no gradient (a result without its tangent
+    would be a derivative of zero); without tangents the ops record nothing, as before."""
+    from test_training_edges import dual_calls
+
+    x = torch.randn(4, 32, device="cuda")
+    index = torch.zeros((8, 8), dtype=torch.long, device="cuda")
+    plan = crumpet.relative_position_buckets(index, 1)
+    table = torch.randn(1, 2, device="cuda")
+    qkv = torch.randn(1, 8, 3, 2, 16, device="cuda")
+    for f, args in ((crumpet.gelu_checkpoint, (x,)),
+                    (lambda t: crumpet.relative_position_bias(t, plan), (table,)),
+                    (lambda q: crumpet.swin_window_attention_train(q, table, plan), (qkv,)),
+                    (lambda t: crumpet.swin_window_attention_train(qkv, t, plan), (table,)),
+                    (lambda b: crumpet.norm_gate_residual(b, x)[0], (x,)),
+                    (lambda w: crumpet.norm_gate_residual(x, x, pre_norm=(w, w))[1], (x[0],)),
+                    (lambda b: crumpet.checkpointed_mlp(b, x, None, x.t(), None), (x,))):
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(f, args, tuple(map(torch.ones_like, args)))
+        with torch.autograd.forward_ad.dual_level():
+            duals = tuple(torch.autograd.forward_ad.make_dual(a, torch.ones_like(a)) for a in args)
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                f(*duals)
+    with torch.autograd.forward_ad.dual_level():
+        for call in dual_calls("cuda"):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    leaf = x.clone().requires_grad_(True)
+    y, kept, scales = torch.ops.crumpet_ops.gelu_checkpoint(leaf)
+    assert not y.requires_grad and torch.equal(y, crumpet.gelu_checkpoint(x)[0])
