@@ -5,7 +5,9 @@
 // one byte is kept: per 32 neighbouring channels of a row the least power of two s = 2^e with
 // max|u| <= 127 s (one byte, e + 127), and q = rint(u / s) as int8.  A power of two makes u / s
 // and q s exact, so what is kept does not depend on how it is computed, and lets one byte serve
-// 32 channels (an fp32 scale would take 12.5 %); it costs up to one of the 8 bits.  A group that
+// 32 channels (an fp32 scale would take 12.5 %); it costs up to one of the 8 bits.  In a group
+// whose largest value would be read back as 64 s = 2^128 (2^16 in fp16), an infinity, |q| stops at
+// 63, so what is finite reads back finite.  A group that
 // holds an infinity or NaN has scale byte 255 and q = 0, which reads back as NaN, so an
 // overflowed step is seen in the gradients.
 //
@@ -137,19 +139,37 @@ __device__ __forceinline__ float code_inverse(uint32_t code) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// The scale byte whose 64 s overflows the element type (rounding reaches 64 there at most); the
+// only one above it is 255.
+template <typename T>
+constexpr uint32_t kTopCode = 249u;
+template <>
+constexpr uint32_t kTopCode<__half> = 137u;
+
 // Rounding to whole numbers by adding 1.5 * 2^23: the sum's low byte is q in two's complement.
 // In a group with an infinity or NaN (code 255) q is 0.
 constexpr float kRound = 12582912.f;
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&b)[4]) {
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+template <typename T>
 __device__ __forceinline__ uint32_t quantise4(const float* x, float inv, uint32_t code) {
   uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(x[i], inv, kRound));
-  const uint32_t w = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040),
-                                 0x5410);
-  return code == 255u ? 0u : w;
+  if (code >= kTopCode<T>) {
+    if (code == 255u) return 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b[i] = __float_as_uint(fminf(fmaxf(__uint_as_float(b[i]), kRound - 63.f), kRound + 63.f));
+  }
+  return low_bytes(b);
 }
+template <typename T>
 __device__ __forceinline__ int quantise(float x, float inv, uint32_t code) {
-  return code == 255u ? 0 : int(int8_t(__float_as_uint(fmaf(x, inv, kRound)) & 0xffu));
+  if (code == 255u) return 0;
+  if (code == kTopCode<T>) return int(fminf(fmaxf(rintf(x * inv), -63.f), 63.f));
+  return int(int8_t(__float_as_uint(fmaf(x, inv, kRound)) & 0xffu));
 }
 // u of four values of a word: a byte with its sign bit flipped, under the exponent of 2^23, is
 // 2^23 + 128 + q
@@ -231,7 +251,7 @@ gelu_keep_kernel(T* y, int8_t* kept, uint8_t* scales, const T* x, Rows r) {
     if (!in) continue;
     const float inv = code_inverse(code);
     stg(reinterpret_cast<uint2*>(kept + at),
-        make_uint2(quantise4(v, inv, code), quantise4(v + 4, inv, code)));
+        make_uint2(quantise4<T>(v, inv, code), quantise4<T>(v + 4, inv, code)));
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       const float2 f = gelu(make_float2(v[i], v[i + 1]));
@@ -259,7 +279,7 @@ gelu_keep_any_kernel(T* y, int8_t* kept, uint8_t* scales, const T* x, Rows r) {
     const uint32_t code = scale_code(__reduce_max_sync(~0u, abs_bits(v)));
     if (lane == 0) scales[grp] = uint8_t(code);
     if (c < r.C) {
-      kept[at] = int8_t(quantise(v, code_inverse(code), code));
+      kept[at] = int8_t(quantise<T>(v, code_inverse(code), code));
       y[at] = from_f32<T>(gelu(both(v)).x);
     }
   }

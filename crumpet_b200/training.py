@@ -374,8 +374,8 @@ def norm_gate_residual_backward(
 # -------------------------------------------------------------- 8-bit activation checkpoints
 class KeptActivation(NamedTuple):
     """An activation ``[..., C]`` in 8 bits: per 32 neighbouring channels one power of two
-    ``2^(scales - 127)`` and int8 multiples of it (``scales`` 255: the group held an infinity
-    or NaN and reads back as NaN)."""
+    ``2^(scales - 127)`` and int8 multiples of it, as finite as the activation (``scales`` 255:
+    the group held an infinity or NaN and reads back as NaN)."""
 
     kept: torch.Tensor    # int8 [..., C]
     scales: torch.Tensor  # uint8 [..., ceil(C / 32)]

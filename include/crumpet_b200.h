@@ -488,8 +488,9 @@ CRUMPET_API int crumpet_norm_gate_residual_backward(
  * GELU (exact, by the normal distribution) whose input is kept in 8 bits for the backward:
  *   y = gelu(x);  kept int8 [M, C], scales uint8 [M, ceil(C / 32)]
  * Per 32 neighbouring channels of a row, s = 2^(scale - 127) is the least power of two (not
- * below 2^-126) with max|x| <= 127 s, and kept = rint(x / s); scale 255 marks a group with an
- * infinity or NaN, which reads back as NaN.  Backward, with u = kept * s:
+ * below 2^-126) with max|x| <= 127 s, and kept = rint(x / s), at most 63 in magnitude where 64 s
+ * is past dtype's largest number; scale 255 marks a group with an infinity or NaN, which reads
+ * back as NaN.  Backward, with u = kept * s:
  *   grad_x = grad_y * gelu'(u), again = gelu(u)   (the weight gradient's input)
  * crumpet_restore_activation writes u itself.  x, y, grad_*, again and u in dtype; C <= 2^24.
  */

@@ -226,3 +226,31 @@ def test_tangents_are_refused():
     leaf = x.clone().requires_grad_(True)
     y, kept, scales = torch.ops.crumpet_ops.gelu_checkpoint(leaf)
     assert not y.requires_grad and torch.equal(y, crumpet.gelu_checkpoint(x)[0])
+
+
+@pytest.mark.parametrize("c", [64, 50])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+def test_gelu_checkpoint_of_the_largest_values(dtype, c):
+    """What is finite reads back finite, within a step (and half a step below the top binade's
+    last step, as everywhere)."""
+    top = torch.finfo(dtype).max
+    scale = 2.0 ** (10 if dtype == F16 else 122)
+    below = [top, 63.75 * scale, 63.5 * scale, 63.25 * scale, 62.75 * scale, 63.5 * scale / 32]
+    x = torch.zeros(2 * len(below), c, dtype=dtype, device="cuda")
+    for i, v in enumerate(below):
+        x[i, 3], x[i, 7], x[i, 35] = v, -v / 2, -v
+        x[i + len(below), 3] = -v
+    y, kept = crumpet.gelu_checkpoint(x)
+    back = crumpet.restore_activation(kept)
+    # (on the CPU: powers of two are exact there)
+    step = (2.0 ** (kept.scales.double().cpu() - 127)).cuda().repeat_interleave(32, 1)[:, :c]
+    want = torch.round(x.double() / step)
+    tops = kept.scales.repeat_interleave(32, 1)[:, :c] == (137 if dtype == F16 else 249)
+    assert tops.any()
+    want = torch.where(tops, want.clamp(-63, 63), want)
+    assert torch.equal(kept.kept.double(), want)
+    assert torch.equal(back.double(), want * step)
+    grad_x, again = crumpet.gelu_checkpoint_backward(torch.ones_like(x), kept)
+    for t in (back, again, grad_x, y):
+        assert torch.isfinite(t).all()
+    assert torch.equal(again, back.clamp(min=0)) and torch.equal(y, x.clamp(min=0))
