@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "common.cuh"
@@ -102,6 +103,21 @@ __device__ __forceinline__ float bias_of(const Params& p, int h, unsigned t) {
   const float v = kLog2e * (p.table_f32 ? __ldg(static_cast<const float*>(p.table) + at)
                                         : load(static_cast<const T*>(p.table), at));
   return t < unsigned(p.table_rows) ? v : 0.f;
+}
+
+// Allows a kernel `bytes` of dynamic shared memory on the current device, once: the most that any
+// call takes.  (Set to each call's own size, one thread would lower it between another's call and
+// its launch.)  `allowed` is the kernel's own, per device.
+template <class K>
+int allow_smem(K kernel, int bytes, std::atomic<bool> (&allowed)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && allowed[dev].load(std::memory_order_acquire)) return kOk;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return set_cuda_error(e, "attention (fp32) smem attribute");
+  if (dev < 64) allowed[dev].store(true, std::memory_order_release);
+  return kOk;
 }
 
 }  // namespace grad_f32

@@ -38,6 +38,7 @@ using namespace grad_f32;
 
 constexpr int kThreads = 128;
 constexpr int kTile = 32;  // tokens streamed at a time
+constexpr int kBiasBytes = 64 * 1024;  // most shared memory for the bias of a CTA's rows
 template <int D>
 struct Shape {
   static constexpr int KL = D <= 32 ? 4 : 1;            // lanes that share out the tokens
@@ -49,10 +50,10 @@ struct Shape {
                                        // different banks
   static constexpr int ROW = TPR * SLICE;
   static constexpr int STAGED = 2 * kTile * ROW * 4 + kTile * 8;  // bytes of a tile and statistics
+  // most of any call: the bias, and a byte per row and per token that it holds
+  static constexpr int MOST = STAGED + kBiasBytes + R + kBiasBytes / (4 * R) + kTile;
   static_assert(E % 4 == 0 && E <= 32, "channels per lane");
 };
-constexpr int kBiasBytes = 64 * 1024;  // most shared memory for the bias of a CTA's rows
-
 template <typename S>
 __device__ __forceinline__ float dot(const float (&a)[S::E], const float* row) {
   float s = 0.f;
@@ -384,13 +385,11 @@ __global__ void __launch_bounds__(kThreads, CH == 16 ? 6 : 1) grad_bias_simt_ker
   }
 }
 
-template <class K>
-int start(K kernel, long long blocks, int smem, const Params& p, cudaStream_t stream) {
-  if (smem > 32 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return set_cuda_error(e, "attention (simt) smem attribute");
-  }
+template <typename T, int D, int MODE>
+int start(long long blocks, int smem, const Params& p, cudaStream_t stream) {
+  const auto kernel = grad_simt_kernel<T, D, MODE>;
+  static std::atomic<bool> allowed[64];  // per device
+  if (int e = allow_smem(kernel, Shape<D>::MOST, allowed)) return e;
   kernel<<<unsigned(blocks), kThreads, smem, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "attention (simt) launch");
@@ -410,9 +409,9 @@ int launch(Params p, bool forward, cudaStream_t stream) {
   p.bias_pitch = S::R * pitch * 4 <= kBiasBytes ? pitch : 0;
   const int smem = S::STAGED + S::R * (p.bias_pitch ? pitch : kTile + 1) * 4 + S::R +
                    (p.bias_pitch ? int(tiles) * kTile : kTile);
-  if (forward) return start(grad_simt_kernel<T, D, kForward>, blocks, smem, p, stream);
-  if (int e = start(grad_simt_kernel<T, D, kRows>, blocks, smem, p, stream)) return e;
-  if (int e = start(grad_simt_kernel<T, D, kCols>, blocks, smem, p, stream)) return e;
+  if (forward) return start<T, D, kForward>(blocks, smem, p, stream);
+  if (int e = start<T, D, kRows>(blocks, smem, p, stream)) return e;
+  if (int e = start<T, D, kCols>(blocks, smem, p, stream)) return e;
   constexpr int CH = D < 32 ? D : 32;
   grad_bias_simt_kernel<T, CH><<<unsigned(bias_blocks), kThreads, 0, stream>>>(p, D);
   const cudaError_t e = cudaGetLastError();

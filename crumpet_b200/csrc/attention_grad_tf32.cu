@@ -96,6 +96,8 @@ template <int D>
 struct Stage {
   static constexpr int CTAS = D == 16 ? 4 : 2;  // per SM, that registers allow
   static constexpr int FLOATS = 2 * kTile * (D + 4) + 2 * kTile;  // x, y and statistics
+  // bytes, most of any call: with the bias, and a byte per token of the longest window
+  static constexpr int MOST = FLOATS * 4 + 64 * 1024 + 46400;
   static constexpr int ROW = D + 4;  // floats from a staged token to the next: both ways of
                                      // reading it (below) find the lanes' words in other banks
 };
@@ -597,12 +599,9 @@ int start(Params p, cudaStream_t stream) {
   const int smem = Stage<D>::FLOATS * 4 + (p.N + kTile - 1) / kTile * kTile +
                    (p.bias_pitch ? bytes
                                  : (MODE == kCols ? kTile * (rows + 4) : rows * (kTile + 8)) * 4);
-  auto kernel = grad_tf32_kernel<D, MODE>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return set_cuda_error(e, "attention (tf32) smem attribute");
-  }
+  const auto kernel = grad_tf32_kernel<D, MODE>;
+  static std::atomic<bool> allowed[64];  // per device
+  if (int e = allow_smem(kernel, Stage<D>::MOST, allowed)) return e;
   kernel<<<unsigned(blocks), 32 * warps, smem, stream>>>(p, int(shares));
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? kOk : set_cuda_error(e, "attention (tf32) launch");

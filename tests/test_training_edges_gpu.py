@@ -254,3 +254,37 @@ def test_gelu_checkpoint_of_the_largest_values(dtype, c):
     for t in (back, again, grad_x, y):
         assert torch.isfinite(t).all()
     assert torch.equal(again, back.clamp(min=0)) and torch.equal(y, x.clamp(min=0))
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 16), (F32, 64), (BF16, 128)], ids=str)
+def test_attention_from_two_threads(dtype, d):
+    """Windows of two sizes, whose kernels take different amounts of shared memory, from two host
+    threads on streams of their own."""
+    import threading
+
+    cases = [attention_case(win, (1, 1, 1), (0, 0, 0), 1, 1, d, dtype, F32)
+             for win in ((6, 6, 6), (5, 5, 7))]
+    want = [attention_both(c) for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(c, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                buckets = crumpet.relative_position_buckets(c["index"], c["table"].shape[0])
+                for _ in range(400):
+                    out = crumpet.swin_window_attention_train(c["qkv"], c["table"], buckets,
+                                                              **c["place"])
+                    got = (out, *crumpet.swin_window_attention_backward(
+                        c["grad"], c["qkv"], c["table"], buckets, **c["place"]))
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, w))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
