@@ -94,7 +94,8 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
         raise ValueError("num_buckets must be positive")
     if index.numel() >= 2 ** 31 or num_buckets >= 2 ** 31:
         raise ValueError("index must hold fewer than 2^31 pairs and buckets")
-    index = index.detach().long().contiguous()
+    # a copy: a later write to the caller's index does not reach a part of the plan
+    index = torch.empty(index.shape, dtype=torch.int64, device=index.device).copy_(index.detach())
     flat = index.reshape(-1)
     if flat.numel() and (int(flat.min()) < 0 or int(flat.max()) >= num_buckets):
         raise ValueError(f"index values must lie in [0, {num_buckets})")

@@ -255,3 +255,12 @@ def test_tangents_are_refused():
 
         torch.func.jvp(lambda x: _ops.require().gelu_checkpoint(x)[0], (torch.ones(2, 32),),
                        (torch.ones(2, 32),))
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_a_plan_does_not_change_with_the_index(dtype):
+    index = torch.arange(12, dtype=dtype).view(3, 4)
+    plan = crumpet.relative_position_buckets(index, 12)
+    index.fill_(99)
+    assert torch.equal(plan.index, torch.arange(12).view(3, 4))
+    assert torch.equal(plan.pairs, plan.index.int())
