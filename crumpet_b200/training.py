@@ -86,7 +86,7 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
     query / key pair) for :func:`relative_position_bias` and
     :func:`swin_window_attention_train`.  Made once for a module's index (for a window clamped
     to a smaller volume, of its slice ``index[:n, :n]``): it sorts the pairs and checks their
-    values, which waits for the device."""
+    values, which waits for the device; the plan is then ready for any stream."""
     if index.ndim != 2 or index.is_floating_point() or index.is_complex() or index.dtype == torch.bool:
         raise ValueError("index must be an integer tensor [rows, cols]")
     num_buckets = int(num_buckets)
@@ -115,8 +115,11 @@ def relative_position_buckets(index: torch.Tensor, num_buckets: int) -> Relative
     items = torch.stack((torch.where(several[bucket], -1, bucket), lo, hi), 1)
     which = torch.nonzero(several).reshape(-1)
     multi = torch.stack((which, first[which], (first + parts)[which]), 1)
-    return RelativePositionBuckets(index, index.int(), order.int(), items.int().contiguous(),
+    plan = RelativePositionBuckets(index, index.int(), order.int(), items.int().contiguous(),
                                    multi.int().contiguous(), num_buckets)
+    if index.is_cuda:  # kept for later calls, whatever their stream
+        torch.cuda.current_stream(index.device).synchronize()
+    return plan
 
 
 def _check_table(table: torch.Tensor, buckets: RelativePositionBuckets) -> None:

@@ -288,3 +288,15 @@ def test_attention_from_two_threads(dtype, d):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_a_plan_is_ready_for_any_stream():
+    """Nothing of it is still to be computed when it is returned (64 M pairs: the last steps take
+    the device longer than the host)."""
+    index = torch.randint(0, 100, (8192, 8192), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        plan = crumpet.relative_position_buckets(index, 100)
+        assert side.query()
+    assert torch.equal(plan.pairs, index.int())
