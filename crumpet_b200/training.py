@@ -435,13 +435,25 @@ class _Mlp(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, w1, w2, kept, scales = ctx.saved_tensors
+        needs = ctx.needs_input_grad  # products of frozen weights are left out
+        grads = [None] * 5
         with torch.autocast("cuda", enabled=False):
             rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
             grad = grad.to(x.dtype)
-            grad_u, y = gelu_checkpoint_backward(grad @ w2, KeptActivation(kept, scales, x.dtype))
-            grads = (grad_u @ w1, rows(grad_u).t() @ rows(x), rows(grad_u).sum(0),
-                     rows(grad).t() @ rows(y), rows(grad).sum(0))
-        return (*(None if dt is None else g.to(dt) for g, dt in zip(grads, ctx.dtypes)), None)
+            if any(needs[:4]):
+                grad_u, y = gelu_checkpoint_backward(grad @ w2,
+                                                     KeptActivation(kept, scales, x.dtype))
+            if needs[0]:
+                grads[0] = grad_u @ w1
+            if needs[1]:
+                grads[1] = rows(grad_u).t() @ rows(x)
+            if needs[2]:
+                grads[2] = rows(grad_u).sum(0)
+            if needs[3]:
+                grads[3] = rows(grad).t() @ rows(y)
+            if needs[4]:
+                grads[4] = rows(grad).sum(0)
+        return (*(None if g is None else g.to(dt) for g, dt in zip(grads, ctx.dtypes)), None)
 
 
 def checkpointed_mlp(x: torch.Tensor, weight1: torch.Tensor, bias1: torch.Tensor | None,

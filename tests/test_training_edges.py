@@ -264,3 +264,54 @@ def test_a_plan_does_not_change_with_the_index(dtype):
     index.fill_(99)
     assert torch.equal(plan.index, torch.arange(12).view(3, 4))
     assert torch.equal(plan.pairs, plan.index.int())
+
+
+def plain_gelu(monkeypatch):
+    """The 8-bit GELU's calls in plain torch, for what is around them."""
+    def keep(x):
+        return torch.nn.functional.gelu(x), training.KeptActivation(x, x, x.dtype)
+
+    def back(grad, kept):
+        u = kept.kept.detach().requires_grad_(True)
+        with torch.enable_grad():
+            y = torch.nn.functional.gelu(u)
+        return torch.autograd.grad(y, u, grad)[0], y.detach()
+
+    monkeypatch.setattr(training, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(training, "gelu_checkpoint", keep)
+    monkeypatch.setattr(training, "gelu_checkpoint_backward", back)
+
+
+@pytest.mark.parametrize("frozen", [(), (1, 2, 3, 4), (1, 2), (3, 4), (0,), (0, 1, 2), (0, 1, 3), (0, 2, 4),
+                                    (0, 1, 2, 3)], ids=str)
+def test_mlp_takes_the_products_that_are_asked_for(monkeypatch, frozen):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        products = sums = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.products += func.overloadpacket in (torch.ops.aten.mm, torch.ops.aten.addmm)
+            self.sums += func.overloadpacket == torch.ops.aten.sum
+            return func(*args, **(kwargs or {}))
+
+    plain_gelu(monkeypatch)
+    g = torch.Generator().manual_seed(0)
+    args = [torch.randn(s, generator=g) for s in ((5, 16), (64, 16), (64,), (16, 64), (16,))]
+    for i, t in enumerate(args):
+        t.requires_grad_(i not in frozen)
+    x, w1, b1, w2, b2 = args
+    want = torch.nn.functional.linear(torch.nn.functional.gelu(
+        torch.nn.functional.linear(x, w1, b1)), w2, b2)
+    got = crumpet.checkpointed_mlp(*args)
+    torch.testing.assert_close(got, want)
+    asked = [t for t in args if t.requires_grad]
+    grad = torch.randn(want.shape, generator=g)
+    wanted = torch.autograd.grad(want, asked, grad)
+    with Count() as count:
+        grads = torch.autograd.grad(got, asked, grad)
+    for a, b in zip(grads, wanted):
+        torch.testing.assert_close(a, b)
+    on = [t.requires_grad for t in args]
+    assert count.products == any(on[:4]) + on[0] + on[1] + on[3]
+    assert count.sums == on[2] + on[4]
