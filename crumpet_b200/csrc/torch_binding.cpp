@@ -874,7 +874,10 @@ std::vector<at::Tensor> norm_gate_residual_backward(
     check_cuda(branch, *grad_normed, "grad_normed");
     gn = grad_normed->contiguous();
   }
-  const at::Tensor x = branch.contiguous(), o = out.contiguous(), go = grad_out.contiguous();
+  // branch is read for the gate's and the post-norm's gradients alone, out for the pre-norm's
+  const bool reads_branch = n.gate.defined() || n.post_w.defined();
+  const at::Tensor x = reads_branch ? branch.contiguous() : branch;
+  const at::Tensor o = n.pre_w.defined() ? out.contiguous() : out, go = grad_out.contiguous();
   std::vector<at::Tensor> res{at::empty(o.sizes(), o.options()), at::empty(x.sizes(), x.options())};
   float* sums[5] = {};  // gate, post weight and bias, pre weight and bias
   const bool has[5] = {n.gate.defined(), n.post_w.defined(), n.post_w.defined(),
@@ -889,7 +892,8 @@ std::vector<at::Tensor> norm_gate_residual_backward(
     partial = f32_like(x, {crumpet_norm_gate_residual_backward_partials(n.M, n.C)});
   check_rc(crumpet_norm_gate_residual_backward(
       res[0].data_ptr(), res[1].data_ptr(), sums[0], sums[1], sums[2], sums[3], sums[4],
-      go.data_ptr(), gn.defined() ? gn.data_ptr() : nullptr, o.data_ptr(), x.data_ptr(),
+      go.data_ptr(), gn.defined() ? gn.data_ptr() : nullptr,
+      n.pre_w.defined() ? o.data_ptr() : nullptr, reads_branch ? x.data_ptr() : nullptr,
       dtype_code(x), dtype_code(o), f32(n.gate), f32(n.row_scale), n.samples, f32(n.post_w),
       f32(n.post_b), f32(n.pre_w), static_cast<float>(eps),
       partial.defined() ? partial.data_ptr<float>() : nullptr, n.M, n.C, cur_stream(x)));

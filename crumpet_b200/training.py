@@ -317,8 +317,8 @@ class _NormGate(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out, grad_normed=None):
         branch, out, *params = ctx.saved_tensors
-        if branch is None:  # not read
-            branch = torch.empty_like(out, dtype=ctx.branch_dtype)
+        if branch is None:  # not read: its shape and dtype, without the memory
+            branch = out.new_empty((), dtype=ctx.branch_dtype).expand(out.shape)
         g = _norm_gate_backward(grad_out, grad_normed, out, branch, *params, ctx.eps)
         gate, *norms = (None if t is None else t.to(dt) for t, dt in zip(g[2:], ctx.dtypes))
         return g.branch, g.residual, gate, None, *norms, None
@@ -690,7 +690,7 @@ def _fake_norm_gate_backward(grad_out, grad_normed, out, branch, gate, row_scale
                              pre_w, eps):
     n = (gate is not None) + 2 * (post_w is not None) + 2 * (pre_w is not None)
     vector = branch.new_empty(branch.shape[-1:], dtype=torch.float32)
-    return [torch.empty_like(out), torch.empty_like(branch),
+    return [out.new_empty(out.shape), branch.new_empty(branch.shape),
             *(torch.empty_like(vector) for _ in range(n))]
 
 

@@ -300,3 +300,25 @@ def test_a_plan_is_ready_for_any_stream():
         plan = crumpet.relative_position_buckets(index, 100)
         assert side.query()
     assert torch.equal(plan.pairs, index.int())
+
+
+@pytest.mark.parametrize("pre", [True, False])
+def test_norm_gate_backward_allocates_its_results(pre):
+    """Without gate and post-norm the branch is not kept, and nothing of its size stands in for it."""
+    rows, c = 1 << 16, 64
+    branch = torch.randn(rows, c, device="cuda", dtype=BF16, requires_grad=True)
+    stream = torch.randn(rows, c, device="cuda", requires_grad=True)
+    norm = (torch.ones(c, device="cuda"), torch.zeros(c, device="cuda"))
+    out, normed = crumpet.norm_gate_residual(branch, stream, pre_norm=norm if pre else None)
+    ends = (out, normed) if pre else (out,)
+    grads = [torch.randn_like(t) for t in ends]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(ends, (branch, stream), grads)
+    torch.cuda.synchronize()
+    # the two results, and the partial column sums (at most two CTAs for each of 148 SMs)
+    most = rows * c * (2 + 4) + (2 * 148 * 5 * c * 4 if pre else 0) + (1 << 14)
+    assert torch.cuda.max_memory_allocated() - before <= most
+    if not pre:
+        assert torch.equal(got[1], grads[0]) and torch.equal(got[0], grads[0].to(BF16))
