@@ -600,8 +600,11 @@ def _train_layer(layer, x, get_window_size):
             branch, x, row_scale=_path_scale(blk, b, x.device),
             pre_norm=(blk.norm2.weight, blk.norm2.bias), eps=blk.norm2.eps)
         mlp = blk.mlp
-        branch = checkpointed_mlp(normed, mlp.linear1.weight, mlp.linear1.bias, mlp.linear2.weight,
-                                  mlp.linear2.bias)
+        if layer.__dict__.get(_EIGHT_BITS, True):
+            branch = checkpointed_mlp(normed, mlp.linear1.weight, mlp.linear1.bias,
+                                      mlp.linear2.weight, mlp.linear2.bias)
+        else:
+            branch = mlp(normed)
         after = blocks[i + 1].norm1 if i + 1 < len(blocks) else None
         x, normed = norm_gate_residual(
             branch, x, row_scale=_path_scale(blk, b, x.device),
@@ -610,6 +613,9 @@ def _train_layer(layer, x, get_window_size):
     if layer.downsample is not None:
         x = layer.downsample(x)
     return x.permute(0, 4, 1, 2, 3).contiguous()
+
+
+_EIGHT_BITS = "_crumpet_eight_bits"  # of a switched stage: keep hidden activations in 8 bits
 
 
 def _stage_trains(layer, x) -> bool:
@@ -662,7 +668,7 @@ def _layers(model):
             and hasattr(sys.modules[type(m).__module__], "get_window_size")]
 
 
-def enable_training_kernels(model: torch.nn.Module) -> int:
+def enable_training_kernels(model: torch.nn.Module, eight_bit_activations: bool = True) -> int:
     """Run the Swin stages (``BasicLayer`` of MONAI or of ``crumpet_b200.swin_unetr``) of
     ``model`` on the training operators while they are in training mode, on CUDA; returns how
     many.  A stage with what they do not compute (attention, projection or MLP dropout,
@@ -670,11 +676,16 @@ def enable_training_kernels(model: torch.nn.Module) -> int:
     MLP or the MLP's Linears anything but the plain class: adapters, parametrizations, pruning,
     hooks) keeps its own forward, and so does eval mode.  Copies of the
     model (replicas, deepcopy, pickles) keep the switch; a file of a pickled model then needs this
-    package to load.  Undone by :func:`disable_training_kernels`."""
+    package to load.
+
+    With ``eight_bit_activations`` the MLPs keep their hidden activation in 8 bits for the backward
+    pass (:func:`checkpointed_mlp`), in fp32 training too: their gradients are then off by about 2^-8
+    in the norm.  Without, the MLPs run as modules, at the memory and precision of eager ones.  Undone by :func:`disable_training_kernels`."""
     layers = [m for m in _layers(model) if "forward" not in m.__dict__]
     for layer in layers:
         if not _is_switched(layer):
             layer.__class__ = _switched_class(type(layer))
+        layer.__dict__[_EIGHT_BITS] = bool(eight_bit_activations)
     return len(layers)
 
 
@@ -683,6 +694,7 @@ def disable_training_kernels(model: torch.nn.Module) -> int:
     layers = [m for m in model.modules() if _is_switched(m)]
     for layer in layers:
         layer.__class__ = type(layer)._crumpet_stage
+        layer.__dict__.pop(_EIGHT_BITS, None)
     return len(layers)
 
 

@@ -315,3 +315,27 @@ def test_mlp_takes_the_products_that_are_asked_for(monkeypatch, frozen):
     on = [t.requires_grad for t in args]
     assert count.products == any(on[:4]) + on[0] + on[1] + on[3]
     assert count.sums == on[2] + on[4]
+
+
+def test_eight_bit_activations_are_a_choice(monkeypatch):
+    kept = []
+    monkeypatch.setattr(training, "checkpointed_mlp", lambda x, *a: kept.append(1) or x)
+    monkeypatch.setattr(training, "_stage_trains", lambda layer, x: True)
+    monkeypatch.setattr(training, "_train_branch", lambda blk, normed, *a: normed)
+    monkeypatch.setattr(training, "norm_gate_residual",
+                        lambda b, x, **k: (b + x, b if k["pre_norm"] else None))
+    layer = stage()
+    called = []
+    x = torch.randn(1, 48, 4, 4, 4)
+    for on in (True, False, True):
+        crumpet.enable_training_kernels(layer, on)
+        kept.clear(), called.clear()
+        handles = [b.mlp.register_forward_hook(lambda *a: called.append(1)) for b in layer.blocks]
+        layer(x)
+        assert (len(kept), len(called)) == ((2, 0) if on else (0, 2))
+        for h in handles:
+            h.remove()
+    for other in copies(crumpet.enable_training_kernels(layer, False) and layer).values():
+        kept.clear()
+        other(x)
+        assert not kept

@@ -322,3 +322,24 @@ def test_norm_gate_backward_allocates_its_results(pre):
     assert torch.cuda.max_memory_allocated() - before <= most
     if not pre:
         assert torch.equal(got[1], grads[0]) and torch.equal(got[0], grads[0].to(BF16))
+
+
+@pytest.mark.parametrize("size", [14, 20])
+def test_stage_without_8_bit_activations(size):
+    """In fp32 the stage's gradients then have fp32 errors: 1e-5 per operator (as above), some ten
+    of them in a row in two blocks."""
+    from crumpet_b200 import swin_unetr
+    from test_training_gpu import _grads
+
+    torch.manual_seed(3)
+    make = lambda: swin_unetr.BasicLayer(48, 2, 3, (7, 7, 7),  # noqa: E731
+                                         downsample=swin_unetr.PatchMerging).cuda()
+    layer, wide = make(), make()
+    wide.load_state_dict(layer.state_dict())
+    x = torch.randn(1, 48, size, size, size - 1, device="cuda")
+    want_out, want = _grads(wide.double(), x.double(), None)
+    assert crumpet.enable_training_kernels(layer, eight_bit_activations=False) == 1
+    out, got = _grads(layer.train(), x, None)
+    assert rel(out, want_out) <= 1e-4
+    for name, w in want.items():
+        assert rel(got[name], w) <= 1e-4, name
