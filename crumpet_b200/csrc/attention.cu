@@ -362,7 +362,9 @@ __device__ __forceinline__ uint32_t window_last_axes(const KParams& p, int b) {
 // Relative-position bias tile of one (head h, query tile mt) for the bias MMA, written
 // to dst (shared or global memory) as the UMMA K-major no-swizzle operand image:
 // elem(elem(bias) / scale) -- rounded to the element type first, as the reference's
-// .to(dtype) -- at rows < N and columns < N; -30000 in padded key columns (their
+// .to(dtype) -- at rows < N and columns < N, and its lowest finite number for less (a bucket
+// switched off by -inf or such: infinite, it would make NaN of the 15 columns that the identity
+// multiplies by 0); -30000 in padded key columns (their
 // scores drop out of the softmax: 30000 scale is at least 117 (kTensorMinScale)); 0 in
 // padded query rows.  Core matrix (row group rg, column group cg) at cg * (kBM / 8) * 128 + rg * 128.
 // Each item is 8 consecutive columns of one row (one 16-byte core-matrix row); two
@@ -446,7 +448,10 @@ __device__ __forceinline__ void build_bias_tile(const KParams& p, int h, int mt,
           uint16_t v16;
           if (grow >= p.N) v16 = 0;
           else if (col >= p.N) v16 = pad_val;
-          else v16 = f32_to_elem<BF16>(to_f32<BF16>(f32_to_elem<BF16>(vals[u][e + z])) * inv_scale);
+          else {
+            v16 = f32_to_elem<BF16>(to_f32<BF16>(f32_to_elem<BF16>(vals[u][e + z])) * inv_scale);
+            if (v16 == (BF16 ? 0xFF80u : 0xFC00u)) v16 = BF16 ? 0xFF7Fu : 0xFBFFu;
+          }
           pair |= uint32_t(v16) << (16 * z);
         }
         wv[e / 2] = pair;

@@ -343,3 +343,21 @@ def test_stage_without_8_bit_activations(size):
     assert rel(out, want_out) <= 1e-4
     for name, w in want.items():
         assert rel(got[name], w) <= 1e-4, name
+
+
+@pytest.mark.parametrize("off", ["-inf", "lowest", "-1e9"])
+@pytest.mark.parametrize("d", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_attention_buckets_switched_off(dtype, d, off):
+    """A bucket whose bias excludes its pairs: they weigh nothing, in both directions, and the
+    pairs beside them are as before."""
+    c = attention_case((3, 4, 5), (2, 1, 2), (1, 0, 2), 1, 2, d, dtype, F32)
+    value = {"-inf": -float("inf"), "lowest": torch.finfo(F32).min, "-1e9": -1e9}[off]
+    c["table"][::4] = value
+    c["table"][c["table"].shape[0] // 2] = 0.25  # a token and itself
+    want = attention_wide(dict(c, table=c["table"].clamp(min=-1e30)))
+    got = attention_both(c)
+    for a, b, tol in zip(got, want, (1.5 * TOL[dtype], TOL[dtype], TOL[F32])):
+        assert torch.isfinite(a.float()).all()
+        assert rel(a, b) <= tol
+    assert not got[2][:4:4].any()
