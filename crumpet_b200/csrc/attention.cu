@@ -20,7 +20,7 @@
 //     adds the relative-position bias on the tensor cores as well: the bias tile
 //     of the (head, query tile), stored as elem(bias)/scale in shared memory,
 //     multiplied by a 16x16 identity (one exact product per sum).  So S holds
-//     q.k + bias/scale; padded key columns carry -30000 and drop out.
+//     q.k + bias/scale; padded key columns carry the type's lowest number and drop out.
 //   * The analytic shifted-window mask is one more MMA: -100 / scale where the roll-side
 //     codes of query and key differ on a "last window" axis.
 //   * Softmax warps pull S into registers, add a dense mask (global loads, read
@@ -364,9 +364,8 @@ __device__ __forceinline__ uint32_t window_last_axes(const KParams& p, int b) {
 // elem(elem(bias) / scale) -- rounded to the element type first, as the reference's
 // .to(dtype) -- at rows < N and columns < N, and its lowest finite number for less (a bucket
 // switched off by -inf or such: infinite, it would make NaN of the 15 columns that the identity
-// multiplies by 0); -30000 in padded key columns (their
-// scores drop out of the softmax: 30000 scale is at least 117 (kTensorMinScale)); 0 in
-// padded query rows.  Core matrix (row group rg, column group cg) at cg * (kBM / 8) * 128 + rg * 128.
+// multiplies by 0); that number in padded key columns too (their scores drop out of the
+// softmax: in fp16, 65504 scale is at least 255 (kTensorMinScale)); 0 in padded query rows.  Core matrix (row group rg, column group cg) at cg * (kBM / 8) * 128 + rg * 128.
 // Each item is 8 consecutive columns of one row (one 16-byte core-matrix row); two
 // items per thread are in flight.  Threads tid = 0 .. nthreads-1 share the work.
 template <int NPAD, bool BF16>
@@ -376,7 +375,7 @@ __device__ __forceinline__ void build_bias_tile(const KParams& p, int h, int mt,
   constexpr int kItems = kBM * (NPAD / 8);
   constexpr int kBatch = 2;
   const float inv_scale = 1.f / p.scale;
-  const uint16_t pad_val = f32_to_elem<BF16>(-30000.f);
+  constexpr uint16_t kLowest = BF16 ? 0xFF7Fu : 0xFBFFu;
   for (int i0 = tid; i0 < kItems; i0 += kBatch * nthreads) {
     float vals[kBatch][8];
     long long idx[kBatch][8];
@@ -447,10 +446,10 @@ __device__ __forceinline__ void build_bias_tile(const KParams& p, int h, int mt,
           const int col = cg * 8 + e + z;
           uint16_t v16;
           if (grow >= p.N) v16 = 0;
-          else if (col >= p.N) v16 = pad_val;
+          else if (col >= p.N) v16 = kLowest;
           else {
             v16 = f32_to_elem<BF16>(to_f32<BF16>(f32_to_elem<BF16>(vals[u][e + z])) * inv_scale);
-            if (v16 == (BF16 ? 0xFF80u : 0xFC00u)) v16 = BF16 ? 0xFF7Fu : 0xFBFFu;
+            if (v16 == (BF16 ? 0xFF80u : 0xFC00u)) v16 = kLowest;
           }
           pair |= uint32_t(v16) << (16 * z);
         }

@@ -35,7 +35,7 @@ extern "C" {
 
 /* Least scale of the 16-bit tensor-core attention kernels, 2^-8: they add bias, mask and the
  * exclusion of padded keys to the scores divided by it, in the element type, which has to hold
- * -100 / scale (fp16: up to 65504) and a padding of -30000 that outweighs it.  Calls with a
+ * -100 / scale and, for the padding, less (fp16: up to 65504 in magnitude).  Calls with a
  * smaller scale run the fp32 kernels (with prebuilt bias tiles: CRUMPET_ERR_UNSUPPORTED). */
 #define CRUMPET_TENSOR_MIN_SCALE 0.00390625f
 

@@ -361,3 +361,16 @@ def test_attention_buckets_switched_off(dtype, d, off):
         assert torch.isfinite(a.float()).all()
         assert rel(a, b) <= tol
     assert not got[2][:4:4].any()
+
+
+@pytest.mark.parametrize("shift", [-1e4, 1e4])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_attention_bias_of_one_value(dtype, shift):
+    """A bias that is the same for all pairs changes nothing, however low (27 tokens: padded
+    keys do not take over).  Scores of 4e4 over the scale lose 2^-9 each in fp32, 1e-3 of p."""
+    c = attention_case((3, 3, 3), (2, 2, 2), (1, 1, 1), 1, 2, 16, dtype, F32)
+    c["table"].fill_(shift)
+    got, want = attention_both(c), attention_wide(c)
+    for a, b, tol in zip(got[:2], want, (1.5 * TOL[dtype], TOL[dtype])):
+        assert torch.isfinite(a.float()).all()
+        assert rel(a, b) <= tol + 2e-3
