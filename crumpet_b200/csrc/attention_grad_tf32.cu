@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
               for (int c = 0; c < D / 8; ++c) acc[c][2 * u] *= alpha, acc[c][2 * u + 1] *= alpha;
             }
           }
-          float now[2][D / 8][4] = {};
+          [[maybe_unused]] float now[2][D / 8][4] = {};
 #pragma unroll
           for (int n = 0; n < TILES; ++n) {
 #pragma unroll
@@ -386,8 +386,10 @@ __global__ void __launch_bounds__(32 * kWarps, Stage<D>::CTAS) grad_tf32_kernel(
               for (int e = 0; e < 4; ++e) dp[e / 2] = fmaf(s[n][e], d[e], dp[e / 2]);
             }
           }
-          if constexpr (MODE == kForward) join<D>(acc, now[0]);
+          if constexpr (MODE == kForward) {
+            join<D>(acc, now[0]);
             join<D>(acc, now[1]);
+          }
         };
         each_block(j0, block);
       }
