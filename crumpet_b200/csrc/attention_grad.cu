@@ -4,8 +4,11 @@
 //   dv = p^T do,   dp = do v^T,   delta_i = sum_j p_ij dp_ij,   ds = p (dp - delta),
 //   dq = ds k * scale,   dk = ds^T q * scale,   dbias[h] = sum over the windows of ds[b,h].
 // Nothing of the forward pass is kept but qkv: the row statistics are taken again here, in
-// fp32 and from the unrounded scores, so dbias (a sum over all windows, returned in fp32 for
-// an fp32 table) is exact to fp32 rounding whatever the element type.
+// fp32 and from unrounded scores, so dbias (a sum over all windows, returned in fp32 for an fp32
+// table) is the gradient at the table's own values to fp32 rounding, whatever the element type.
+// (The forward rounds an fp32 table's bias to the element type for its tensor-core operand,
+// scores moved by up to 2^-8 |bias| in bf16; kept unrounded there it would take a second operand
+// as large as the first.)
 //
 // What bounds it: one exponential per score and pass on the SFU (16 per SM and cycle) and
 // about six fp32 operations per score; the products have depth head_dim = 16 or 32, a few
@@ -30,12 +33,14 @@
 // the loads are bounded like the forward kernel's (2 s, then the device error word).  No wait
 // depends on another CTA; sums have a fixed order, so results do not change from run to run.
 //
-// Measured, three heads of 16 channels and 343 tokens: 1372 windows in bf16 rows 561 us, columns
-// 325 us (the exponentials alone 117 us each, with the padding); 343 windows in fp16 178 and 114
-// us, issue slots 42 % and 37 % busy: latency bounds both, in the rows kernel that of the exchange
+// Measured, three heads of 16 channels and 343 tokens: 1372 windows in bf16 rows 557 us, columns
+// 321 us (the exponentials alone 117 us each, with the padding); 343 windows in fp16 162 and 107
+// us, issue slots 42 % and 34 % busy: latency bounds both, in the rows kernel that of the exchange
 // between the warps of a row (its largest stall; one row group alone on an SM takes 348 of 571
-// us).  Measured and not kept in the rows kernel, against 571 us: dp held in registers as well (595
-// to 661 us), two windows' halves in flight (740 us, registers spill).
+// us).  Nearly all columns kernels and the rows kernels of the widest shapes spill (8 to 100 bytes
+// per thread, at 128 to 168 registers).  Measured and not kept in the rows kernel, against 571 us:
+// dp held in registers as well (595 to 661 us), two windows' halves in flight (740 us, registers
+// spill).
 #include <cmath>
 #include <mutex>
 #include <type_traits>

@@ -23,7 +23,8 @@
 // loads from shared memory take 62 % and 69 % of their rate in the first two, FMA 20 %.  Two rows
 // per lane halve those loads but need twice the registers, and came out level (33, 50 us); a tile
 // loaded ahead into registers, too (28, 51, 49 us).  At 16 windows of 216 tokens, three heads of
-// 64 channels, fp32: 69 us forward, 129 us rows, 98 us columns, 92 us bias.
+// 64 channels, fp32: 68 us forward, 127 us rows, 96 us columns, 92 us bias.  (16-bit tensors are
+// multiplied in fp32 here too, at the same rate.)
 #include <cmath>
 
 #include "attention_grad_f32.cuh"

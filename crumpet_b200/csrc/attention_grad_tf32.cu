@@ -2,8 +2,9 @@
 //
 // The formulas of attention_grad.cu.  A product of fp32 numbers is taken as three products of
 // 11-bit (tf32) halves: x = hi + lo with hi = x cut to 11 bits and lo = x - hi (exact) cut
-// likewise, and x y = hi hi + hi lo + lo hi; what is left out, lo lo and the bits cut from lo, is
-// below 2^-20 of |x y| and about 2^-22 on average, the size of an fp32 sum's own rounding.  The
+// likewise, and x y = hi hi + hi lo + lo hi; what is left out, lo lo (below 2^-20 of |x y|) and the
+// bits cut from either lo (below 2^-21 each), is below 2^-19 and about 2^-22 on average, the size of
+// an fp32 sum's own rounding.  The
 // tensor core cuts its sums instead of rounding them, so sums over the tokens are kept in
 // fragments for 32 tokens only and added to fp32 registers.  (An infinity comes out as NaN.)
 //
@@ -19,11 +20,11 @@
 //              operands come straight from global memory, nothing is shared between warps.
 //
 // What bounds it: instructions, not the tensor cores (8.5 cycles per product and SM quarter when
-// they are alone, 16 to 20 % busy here): splitting the staged operands, which every warp does for
+// they are alone, 11 to 24 % busy here): splitting the staged operands, which every warp does for
 // itself, and the softmax.  The bias kernel reads 6 KB per 16 x 32 pairs and window from L2 (3.4
-// TB/s at 343 tokens).  At 64 windows of 125 tokens, three heads of 16 channels: forward 19 us,
-// rows 26 us, columns 21 us, bias 22 us (fp32 arithmetic of attention_grad_simt.cu: 28, 48, 49,
-// 33 us); of 343 tokens: 94, 179, 123 and 81 us, with 32 channels 188, 332, 195 and 110 us.
+// TB/s at 343 tokens).  At 64 windows of 125 tokens, three heads of 16 channels: forward 16 us,
+// rows 26 us, columns 21 us, bias 25 us (fp32 arithmetic of attention_grad_simt.cu: 28, 48, 49,
+// 33 us); of 343 tokens: 93, 181, 123 and 84 us, with 32 channels 156, 331, 193 and 113 us.
 // Measured and not kept, at 125 tokens: two warps per 16 rows that share out the tokens (96 us in
 // all, against 84 us before the third part was added to the sums' operands); tokens staged a tile
 // ahead by asynchronous copies (94 us, the same, and 285 against 202 us at 144 tokens, where the

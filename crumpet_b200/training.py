@@ -233,7 +233,8 @@ def swin_window_attention_train(
     scale: float | None = None,
 ) -> torch.Tensor:
     """:func:`~crumpet_b200.swin_window_attention_qkv` for training: the same result (in
-    fp32 to rounding, about 1e-6), from ``qkv [B, N, 3, H, head_dim]``, the bias ``table
+    fp32 to rounding, about 1e-6; in 16 bits the bias is rounded to them, which the gradient does
+    not see), from ``qkv [B, N, 3, H, head_dim]``, the bias ``table
     [num_buckets, H]`` and its ``buckets`` (of the ``[N, N]`` index), differentiable in ``qkv`` and
     ``table``."""
     place = _place(qkv, table, buckets, num_windows, window_size, shift_size, scale)
@@ -387,8 +388,8 @@ class KeptActivation(NamedTuple):
 
 
 def gelu_checkpoint(x: torch.Tensor) -> tuple[torch.Tensor, KeptActivation]:
-    """``gelu(x)`` (exact, as ``torch.nn.GELU()``) and ``x`` in 8 bits for
-    :func:`gelu_checkpoint_backward`.  Called outside autograd (:func:`checkpointed_mlp` is the
+    """``gelu(x)`` (of the normal distribution, as ``torch.nn.GELU()``; off by at most 0.75e-7 |x|
+    before rounding) and ``x`` in 8 bits for :func:`gelu_checkpoint_backward`.  Called outside autograd (:func:`checkpointed_mlp` is the
     differentiable form)."""
     if _needs_grad(x):
         raise RuntimeError("gelu_checkpoint is not differentiable by itself; use "

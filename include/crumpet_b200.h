@@ -485,7 +485,7 @@ CRUMPET_API int crumpet_norm_gate_residual_backward(
     void* stream);
 
 /*
- * GELU (exact, by the normal distribution) whose input is kept in 8 bits for the backward:
+ * GELU (by the normal distribution, to 0.75e-7 |x|) whose input is kept in 8 bits for the backward:
  *   y = gelu(x);  kept int8 [M, C], scales uint8 [M, ceil(C / 32)]
  * Per 32 neighbouring channels of a row, s = 2^(scale - 127) is the least power of two (not
  * below 2^-126) with max|x| <= 127 s, and kept = rint(x / s), at most 63 in magnitude where 64 s

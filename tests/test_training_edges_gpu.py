@@ -374,3 +374,15 @@ def test_attention_bias_of_one_value(dtype, shift):
     for a, b, tol in zip(got[:2], want, (1.5 * TOL[dtype], TOL[dtype])):
         assert torch.isfinite(a.float()).all()
         assert rel(a, b) <= tol + 2e-3
+
+
+def test_gelu_tails():
+    """Formula 7.1.26 bounds erf's error by 1.5e-7 absolutely, so gelu(x) = x F(x) is off by at most
+    0.75e-7 |x| in all of the tail (and the hardware's exponential and reciprocal, and fp32
+    rounding, by 2^-20 of the value), though not by a part of the value itself."""
+    x = torch.linspace(-14, 14, 1 << 16, device="cuda").view(-1, 32)
+    y, _ = crumpet.gelu_checkpoint(x)
+    want = torch.nn.functional.gelu(x.double())
+    off = (y.double() - want).abs()
+    assert (off <= 0.75e-7 * x.double().abs() + 2.0 ** -20 * want.abs()).all()
+    assert (y[x < -13.5] == 0).all() and torch.equal(y[x > 6], x[x > 6])
