@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import crumpet_b200 as crumpet
-from crumpet_b200 import training
+from crumpet_b200 import fused_attention, training
 from test_training_gpu import BF16, F16, F32, TOL, attention64, attention_case, rel
 
 pytestmark = pytest.mark.gpu
@@ -386,3 +386,20 @@ def test_gelu_tails():
     off = (y.double() - want).abs()
     assert (off <= 0.75e-7 * x.double().abs() + 2.0 ** -20 * want.abs()).all()
     assert (y[x < -13.5] == 0).all() and torch.equal(y[x > 6], x[x > 6])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_inference_attention_small_scale(dtype):
+    """The inference functions follow the same rule, with and without prebuilt tiles."""
+    c = attention_case((3, 3, 3), (2, 2, 2), (1, 1, 1), 1, 2, 16, dtype, F32)
+    c["qkv"][:, :, :2] *= 16
+    c["scale"] = scale = 1e-3
+    want = attention_wide(c)[0]
+    tiles = fused_attention.attention_bias_tiles(c["table"], c["index"], 27, scale, dtype)
+    for t in (None, tiles):
+        got = crumpet.swin_window_attention_qkv(c["qkv"], c["table"], c["index"], **c["place"],
+                                                scale=scale, bias_tiles=t)
+        assert rel(got, want) <= 1.5 * TOL[dtype]
+    with pytest.raises(RuntimeError, match="scale"):
+        torch.ops.crumpet_ops.swin_window_attention_qkv_tiles(
+            torch.empty_like(got), c["qkv"], tiles, [2, 2, 2], [3, 3, 3], [1, 1, 1], scale)
