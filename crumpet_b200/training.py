@@ -534,7 +534,9 @@ def _block_trains(blk, C: int) -> bool:
     path = getattr(blk, "drop_path", None)
     softmax = getattr(attn, "softmax", None)
     heads = int(attn.num_heads)
-    called = {id(m) for top in (attn.qkv, attn.proj) for m in top.modules()}
+    passed_by = (blk, blk.norm1, blk.norm2, path, attn, softmax, attn.attn_drop, attn.proj_drop, mlp,
+                 mlp.linear1, mlp.linear2, mlp.fn, getattr(mlp, "drop1", None),
+                 getattr(mlp, "drop2", None))
     return (C <= MAX_CHANNELS and _fits(blk.norm1, C) and _fits(blk.norm2, C)
             and C % heads == 0 and head_dim_supported(C // heads)
             and (softmax is None or _plain(softmax, torch.nn.Softmax) and softmax.dim == -1)
@@ -547,7 +549,7 @@ def _block_trains(blk, C: int) -> bool:
                                 and getattr(path, "scale_by_keep", True)))
             and not getattr(blk, "use_checkpoint", False)
             and not torch.nn.modules.module._has_any_global_hook()
-            and not any(_hooked(m) for m in blk.modules() if id(m) not in called))
+            and not any(m is not None and _hooked(m) for m in passed_by))
 
 
 def _path_scale(blk, samples: int, device) -> torch.Tensor | None:
